@@ -81,16 +81,18 @@ public:
         if (!handle_) throw Error(err, "tt_hip_kv_create_quantized");
     }
     // A ring for sliding-window layers: the row of position p lives at p % ringCapacity (KVCacheManager.ringCapacity).
+    // With sinks, the first that many positions keep rows of their own in front of it.
     struct Ring {
         int capacity;
+        int sinks = 0;
     };
     KVCacheManager(Context &context, int layers, int kvHeads, int headDim, int slots, int maxContext, Ring ring,
                    KVCachePrecision precision = KVCachePrecision::fp16)
         : context_(context) {
         int err = 0;
-        handle_ = tt_hip_kv_create_ring(context.handle(), layers, kvHeads, headDim, slots, ring.capacity, maxContext,
-                                        (int)precision, &err);
-        if (!handle_) throw Error(err, "tt_hip_kv_create_ring");
+        handle_ = tt_hip_kv_create_ring_sinks(context.handle(), layers, kvHeads, headDim, slots, ring.capacity, ring.sinks, maxContext,
+                                              (int)precision, &err);
+        if (!handle_) throw Error(err, "tt_hip_kv_create_ring_sinks");
     }
     KVCachePrecision precision() const { return (KVCachePrecision)tt_hip_kv_precision_bits(handle_); }
     // Rows in the stored row format (device memory, rowStrideBytes apart); null skips a side on export.
@@ -178,11 +180,11 @@ public:
                                          scale, out),
               "Attention.encodeFullNoAlloc");
     }
-    // Attention.encodeSWA (Attention.swift:229-266): keys [max(0, seqLen - window), seqLen); no ring storage.
+    // Attention.encodeSWA (Attention.swift:229-266): keys [max(0, seqLen - window), seqLen), and with sinks the keys [0, sinks) beside them.
     void encodeSWA(KVCacheManager &kv, int layer, const tt_half *q, tt_half *out, int numQHeads, int seqLen, int window,
-                   float scale, int slot = 0, const tt_half *gate = nullptr) {
-        check(tt_hip_attn_decode_swa(context_.handle(), kv.handle(), layer, 1, &slot, &seqLen, window, numQHeads, q, gate,
-                                     scale, out),
+                   float scale, int slot = 0, const tt_half *gate = nullptr, int sinks = 0) {
+        check(tt_hip_attn_decode_sinks(context_.handle(), kv.handle(), layer, 1, &slot, &seqLen, window, sinks, numQHeads, q, gate,
+                                       scale, out),
               "Attention.encodeSWA");
     }
     // Attention.encodeFull(..., keepMask:): one byte per key position, 0 drops the key (a QSA layer's selection).
@@ -211,10 +213,10 @@ public:
     // encodeFullAttentionDecodeOrderRows: row r attends start + r + 1 keys.
     void encodeVerifyRows(KVCacheManager &kv, int layer, const std::vector<int> &slots,
                           const std::vector<int> &startPositions, int rows, const tt_half *q, tt_half *out,
-                          int numQHeads, float scale, const tt_half *gate = nullptr, int window = 0) {
+                          int numQHeads, float scale, const tt_half *gate = nullptr, int window = 0, int sinks = 0) {
         if (slots.size() != startPositions.size()) throw Error(TT_HIP_ERR_INVALID_ARGUMENT, "Attention.encodeVerifyRows");
-        check(tt_hip_attn_verify_swa(context_.handle(), kv.handle(), layer, (int)slots.size(), slots.data(),
-                                     startPositions.data(), rows, window, numQHeads, q, gate, scale, out),
+        check(tt_hip_attn_verify_sinks(context_.handle(), kv.handle(), layer, (int)slots.size(), slots.data(),
+                                       startPositions.data(), rows, window, sinks, numQHeads, q, gate, scale, out),
               "Attention.encodeVerifyRows");
     }
 
@@ -233,6 +235,7 @@ struct PrefillAttentionParams {
     size_t oStride = 0;
     size_t gateStride = 0;
     int slidingWindow = 0;  // 0: every key up to the row's own
+    int sinks = 0;          // with a window: the first keys that stay visible
 };
 
 class PrefillAttention {
@@ -240,9 +243,9 @@ public:
     explicit PrefillAttention(Context &context) : context_(context) {}
     void encodeCausal(KVCacheManager &kv, int layer, int slot, const tt_half *q, tt_half *out,
                       const PrefillAttentionParams &p, const tt_half *gate = nullptr) {
-        check(tt_hip_attn_prefill_swa(context_.handle(), kv.handle(), layer, slot, p.startPosition, p.queryCount,
-                                      p.kvValidCount, p.slidingWindow, p.numQHeads, q, p.qStride, gate,
-                                      p.gateStride ? p.gateStride : p.qStride, p.scale, out, p.oStride),
+        check(tt_hip_attn_prefill_sinks(context_.handle(), kv.handle(), layer, slot, p.startPosition, p.queryCount,
+                                        p.kvValidCount, p.slidingWindow, p.sinks, p.numQHeads, q, p.qStride, gate,
+                                        p.gateStride ? p.gateStride : p.qStride, p.scale, out, p.oStride),
               "PrefillAttention.encodeCausal");
     }
     // encodeCausal(..., keepMask:, keepStride:) of a QSA chunk, mask form: a row of keepStride bytes per query.

@@ -237,6 +237,21 @@ TT_HIP_API int tt_hip_kv_precision_bits(const tt_hip_kv *kv); /* 16, 8 or 4; -1 
 TT_HIP_API tt_hip_kv *tt_hip_kv_create_ring(tt_hip_ctx *ctx, int n_layers, int n_kv_heads, int head_dim, int n_slots,
                                             int ring_capacity_tokens, int max_context_tokens, int bits, int *out_err);
 
+/* Such a ring for layers whose window has sinks (tt_hip_attn_decode_sinks): the first sink_tokens positions, rounded up to a
+ * whole block of 32, keep rows of their own at the page's front, and the ring of ring_capacity_tokens goes round behind them: with
+ * S the rounded sinks and R the rounded ring, the row of position p lives at p for p < S and at S + (p - S) % R from there on.
+ * A session then runs to max_context_tokens in S + R rows of memory and never loses its first tokens.  No counterpart in the
+ * reference, whose ring overwrites them.  Everything as for tt_hip_kv_create_ring, but:
+ *   capacity  S + R (or max_context_tokens where that is less: then nothing ever comes round and nothing is pinned);
+ *   rows      a range may not cross the place where the ring comes round;
+ *   keys      the windowed calls (_swa, _sinks; window + rows + 30 <= R serves every position) know where the rows lie; the calls
+ *             without a window and those over key selections serve such a cache while the sequence fits the capacity, else
+ *             TT_HIP_ERR_CAPACITY.
+ * sink_tokens 0 is tt_hip_kv_create_ring. */
+TT_HIP_API tt_hip_kv *tt_hip_kv_create_ring_sinks(tt_hip_ctx *ctx, int n_layers, int n_kv_heads, int head_dim, int n_slots,
+                                                  int ring_capacity_tokens, int sink_tokens, int max_context_tokens, int bits,
+                                                  int *out_err);
+
 /* KVCacheManager.rowLayout (KVCacheManager+Validation.swift:30-41): bytes per stored token row and
  * bytes of its packed levels (rounded up to 2), for a row of `elements` values.  Pure host
  * arithmetic; 512 elements -> 1024 / 544 / 288 bytes at 16 / 8 / 4 bits. */
@@ -449,6 +464,24 @@ TT_HIP_API int tt_hip_attn_prefill_swa(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer
 TT_HIP_API int tt_hip_attn_verify_swa(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, const int *slots,
                                       const int *start_positions, int rows, int window, int n_q_heads,
                                       const tt_half *q, const tt_half *gate, float scale, tt_half *out);
+
+/* A sliding window and a few first tokens that stay visible, the sinks: the row at absolute position p attends keys j <= p with
+ * j > p - window or j < sinks.  What a model needs that keeps a part of its attention on the first tokens when a session outgrows
+ * its window (no counterpart in the reference); sinks 0 is the _swa form, window 0 every key, and a row whose window reaches down to
+ * the sinks sees every key once.  Decode, verify and chunk as in the _swa forms, which they extend by one argument; caches of every
+ * precision, linear or ring.  A ring has to keep the sinks: tt_hip_kv_create_ring_sinks with at least `sinks` tokens, else
+ * TT_HIP_ERR_CAPACITY as soon as the sequence has outgrown the ring.
+ * A call reads the blocks of the sinks and of the window, as one run of blocks, and nothing between them. */
+TT_HIP_API int tt_hip_attn_decode_sinks(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, const int *slots,
+                                        const int *seq_lens, int window, int sinks, int n_q_heads, const tt_half *q,
+                                        const tt_half *gate, float scale, tt_half *out);
+TT_HIP_API int tt_hip_attn_verify_sinks(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, const int *slots,
+                                        const int *start_positions, int rows, int window, int sinks, int n_q_heads,
+                                        const tt_half *q, const tt_half *gate, float scale, tt_half *out);
+TT_HIP_API int tt_hip_attn_prefill_sinks(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int slot, int start_pos, int q_len,
+                                         int kv_valid, int sliding_window, int sinks, int n_q_heads, const tt_half *q,
+                                         size_t q_stride, const tt_half *gate, size_t gate_stride, float scale, tt_half *out,
+                                         size_t o_stride);
 
 /* Multi-row verify (MTP pair / wide verify): replaces
  * encodeFullAttentionDecodeOrderRows (RealForwardRunner+VerifyDecodeOrderAttention.swift:52-110)

@@ -64,6 +64,7 @@ _SIGNATURES = {
     "tt_hip_kv_create": (_vp, [_vp, _i, _i, _i, _i, _i, _i, _c_int_p]),
     "tt_hip_kv_create_quantized": (_vp, [_vp, _i, _i, _i, _i, _i, _i, _i, _c_int_p]),
     "tt_hip_kv_create_ring": (_vp, [_vp, _i, _i, _i, _i, _i, _i, _i, _c_int_p]),
+    "tt_hip_kv_create_ring_sinks": (_vp, [_vp, _i, _i, _i, _i, _i, _i, _i, _i, _c_int_p]),
     "tt_hip_kv_precision_bits": (_i, [_vp]),
     "tt_hip_kv_row_layout": (_i, [_i, _i, ctypes.POINTER(ctypes.c_size_t), ctypes.POINTER(ctypes.c_size_t)]),
     "tt_hip_kv_export_rows": (_i, [_vp, _i, _i, _i, _i, _vp, _vp, _sz]),
@@ -95,6 +96,9 @@ _SIGNATURES = {
                                               _sz]),
     "tt_hip_attn_prefill_swa": (_i, [_vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _sz, _vp, _sz, ctypes.c_float, _vp, _sz]),
     "tt_hip_attn_verify_swa": (_i, [_vp, _vp, _i, _i, _c_int_p, _c_int_p, _i, _i, _i, _vp, _vp, ctypes.c_float, _vp]),
+    "tt_hip_attn_decode_sinks": (_i, [_vp, _vp, _i, _i, _c_int_p, _c_int_p, _i, _i, _i, _vp, _vp, ctypes.c_float, _vp]),
+    "tt_hip_attn_verify_sinks": (_i, [_vp, _vp, _i, _i, _c_int_p, _c_int_p, _i, _i, _i, _i, _vp, _vp, ctypes.c_float, _vp]),
+    "tt_hip_attn_prefill_sinks": (_i, [_vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _sz, _vp, _sz, ctypes.c_float, _vp, _sz]),
     "tt_hip_attn_verify": (_i, [_vp, _vp, _i, _i, _c_int_p, _c_int_p, _i, _i, _vp, _vp, ctypes.c_float, _vp]),
     "tt_hip_kv_snapshot_segment_count": (_i, [_vp]),
     "tt_hip_kv_snapshot_segment_lengths": (_i, [_vp, _i, ctypes.POINTER(ctypes.c_size_t), _i]),

@@ -58,8 +58,12 @@ __device__ __forceinline__ h8 load_h8(global_halves p) {
 struct TileInfo {
     int kvh, hsub, tok_tile, t0, tile_rows, tile_end, start, total;
     int k0;  // first key of split 0: 0, or the block that holds the first key the tile's first row sees through its window
+    // A window with sinks: the tile walks the blocks [0, sink_blocks) and, `skipped` blocks further on, those of its window, one
+    // behind the other: k0 and tile_end count along that walk.
+    int sink_blocks, skipped;
 };
 
+template <bool SINKS = false>
 __device__ __forceinline__ TileInfo tile_info(const SplitKHot &a, const SplitKSeq &sq, int tile) {
     TileInfo t;
     if (a.tok_tiles == 1 && a.hsubs == 1) {  // a decode step, a verify pass of a few rows: a tile is a KV head
@@ -78,6 +82,12 @@ __device__ __forceinline__ TileInfo tile_info(const SplitKHot &a, const SplitKSe
     t.tile_end = max(0, min(t.total, t.start + t.t0 + t.tile_rows));  // keys visible to the tile's last row
     const int first_lim = min(t.total, t.start + t.t0 + 1);
     t.k0 = (a.window > 0 && first_lim > a.window) ? ((first_lim - a.window) & ~31) : 0;
+    if constexpr (SINKS) {
+        t.sink_blocks = min((a.keep_words + 31) >> 5, t.k0 >> 5);  // (a window that reaches down to the sinks: one run of blocks)
+        t.skipped = (t.k0 >> 5) - t.sink_blocks;
+        t.k0 = 0;
+        t.tile_end = max(0, t.tile_end - 32 * t.skipped);
+    }
     return t;
 }
 
@@ -353,7 +363,8 @@ template <int D, int NT>
 __device__ __forceinline__ void block_softmax(RowState<D, NT> &st, Scores<D, NT> &sc, Probs<D, NT> &pr,
                                               const Lane<D, NT> &ln, int kbase, int lo, int lim, float scale_log2e,
                                               typename RowState<D, NT>::acc_t *extra = nullptr, unsigned kept = ~0u,
-                                              const unsigned *row_keep = nullptr, unsigned row_bits = ~0u) {
+                                              const unsigned *row_keep = nullptr, unsigned row_bits = ~0u, int sinks = 0) {
+    // sinks: keys below it are seen although they lie below `lo`.
     // kept: bit i set = key kbase + i takes part (a sparse selection shared by the tile's rows; all ones without one).
     // row_keep: this lane's own row's 32 selection bytes of the block, as 8 words (a per-query selection).
     // row_bits: the same as one bit per key (a per-query selection that came as index lists); all ones without one.
@@ -382,7 +393,7 @@ __device__ __forceinline__ void block_softmax(RowState<D, NT> &st, Scores<D, NT>
 #pragma unroll
             for (int v = 0; v < 16; ++v) {
                 const int key = kbase + 8 * (v >> 2) + 4 * ln.g + (v & 3);
-                if (key >= lim || key < lo) s[v] = -INFINITY;
+                if (key >= lim || (key < lo && key >= sinks)) s[v] = -INFINITY;
             }
         }
         if (kept != ~0u) {
@@ -429,9 +440,9 @@ __device__ __forceinline__ void block_softmax(RowState<D, NT> &st, Scores<D, NT>
         for (int v = 0; v < 4; ++v) {
             float xa = sa[v] * scale_log2e, xb = sb[v] * scale_log2e;
             if (need_mask) {
-                if (key0 + v >= lim || key0 + v < lo || !((kept & row_bits) >> (key0 + v - kbase) & 1u) || !((rk[0] >> (8 * v)) & 0xffu))
+                if (key0 + v >= lim || (key0 + v < lo && key0 + v >= sinks) || !((kept & row_bits) >> (key0 + v - kbase) & 1u) || !((rk[0] >> (8 * v)) & 0xffu))
                     xa = -INFINITY;
-                if (key0 + 8 + v >= lim || key0 + 8 + v < lo || !((kept & row_bits) >> (key0 + 8 + v - kbase) & 1u) ||
+                if (key0 + 8 + v >= lim || (key0 + 8 + v < lo && key0 + 8 + v >= sinks) || !((kept & row_bits) >> (key0 + 8 + v - kbase) & 1u) ||
                     !((rk[1] >> (8 * v)) & 0xffu))
                     xb = -INFINITY;
             }
@@ -460,13 +471,49 @@ __device__ __forceinline__ void block_softmax(RowState<D, NT> &st, Scores<D, NT>
     }
 }
 
+// Halves 8 c .. 8 c + 7 of a V block's chunk c (fp16 values, or scales or biases of a quantised block) without those of keys that no
+// row of the tile sees (`seen`: bit i = key i of the block is seen): whatever such a row of the cache holds -- an older sequence's
+// values, an infinity -- a probability of zero would make NaN of it.
+__device__ __forceinline__ void seen_words(unsigned (&mask)[4], int chunk, unsigned seen) {
+    const unsigned lo = seen >> (16 * (chunk >> 1) + 4 * (chunk & 1)), hi = lo >> 8;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        mask[w] = ((lo >> (2 * w)) & 1u ? 0xffffu : 0u) | ((lo >> (2 * w + 1)) & 1u ? 0xffff0000u : 0u);
+        mask[2 + w] = ((hi >> (2 * w)) & 1u ? 0xffffu : 0u) | ((hi >> (2 * w + 1)) & 1u ? 0xffff0000u : 0u);
+    }
+}
+__device__ __forceinline__ h8 only_seen(h8 x, const unsigned (&mask)[4]) {
+    typedef unsigned words __attribute__((ext_vector_type(4)));
+    const words m = {mask[0], mask[1], mask[2], mask[3]};
+    return __builtin_bit_cast(h8, __builtin_bit_cast(words, x) & m);
+}
+template <int D, int NT>
+__device__ __forceinline__ void drop_unseen(VTile<D, NT> &vt, const Lane<D, NT> &ln, unsigned seen) {
+    if constexpr (NT == 32) {
+        unsigned mask[2][4];
+        seen_words(mask[0], ln.g, seen);
+        seen_words(mask[1], 2 + ln.g, seen);
+#pragma unroll
+        for (int mt = 0; mt < D / 32; ++mt)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) vt.f[mt][t] = only_seen(vt.f[mt][t], mask[t]);
+    } else {
+        unsigned mask[4];
+        seen_words(mask, ln.g, seen);
+#pragma unroll
+        for (int mt = 0; mt < D / 16; ++mt) vt.f[mt] = only_seen(vt.f[mt], mask);
+    }
+}
+
 // Phase 2b: O^T += V^T P^T.
 template <int D, int NT>
-__device__ __forceinline__ void block_softmax_pv(RowState<D, NT> &st, Scores<D, NT> &sc, const VTile<D, NT> &vt,
+__device__ __forceinline__ void block_softmax_pv(RowState<D, NT> &st, Scores<D, NT> &sc, VTile<D, NT> &vt,
                                                  const Lane<D, NT> &ln, int kbase, int lo, int lim, float scale_log2e,
-                                                 unsigned kept = ~0u, const unsigned *row_keep = nullptr, unsigned row_bits = ~0u) {
+                                                 unsigned kept = ~0u, const unsigned *row_keep = nullptr, unsigned row_bits = ~0u,
+                                                 int sinks = 0, unsigned seen = ~0u) {
     Probs<D, NT> pr;
-    block_softmax<D, NT>(st, sc, pr, ln, kbase, lo, lim, scale_log2e, nullptr, kept, row_keep, row_bits);
+    block_softmax<D, NT>(st, sc, pr, ln, kbase, lo, lim, scale_log2e, nullptr, kept, row_keep, row_bits, sinks);
+    if (seen != ~0u) drop_unseen<D, NT>(vt, ln, seen);
     if constexpr (NT == 32) {
 #pragma unroll
         for (int mt = 0; mt < D / 32; ++mt)
@@ -501,9 +548,10 @@ template <int AUX, int D>
 __device__ __forceinline__ void block_softmax_pv_refill(RowState<D, 32> &st, Scores<D, 32> &sc, VTile<D, 32> &vt,
                                                         const Lane<D, 32> &ln, int kbase, int lo, int lim, float scale_log2e,
                                                         __amdgpu_buffer_rsrc_t rv, unsigned next_bytes, const Voids<D, 32> &vo,
-                                                        unsigned kept, const unsigned *row_keep, unsigned row_bits) {
+                                                        unsigned kept, const unsigned *row_keep, unsigned row_bits, int sinks, unsigned seen) {
     Probs<D, 32> pr;
-    block_softmax<D, 32>(st, sc, pr, ln, kbase, lo, lim, scale_log2e, nullptr, kept, row_keep, row_bits);
+    block_softmax<D, 32>(st, sc, pr, ln, kbase, lo, lim, scale_log2e, nullptr, kept, row_keep, row_bits, sinks);
+    if (seen != ~0u) drop_unseen<D, 32>(vt, ln, seen);
     const unsigned lane_bytes[2] = {(unsigned)ln.voff * 2u + vo.v[0], (unsigned)ln.voff * 2u + vo.v[1]};
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -860,14 +908,39 @@ __device__ __forceinline__ void block_softmax_pv(RowState<D, NT> &st, Scores<D, 
                                                  const Lane<D, NT> &ln, int kbase, int lo, int lim, float scale_log2e,
                                                  typename RowState<D, NT>::acc_t &bias_acc, __amdgpu_buffer_rsrc_t rv,
                                                  unsigned next_bytes, const Voids<D, NT> &vo, unsigned kept = ~0u,
-                                                 const unsigned *row_keep = nullptr, unsigned row_bits = ~0u) {
+                                                 const unsigned *row_keep = nullptr, unsigned row_bits = ~0u, int sinks = 0,
+                                                 unsigned seen = ~0u) {
     typedef QuantOffsets<D, NT, BITS> O;
     constexpr int GPH = D / 64;
     const unsigned lane_bytes = O::v_lane(ln);
     const unsigned param_lane = (unsigned)ln.g * 16 + vo.all;
     const unsigned bias_lane = (unsigned)ln.li * 64 + (unsigned)ln.g * 16 + ((unsigned)ln.li < (unsigned)GPH ? vo.all : kVoidLoad);
     Probs<D, NT> pr;
-    block_softmax<D, NT>(st, sc, pr, ln, kbase, lo, lim, scale_log2e, &bias_acc, kept, row_keep, row_bits);
+    block_softmax<D, NT>(st, sc, pr, ln, kbase, lo, lim, scale_log2e, &bias_acc, kept, row_keep, row_bits, sinks);
+    if (seen != ~0u) {  // (levels are finite whatever they are)
+        if constexpr (NT == 32) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                unsigned mask[4];
+                seen_words(mask, 2 * t + ln.g, seen);
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    vt.bias[t][w] &= mask[w];
+#pragma unroll
+                    for (int grp = 0; grp < GPH; ++grp) vt.sc[grp][t][w] &= mask[w];
+                }
+            }
+        } else {
+            unsigned mask[4];
+            seen_words(mask, ln.g, seen);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                vt.bias[w] &= mask[w];
+#pragma unroll
+                for (int grp = 0; grp < GPH; ++grp) vt.sc[grp][w] &= mask[w];
+            }
+        }
+    }
     if constexpr (NT == 32) {
         h8 ps[GPH][2];
 #pragma unroll
@@ -941,6 +1014,9 @@ __device__ __forceinline__ void block_softmax_pv(RowState<D, NT> &st, Scores<D, 
 // KEEP = 4: the same, where few of a touched block's keys are listed (fp16 pages, tiles of 32): the plan lists groups of
 // four keys, and eight listed groups, wherever they lie, make a turn of the loop.
 // KEEP = 5: KEEP = 3 whose blocks' loads cover the listed keys only (lists_fetch_by_key).
+// KEEP = kKeepSinks: a window whose rows also see the first tokens, the sinks.  A tile walks the sinks' blocks and its window's as
+// one run (TileInfo), so a wavefront goes from one to the other like from block to block -- no pass of its own for a piece that
+// is mostly one block -- and a block's place is looked up from its number in the walk.
 // The hot arguments, this workgroup's sequence entry and where the rows go and their gate beside them, by five scalar loads issued
 // together (the compiler would fetch each field where it is first used: five or six dependent trips to the kernarg segment before
 // the first K/V load can go out, about 0.15 us each, and another ahead of the gate's loads).
@@ -998,7 +1074,7 @@ __device__ __forceinline__ void load_row_words(unsigned (&dst)[8], __amdgpu_buff
 }
 
 template <int D, int NT, int WAVES, int BITS, int KEEP = 0, int STREAM = 0>
-__global__ __launch_bounds__(WAVES * 64, (NT == 16 && KEEP < 2 ? 2 : 1)) void attn_splitk_kernel(const SplitKArgs args) {
+__global__ __launch_bounds__(WAVES * 64, (NT == 16 && (KEEP < 2 || KEEP == kKeepSinks) ? 2 : 1)) void attn_splitk_kernel(const SplitKArgs args) {
     constexpr bool PAIRED = STREAM == 2;
     static_assert(!PAIRED || (D == 256 && NT == 32 && BITS == 16 && KEEP == 0));
     constexpr int AUX = (STREAM ? kStreamed : 0) | (PAIRED ? kPaired : 0);
@@ -1032,7 +1108,8 @@ __global__ __launch_bounds__(WAVES * 64, (NT == 16 && KEEP < 2 ? 2 : 1)) void at
         split = (int)(pair / (unsigned)a.n_tiles);
         tile = (int)(pair - (unsigned)split * (unsigned)a.n_tiles);
     }
-    const TileInfo ti = tile_info(a, sq, tile);
+    constexpr bool SINKS = KEEP == kKeepSinks;
+    const TileInfo ti = tile_info<SINKS>(a, sq, tile);
     const int k_begin = ti.k0 + split * a.split_len;
     if (k_begin >= ti.tile_end && split != 0) return;  // split 0 always runs so that an empty range yields zeros
     const int k_end = min(k_begin + a.split_len, ti.tile_end);
@@ -1255,8 +1332,21 @@ __global__ __launch_bounds__(WAVES * 64, (NT == 16 && KEEP < 2 ? 2 : 1)) void at
         plan_bits_tile = args.plan_bits + (size_t)ti.tok_tile * (args.plan_cap >> 3) * a.tt;
         b = b_end;  // (the walk over blocks finds nothing)
     }
+    // Block `i` of the walk: its number among the sequence's blocks, and that one's place in the page.
+    auto walked_block = [&](int i) { return SINKS && i >= ti.sink_blocks ? i + ti.skipped : i; };
+    auto page_block = [&](int i) {
+        const int block = walked_block(i);
+        if constexpr (SINKS) {
+            const int pinned = a.flags >> kHotPinnedShift;
+            return a.ring_blocks && block >= pinned ? pinned + (block - pinned) % a.ring_blocks : block;
+        }
+        return a.ring_blocks ? block % a.ring_blocks : block;
+    };
+    const int sinks = SINKS ? a.keep_words : 0;
+    const int first_lim = min(ti.total, ti.start + ti.t0 + 1), seen_from = a.window > 0 ? max(first_lim - a.window, 0) : 0;
+    const int seen_end = ti.tile_end + 32 * ti.skipped;  // (SINKS) keys up to the tile's last row's own
     const bool first_real = b < b_end;
-    const unsigned first_bytes = first_real ? (unsigned)(a.ring_blocks ? b % a.ring_blocks : b) * BLK_BYTES : 0u;
+    const unsigned first_bytes = first_real ? (unsigned)page_block(b) * BLK_BYTES : 0u;
     Voids<D, NT> first_void(first_real ? 0u : kVoidLoad);
     if constexpr (BY_KEY) first_void = Voids<D, NT>(first_real ? 0u : kVoidLoad, first_keys, ln);
     if constexpr (KEEP == 4) {
@@ -1384,21 +1474,27 @@ __global__ __launch_bounds__(WAVES * 64, (NT == 16 && KEEP < 2 ? 2 : 1)) void at
             row_bits = bits_cur;
         }
         const bool real = nb < b_end && next_kept;
-        const unsigned next = real ? (unsigned)(a.ring_blocks ? nb % a.ring_blocks : nb) * BLK_BYTES : 0u;
+        const unsigned next = real ? (unsigned)page_block(nb) * BLK_BYTES : 0u;
+        const int kbase = walked_block(b) << 5;
+        unsigned seen = ~0u;  // the block's keys that some row of the tile sees
+        if constexpr (SINKS) {
+            auto below = [](int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; };
+            seen = below(seen_end - kbase) & (below(sinks - kbase) | ~below(seen_from - kbase));
+        }
         Voids<D, NT> vo(real ? 0u : kVoidLoad);
         if constexpr (BY_KEY) vo = Voids<D, NT>(real ? 0u : kVoidLoad, next_keys, ln);
         if constexpr (BITS == 16 && NT == 32) {
             block_scores_refill<AUX, D>(sc, kt, qf, rk, next, ln, vo);
-            block_softmax_pv_refill<AUX, D>(st, sc, vt, ln, b << 5, lo, lim, a.scale_log2e, rv, next, vo, kept, row_keep, row_bits);
+            block_softmax_pv_refill<AUX, D>(st, sc, vt, ln, kbase, lo, lim, a.scale_log2e, rv, next, vo, kept, row_keep, row_bits, sinks, seen);
         } else if constexpr (BITS == 16) {
             block_scores(sc, kt, qf, qlds, lane);
             load_k<AUX>(kt, rk, next, ln, vo);
-            block_softmax_pv<D, NT>(st, sc, vt, ln, b << 5, lo, lim, a.scale_log2e, kept, row_keep, row_bits);
+            block_softmax_pv<D, NT>(st, sc, vt, ln, kbase, lo, lim, a.scale_log2e, kept, row_keep, row_bits, sinks, seen);
             load_v<AUX>(vt, rv, next, ln, vo);
         } else {  // the phases refill their tiles as they go
             block_scores<AUX, D, NT, BITS>(sc, kt, qf, qlds, lane, rk, next, ln, vo);
-            block_softmax_pv<AUX, D, NT, BITS>(st, sc, vt, ln, b << 5, lo, lim, a.scale_log2e, bias_acc, rv, next, vo, kept,
-                                          row_keep, row_bits);
+            block_softmax_pv<AUX, D, NT, BITS>(st, sc, vt, ln, kbase, lo, lim, a.scale_log2e, bias_acc, rv, next, vo, kept,
+                                          row_keep, row_bits, sinks, seen);
         }
         if constexpr (KEEP == 1) {
             keep_cur = keep_next;
@@ -1539,7 +1635,7 @@ __device__ __forceinline__ int splits_of(const TileInfo &ti, int split_len) {
     return (int)((unsigned)(max(ti.tile_end - ti.k0, 1) + split_len - 1) / (unsigned)split_len);  // (an empty range has one, of zeros)
 }
 
-template <int D, int NT>
+template <int D, int NT, bool SINKS>
 __global__ __launch_bounds__(256) void attn_combine_kernel([[maybe_unused]] const SplitKArgs args) {  // (load_args reads them)
     constexpr int DCH = D / 64;
     __shared__ float sm[4][68];
@@ -1549,7 +1645,7 @@ __global__ __launch_bounds__(256) void attn_combine_kernel([[maybe_unused]] cons
     SplitKSeq sq;
     SplitKOut out;
     load_args(a, sq, out, seq);
-    const TileInfo ti = tile_info(a, sq, tile);
+    const TileInfo ti = tile_info<SINKS>(a, sq, tile);
     if (n >= ti.tile_rows * a.gh) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int n_splits = splits_of(ti, a.split_len);
@@ -1646,7 +1742,7 @@ __global__ __launch_bounds__(256) void attn_combine_kernel([[maybe_unused]] cons
 // grid = (NT / 4, tile, sequence), 256 threads.
 constexpr int kCombineRowsSplits = 16;
 
-template <int D, int NT>
+template <int D, int NT, bool SINKS>
 __global__ __launch_bounds__(256) void attn_combine_rows_kernel([[maybe_unused]] const SplitKArgs args) {  // (load_args reads them)
     constexpr int D4 = D / 4, ROWS = 4;
     static_assert(ROWS * D4 <= 256, "an item a thread");
@@ -1655,7 +1751,7 @@ __global__ __launch_bounds__(256) void attn_combine_rows_kernel([[maybe_unused]]
     SplitKSeq sq;
     SplitKOut out;
     load_args(a, sq, out, seq);
-    const TileInfo ti = tile_info(a, sq, tile);
+    const TileInfo ti = tile_info<SINKS>(a, sq, tile);
     const int n = blockIdx.x * ROWS + (int)threadIdx.x / D4, d = ((int)threadIdx.x % D4) * 4;
     if ((int)threadIdx.x >= ROWS * D4 || n >= ti.tile_rows * a.gh) return;
     const int n_splits = splits_of(ti, a.split_len);
@@ -1829,7 +1925,7 @@ int plan_launch(const tt_hip_ctx *ctx, int kind, int n_seq, int n_q_heads, int n
     return TT_HIP_OK;
 }
 
-template <int D, int NT>
+template <int D, int NT, bool SINKS>
 static int launch_combine_one(tt_hip_ctx *ctx, const LaunchPlan &plan, int n_seq, const SplitKArgs &args) {
     // Many tiles with few splits each: from 64 of its workgroups on (8 sequences' decode rows, 4 sequences' verify
     // rows; a verify pass of 8 x 4 rows at 65k keys 174.5 -> 170.1 us a step, 8 sequences x 8 rows at 4k keys 36.9 ->
@@ -1838,12 +1934,12 @@ static int launch_combine_one(tt_hip_ctx *ctx, const LaunchPlan &plan, int n_seq
     const bool near = (unsigned long long)plan.n_tiles * NT * D * sizeof(float) * kCombineRowsSplits <= 0xffffffffull;
     if (near && plan.n_splits_max <= 2 * kCombineRowsSplits && (long long)plan.n_tiles * n_seq * (NT / 4) >= 64) {
         dim3 cgrid((unsigned)(NT / 4), (unsigned)plan.n_tiles, (unsigned)n_seq);
-        hipLaunchKernelGGL((attn_combine_rows_kernel<D, NT>), cgrid, dim3(256), 0, ctx->stream, args);
+        hipLaunchKernelGGL((attn_combine_rows_kernel<D, NT, SINKS>), cgrid, dim3(256), 0, ctx->stream, args);
     } else {
         // (a workgroup per row that a tile can have and 64 dims of it: tiles of 16 with 8 rows in use launch no idle half)
         const int tile_rows = args.hot.rows < plan.tt ? args.hot.rows : plan.tt;
         dim3 cgrid((unsigned)(tile_rows * plan.gh * (D / 64)), (unsigned)plan.n_tiles, (unsigned)n_seq);
-        hipLaunchKernelGGL((attn_combine_kernel<D, NT>), cgrid, dim3(256), 0, ctx->stream, args);
+        hipLaunchKernelGGL((attn_combine_kernel<D, NT, SINKS>), cgrid, dim3(256), 0, ctx->stream, args);
     }
     hipError_t e = hipGetLastError();
     return e == hipSuccess ? TT_HIP_OK : hip_fail(ctx, e, "attn_combine_kernel launch");
@@ -1858,7 +1954,7 @@ static int launch_one(tt_hip_ctx *ctx, const LaunchPlan &plan, int n_seq, const 
     launch_profiled(ctx, kernel, grid, dim3(WAVES * 64), (unsigned)(plan.lds_bytes + keep_list_bytes(KEEP, WAVES)), args);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return hip_fail(ctx, e, "attn_splitk_kernel launch");
-    if (plan.n_splits_max > 1 && !ctx->pass_only) return launch_combine_one<D, NT>(ctx, plan, n_seq, args);
+    if (plan.n_splits_max > 1 && !ctx->pass_only) return launch_combine_one<D, NT, KEEP == kKeepSinks>(ctx, plan, n_seq, args);
     return TT_HIP_OK;
 }
 
@@ -1875,7 +1971,7 @@ static hipError_t configure_one() {
             e = hipFuncSetAttribute(reinterpret_cast<const void *>(attn_splitk_kernel<D, NT, 4, BITS, KEEP, 2>),
                                     hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_bytes_for(D, NT, 4));
     }
-    if constexpr (KEEP < 2) {  // (a chunk's per-query selections come with many token tiles: never streamed)
+    if constexpr (KEEP < 2 || KEEP == kKeepSinks) {  // (a chunk's per-query selections come with many token tiles: never streamed)
         if (e == hipSuccess)
             e = hipFuncSetAttribute(reinterpret_cast<const void *>(attn_splitk_kernel<D, NT, 4, BITS, KEEP, 1>),
                                     hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_bytes_for(D, NT, 4));
@@ -1894,6 +1990,7 @@ static hipError_t configure_tile() {
     TT_CFG(8, 3) TT_CFG(4, 3)
     if constexpr (NT == 32) { TT_CFG(16, 4) }
     if constexpr (lists_fetch_by_key(D, 16)) { TT_CFG(16, 5) }
+    TT_CFG(16, kKeepSinks) TT_CFG(8, kKeepSinks) TT_CFG(4, kKeepSinks)
 #undef TT_CFG
     return e;
 }
@@ -1911,7 +2008,7 @@ int configure_splitk_kernels(tt_hip_ctx *ctx) {
 int launch_combine(tt_hip_ctx *ctx, const LaunchPlan &plan, int head_dim, int n_seq, const SplitKArgs &args) {
     if (plan.n_tiles > 65535 || n_seq > 65535) return TT_HIP_ERR_SHAPE;
 #define TT_CASE(DD, NN) \
-    if (head_dim == DD && plan.nt == NN) return launch_combine_one<DD, NN>(ctx, plan, n_seq, args);
+    if (head_dim == DD && plan.nt == NN) return launch_combine_one<DD, NN, false>(ctx, plan, n_seq, args);
     TT_CASE(256, 16)
     TT_CASE(256, 32)
     TT_CASE(128, 16)
@@ -1954,6 +2051,16 @@ int launch_splitk(tt_hip_ctx *ctx, const LaunchPlan &plan, int head_dim, int n_s
             if (kv_bits == 16) return launch_one<DD, NN, 4, 16, 1>(ctx, plan, n_seq, args);          \
             if (kv_bits == 8) return launch_one<DD, NN, 4, 8, 1>(ctx, plan, n_seq, args);            \
             if (kv_bits == 4) return launch_one<DD, NN, 4, 4, 1>(ctx, plan, n_seq, args);            \
+        }                                                                                            \
+        if ((args.hot.flags & kHotSinks) && plan.stream) {                                           \
+            if (kv_bits == 16) return launch_one<DD, NN, 4, 16, kKeepSinks, 1>(ctx, plan, n_seq, args); \
+            if (kv_bits == 8) return launch_one<DD, NN, 4, 8, kKeepSinks, 1>(ctx, plan, n_seq, args); \
+            if (kv_bits == 4) return launch_one<DD, NN, 4, 4, kKeepSinks, 1>(ctx, plan, n_seq, args); \
+        }                                                                                            \
+        if (args.hot.flags & kHotSinks) {                                                            \
+            if (kv_bits == 16) return launch_one<DD, NN, 4, 16, kKeepSinks>(ctx, plan, n_seq, args); \
+            if (kv_bits == 8) return launch_one<DD, NN, 4, 8, kKeepSinks>(ctx, plan, n_seq, args);   \
+            if (kv_bits == 4) return launch_one<DD, NN, 4, 4, kKeepSinks>(ctx, plan, n_seq, args);   \
         }                                                                                            \
         if (plan.stream) {                                                                           \
             if constexpr (DD == 256 && NN == 32) {                                                   \

@@ -296,6 +296,7 @@ struct KeepLists {
 //   kind 1: causal chunk of one sequence.
 //   chunk_splits > 1 (kind 1, one sequence): the chunk kernel over chunk_splits key ranges of
 //   chunk_split_blocks blocks, then the combine pass.
+//   sinks >= 0 (kind 0): the keys [0, sinks) stay visible beside the window; pinned rows of a ring are known.  -1: neither.
 static int run_attention(tt_hip_ctx *ctx, tt_hip_kv *kv, int kind, int layer, int n_seq, const int *slots,
                          const int *starts, const int *totals, int rows, int n_q_heads, const tt_half *q,
                          long long q_seq_stride, long long q_tok_stride, const tt_half *gate, long long g_seq_stride,
@@ -303,7 +304,7 @@ static int run_attention(tt_hip_ctx *ctx, tt_hip_kv *kv, int kind, int layer, in
                          long long o_tok_stride, int chunk_splits = 1, int chunk_split_blocks = 0,
                          const PageSource *pages = nullptr, int window = 0, const uint8_t *keep = nullptr,
                          long long keep_seq_stride = 0, long long keep_row_stride = 0, bool static_partials = false,
-                         const KeepLists *lists = nullptr) {
+                         const KeepLists *lists = nullptr, int sinks = -1) {
     const int D = kv->head_dim;
     hipError_t e = hipSetDevice(ctx->device);
     if (e != hipSuccess) return hip_fail(ctx, e, "hipSetDevice");
@@ -314,7 +315,7 @@ static int run_attention(tt_hip_ctx *ctx, tt_hip_kv *kv, int kind, int layer, in
         // Keys a tile walks: all of them, or with a sliding window at most the window, the tile's
         // rows and the partial block in front.
         auto walked = [&](int i) {
-            const long long reach = (long long)window + rows + 32;
+            const long long reach = (long long)window + rows + 32 + (sinks > 0 ? (sinks + 31LL) / 32 * 32 : 0);
             return window > 0 && totals[base + i] > reach ? (int)reach : totals[base + i];
         };
         min_keys = walked(0);
@@ -530,6 +531,10 @@ static int run_attention(tt_hip_ctx *ctx, tt_hip_kv *kv, int kind, int layer, in
         h.scale_log2e = scale * 1.4426950408889634f;
         h.window = window;
         h.ring_blocks = walks_pages ? pages->ring_blocks : kv->ring_blocks();
+        if (sinks >= 0) {
+            h.flags |= kHotSinks | (kv->pinned / kBlockTokens) << kHotPinnedShift;
+            h.ring_blocks = kv->ring ? (kv->capacity - kv->pinned) / kBlockTokens : 0;
+        }
         a.keep = keep ? keep + base * keep_seq_stride : nullptr;
         a.keep_seq_stride = keep_seq_stride;
         a.keep_row_stride = keep_row_stride;
@@ -546,6 +551,7 @@ static int run_attention(tt_hip_ctx *ctx, tt_hip_kv *kv, int kind, int layer, in
         const int listed_blocks = keep_row_stride > 0 ? 8 : D == 256 && kv_bits == 16 ? 2 : max_keys >= 50000 ? 4 : 6;
         h.keep_words = a.keep && (uintptr_t)a.keep % 4 == 0 && (n == 1 || keep_seq_stride % 4 == 0) &&
                        plan.split_len >= listed_blocks * plan.waves * 32;
+        if (sinks >= 0) h.keep_words = sinks;
         for (int i = 0; i < n; ++i) {
             a.seq[i].slot = walks_pages ? 0 : slots[base + i];
             a.seq[i].start = starts[base + i];
@@ -948,21 +954,37 @@ int tt_hip_attn_decode(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, con
 
 int tt_hip_attn_decode_swa(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, const int *slots, const int *seq_lens,
                            int window, int n_q_heads, const tt_half *q, const tt_half *gate, float scale, tt_half *out) {
+    return tt_hip_attn_decode_sinks(ctx, kv, layer, n_seq, slots, seq_lens, window, 0, n_q_heads, q, gate, scale, out);
+}
+
+// Whether a call goes through the kernels that know of sinks and pinned rows: a ring with pinned rows behind any window, else where
+// a row's window leaves keys out and sinks stay.
+static bool needs_sinks(const tt_hip_kv *kv, int window, int sinks, bool clipped) {
+    return window > 0 && (kv->pinned > 0 || (sinks > 0 && clipped));
+}
+
+int tt_hip_attn_decode_sinks(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, const int *slots, const int *seq_lens,
+                             int window, int sinks, int n_q_heads, const tt_half *q, const tt_half *gate, float scale, tt_half *out) {
     int st = check_common(ctx, kv, layer, n_q_heads, q, out);
     if (st != TT_HIP_OK) return st;
-    if (n_seq <= 0 || !slots || !seq_lens || window < 0) return TT_HIP_ERR_INVALID_ARGUMENT;
+    if (n_seq <= 0 || !slots || !seq_lens || window < 0 || sinks < 0) return TT_HIP_ERR_INVALID_ARGUMENT;
     IntTable starts(n_seq);
+    bool clipped = false;
+    int longest = 0;
     for (int i = 0; i < n_seq; ++i) {
         if (slots[i] < 0 || slots[i] >= kv->n_slots || seq_lens[i] < 0) return TT_HIP_ERR_INVALID_ARGUMENT;
-        const long long first = window > 0 && seq_lens[i] > window ? seq_lens[i] - window : 0;
-        if (!kv->holds_keys(first, seq_lens[i])) return TT_HIP_ERR_CAPACITY;
+        const int first = window > 0 && seq_lens[i] > window ? seq_lens[i] - window : 0;
+        if (!kv->holds_keys_and_sinks(std::min(sinks, first), first, seq_lens[i])) return TT_HIP_ERR_CAPACITY;
+        clipped = clipped || first > 0;
+        longest = std::max(longest, seq_lens[i]);
         starts[i] = seq_lens[i] - 1;
     }
     BusyGuard guard(ctx);
     if (!guard.ok) return TT_HIP_ERR_BUSY;
     const long long row = (long long)n_q_heads * kv->head_dim;
     return run_attention(ctx, kv, 0, layer, n_seq, slots, starts.data(), seq_lens, 1, n_q_heads, q, row, row, gate, row,
-                         row, scale, out, row, row, 1, 0, nullptr, window);
+                         row, scale, out, row, row, 1, 0, nullptr, window, nullptr, 0, 0, false, nullptr,
+                         needs_sinks(kv, window, sinks, clipped) ? std::min(sinks, longest) : -1);
 }
 
 // Same kernels and planner as tt_hip_attn_decode; the partials live in this device's copy of `scratch`
@@ -1145,22 +1167,34 @@ int tt_hip_attn_verify(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, con
 int tt_hip_attn_verify_swa(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, const int *slots,
                            const int *start_positions, int rows, int window, int n_q_heads, const tt_half *q,
                            const tt_half *gate, float scale, tt_half *out) {
+    return tt_hip_attn_verify_sinks(ctx, kv, layer, n_seq, slots, start_positions, rows, window, 0, n_q_heads, q, gate, scale, out);
+}
+
+int tt_hip_attn_verify_sinks(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, const int *slots,
+                             const int *start_positions, int rows, int window, int sinks, int n_q_heads, const tt_half *q,
+                             const tt_half *gate, float scale, tt_half *out) {
     int st = check_common(ctx, kv, layer, n_q_heads, q, out);
     if (st != TT_HIP_OK) return st;
-    if (n_seq <= 0 || rows <= 0 || !slots || !start_positions || window < 0) return TT_HIP_ERR_INVALID_ARGUMENT;
+    if (n_seq <= 0 || rows <= 0 || !slots || !start_positions || window < 0 || sinks < 0) return TT_HIP_ERR_INVALID_ARGUMENT;
     IntTable totals(n_seq);
+    bool clipped = false;
+    int longest = 0;
     for (int i = 0; i < n_seq; ++i) {
         if (slots[i] < 0 || slots[i] >= kv->n_slots || start_positions[i] < 0) return TT_HIP_ERR_INVALID_ARGUMENT;
-        const long long first = window > 0 && start_positions[i] + 1 > window ? start_positions[i] + 1 - window : 0;
-        if (!kv->holds_keys(first, (long long)start_positions[i] + rows)) return TT_HIP_ERR_CAPACITY;
-        totals[i] = start_positions[i] + rows;
+        const long long end = (long long)start_positions[i] + rows;
+        const long long first = window > 0 && start_positions[i] + 1LL > window ? start_positions[i] + 1LL - window : 0;
+        if (!kv->holds_keys_and_sinks((int)std::min<long long>(sinks, std::max(end - window, 0ll)), first, end)) return TT_HIP_ERR_CAPACITY;
+        clipped = clipped || end > window;
+        totals[i] = (int)end;
+        longest = std::max(longest, totals[i]);
     }
     BusyGuard guard(ctx);
     if (!guard.ok) return TT_HIP_ERR_BUSY;
     const long long tok = (long long)n_q_heads * kv->head_dim;
     const long long seq = tok * rows;
     return run_attention(ctx, kv, 0, layer, n_seq, slots, start_positions, totals.data(), rows, n_q_heads, q, seq, tok,
-                         gate, seq, tok, scale, out, seq, tok, 1, 0, nullptr, window);
+                         gate, seq, tok, scale, out, seq, tok, 1, 0, nullptr, window, nullptr, 0, 0, false, nullptr,
+                         needs_sinks(kv, window, sinks, clipped) ? std::min(sinks, longest) : -1);
 }
 
 int tt_hip_attn_prefill(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int slot, int start_pos, int q_len, int kv_valid,
@@ -1170,9 +1204,34 @@ int tt_hip_attn_prefill(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int slot, int
                                    gate_stride, scale, out, o_stride);
 }
 
+int tt_hip_attn_prefill_sinks(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int slot, int start_pos, int q_len, int kv_valid,
+                              int sliding_window, int sinks, int n_q_heads, const tt_half *q, size_t q_stride, const tt_half *gate,
+                              size_t gate_stride, float scale, tt_half *out, size_t o_stride) {
+    int st = check_common(ctx, kv, layer, n_q_heads, q, out);
+    if (st != TT_HIP_OK) return st;
+    if (slot < 0 || slot >= kv->n_slots || start_pos < 0 || q_len <= 0 || sliding_window < 0 || sinks < 0) return TT_HIP_ERR_INVALID_ARGUMENT;
+    const long long end = (long long)start_pos + q_len;
+    if (!needs_sinks(kv, sliding_window, sinks, end > sliding_window))
+        return tt_hip_attn_prefill_swa(ctx, kv, layer, slot, start_pos, q_len, kv_valid, sliding_window, n_q_heads, q, q_stride, gate,
+                                       gate_stride, scale, out, o_stride);
+    const size_t packed = (size_t)n_q_heads * kv->head_dim;
+    if (q_stride < packed || o_stride < packed || (gate && gate_stride < packed)) return TT_HIP_ERR_SHAPE;
+    if (end > kv_valid) return TT_HIP_ERR_INVALID_ARGUMENT;
+    const long long first = start_pos + 1LL > sliding_window ? start_pos + 1LL - sliding_window : 0;
+    if (!kv->holds_keys_and_sinks((int)std::min<long long>(sinks, std::max(end - sliding_window, 0ll)), first, kv_valid)) return TT_HIP_ERR_CAPACITY;
+    BusyGuard guard(ctx);
+    if (!guard.ok) return TT_HIP_ERR_BUSY;
+    return run_attention(ctx, kv, 0, layer, 1, &slot, &start_pos, &kv_valid, q_len, n_q_heads, q, 0, (long long)q_stride, gate, 0,
+                         (long long)gate_stride, scale, out, 0, (long long)o_stride, 1, 0, nullptr, sliding_window, nullptr, 0, 0, false,
+                         nullptr, std::min(sinks, kv_valid));
+}
+
 int tt_hip_attn_prefill_swa(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int slot, int start_pos, int q_len, int kv_valid,
                             int sliding_window, int n_q_heads, const tt_half *q, size_t q_stride, const tt_half *gate,
                             size_t gate_stride, float scale, tt_half *out, size_t o_stride) {
+    if (kv && kv->pinned > 0 && sliding_window > 0)
+        return tt_hip_attn_prefill_sinks(ctx, kv, layer, slot, start_pos, q_len, kv_valid, sliding_window, 0, n_q_heads, q, q_stride, gate,
+                                         gate_stride, scale, out, o_stride);
     int st = check_common(ctx, kv, layer, n_q_heads, q, out);
     if (st != TT_HIP_OK) return st;
     if (slot < 0 || slot >= kv->n_slots || start_pos < 0 || q_len <= 0 || sliding_window < 0) return TT_HIP_ERR_INVALID_ARGUMENT;

@@ -34,6 +34,10 @@ constexpr int kHotAligned = 1;  // q/gate/out rows are 16-byte aligned
 constexpr int kHotXcdGrid = 2;
 // The grid is (splits of all sequences, tiles): split x belongs to the sequence whose first_split it falls behind.
 constexpr int kHotPackedSplits = 4;
+// A window with sinks: keep_words is the number of first tokens that stay visible, and from kHotPinnedShift on the flags hold the
+// blocks at the page's front that its ring leaves alone.
+constexpr int kHotSinks = 8, kHotPinnedShift = 8;
+constexpr int kKeepSinks = 6;  // that kernel's KEEP (attn_splitk.hip)
 struct SplitKHot {                         // dword
     const _Float16 *k_layer;               //  0
     const _Float16 *v_layer;               //  2
@@ -49,12 +53,12 @@ struct SplitKHot {                         // dword
     int tok_tiles;                         // 18  ceil(rows / tt)
     int split_len;                         // 19  keys per split, multiple of 32
     int window;       // 20  sliding window: a row at position p sees keys [max(0, p + 1 - window), p + 1); 0 = every key
-    int ring_blocks;  // 21  ring cache: key block b lives in block b % ring_blocks of the page; 0 = where it is
+    int ring_blocks;  // 21  ring cache: key block b lives in block b % ring_blocks of the page (kHotSinks: of what lies behind the pinned blocks); 0 = where it is
     float scale_log2e;                     // 22
     int n_splits_max;                      // 23
     int n_tiles;                           // 24  n_kv_heads * hsubs * tok_tiles
-    int flags;                             // 25  kHotAligned | kHotXcdGrid | kHotPackedSplits
-    int keep_words;   // 26  per-sequence masks start on 4-byte boundaries: a wavefront may read its blocks' bytes as words
+    int flags;                             // 25  kHotAligned | kHotXcdGrid | kHotPackedSplits | kHotSinks
+    int keep_words;   // 26  (kHotSinks: the sinks) per-sequence masks start on 4-byte boundaries: a wavefront may read its blocks' bytes as words
     int gh_inv;       // 27  ceil(65536 / gh): (i * gh_inv) >> 16 == i / gh for 0 <= i < 64, gh <= 32
     float *part_o;    // 28  [first_split(seq) + split][tile][NT][D]
     float *part_ml;   // 30  [first_split(seq) + split][tile][NT][2]  (max in log2 domain, sum)
@@ -180,6 +184,7 @@ struct tt_hip_kv {
     int capacity = 0, max_context = 0;
     int bits = 16;                 // 16: fp16 values; 8 / 4: affine levels with per-group fp16 scale and bias
     bool ring = false;             // row of position p lives at p % capacity; capacity is fixed
+    int pinned = 0;                // ring: its first rows (whole blocks) that later ones leave alone; the ring goes round behind them
     uint64_t generation = 0;       // bumped when the stores are reallocated
     std::vector<_Float16 *> k, v;  // one K and one V store per layer (bytes at 8 / 4 bits)
     std::vector<int> positions;
@@ -187,19 +192,27 @@ struct tt_hip_kv {
     size_t page_bytes() const { return (size_t)(capacity / tt::kBlockTokens) * block_bytes(); }
     size_t layer_bytes() const { return (size_t)n_slots * n_kv_heads * page_bytes(); }
     size_t page_elems() const { return page_bytes() / 2; }  // halves per (slot, kv head) page, whatever they hold
-    int physical(int position) const { return ring ? position % capacity : position; }
+    int physical(int position) const { return ring && position >= pinned ? pinned + (position - pinned) % (capacity - pinned) : position; }
     // Rows [position, position + n) must be storable in one piece: inside capacity, and on a ring
     // inside max_context without wrapping (KVCacheManager+Validation.swift:52-59).
     bool holds_rows(int position, int n) const {
         if (!ring) return (long long)position + n <= capacity;
         return (long long)position + n <= max_context && (long long)physical(position) + n <= capacity;
     }
-    // Keys [first, last) readable by an attention call: on a ring only the last `capacity` rows exist.
+    // Keys [first, last) readable by an attention call: on a ring only the last `capacity` rows exist, or the pinned ones and the
+    // last of those behind them.
     bool holds_keys(long long first, long long last) const {
         if (!ring) return last <= capacity;
-        return last <= max_context && last - (first & ~31LL) <= capacity;
+        const long long from = (first & ~31LL) > pinned ? (first & ~31LL) : pinned;
+        return last <= max_context && last - from <= capacity - pinned;
     }
-    int ring_blocks() const { return ring ? capacity / tt::kBlockTokens : 0; }
+    // ... and the keys [0, sinks) beside them.
+    bool holds_keys_and_sinks(int sinks, long long first, long long last) const {
+        return holds_keys(first, last) && (!ring || sinks <= pinned || last <= capacity);
+    }
+    // For the kernels that know nothing of pinned rows: their calls may read such a ring only as long as it has not come round
+    // (holds_keys from key 0 on), when every row lies at its position.
+    int ring_blocks() const { return ring && pinned == 0 ? capacity / tt::kBlockTokens : 0; }
 };
 
 namespace tt {

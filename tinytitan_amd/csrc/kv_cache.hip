@@ -3,6 +3,7 @@
 //
 // Bookkeeping follows KVCacheManager (sources/TinyTitan/Runtime/KVCache/
 // KVCacheManager.swift:62-333, KVCacheManager+Storage.swift:99-139, :266-309).
+#include <algorithm>
 #include <cstdint>
 #include <new>
 
@@ -36,7 +37,7 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const _Float16 *__restrict
                                                       _Float16 *__restrict__ v_dst, long long dst_stride,
                                                       long long page_elems, int slot, int n_kv_heads, int head_dim,
                                                       int position, int n_tokens, const int *__restrict__ positions,
-                                                      int limit, int ring_capacity) {
+                                                      int limit, int ring_capacity, int pinned) {
     // positions: row t is the row of position positions[t] (a gather); a position outside [0, limit) gives zeros
     const long long per_token = (long long)n_kv_heads * head_dim;
     const long long idx = (long long)blockIdx.x * blockDim.x + threadIdx.x;
@@ -52,7 +53,8 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const _Float16 *__restrict
     if (positions) {
         pos = positions[t];
         inside = pos >= 0 && pos < limit;
-        pos = inside ? (ring_capacity > 0 ? pos % ring_capacity : pos) : 0;
+        pos = inside ? pos : 0;
+        if (ring_capacity > 0 && pos >= pinned) pos = pinned + (pos - pinned) % ring_capacity;
     }
     if (k_dst) k_dst[dst] = inside ? k_layer[page + k_offset(head_dim, pos, d)] : (_Float16)0;
     if (v_dst) v_dst[dst] = inside ? v_layer[page + v_offset(head_dim, pos, d)] : (_Float16)0;
@@ -183,7 +185,7 @@ static int launch_kv_read_rows(tt_hip_kv *kv, int layer, int slot, int position,
     const unsigned blocks = (unsigned)((total + 255) / 256);
     hipLaunchKernelGGL(kv_read_kernel, dim3(blocks), dim3(256), 0, kv->ctx->stream, kv->k[layer], kv->v[layer], k, v,
                        (long long)stride, (long long)kv->page_elems(), slot, kv->n_kv_heads, kv->head_dim, position, n_tokens,
-                       positions, limit, kv->ring ? kv->capacity : 0);
+                       positions, limit, kv->ring ? kv->capacity - kv->pinned : 0, kv->pinned);
     hipError_t e = hipGetLastError();
     return e == hipSuccess ? TT_HIP_OK : hip_fail(kv->ctx, e, "kv_read_kernel launch");
 }
@@ -258,9 +260,24 @@ tt_hip_kv *tt_hip_kv_create(tt_hip_ctx *ctx, int n_layers, int n_kv_heads, int h
 
 tt_hip_kv *tt_hip_kv_create_ring(tt_hip_ctx *ctx, int n_layers, int n_kv_heads, int head_dim, int n_slots,
                                  int ring_capacity_tokens, int max_context_tokens, int bits, int *out_err) {
-    tt_hip_kv *kv = tt_hip_kv_create_quantized(ctx, n_layers, n_kv_heads, head_dim, n_slots, ring_capacity_tokens,
-                                               max_context_tokens, bits, out_err);
-    if (kv) kv->ring = true;  // capacity = min(ring capacity, max context), both rounded up to whole blocks, and fixed
+    return tt_hip_kv_create_ring_sinks(ctx, n_layers, n_kv_heads, head_dim, n_slots, ring_capacity_tokens, 0, max_context_tokens, bits, out_err);
+}
+
+tt_hip_kv *tt_hip_kv_create_ring_sinks(tt_hip_ctx *ctx, int n_layers, int n_kv_heads, int head_dim, int n_slots,
+                                       int ring_capacity_tokens, int sink_tokens, int max_context_tokens, int bits, int *out_err) {
+    if (ring_capacity_tokens <= 0 || sink_tokens < 0) {
+        if (out_err) *out_err = TT_HIP_ERR_INVALID_ARGUMENT;
+        return nullptr;
+    }
+    // capacity = min(the sinks' blocks + ring capacity, max context), rounded up to whole blocks, and fixed
+    const long long sink_blocks = ((long long)sink_tokens + kBlockTokens - 1) / kBlockTokens;
+    const long long ring_blocks = ((long long)ring_capacity_tokens + kBlockTokens - 1) / kBlockTokens;
+    const long long rows = std::min<long long>((sink_blocks + ring_blocks) * kBlockTokens, std::max(max_context_tokens, 1));
+    tt_hip_kv *kv = tt_hip_kv_create_quantized(ctx, n_layers, n_kv_heads, head_dim, n_slots, (int)rows, max_context_tokens, bits, out_err);
+    if (!kv) return nullptr;
+    kv->ring = true;
+    // (a ring that holds every position never comes round: nothing to pin)
+    kv->pinned = kv->capacity < kv->max_context ? (int)(sink_blocks * kBlockTokens) : 0;
     return kv;
 }
 

@@ -22,7 +22,7 @@ struct QuantArgs {
     long long page_bytes;
     int slot, n_kv_heads, head_dim, position, n_tokens;
     const int *positions;  // the read kernel only: row t is the row of positions[t]; outside [0, limit) gives zeros
-    int limit, ring_capacity;
+    int limit, ring_capacity, pinned;  // (the ring goes round behind the pinned rows)
 };
 
 __device__ __forceinline__ uint8_t *block_of(const QuantArgs &a, bool is_v, int kvh, int pos, int bits) {
@@ -176,7 +176,7 @@ __global__ __launch_bounds__(256) void kvq_read_kernel(const QuantArgs a, _Float
             dst[(long long)token * dst_stride + flat] = (_Float16)0;
             return;
         }
-        if (a.ring_capacity > 0) pos %= a.ring_capacity;
+        if (a.ring_capacity > 0 && pos >= a.pinned) pos = a.pinned + (pos - a.pinned) % a.ring_capacity;
     }
     const int key = pos & 31;
     const uint8_t *block = block_of(a, is_v, kvh, pos, BITS);
@@ -294,7 +294,8 @@ QuantArgs quant_args(tt_hip_kv *kv, int layer, int slot, int position, int n_tok
     a.n_tokens = n_tokens;
     a.positions = nullptr;
     a.limit = 0;
-    a.ring_capacity = kv->ring ? kv->capacity : 0;
+    a.ring_capacity = kv->ring ? kv->capacity - kv->pinned : 0;
+    a.pinned = kv->pinned;
     return a;
 }
 

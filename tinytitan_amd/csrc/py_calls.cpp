@@ -23,6 +23,9 @@ namespace {
     F(tt_hip_attn_decode_keep)                                                                                           \
     F(tt_hip_attn_decode_keep_indices)                                                                                   \
     F(tt_hip_attn_verify_swa)                                                                                            \
+    F(tt_hip_attn_decode_sinks)                                                                                          \
+    F(tt_hip_attn_verify_sinks)                                                                                          \
+    F(tt_hip_attn_prefill_sinks)                                                                                         \
     F(tt_hip_attn_prefill)                                                                                               \
     F(tt_hip_attn_prefill_swa)                                                                                           \
     F(tt_hip_attn_prefill_keep)                                                                                          \
@@ -316,6 +319,48 @@ TT_CALL(attn_verify_swa) {
     });
 }
 
+// (ctx, kv, layer, slots, lengths, window, sinks, heads, q, gate, scale, out)
+TT_CALL(attn_decode_sinks) {
+    Args a(args, n, 12);
+    if (!a.ok) return nullptr;
+    auto *ctx = a.handle<tt_hip_ctx>();
+    auto *kv = a.handle<tt_hip_kv>();
+    const int layer = a.i();
+    Ints slots, lens;
+    slots.take(a);
+    lens.take(a);
+    const int window = a.i(), sinks = a.i(), heads = a.i();
+    const tt_half *q = a.half(), *gate = a.half();
+    const float scale = a.real();
+    tt_half *out = a.half();
+    return finish(a, [&] {
+        if (slots.count != lens.count) return (int)TT_HIP_ERR_INVALID_ARGUMENT;
+        return lib.tt_hip_attn_decode_sinks(ctx, kv, layer, slots.count, slots.values, lens.values, window, sinks, heads, q, gate, scale,
+                                            out);
+    });
+}
+
+// (ctx, kv, layer, slots, start_positions, rows, window, sinks, heads, q, gate, scale, out)
+TT_CALL(attn_verify_sinks) {
+    Args a(args, n, 13);
+    if (!a.ok) return nullptr;
+    auto *ctx = a.handle<tt_hip_ctx>();
+    auto *kv = a.handle<tt_hip_kv>();
+    const int layer = a.i();
+    Ints slots, starts;
+    slots.take(a, true);
+    starts.take(a, true);
+    const int rows = a.i(), window = a.i(), sinks = a.i(), heads = a.i();
+    const tt_half *q = a.half(), *gate = a.half();
+    const float scale = a.real();
+    tt_half *out = a.half();
+    return finish(a, [&] {
+        if (slots.count > starts.count) return (int)TT_HIP_ERR_INVALID_ARGUMENT;  // (positions may be a longer table than the step's)
+        return lib.tt_hip_attn_verify_sinks(ctx, kv, layer, slots.count, slots.values, starts.values, rows, window, sinks, heads, q, gate,
+                                            scale, out);
+    });
+}
+
 // What the chunk calls have in common behind their own arguments: (heads, q, q_stride, gate, gate_stride, scale, out, o_stride)
 struct Rows {
     int heads;
@@ -344,6 +389,20 @@ TT_CALL(attn_prefill) {
                                                r.gate_stride, r.scale, r.out, r.o_stride);
         return lib.tt_hip_attn_prefill(ctx, kv, layer, slot, start, count, valid, r.heads, r.q, r.q_stride, r.gate, r.gate_stride, r.scale,
                                        r.out, r.o_stride);
+    });
+}
+
+// (ctx, kv, layer, slot, start, query_count, kv_valid, window, sinks, <rows>)
+TT_CALL(attn_prefill_sinks) {
+    Args a(args, n, 17);
+    if (!a.ok) return nullptr;
+    auto *ctx = a.handle<tt_hip_ctx>();
+    auto *kv = a.handle<tt_hip_kv>();
+    const int layer = a.i(), slot = a.i(), start = a.i(), count = a.i(), valid = a.i(), window = a.i(), sinks = a.i();
+    const Rows r(a);
+    return finish(a, [&] {
+        return lib.tt_hip_attn_prefill_sinks(ctx, kv, layer, slot, start, count, valid, window, sinks, r.heads, r.q, r.q_stride, r.gate,
+                                             r.gate_stride, r.scale, r.out, r.o_stride);
     });
 }
 
@@ -538,7 +597,8 @@ PyObject *bind(PyObject *, PyObject *arg) {
 PyMethodDef methods[] = {
     {"bind", bind, METH_O, nullptr},
     TT_METHOD(attn_decode) TT_METHOD(attn_decode_swa) TT_METHOD(attn_decode_keep) TT_METHOD(attn_decode_keep_indices)
-    TT_METHOD(attn_verify_swa) TT_METHOD(attn_prefill) TT_METHOD(attn_prefill_keep) TT_METHOD(attn_prefill_keep_indices)
+    TT_METHOD(attn_verify_swa) TT_METHOD(attn_decode_sinks) TT_METHOD(attn_verify_sinks) TT_METHOD(attn_prefill_sinks)
+    TT_METHOD(attn_prefill) TT_METHOD(attn_prefill_keep) TT_METHOD(attn_prefill_keep_indices)
     TT_METHOD(kv_append) TT_METHOD(qkv_epilogue_append) TT_METHOD(affine_projection) TT_METHOD(qsa_pool_blocks)
     TT_METHOD(qsa_norm_rope_rows) TT_METHOD(qsa_block_scores) TT_METHOD(qsa_decode_scores) TT_METHOD(qsa_select)
     {nullptr, nullptr, 0, nullptr}};

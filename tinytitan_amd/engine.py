@@ -182,22 +182,29 @@ class KVCacheManager:
 
     def __init__(self, ctx: HIPContext, layers: int, kv_heads: int, head_dim: int, slots: int = 1,
                  max_context: int = 262144, initial_capacity: Optional[int] = None, precision_bits: int = 16,
-                 ring_capacity: int = 0):
-        """``ring_capacity`` > 0: a ring for sliding-window layers (row of position p at p % capacity)."""
+                 ring_capacity: int = 0, sink_tokens: int = 0):
+        """``ring_capacity`` > 0: a ring for sliding-window layers (row of position p at p % capacity); with ``sink_tokens`` > 0
+        the first that many positions keep rows of their own in front of it (for ``Attention.encode_swa(..., sinks=)``)."""
         self.ctx = ctx
         self._lib = ctx._lib
         self._calls = ctx._calls
         if initial_capacity is None:
             initial_capacity = min(max_context, 8192)  # KVCacheManager.swift:270-285
         err = ctypes.c_int(0)
-        if ring_capacity > 0:
+        if sink_tokens and ring_capacity <= 0:
+            raise TinyTitanHIPError(capi.ERR_INVALID_ARGUMENT, "KVCacheManager")  # (a cache that keeps every row keeps the first ones)
+        if sink_tokens:
+            self.handle = self._lib.tt_hip_kv_create_ring_sinks(ctx.handle, layers, kv_heads, head_dim, slots, ring_capacity, sink_tokens,
+                                                                max_context, precision_bits, ctypes.byref(err))
+        elif ring_capacity > 0:
             self.handle = self._lib.tt_hip_kv_create_ring(ctx.handle, layers, kv_heads, head_dim, slots, ring_capacity,
                                                           max_context, precision_bits, ctypes.byref(err))
         else:
             self.handle = self._lib.tt_hip_kv_create_quantized(ctx.handle, layers, kv_heads, head_dim, slots,
                                                                initial_capacity, max_context, precision_bits, ctypes.byref(err))
         if not self.handle:
-            raise TinyTitanHIPError(err.value, "tt_hip_kv_create_ring" if ring_capacity > 0 else "tt_hip_kv_create_quantized")
+            raise TinyTitanHIPError(err.value, "tt_hip_kv_create_ring_sinks" if sink_tokens else
+                                    "tt_hip_kv_create_ring" if ring_capacity > 0 else "tt_hip_kv_create_quantized")
         self.layers, self.kv_heads, self.head_dim, self.slots = layers, kv_heads, head_dim, slots
         self.precision_bits = precision_bits
 
@@ -352,8 +359,15 @@ class Attention:
             self.ctx._check(status, "tt_hip_attn_decode")
 
     def encode_swa(self, kv: KVCacheManager, layer: int, q: torch.Tensor, out: torch.Tensor, num_q_heads: int,
-                   seq_len, window: int, scale: float, slot=0, gate: Optional[torch.Tensor] = None) -> None:
-        """``Attention.encodeSWA`` (Attention.swift:229-266): keys ``[max(0, seq_len - window), seq_len)``."""
+                   seq_len, window: int, scale: float, slot=0, gate: Optional[torch.Tensor] = None, sinks: int = 0) -> None:
+        """``Attention.encodeSWA`` (Attention.swift:229-266): keys ``[max(0, seq_len - window), seq_len)``, and with ``sinks`` > 0
+        the keys ``[0, sinks)`` beside them."""
+        if sinks:
+            status = self._calls.attn_decode_sinks(self.ctx.handle, kv.handle, layer, slot, seq_len, window, sinks, num_q_heads, q, gate,
+                                                   scale, out)
+            if status:
+                self.ctx._check(status, "tt_hip_attn_decode_sinks")
+            return
         status = self._calls.attn_decode_swa(self.ctx.handle, kv.handle, layer, slot, seq_len, window, num_q_heads, q, gate, scale, out)
         if status:
             self.ctx._check(status, "tt_hip_attn_decode_swa")
@@ -387,8 +401,15 @@ class Attention:
 
     def encode_verify_rows(self, kv: KVCacheManager, layer: int, q: torch.Tensor, out: torch.Tensor,
                            num_q_heads: int, start_positions: Sequence[int], rows: int, scale: float,
-                           slots: Sequence[int], gate: Optional[torch.Tensor] = None, window: int = 0) -> None:
-        """Row r of sequence i attends like a decode at ``start_positions[i] + r`` (over its last ``window`` keys)."""
+                           slots: Sequence[int], gate: Optional[torch.Tensor] = None, window: int = 0, sinks: int = 0) -> None:
+        """Row r of sequence i attends like a decode at ``start_positions[i] + r`` (over its last ``window`` keys, and beside them
+        the first ``sinks``)."""
+        if sinks:
+            status = self._calls.attn_verify_sinks(self.ctx.handle, kv.handle, layer, slots, start_positions, rows, window, sinks,
+                                                   num_q_heads, q, gate, scale, out)
+            if status:
+                self.ctx._check(status, "tt_hip_attn_verify_sinks")
+            return
         status = self._calls.attn_verify_swa(self.ctx.handle, kv.handle, layer, slots, start_positions, rows, window, num_q_heads, q,
                                              gate, scale, out)
         if status:
@@ -407,6 +428,7 @@ class PrefillAttentionParams:
     o_stride: int
     gate_stride: int = 0
     sliding_window: int = 0  # 0: every key up to the row's own
+    sinks: int = 0  # with a window: the first keys that stay visible
 
 
 class PrefillAttention:
@@ -426,7 +448,7 @@ class PrefillAttention:
         p = params
         gate_stride = p.gate_stride or p.q_stride
         if keep_indices is not None:
-            if (keep_counts is None or keep_mask is not None or p.sliding_window or keep_indices.dtype != torch.int32
+            if (keep_counts is None or keep_mask is not None or p.sliding_window or p.sinks or keep_indices.dtype != torch.int32
                     or keep_counts.dtype != torch.int32):
                 raise TinyTitanHIPError(capi.ERR_INVALID_ARGUMENT, "PrefillAttention.encode_causal")
             status = self._calls.attn_prefill_keep_indices(
@@ -437,13 +459,20 @@ class PrefillAttention:
                 self.ctx._check(status, "tt_hip_attn_prefill_keep_indices")
             return
         if keep_mask is not None:
-            if keep_mask.dtype != torch.uint8 or p.sliding_window:
+            if keep_mask.dtype != torch.uint8 or p.sliding_window or p.sinks:
                 raise TinyTitanHIPError(capi.ERR_INVALID_ARGUMENT, "PrefillAttention.encode_causal")
             status = self._calls.attn_prefill_keep(
                 self.ctx.handle, kv.handle, layer, slot, p.start_position, p.query_count, p.kv_valid_count, keep_mask,
                 keep_stride or keep_mask.shape[-1], p.num_q_heads, q, p.q_stride, gate, gate_stride, p.scale, out, p.o_stride)
             if status:
                 self.ctx._check(status, "tt_hip_attn_prefill_keep")
+            return
+        if p.sinks:
+            status = self._calls.attn_prefill_sinks(self.ctx.handle, kv.handle, layer, slot, p.start_position, p.query_count,
+                                                    p.kv_valid_count, p.sliding_window, p.sinks, p.num_q_heads, q, p.q_stride, gate,
+                                                    gate_stride, p.scale, out, p.o_stride)
+            if status:
+                self.ctx._check(status, "tt_hip_attn_prefill_sinks")
             return
         status = self._calls.attn_prefill(self.ctx.handle, kv.handle, layer, slot, p.start_position, p.query_count, p.kv_valid_count,
                                           p.sliding_window, p.num_q_heads, q, p.q_stride, gate, gate_stride, p.scale, out, p.o_stride)

@@ -144,6 +144,10 @@ public:
     void expectPosition(int slot, int position) const {
         check(tt_hip_kv_expect_position(handle_, slot, position), "KVCacheManager.expectPosition");
     }
+    // The slots start from rows [0, length) of prefixSlot, which keeps them (see tt_hip_kv_share_prefix).
+    void sharePrefix(int prefixSlot, int length, const std::vector<int> &slots) {
+        check(tt_hip_kv_share_prefix(handle_, prefixSlot, length, (int)slots.size(), slots.data()), "KVCacheManager.sharePrefix");
+    }
     // The reference hands out write targets (kSlot / vSlot / kRange / vRange) into token-major rows;
     // here the rows are written through the cache, which owns their layout.
     void write(int layer, int slot, int position, int count, const tt_half *k, const tt_half *v, size_t tokenStride) {
@@ -160,6 +164,11 @@ public:
 private:
     Context &context_;
     tt_hip_kv *handle_ = nullptr;
+};
+
+// A prefix that slots share (KVCacheManager::sharePrefix): the first `length` rows of `slot`.
+struct SharedPrefix {
+    int slot, length;
 };
 
 class Attention {
@@ -210,6 +219,14 @@ public:
                                  numQHeads, q, gate, scale, out),
               "Attention.encodeBatch");
     }
+    // The same for slots that share a prefix, which is read once for all of them.
+    void encodeBatch(KVCacheManager &kv, int layer, const std::vector<int> &slots, const std::vector<int> &seqLens, SharedPrefix prefix,
+                     const tt_half *q, tt_half *out, int numQHeads, float scale, const tt_half *gate = nullptr) {
+        if (slots.size() != seqLens.size()) throw Error(TT_HIP_ERR_INVALID_ARGUMENT, "Attention.encodeBatch");
+        check(tt_hip_attn_decode_shared(context_.handle(), kv.handle(), layer, (int)slots.size(), slots.data(), seqLens.data(),
+                                        prefix.slot, prefix.length, numQHeads, q, gate, scale, out),
+              "Attention.encodeBatch");
+    }
     // encodeFullAttentionDecodeOrderRows: row r attends start + r + 1 keys.
     void encodeVerifyRows(KVCacheManager &kv, int layer, const std::vector<int> &slots,
                           const std::vector<int> &startPositions, int rows, const tt_half *q, tt_half *out,
@@ -217,6 +234,13 @@ public:
         if (slots.size() != startPositions.size()) throw Error(TT_HIP_ERR_INVALID_ARGUMENT, "Attention.encodeVerifyRows");
         check(tt_hip_attn_verify_sinks(context_.handle(), kv.handle(), layer, (int)slots.size(), slots.data(),
                                        startPositions.data(), rows, window, sinks, numQHeads, q, gate, scale, out),
+              "Attention.encodeVerifyRows");
+    }
+    void encodeVerifyRows(KVCacheManager &kv, int layer, const std::vector<int> &slots, const std::vector<int> &startPositions, int rows,
+                          SharedPrefix prefix, const tt_half *q, tt_half *out, int numQHeads, float scale, const tt_half *gate = nullptr) {
+        if (slots.size() != startPositions.size()) throw Error(TT_HIP_ERR_INVALID_ARGUMENT, "Attention.encodeVerifyRows");
+        check(tt_hip_attn_verify_shared(context_.handle(), kv.handle(), layer, (int)slots.size(), slots.data(), startPositions.data(), rows,
+                                        prefix.slot, prefix.length, numQHeads, q, gate, scale, out),
               "Attention.encodeVerifyRows");
     }
 
@@ -246,6 +270,15 @@ public:
         check(tt_hip_attn_prefill_sinks(context_.handle(), kv.handle(), layer, slot, p.startPosition, p.queryCount,
                                         p.kvValidCount, p.slidingWindow, p.sinks, p.numQHeads, q, p.qStride, gate,
                                         p.gateStride ? p.gateStride : p.qStride, p.scale, out, p.oStride),
+              "PrefillAttention.encodeCausal");
+    }
+    // A chunk of a slot that shares a prefix.
+    void encodeCausal(KVCacheManager &kv, int layer, int slot, SharedPrefix prefix, const tt_half *q, tt_half *out,
+                      const PrefillAttentionParams &p, const tt_half *gate = nullptr) {
+        if (p.slidingWindow || p.sinks) throw Error(TT_HIP_ERR_INVALID_ARGUMENT, "PrefillAttention.encodeCausal");
+        check(tt_hip_attn_prefill_shared(context_.handle(), kv.handle(), layer, slot, p.startPosition, p.queryCount, p.kvValidCount,
+                                         prefix.slot, prefix.length, p.numQHeads, q, p.qStride, gate,
+                                         p.gateStride ? p.gateStride : p.qStride, p.scale, out, p.oStride),
               "PrefillAttention.encodeCausal");
     }
     // encodeCausal(..., keepMask:, keepStride:) of a QSA chunk, mask form: a row of keepStride bytes per query.

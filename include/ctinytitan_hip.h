@@ -321,6 +321,16 @@ TT_HIP_API int tt_hip_kv_reserve(tt_hip_kv *kv, int tokens);
  * produceToken makes before a step (RealForwardRunner+Decode.swift:222-226). */
 TT_HIP_API int tt_hip_kv_expect_position(const tt_hip_kv *kv, int slot, int position);
 
+/* Slots that start from one prefix: rows [0, prefix_len) of prefix_slot -- written, its cursor at prefix_len or beyond -- become the
+ * first rows of the listed slots without being copied: only the last block of 32 is, where the prefix ends inside one (one launch for
+ * all layers and slots), and the slots' cursors are set to prefix_len, whatever they held before.  From then on a listed slot's rows
+ * below prefix_len & ~31 are read by the _shared attention calls only, from prefix_slot, whose first prefix_len rows have to stay as they
+ * are; other readers of such a slot (plain attention calls, tt_hip_kv_read, snapshots) find what its own pages hold there.
+ * The rows from prefix_len on are the slot's own, at their own positions: append, epilogue, advance and rewind as ever.
+ * TT_HIP_ERR_INVALID_ARGUMENT: a slot out of range, or prefix_slot itself among the slots; TT_HIP_ERR_CURSOR: prefix_slot has fewer
+ * rows; TT_HIP_ERR_SHAPE: a ring. */
+TT_HIP_API int tt_hip_kv_share_prefix(tt_hip_kv *kv, int prefix_slot, int prefix_len, int n_slots, const int *slots);
+
 /* Element offsets (in halves, within one [slot][kv_head] page) of key/value
  * element (position, d).  Pure host arithmetic, the same functions the kernels
  * use; exported so that the layout is testable and documented in one place. */
@@ -482,6 +492,26 @@ TT_HIP_API int tt_hip_attn_prefill_sinks(tt_hip_ctx *ctx, tt_hip_kv *kv, int lay
                                          int kv_valid, int sliding_window, int sinks, int n_q_heads, const tt_half *q,
                                          size_t q_stride, const tt_half *gate, size_t gate_stride, float scale, tt_half *out,
                                          size_t o_stride);
+
+/* Sequences that share a prefix (tt_hip_kv_share_prefix): tt_hip_attn_decode, _verify and _prefill with the keys of positions
+ * [0, prefix_len) taken from prefix_slot, which the call reads once for all of its rows -- as it reads a chunk's keys -- and not
+ * once per sequence: many samples of one prompt, many users behind one system prompt, and a session's own first chunk behind it.
+ * The rest of a row's keys are its own slot's.  Every sequence of a call starts from the same prefix (one call per prefix); a
+ * sequence has prefix_len keys at least (seq_lens[i] >= prefix_len, start positions + 1 >= prefix_len), else
+ * TT_HIP_ERR_INVALID_ARGUMENT.  prefix_slot may be one of the slots; prefix_len below 32 is the plain call.  Results are those of the
+ * plain call over slots that hold the prefix's rows themselves, up to the order of the additions.  Not over a ring (TT_HIP_ERR_SHAPE).
+ * The partial results of the pass over the prefix live in a store the context owns (grown on demand: TT_HIP_ERR_BUSY inside a
+ * graph capture if it has to grow).  No counterpart in the reference, whose slots each hold their prompt. */
+TT_HIP_API int tt_hip_attn_decode_shared(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, const int *slots,
+                                         const int *seq_lens, int prefix_slot, int prefix_len, int n_q_heads, const tt_half *q,
+                                         const tt_half *gate, float scale, tt_half *out);
+TT_HIP_API int tt_hip_attn_verify_shared(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, const int *slots,
+                                         const int *start_positions, int rows, int prefix_slot, int prefix_len, int n_q_heads,
+                                         const tt_half *q, const tt_half *gate, float scale, tt_half *out);
+TT_HIP_API int tt_hip_attn_prefill_shared(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int slot, int start_pos, int q_len,
+                                          int kv_valid, int prefix_slot, int prefix_len, int n_q_heads, const tt_half *q,
+                                          size_t q_stride, const tt_half *gate, size_t gate_stride, float scale, tt_half *out,
+                                          size_t o_stride);
 
 /* Multi-row verify (MTP pair / wide verify): replaces
  * encodeFullAttentionDecodeOrderRows (RealForwardRunner+VerifyDecodeOrderAttention.swift:52-110)

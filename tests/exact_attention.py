@@ -41,7 +41,7 @@ def stored_rows(values, bits):
     levels = np.clip(np.rint((x - bias.astype(np.float32)[..., None]) / safe), 0, 2 ** bits - 1).astype(np.uint8).reshape(n, width)
     if bits == 4:
         levels = levels[:, 0::2] | (levels[:, 1::2] << 4)
-    return np.concatenate([levels, scale.view(np.uint8).reshape(n, -1), bias.view(np.uint8).reshape(n, -1)], 1)
+    return np.concatenate([levels, *(p.view(np.uint8).reshape(n, width // 32) for p in (scale, bias))], 1)
 
 
 def attend(q, k, v, seen, scale, gate=None, bits=16):
@@ -56,12 +56,14 @@ def attend(q, k, v, seen, scale, gate=None, bits=16):
         return out, bound
     q = q.astype(np.float64)
     for h in range(heads):
-        cols = slice(h // group * dim, (h // group + 1) * dim)
-        kk = (k[0][at, cols] + k[1][at, cols])
-        v_level, v_bias = v[0][at, cols], v[1][at, cols]
-        vv = v_level + v_bias
+        if h % group == 0:
+            cols = slice(h // group * dim, (h // group + 1) * dim)
+            v_level, v_bias = v[0][at, cols], v[1][at, cols]
+            kk, vv = k[0][at, cols] + k[1][at, cols], v_level + v_bias
+            abs_k, abs_v, abs_level, abs_bias, top_v, top_bias = (np.abs(kk), np.abs(vv), np.abs(v_level), np.abs(v_bias), np.abs(vv).max(0),
+                                                                 np.abs(v_bias).max(0))
         s = kk @ q[h] * scale
-        mags = np.abs(kk) @ np.abs(q[h]) * abs(scale)
+        mags = abs_k @ np.abs(q[h]) * abs(scale)
         ds = mags * ((dim + 4) * HALF32 + (0.0 if bits == 16 else HALF16)) + np.abs(s) * 2.0 ** -22
         w = np.exp(s - s.max())
         total = w.sum()
@@ -70,10 +72,10 @@ def attend(q, k, v, seen, scale, gate=None, bits=16):
         eps = 2.0 * 2.0 * ds.max() + 2.0 ** -20
         tiny = (w * total < 2.0 ** -13 * (1.0 if bits == 16 else 2.0 ** 8)).sum() / total
         if bits == 16:
-            err = (w @ np.abs(vv)) * (eps + 2 * HALF16) + tiny * 2.0 ** -25 * np.abs(vv).max(0)
+            err = (w @ abs_v) * (eps + 2 * HALF16) + tiny * 2.0 ** -25 * top_v
         else:
-            err = (w @ np.abs(vv)) * eps + (w @ np.abs(v_level)) * 3 * HALF16 + (w @ np.abs(v_bias)) * 2 * HALF16
-            err += tiny * 2.0 ** -25 * ((2 ** bits - 1) / 4.0 + np.abs(v_bias).max(0))
+            err = (w @ abs_v) * eps + (w @ abs_level) * 3 * HALF16 + (w @ abs_bias) * 2 * HALF16
+            err += tiny * 2.0 ** -25 * ((2 ** bits - 1) / 4.0 + top_bias)
         bound[h] = err
     if gate is not None:
         g = 1.0 / (1.0 + np.exp(-gate.astype(np.float64)))

@@ -83,6 +83,7 @@ _SIGNATURES = {
     "tt_hip_kv_reset": (_i, [_vp, _i]),
     "tt_hip_kv_reserve": (_i, [_vp, _i]),
     "tt_hip_kv_expect_position": (_i, [_vp, _i, _i]),
+    "tt_hip_kv_share_prefix": (_i, [_vp, _i, _i, _i, _c_int_p]),
     "tt_hip_kv_k_offset": (_sz, [_i, _i, _i]),
     "tt_hip_kv_v_offset": (_sz, [_i, _i, _i]),
     "tt_hip_attn_decode": (_i, [_vp, _vp, _i, _i, _c_int_p, _c_int_p, _i, _vp, _vp, ctypes.c_float, _vp]),
@@ -99,6 +100,9 @@ _SIGNATURES = {
     "tt_hip_attn_decode_sinks": (_i, [_vp, _vp, _i, _i, _c_int_p, _c_int_p, _i, _i, _i, _vp, _vp, ctypes.c_float, _vp]),
     "tt_hip_attn_verify_sinks": (_i, [_vp, _vp, _i, _i, _c_int_p, _c_int_p, _i, _i, _i, _i, _vp, _vp, ctypes.c_float, _vp]),
     "tt_hip_attn_prefill_sinks": (_i, [_vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _sz, _vp, _sz, ctypes.c_float, _vp, _sz]),
+    "tt_hip_attn_decode_shared": (_i, [_vp, _vp, _i, _i, _c_int_p, _c_int_p, _i, _i, _i, _vp, _vp, ctypes.c_float, _vp]),
+    "tt_hip_attn_verify_shared": (_i, [_vp, _vp, _i, _i, _c_int_p, _c_int_p, _i, _i, _i, _i, _vp, _vp, ctypes.c_float, _vp]),
+    "tt_hip_attn_prefill_shared": (_i, [_vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _sz, _vp, _sz, ctypes.c_float, _vp, _sz]),
     "tt_hip_attn_verify": (_i, [_vp, _vp, _i, _i, _c_int_p, _c_int_p, _i, _i, _vp, _vp, ctypes.c_float, _vp]),
     "tt_hip_kv_snapshot_segment_count": (_i, [_vp]),
     "tt_hip_kv_snapshot_segment_lengths": (_i, [_vp, _i, ctypes.POINTER(ctypes.c_size_t), _i]),

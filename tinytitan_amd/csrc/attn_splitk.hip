@@ -1954,7 +1954,7 @@ static int launch_one(tt_hip_ctx *ctx, const LaunchPlan &plan, int n_seq, const 
     launch_profiled(ctx, kernel, grid, dim3(WAVES * 64), (unsigned)(plan.lds_bytes + keep_list_bytes(KEEP, WAVES)), args);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return hip_fail(ctx, e, "attn_splitk_kernel launch");
-    if (plan.n_splits_max > 1 && !ctx->pass_only) return launch_combine_one<D, NT, KEEP == kKeepSinks>(ctx, plan, n_seq, args);
+    if (plan.n_splits_max > 1 && !plan.partials_only && !ctx->pass_only) return launch_combine_one<D, NT, KEEP == kKeepSinks>(ctx, plan, n_seq, args);
     return TT_HIP_OK;
 }
 

@@ -25,29 +25,31 @@ int hip_fail(tt_hip_ctx *ctx, hipError_t err, const char *what) {
     return err == hipErrorOutOfMemory ? TT_HIP_ERR_OUT_OF_MEMORY : TT_HIP_ERR_HIP;
 }
 
-int ensure_partials(tt_hip_ctx *ctx, size_t rows, int head_dim) {
+int ensure_partials(tt_hip_ctx *ctx, size_t rows, int head_dim, bool front) {
     // Sized for head_dim 256 so that a context serves every supported head_dim.
     (void)head_dim;
-    if (rows <= ctx->part_rows) return TT_HIP_OK;
+    float *&part_o = front ? ctx->front_o : ctx->part_o, *&part_ml = front ? ctx->front_ml : ctx->part_ml;
+    size_t &part_rows = front ? ctx->front_rows : ctx->part_rows;
+    if (rows <= part_rows) return TT_HIP_OK;
     if (ctx->capturing) return TT_HIP_ERR_BUSY;  // growing would synchronise and allocate inside a capture
     hipError_t e = hipStreamSynchronize(ctx->stream);
     if (e != hipSuccess) return hip_fail(ctx, e, "hipStreamSynchronize");
-    if (ctx->part_o) (void)hipFree(ctx->part_o);
-    if (ctx->part_ml) (void)hipFree(ctx->part_ml);
-    ctx->part_o = nullptr;
-    ctx->part_ml = nullptr;
-    ctx->part_rows = 0;
+    if (part_o) (void)hipFree(part_o);
+    if (part_ml) (void)hipFree(part_ml);
+    part_o = nullptr;
+    part_ml = nullptr;
+    part_rows = 0;
     ++ctx->generation;
     size_t want = rows + rows / 4;
-    e = hipMalloc(reinterpret_cast<void **>(&ctx->part_o), want * 256 * sizeof(float));
+    e = hipMalloc(reinterpret_cast<void **>(&part_o), want * 256 * sizeof(float));
     if (e != hipSuccess) return hip_fail(ctx, e, "hipMalloc(split partial O)");
-    e = hipMalloc(reinterpret_cast<void **>(&ctx->part_ml), want * 2 * sizeof(float));
+    e = hipMalloc(reinterpret_cast<void **>(&part_ml), want * 2 * sizeof(float));
     if (e != hipSuccess) {
-        (void)hipFree(ctx->part_o);
-        ctx->part_o = nullptr;
+        (void)hipFree(part_o);
+        part_o = nullptr;
         return hip_fail(ctx, e, "hipMalloc(split partial m/l)");
     }
-    ctx->part_rows = want;
+    part_rows = want;
     return TT_HIP_OK;
 }
 
@@ -297,6 +299,14 @@ struct KeepLists {
 //   chunk_splits > 1 (kind 1, one sequence): the chunk kernel over chunk_splits key ranges of
 //   chunk_split_blocks blocks, then the combine pass.
 //   sinks >= 0 (kind 0): the keys [0, sinks) stay visible beside the window; pinned rows of a ring are known.  -1: neither.
+//   piece: the pass takes one piece of the rows' keys and leaves its partial results there, for launch_join (at most
+//   kMaxSeqPerLaunch sequences).
+struct KeyPiece {
+    bool front;  // the keys that the sequences share, with a store for partial results of its own
+    int first_block = 0;  // the pages' blocks in front of the piece: starts and totals count from here
+    PassParts parts{};
+    int first_split[kMaxSeqPerLaunch] = {};
+};
 static int run_attention(tt_hip_ctx *ctx, tt_hip_kv *kv, int kind, int layer, int n_seq, const int *slots,
                          const int *starts, const int *totals, int rows, int n_q_heads, const tt_half *q,
                          long long q_seq_stride, long long q_tok_stride, const tt_half *gate, long long g_seq_stride,
@@ -304,7 +314,7 @@ static int run_attention(tt_hip_ctx *ctx, tt_hip_kv *kv, int kind, int layer, in
                          long long o_tok_stride, int chunk_splits = 1, int chunk_split_blocks = 0,
                          const PageSource *pages = nullptr, int window = 0, const uint8_t *keep = nullptr,
                          long long keep_seq_stride = 0, long long keep_row_stride = 0, bool static_partials = false,
-                         const KeepLists *lists = nullptr, int sinks = -1) {
+                         const KeepLists *lists = nullptr, int sinks = -1, KeyPiece *piece = nullptr) {
     const int D = kv->head_dim;
     hipError_t e = hipSetDevice(ctx->device);
     if (e != hipSuccess) return hip_fail(ctx, e, "hipSetDevice");
@@ -487,12 +497,14 @@ static int run_attention(tt_hip_ctx *ctx, tt_hip_kv *kv, int kind, int layer, in
         // of 16/2 of 256 behind 336 .. 433 10.39 / 11.00; two tiles, 3 rows x 2 sequences of 24/2 of 256, 11.94 against 11.32).
         plan.packed_splits = ragged && (plan.workgroups > ctx->n_cus || plan.tok_tiles > 1) ? (int)total_splits : 0;
         if (plan.packed_splits > 0 && plan.tok_tiles > 1) plan.packed_splits = (plan.packed_splits + 7) & ~7;
-        if (plan.n_splits_max > 1) {
+        plan.partials_only = piece != nullptr;
+        const bool front = piece && piece->front;
+        if (plan.n_splits_max > 1 || piece) {
             const size_t part_rows = total_splits * plan.n_tiles * plan.nt;
             if (static_partials) {
                 if (part_rows > kStaticPartialRows) return TT_HIP_ERR_SCRATCH;
             } else {
-                st = ensure_partials(ctx, part_rows, D);
+                st = ensure_partials(ctx, part_rows, D, front);
                 if (st != TT_HIP_OK) return st;
             }
         }
@@ -501,11 +513,15 @@ static int run_attention(tt_hip_ctx *ctx, tt_hip_kv *kv, int kind, int layer, in
         SplitKHot &h = a.hot;
         h.k_layer = walks_pages ? pages->k : kv->k[layer];
         h.v_layer = walks_pages ? pages->v : kv->v[layer];
+        if (piece) {
+            h.k_layer += piece->first_block * (kv->block_bytes() / 2);
+            h.v_layer += piece->first_block * (kv->block_bytes() / 2);
+        }
         h.q = reinterpret_cast<const _Float16 *>(q) + base * q_seq_stride;
         a.gate = gate ? reinterpret_cast<const _Float16 *>(gate) + base * g_seq_stride : nullptr;
         a.out = reinterpret_cast<_Float16 *>(out) + base * o_seq_stride;
-        h.part_o = static_partials ? ctx->static_scratch : ctx->part_o;
-        h.part_ml = static_partials ? ctx->static_scratch + kStaticPartialRows * 256 : ctx->part_ml;
+        h.part_o = static_partials ? ctx->static_scratch : front ? ctx->front_o : ctx->part_o;
+        h.part_ml = static_partials ? ctx->static_scratch + kStaticPartialRows * 256 : front ? ctx->front_ml : ctx->part_ml;
         h.page_elems = walks_pages ? pages->page_elems : (long long)kv->page_elems();
         h.q_seq_stride = q_seq_stride;
         h.q_tok_stride = q_tok_stride;
@@ -524,6 +540,12 @@ static int run_attention(tt_hip_ctx *ctx, tt_hip_kv *kv, int kind, int layer, in
         h.n_tiles = plan.n_tiles;
         h.split_len = plan.split_len;
         h.n_splits_max = plan.n_splits_max;
+        if (piece) {
+            // (a launch of one split would write the final rows: it is told of a second one, which no tile has)
+            if (h.n_splits_max == 1) h.n_splits_max = 2;
+            piece->parts = PassParts{h.part_o, h.part_ml, plan.nt, plan.gh, plan.tt, plan.hsubs, plan.tok_tiles, plan.n_tiles, plan.split_len};
+            std::copy(first_split, first_split + n, piece->first_split);
+        }
         const bool aligned = aligned16(h.q) && aligned16(a.out) && (!a.gate || aligned16(a.gate)) && q_seq_stride % 8 == 0 &&
                              q_tok_stride % 8 == 0 && g_seq_stride % 8 == 0 && g_tok_stride % 8 == 0 && o_seq_stride % 8 == 0 &&
                              o_tok_stride % 8 == 0;
@@ -591,9 +613,8 @@ static int run_attention(tt_hip_ctx *ctx, tt_hip_kv *kv, int kind, int layer, in
         }
         if (chunk_splits > 1) {
             st = launch_prefill(ctx, kv, layer, slots[base], starts[base], rows, totals[base], n_q_heads, q, q_tok_stride, gate,
-                                g_tok_stride, scale, out, o_tok_stride, chunk_splits, chunk_split_blocks, ctx->part_o,
-                                ctx->part_ml, pages, window);
-            if (st == TT_HIP_OK) st = launch_combine(ctx, plan, D, n, a);
+                                g_tok_stride, scale, out, o_tok_stride, chunk_splits, chunk_split_blocks, h.part_o, h.part_ml, pages, window);
+            if (st == TT_HIP_OK && !piece) st = launch_combine(ctx, plan, D, n, a);
         } else {
             st = launch_splitk(ctx, plan, D, n, a, kv_bits);
         }
@@ -691,6 +712,8 @@ void tt_hip_ctx_destroy(tt_hip_ctx *ctx) {
     (void)hipStreamSynchronize(ctx->stream);  // (null: the default stream)
     if (ctx->part_o) (void)hipFree(ctx->part_o);
     if (ctx->part_ml) (void)hipFree(ctx->part_ml);
+    if (ctx->front_o) (void)hipFree(ctx->front_o);
+    if (ctx->front_ml) (void)hipFree(ctx->front_ml);
     if (ctx->stage_k) (void)hipFree(ctx->stage_k);
     if (ctx->stage_v) (void)hipFree(ctx->stage_v);
     if (ctx->select_ws) (void)hipFree(ctx->select_ws);
@@ -1400,6 +1423,183 @@ int tt_hip_attn_prefill_swa(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int slot,
     // (without memory for the splits' partial results, as inside a capture that would have to grow it: tiles of one head, which have none)
     if (plentiful && (st == TT_HIP_ERR_BUSY || st == TT_HIP_ERR_OUT_OF_MEMORY)) st = in_tiles(1);
     return st;
+}
+
+// ---- sequences that share a prefix ------------------------------------------
+
+// Rows of sequences whose keys [0, front) -- whole blocks -- are another slot's rows: a pass over those with the tokens of all
+// sequences as rows of one, a pass over each sequence's own keys from there on, and the join.  The shared keys are then read once per
+// tile of rows, as a chunk's are, and not once per sequence.
+static int run_shared(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, const int *slots, const int *starts, const int *totals, int rows,
+                      int prefix_slot, int front, int n_q_heads, const tt_half *q, long long q_seq_stride, long long q_tok_stride,
+                      const tt_half *gate, long long g_seq_stride, long long g_tok_stride, float scale, tt_half *out,
+                      long long o_seq_stride, long long o_tok_stride) {
+    if (hipSetDevice(ctx->device) != hipSuccess) return TT_HIP_ERR_HIP;
+    const int D = kv->head_dim, tokens = n_seq * rows;
+    const int front_from = front;  // (no row's own position limits what it sees of the shared keys)
+    const bool aligned = aligned16(q) && q_tok_stride % 8 == 0;
+    const bool serves = prefill_kernel_serves(n_q_heads, kv->n_kv_heads, D, aligned) && scale > 0.0f;
+    // The shared keys: as behind a long context, the chunk kernel over ranges of the keys from some rows and keys on, else the split-K tiles.
+    const int rows_from = kv->bits == 16 ? (front >= 32768 ? 32 : 64) : 64;
+    const long long keys_from = std::max<long long>(786432 / tokens, kv->bits == 16 ? 4096 : 2560);
+    KeyPiece shared{true}, own{false, front / kBlockTokens};
+    KeyRanges ranges;
+    PageSource staged{};
+    const PageSource *pages = nullptr;
+    int st = TT_HIP_OK;
+    if (serves && tokens >= rows_from && front >= keys_from)
+        ranges = plan_key_ranges(ctx->n_cus, D, n_q_heads, kv->n_kv_heads, tokens, front / kBlockTokens);
+    if (ranges.n_splits >= 2 && kv->bits != 16) {
+        const size_t page = (size_t)front * D;
+        st = ensure_stage(ctx, page * kv->n_kv_heads);
+        if (st == TT_HIP_OK) st = launch_kvq_dequant_blocks(kv, layer, prefix_slot, front / kBlockTokens, ctx->stage_k, ctx->stage_v, page);
+        else if (st == TT_HIP_ERR_BUSY || st == TT_HIP_ERR_OUT_OF_MEMORY) ranges.n_splits = 1, st = TT_HIP_OK;  // (the pages as they are)
+        if (st != TT_HIP_OK) return st;
+        staged = PageSource{ctx->stage_k, ctx->stage_v, (long long)page, 0};
+        pages = &staged;
+    }
+    const bool by_ranges = ranges.n_splits >= 2;
+    st = run_attention(ctx, kv, by_ranges ? 1 : 0, layer, 1, &prefix_slot, &front_from, &front, tokens, n_q_heads, q, 0, q_tok_stride, nullptr,
+                       0, 0, scale, out, 0, o_tok_stride, by_ranges ? ranges.n_splits : 1, ranges.split_blocks, by_ranges ? pages : nullptr, 0,
+                       nullptr, 0, 0, false, nullptr, -1, &shared);
+    if (st != TT_HIP_OK) return st;
+    IntTable own_starts(n_seq), own_totals(n_seq);
+    for (int i = 0; i < n_seq; ++i) {
+        own_starts[i] = starts[i] - front;
+        own_totals[i] = totals[i] - front;
+    }
+    st = run_attention(ctx, kv, 0, layer, n_seq, slots, own_starts.data(), own_totals.data(), rows, n_q_heads, q, q_seq_stride, q_tok_stride,
+                       nullptr, 0, 0, scale, out, o_seq_stride, o_tok_stride, 1, 0, nullptr, 0, nullptr, 0, 0, false, nullptr, 0, &own);
+    if (st != TT_HIP_OK) return st;
+    JoinArgs j{};
+    j.front = shared.parts;
+    j.own = own.parts;
+    j.front_splits = std::max((front + shared.parts.split_len - 1) / shared.parts.split_len, 1);
+    j.rows = rows;
+    j.heads = n_q_heads;
+    j.group = n_q_heads / kv->n_kv_heads;
+    j.gate = reinterpret_cast<const _Float16 *>(gate);
+    j.out = reinterpret_cast<_Float16 *>(out);
+    j.g_seq_stride = g_seq_stride;
+    j.g_tok_stride = g_tok_stride;
+    j.o_seq_stride = o_seq_stride;
+    j.o_tok_stride = o_tok_stride;
+    j.aligned = aligned16(out) && o_seq_stride % 8 == 0 && o_tok_stride % 8 == 0;
+    for (int i = 0; i < n_seq; ++i) j.seq[i] = JoinSeq{own_starts[i], own_totals[i], own.first_split[i]};
+    return launch_join(ctx, D, n_seq, j);
+}
+
+// ... of any number of sequences and rows, in pieces of at most kMaxSeqPerLaunch sequences and kSharedTokens rows of all together, so that
+// the partial results stay small.  (Several sequences in a piece come with all of their rows: these then lie one behind the other, as
+// the pass over the shared keys takes them.)
+constexpr int kSharedTokens = 1024;
+static int run_shared_rows(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, const int *slots, const int *starts, const int *totals,
+                           int rows, int prefix_slot, int front, int n_q_heads, const tt_half *q, long long q_seq_stride,
+                           long long q_tok_stride, const tt_half *gate, long long g_seq_stride, long long g_tok_stride, float scale,
+                           tt_half *out, long long o_seq_stride, long long o_tok_stride) {
+    const int seqs_at_once = std::min(std::max(kSharedTokens / rows, 1), kMaxSeqPerLaunch), rows_at_once = std::min(rows, kSharedTokens);
+    for (int base = 0; base < n_seq; base += seqs_at_once) {
+        const int n = std::min(n_seq - base, seqs_at_once);
+        for (int r = 0; r < rows; r += rows_at_once) {
+            int first[kMaxSeqPerLaunch];
+            for (int i = 0; i < n; ++i) first[i] = starts[base + i] + r;
+            const int st = run_shared(ctx, kv, layer, n, slots + base, first, totals + base, std::min(rows - r, rows_at_once), prefix_slot, front,
+                                      n_q_heads, q + base * q_seq_stride + r * q_tok_stride, q_seq_stride, q_tok_stride,
+                                      gate ? gate + base * g_seq_stride + r * g_tok_stride : nullptr, g_seq_stride, g_tok_stride, scale,
+                                      out + base * o_seq_stride + r * o_tok_stride, o_seq_stride, o_tok_stride);
+            if (st != TT_HIP_OK) return st;
+        }
+    }
+    return TT_HIP_OK;
+}
+
+static int check_prefix(const tt_hip_kv *kv, int prefix_slot, int prefix_len) {
+    if (prefix_slot < 0 || prefix_slot >= kv->n_slots || prefix_len < 0) return TT_HIP_ERR_INVALID_ARGUMENT;
+    if (kv->ring) return TT_HIP_ERR_SHAPE;  // (whose rows the prefix's slot itself overwrites)
+    return prefix_len <= kv->capacity ? TT_HIP_OK : TT_HIP_ERR_CAPACITY;
+}
+
+int tt_hip_kv_share_prefix(tt_hip_kv *kv, int prefix_slot, int prefix_len, int n_slots, const int *slots) {
+    if (!kv || n_slots <= 0 || !slots) return TT_HIP_ERR_INVALID_ARGUMENT;
+    int st = check_prefix(kv, prefix_slot, prefix_len);
+    if (st != TT_HIP_OK) return st;
+    for (int i = 0; i < n_slots; ++i)
+        if (slots[i] < 0 || slots[i] >= kv->n_slots || slots[i] == prefix_slot) return TT_HIP_ERR_INVALID_ARGUMENT;
+    if (kv->positions[prefix_slot] < prefix_len) return TT_HIP_ERR_CURSOR;
+    BusyGuard guard(kv->ctx);
+    if (!guard.ok) return TT_HIP_ERR_BUSY;
+    if (prefix_len % kBlockTokens != 0) {
+        if (hipSetDevice(kv->ctx->device) != hipSuccess) return TT_HIP_ERR_HIP;
+        st = launch_kv_copy_block(kv, prefix_slot, prefix_len / kBlockTokens, n_slots, slots);
+        if (st != TT_HIP_OK) return st;
+    }
+    for (int i = 0; i < n_slots; ++i) kv->positions[slots[i]] = prefix_len;
+    return TT_HIP_OK;
+}
+
+int tt_hip_attn_verify_shared(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, const int *slots, const int *start_positions, int rows,
+                              int prefix_slot, int prefix_len, int n_q_heads, const tt_half *q, const tt_half *gate, float scale,
+                              tt_half *out) {
+    int st = check_common(ctx, kv, layer, n_q_heads, q, out);
+    if (st != TT_HIP_OK) return st;
+    if (n_seq <= 0 || rows <= 0 || !slots || !start_positions) return TT_HIP_ERR_INVALID_ARGUMENT;
+    st = check_prefix(kv, prefix_slot, prefix_len);
+    if (st != TT_HIP_OK) return st;
+    IntTable totals(n_seq);
+    for (int i = 0; i < n_seq; ++i) {
+        if (slots[i] < 0 || slots[i] >= kv->n_slots || start_positions[i] < 0 || start_positions[i] + 1LL < prefix_len) return TT_HIP_ERR_INVALID_ARGUMENT;
+        if (!kv->holds_keys(0, (long long)start_positions[i] + rows)) return TT_HIP_ERR_CAPACITY;
+        totals[i] = start_positions[i] + rows;
+    }
+    const int front = prefix_len / kBlockTokens * kBlockTokens;
+    if (front == 0) return tt_hip_attn_verify(ctx, kv, layer, n_seq, slots, start_positions, rows, n_q_heads, q, gate, scale, out);
+    BusyGuard guard(ctx);
+    if (!guard.ok) return TT_HIP_ERR_BUSY;
+    const long long tok = (long long)n_q_heads * kv->head_dim, seq = tok * rows;
+    return run_shared_rows(ctx, kv, layer, n_seq, slots, start_positions, totals.data(), rows, prefix_slot, front, n_q_heads, q, seq, tok,
+                           gate, seq, tok, scale, out, seq, tok);
+}
+
+int tt_hip_attn_decode_shared(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, const int *slots, const int *seq_lens, int prefix_slot,
+                              int prefix_len, int n_q_heads, const tt_half *q, const tt_half *gate, float scale, tt_half *out) {
+    int st = check_common(ctx, kv, layer, n_q_heads, q, out);
+    if (st != TT_HIP_OK) return st;
+    if (n_seq <= 0 || !seq_lens || !slots) return TT_HIP_ERR_INVALID_ARGUMENT;
+    st = check_prefix(kv, prefix_slot, prefix_len);
+    if (st != TT_HIP_OK) return st;
+    if (prefix_len < kBlockTokens) {  // (a sequence without keys is the plain call's to serve)
+        for (int i = 0; i < n_seq; ++i)
+            if (seq_lens[i] < prefix_len) return TT_HIP_ERR_INVALID_ARGUMENT;
+        return tt_hip_attn_decode(ctx, kv, layer, n_seq, slots, seq_lens, n_q_heads, q, gate, scale, out);
+    }
+    IntTable starts(n_seq);
+    for (int i = 0; i < n_seq; ++i) {
+        if (seq_lens[i] < prefix_len) return TT_HIP_ERR_INVALID_ARGUMENT;
+        starts[i] = seq_lens[i] - 1;
+    }
+    return tt_hip_attn_verify_shared(ctx, kv, layer, n_seq, slots, starts.data(), 1, prefix_slot, prefix_len, n_q_heads, q, gate, scale, out);
+}
+
+int tt_hip_attn_prefill_shared(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int slot, int start_pos, int q_len, int kv_valid,
+                               int prefix_slot, int prefix_len, int n_q_heads, const tt_half *q, size_t q_stride, const tt_half *gate,
+                               size_t gate_stride, float scale, tt_half *out, size_t o_stride) {
+    int st = check_common(ctx, kv, layer, n_q_heads, q, out);
+    if (st != TT_HIP_OK) return st;
+    st = check_prefix(kv, prefix_slot, prefix_len);
+    if (st != TT_HIP_OK) return st;
+    if (slot < 0 || slot >= kv->n_slots || start_pos < 0 || q_len <= 0 || start_pos + 1LL < prefix_len) return TT_HIP_ERR_INVALID_ARGUMENT;
+    const int front = prefix_len / kBlockTokens * kBlockTokens;
+    if (front == 0 || slot == prefix_slot)
+        return tt_hip_attn_prefill(ctx, kv, layer, slot, start_pos, q_len, kv_valid, n_q_heads, q, q_stride, gate, gate_stride, scale, out,
+                                   o_stride);
+    const size_t packed = (size_t)n_q_heads * kv->head_dim;
+    if (q_stride < packed || o_stride < packed || (gate && gate_stride < packed)) return TT_HIP_ERR_SHAPE;
+    if ((long long)start_pos + q_len > kv_valid) return TT_HIP_ERR_INVALID_ARGUMENT;
+    if (!kv->holds_keys(0, kv_valid)) return TT_HIP_ERR_CAPACITY;
+    BusyGuard guard(ctx);
+    if (!guard.ok) return TT_HIP_ERR_BUSY;
+    return run_shared_rows(ctx, kv, layer, 1, &slot, &start_pos, &kv_valid, q_len, prefix_slot, front, n_q_heads, q, 0, (long long)q_stride,
+                           gate, 0, (long long)gate_stride, scale, out, 0, (long long)o_stride);
 }
 
 }  // extern "C"

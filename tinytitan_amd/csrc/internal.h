@@ -118,6 +118,29 @@ struct LaunchPlan {
     bool xcd_grid;  // launch with kHotXcdGrid
     int slots_per_cu;  // workgroups that the planner's rule for unlike lengths counts on
     int packed_splits;  // > 0: launch with kHotPackedSplits over this many splits
+    bool partials_only;  // the partial results are somebody else's to combine (PassParts)
+};
+
+// Where a pass over one piece of the keys has left its partial results: row n of a tile's split lies at
+// ((first_split(sequence) + split) * n_tiles + tile) * nt + n, D floats of `o` and a (maximum, sum) pair of `ml`.
+struct PassParts {
+    const float *o, *ml;
+    int nt, gh, tt, hsubs, tok_tiles, n_tiles;
+    int split_len;  // keys of a split; a tile of a sequence has as many splits as its last row's keys need, one at least
+};
+// A sequence of a join: its own piece of the keys as the pass over that saw it.
+struct JoinSeq {
+    int start, total, first_split;
+};
+struct JoinArgs {
+    PassParts front, own;  // the piece that all sequences share -- all tokens are rows of one sequence there -- and each one's own
+    int front_splits;
+    int rows;              // tokens per sequence
+    int heads, group, aligned;
+    const _Float16 *gate;  // nullptr: no gate
+    _Float16 *out;
+    long long g_seq_stride, g_tok_stride, o_seq_stride, o_tok_stride;
+    JoinSeq seq[kMaxSeqPerLaunch];
 };
 
 }  // namespace tt
@@ -134,6 +157,8 @@ struct tt_hip_ctx {
     float *part_ml = nullptr;
     float *static_scratch = nullptr;  // this device's address of the library's fixed scratch array
     size_t part_rows = 0;  // capacity in (seq, tile, split, n) rows
+    float *front_o = nullptr, *front_ml = nullptr;  // the same of a pass over the keys that sequences share
+    size_t front_rows = 0;
     _Float16 *stage_k = nullptr, *stage_v = nullptr;  // fp16 pages of one slot, dequantised for a prefill chunk
     size_t stage_elems = 0;                           // halves in each
     void *select_ws = nullptr;  // the multi-workgroup key selection's sorted chunks and their tables
@@ -235,7 +260,7 @@ int configure_splitk_kernels(tt_hip_ctx *ctx);
 int configure_prefill_kernels(tt_hip_ctx *ctx);
 int configure_affine_kernels(tt_hip_ctx *ctx);
 
-int ensure_partials(tt_hip_ctx *ctx, size_t rows, int head_dim);
+int ensure_partials(tt_hip_ctx *ctx, size_t rows, int head_dim, bool front = false);
 int ensure_stage(tt_hip_ctx *ctx, size_t elems);
 
 // K/V pages the chunk kernel reads instead of the cache's own (one slot's, kv head pages page_elems apart).
@@ -262,6 +287,11 @@ int launch_prefill(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int slot, int star
                    float scale, tt_half *out, long long o_stride, int n_splits = 1, int split_blocks = 0,
                    float *part_o = nullptr, float *part_ml = nullptr, const PageSource *pages = nullptr, int window = 0, bool single_tiles = false);
 int launch_combine(tt_hip_ctx *ctx, const LaunchPlan &plan, int head_dim, int n_seq, const SplitKArgs &args);
+// The rows of n_seq sequences from the partial results of two passes (attn_join.hip).
+int launch_join(tt_hip_ctx *ctx, int head_dim, int n_seq, const JoinArgs &args);
+
+// A prefix that slots share: block `block` of `slot`'s pages, every layer, into the same place of `n_slots` others.
+int launch_kv_copy_block(tt_hip_kv *kv, int slot, int block, int n_slots, const int *slots);
 
 int launch_kv_append(tt_hip_kv *kv, int layer, int slot, int position, int n_tokens, const tt_half *k, const tt_half *v,
                      size_t stride);

@@ -218,6 +218,48 @@ static int round_up_block(long long tokens) {
     return (int)(((tokens + kBlockTokens - 1) / kBlockTokens) * kBlockTokens);
 }
 
+// One block of a slot's pages into other slots' pages, as it is stored, whatever that is: (slot, kv head, K or V of a layer) a workgroup.
+constexpr int kCopyLayers = 64;
+struct CopyBlockArgs {
+    uint8_t *store[kCopyLayers][2];
+    long long page_bytes, block_at;
+    int block_bytes, n_kv_heads, from;
+    uint8_t to[TT_HIP_MAX_SLOTS];
+};
+static_assert(TT_HIP_MAX_SLOTS <= 256, "a slot is a byte");
+__global__ __launch_bounds__(256) void kv_copy_block_kernel(const CopyBlockArgs a) {
+    typedef unsigned u4 __attribute__((ext_vector_type(4)));
+    uint8_t *const store = a.store[blockIdx.z >> 1][blockIdx.z & 1];
+    const u4 *src = reinterpret_cast<const u4 *>(store + ((long long)a.from * a.n_kv_heads + blockIdx.y) * a.page_bytes + a.block_at);
+    u4 *dst = reinterpret_cast<u4 *>(store + ((long long)a.to[blockIdx.x] * a.n_kv_heads + blockIdx.y) * a.page_bytes + a.block_at);
+    for (int i = threadIdx.x; i < a.block_bytes / 16; i += 256) dst[i] = src[i];
+}
+
+int launch_kv_copy_block(tt_hip_kv *kv, int slot, int block, int n_slots, const int *slots) {
+    CopyBlockArgs a;
+    a.page_bytes = (long long)kv->page_bytes();
+    a.block_bytes = (int)kv->block_bytes();
+    a.block_at = (long long)block * a.block_bytes;
+    a.n_kv_heads = kv->n_kv_heads;
+    a.from = slot;
+    for (int first = 0; first < n_slots; first += TT_HIP_MAX_SLOTS) {
+        const int n = std::min(n_slots - first, TT_HIP_MAX_SLOTS);
+        for (int i = 0; i < n; ++i) a.to[i] = (uint8_t)slots[first + i];
+        for (int layer = 0; layer < kv->n_layers; layer += kCopyLayers) {
+            const int layers = std::min(kv->n_layers - layer, kCopyLayers);
+            for (int i = 0; i < layers; ++i) {
+                a.store[i][0] = reinterpret_cast<uint8_t *>(kv->k[layer + i]);
+                a.store[i][1] = reinterpret_cast<uint8_t *>(kv->v[layer + i]);
+            }
+            hipLaunchKernelGGL(kv_copy_block_kernel, dim3((unsigned)n, (unsigned)kv->n_kv_heads, (unsigned)(2 * layers)), dim3(256), 0,
+                               kv->ctx->stream, a);
+            const hipError_t e = hipGetLastError();
+            if (e != hipSuccess) return hip_fail(kv->ctx, e, "kv_copy_block_kernel launch");
+        }
+    }
+    return TT_HIP_OK;
+}
+
 // Allocates zero-filled stores for every layer at `capacity` tokens per slot.
 // Zero fill matters: rows past a sequence's end inside its last 32-token block
 // are multiplied by probability 0 in the P.V contraction and must be finite.

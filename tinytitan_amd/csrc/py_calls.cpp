@@ -26,6 +26,9 @@ namespace {
     F(tt_hip_attn_decode_sinks)                                                                                          \
     F(tt_hip_attn_verify_sinks)                                                                                          \
     F(tt_hip_attn_prefill_sinks)                                                                                         \
+    F(tt_hip_attn_decode_shared)                                                                                         \
+    F(tt_hip_attn_verify_shared)                                                                                         \
+    F(tt_hip_attn_prefill_shared)                                                                                        \
     F(tt_hip_attn_prefill)                                                                                               \
     F(tt_hip_attn_prefill_swa)                                                                                           \
     F(tt_hip_attn_prefill_keep)                                                                                          \
@@ -361,6 +364,48 @@ TT_CALL(attn_verify_sinks) {
     });
 }
 
+// (ctx, kv, layer, slots, lengths, prefix_slot, prefix_len, heads, q, gate, scale, out)
+TT_CALL(attn_decode_shared) {
+    Args a(args, n, 12);
+    if (!a.ok) return nullptr;
+    auto *ctx = a.handle<tt_hip_ctx>();
+    auto *kv = a.handle<tt_hip_kv>();
+    const int layer = a.i();
+    Ints slots, lens;
+    slots.take(a);
+    lens.take(a);
+    const int prefix_slot = a.i(), prefix_len = a.i(), heads = a.i();
+    const tt_half *q = a.half(), *gate = a.half();
+    const float scale = a.real();
+    tt_half *out = a.half();
+    return finish(a, [&] {
+        if (slots.count != lens.count) return (int)TT_HIP_ERR_INVALID_ARGUMENT;
+        return lib.tt_hip_attn_decode_shared(ctx, kv, layer, slots.count, slots.values, lens.values, prefix_slot, prefix_len, heads, q,
+                                             gate, scale, out);
+    });
+}
+
+// (ctx, kv, layer, slots, start_positions, rows, prefix_slot, prefix_len, heads, q, gate, scale, out)
+TT_CALL(attn_verify_shared) {
+    Args a(args, n, 13);
+    if (!a.ok) return nullptr;
+    auto *ctx = a.handle<tt_hip_ctx>();
+    auto *kv = a.handle<tt_hip_kv>();
+    const int layer = a.i();
+    Ints slots, starts;
+    slots.take(a, true);
+    starts.take(a, true);
+    const int rows = a.i(), prefix_slot = a.i(), prefix_len = a.i(), heads = a.i();
+    const tt_half *q = a.half(), *gate = a.half();
+    const float scale = a.real();
+    tt_half *out = a.half();
+    return finish(a, [&] {
+        if (slots.count > starts.count) return (int)TT_HIP_ERR_INVALID_ARGUMENT;  // (positions may be a longer table than the step's)
+        return lib.tt_hip_attn_verify_shared(ctx, kv, layer, slots.count, slots.values, starts.values, rows, prefix_slot, prefix_len, heads,
+                                             q, gate, scale, out);
+    });
+}
+
 // What the chunk calls have in common behind their own arguments: (heads, q, q_stride, gate, gate_stride, scale, out, o_stride)
 struct Rows {
     int heads;
@@ -403,6 +448,20 @@ TT_CALL(attn_prefill_sinks) {
     return finish(a, [&] {
         return lib.tt_hip_attn_prefill_sinks(ctx, kv, layer, slot, start, count, valid, window, sinks, r.heads, r.q, r.q_stride, r.gate,
                                              r.gate_stride, r.scale, r.out, r.o_stride);
+    });
+}
+
+// (ctx, kv, layer, slot, start, query_count, kv_valid, prefix_slot, prefix_len, <rows>)
+TT_CALL(attn_prefill_shared) {
+    Args a(args, n, 17);
+    if (!a.ok) return nullptr;
+    auto *ctx = a.handle<tt_hip_ctx>();
+    auto *kv = a.handle<tt_hip_kv>();
+    const int layer = a.i(), slot = a.i(), start = a.i(), count = a.i(), valid = a.i(), prefix_slot = a.i(), prefix_len = a.i();
+    const Rows r(a);
+    return finish(a, [&] {
+        return lib.tt_hip_attn_prefill_shared(ctx, kv, layer, slot, start, count, valid, prefix_slot, prefix_len, r.heads, r.q, r.q_stride,
+                                              r.gate, r.gate_stride, r.scale, r.out, r.o_stride);
     });
 }
 
@@ -598,6 +657,7 @@ PyMethodDef methods[] = {
     {"bind", bind, METH_O, nullptr},
     TT_METHOD(attn_decode) TT_METHOD(attn_decode_swa) TT_METHOD(attn_decode_keep) TT_METHOD(attn_decode_keep_indices)
     TT_METHOD(attn_verify_swa) TT_METHOD(attn_decode_sinks) TT_METHOD(attn_verify_sinks) TT_METHOD(attn_prefill_sinks)
+    TT_METHOD(attn_decode_shared) TT_METHOD(attn_verify_shared) TT_METHOD(attn_prefill_shared)
     TT_METHOD(attn_prefill) TT_METHOD(attn_prefill_keep) TT_METHOD(attn_prefill_keep_indices)
     TT_METHOD(kv_append) TT_METHOD(qkv_epilogue_append) TT_METHOD(affine_projection) TT_METHOD(qsa_pool_blocks)
     TT_METHOD(qsa_norm_rope_rows) TT_METHOD(qsa_block_scores) TT_METHOD(qsa_decode_scores) TT_METHOD(qsa_select)

@@ -246,6 +246,12 @@ class KVCacheManager:
     def expect_position(self, slot: int, position: int) -> None:
         self.ctx._check(self._lib.tt_hip_kv_expect_position(self.handle, slot, position), "tt_hip_kv_expect_position")
 
+    def share_prefix(self, prefix_slot: int, length: int, slots: Sequence[int]) -> None:
+        """The listed slots start from rows ``[0, length)`` of ``prefix_slot``: nothing is copied but the last part block, and the
+        slots' cursors are set to ``length``.  Attention calls then take ``prefix=SharedPrefix(prefix_slot, length)``."""
+        table = capi.int_array(slots)
+        self.ctx._check(self._lib.tt_hip_kv_share_prefix(self.handle, prefix_slot, length, len(table), table), "tt_hip_kv_share_prefix")
+
     # -- rows ----------------------------------------------------------------
     def append(self, layer: int, slot: int, position: int, k: torch.Tensor, v: torch.Tensor,
                token_stride: Optional[int] = None, n_tokens: Optional[int] = None) -> None:
@@ -343,6 +349,13 @@ class KVCacheManager:
             pass
 
 
+@dataclass(frozen=True)
+class SharedPrefix:
+    """A prefix that slots share (``KVCacheManager.share_prefix``): the first ``length`` rows of ``slot``."""
+    slot: int
+    length: int
+
+
 class Attention:
     """Decode attention over the cache (``Attention.encodeFull`` + the sigmoid gate pass)."""
 
@@ -351,9 +364,17 @@ class Attention:
         self._calls = ctx._calls
 
     def encode_full(self, kv: KVCacheManager, layer: int, q: torch.Tensor, out: torch.Tensor, num_q_heads: int,
-                    seq_len, scale: float, slot=0, gate: Optional[torch.Tensor] = None) -> None:
+                    seq_len, scale: float, slot=0, gate: Optional[torch.Tensor] = None,
+                    prefix: Optional[SharedPrefix] = None) -> None:
         """``seq_len`` is the exclusive key count (position + 1).  ``slot``/``seq_len`` may be
-        lists for the batched form (one query token per sequence)."""
+        lists for the batched form (one query token per sequence).  With ``prefix`` the keys of its positions are its slot's, read
+        once for all sequences."""
+        if prefix is not None:
+            status = self._calls.attn_decode_shared(self.ctx.handle, kv.handle, layer, slot, seq_len, prefix.slot, prefix.length, num_q_heads,
+                                                    q, gate, scale, out)
+            if status:
+                self.ctx._check(status, "tt_hip_attn_decode_shared")
+            return
         status = self._calls.attn_decode(self.ctx.handle, kv.handle, layer, slot, seq_len, num_q_heads, q, gate, scale, out)
         if status:
             self.ctx._check(status, "tt_hip_attn_decode")
@@ -401,9 +422,18 @@ class Attention:
 
     def encode_verify_rows(self, kv: KVCacheManager, layer: int, q: torch.Tensor, out: torch.Tensor,
                            num_q_heads: int, start_positions: Sequence[int], rows: int, scale: float,
-                           slots: Sequence[int], gate: Optional[torch.Tensor] = None, window: int = 0, sinks: int = 0) -> None:
+                           slots: Sequence[int], gate: Optional[torch.Tensor] = None, window: int = 0, sinks: int = 0,
+                           prefix: Optional[SharedPrefix] = None) -> None:
         """Row r of sequence i attends like a decode at ``start_positions[i] + r`` (over its last ``window`` keys, and beside them
-        the first ``sinks``)."""
+        the first ``sinks``; or over all of them, those of a ``prefix`` from its slot)."""
+        if prefix is not None:
+            if window or sinks:
+                raise TinyTitanHIPError(capi.ERR_INVALID_ARGUMENT, "Attention.encode_verify_rows")
+            status = self._calls.attn_verify_shared(self.ctx.handle, kv.handle, layer, slots, start_positions, rows, prefix.slot,
+                                                    prefix.length, num_q_heads, q, gate, scale, out)
+            if status:
+                self.ctx._check(status, "tt_hip_attn_verify_shared")
+            return
         if sinks:
             status = self._calls.attn_verify_sinks(self.ctx.handle, kv.handle, layer, slots, start_positions, rows, window, sinks,
                                                    num_q_heads, q, gate, scale, out)
@@ -440,13 +470,22 @@ class PrefillAttention:
                       params: PrefillAttentionParams, gate: Optional[torch.Tensor] = None,
                       keep_mask: Optional[torch.Tensor] = None, keep_stride: int = 0,
                       keep_indices: Optional[torch.Tensor] = None, keep_index_stride: int = 0,
-                      keep_counts: Optional[torch.Tensor] = None) -> None:
+                      keep_counts: Optional[torch.Tensor] = None, prefix: Optional[SharedPrefix] = None) -> None:
         """``keep_mask`` / ``keep_stride``: a QSA chunk's per-query selection in its mask form (one row of
         ``keep_stride`` bytes per query, a zero byte drops that key for that query).  ``keep_indices`` /
         ``keep_index_stride`` / ``keep_counts``: the same selection compacted (int32 key ids per query and how
-        many of them), as ``encodeCausal`` takes it for the tiled kernel."""
+        many of them), as ``encodeCausal`` takes it for the tiled kernel.  ``prefix``: the keys of its positions are its slot's."""
         p = params
         gate_stride = p.gate_stride or p.q_stride
+        if prefix is not None:
+            if keep_mask is not None or keep_indices is not None or p.sliding_window or p.sinks:
+                raise TinyTitanHIPError(capi.ERR_INVALID_ARGUMENT, "PrefillAttention.encode_causal")
+            status = self._calls.attn_prefill_shared(self.ctx.handle, kv.handle, layer, slot, p.start_position, p.query_count,
+                                                     p.kv_valid_count, prefix.slot, prefix.length, p.num_q_heads, q, p.q_stride, gate,
+                                                     gate_stride, p.scale, out, p.o_stride)
+            if status:
+                self.ctx._check(status, "tt_hip_attn_prefill_shared")
+            return
         if keep_indices is not None:
             if (keep_counts is None or keep_mask is not None or p.sliding_window or p.sinks or keep_indices.dtype != torch.int32
                     or keep_counts.dtype != torch.int32):

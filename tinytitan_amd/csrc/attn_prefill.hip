@@ -74,6 +74,10 @@ struct PrefillArgs {
     int xcd_chunk;  // key ranges with xs > 0: (range, tile, head set) items one XCD takes, ceil(per_kvh * n_splits / xs)
     float *part_o;   // [split][head * n_tiles + tile][32 rows][D]
     float *part_ml;  // [split][head * n_tiles + tile][32 rows][2]
+    // Keys in two pieces (the kernels' PIECES): the first `sinks` stay visible beside the window, the ring's blocks lie behind `pinned`
+    // ones, and the first front_blocks blocks are another slot's.
+    int sinks, pinned, front_blocks;
+    const _Float16 *k_front, *v_front;  // page of kv head 0 of that slot
 };
 
 namespace {
@@ -146,8 +150,9 @@ __device__ __forceinline__ void rescale_tile(f16v &o, float alpha) {
 // waits until the matrix pipe is free: 64 of them beside another wavefront's MFMAs take as long as those do, 64 of any other instruction
 // here 1.25 times their own time.  64/8 heads of 64, 2,048 rows behind 4,000 keys 252.0 -> 235.3 us; 32/8 of 128, 4,096 behind 8,000
 // 729 -> 719; heads of 256, whose softmax is a smaller part, the same.)  Returns the factor the row's accumulators must be scaled by before this block is added.
+template <bool SINKS>
 __device__ __forceinline__ float softmax_step(const f16v &s_raw, bool mask, int kbase, int lo, int lim, int g, float scale_log2e, float &m,
-                                              float &l, h8 (&pf)[2]) {
+                                              float &l, h8 (&pf)[2], [[maybe_unused]] int sinks) {
     // The maximum is taken over the raw scores and scaled once (the host sends only chunks with scale > 0 here), and a
     // probability is one fused multiply-add and one exp2 off its raw score.
     float t[16];
@@ -157,7 +162,11 @@ __device__ __forceinline__ float softmax_step(const f16v &s_raw, bool mask, int 
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
             const int key = kbase + 8 * (v >> 2) + 4 * g + (v & 3);
-            if (key >= lim || key < lo) t[v] = -INFINITY;
+            if constexpr (SINKS) {
+                if (key >= lim || (key < lo && key >= sinks)) t[v] = -INFINITY;
+            } else {
+                if (key >= lim || key < lo) t[v] = -INFINITY;
+            }
         }
     }
     float mx = fmaxf(t[0], t[1]);
@@ -180,6 +189,44 @@ __device__ __forceinline__ float softmax_step(const f16v &s_raw, bool mask, int 
     }
     l += l_odd;
     return alpha;
+}
+
+// The keys in two pieces that a tile walks as one run of blocks: the sinks' blocks, then, `skipped` blocks further on, those of its window.
+// (Without sinks nothing is skipped that is not skipped anyway; a front piece in another slot's pages changes where a block lies only.)
+template <bool PIECES>
+struct Walk {
+    int sink_blocks = 0, skipped = 0;
+    __device__ __forceinline__ Walk([[maybe_unused]] const PrefillArgs &a, [[maybe_unused]] int window_block) {
+        if constexpr (PIECES) {
+            sink_blocks = min((a.sinks + 31) >> 5, window_block);
+            skipped = window_block - sink_blocks;
+        }
+    }
+    __device__ __forceinline__ int block(int at) const { return at < sink_blocks ? at : at + skipped; }
+};
+// The keys of block `block`, bit by bit, that some row of a tile sees whose rows see keys up to `end` in all and, its first one, those from `from` on.
+__device__ __forceinline__ unsigned seen_keys(const PrefillArgs &a, int block, int from, int end) {
+    auto below = [](int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; };
+    const int key = block << 5;
+    return below(end - key) & (below(a.sinks - key) | ~below(from - key));
+}
+// V fragments (2 mt + t: chunk 2 t + g of 32 dims) without the values of keys that no row sees: whatever such a row of the cache
+// holds, an infinity for one, a probability of zero would make NaN of it.
+template <int N>
+__device__ __forceinline__ void drop_unseen(h8 (&vf)[N], int g, unsigned seen) {
+    typedef unsigned words __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const unsigned lo = seen >> (16 * t + 4 * g), hi = lo >> 8;
+        words mask;
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            mask[w] = ((lo >> (2 * w)) & 1u ? 0xffffu : 0u) | ((lo >> (2 * w + 1)) & 1u ? 0xffff0000u : 0u);
+            mask[2 + w] = ((hi >> (2 * w)) & 1u ? 0xffffu : 0u) | ((hi >> (2 * w + 1)) & 1u ? 0xffff0000u : 0u);
+        }
+#pragma unroll
+        for (int c = t; c < N; c += 2) vf[c] = __builtin_bit_cast(h8, __builtin_bit_cast(words, vf[c]) & mask);
+    }
 }
 
 // Workgroup -> (kv head, head sub-group, tile pair); kv heads are spread over XCDs so
@@ -225,7 +272,7 @@ __device__ __forceinline__ bool chunk_item(const PrefillArgs &a, ChunkItem &item
 
 }  // namespace
 
-template <int D>
+template <int D, bool PIECES>
 __global__ __launch_bounds__(512, D == 64 ? 4 : 1) void attn_prefill_kernel(const PrefillArgs a) {
     constexpr int KS = D / 16;  // k-steps of S^T
     constexpr int MT = D / 32;  // 32-dim tiles of O^T
@@ -270,7 +317,11 @@ __global__ __launch_bounds__(512, D == 64 ? 4 : 1) void attn_prefill_kernel(cons
     // and one of V are in LDS when the first tile's last step ends, in the slots that follow on, and the second tile starts
     // without waiting for memory.  (A wave copies and reads K or V, so the offset is that of its own ring.)
     int slot_off = 0, carry_nb = 0;
-    auto page_block = [&](int block) { return a.ring_blocks ? block % a.ring_blocks : block; };
+    Walk<PIECES> walk(a, 0);  // (the tile's in hand)
+    auto page_block = [&](int block) {
+        if constexpr (PIECES) return a.ring_blocks && block >= a.pinned ? a.pinned + (block - a.pinned) % a.ring_blocks : block;
+        return a.ring_blocks ? block % a.ring_blocks : block;
+    };
     const int my_chunk = w4 * CPW;
     // A step's copies: this wave's CPW one-KiB chunks of ONE block -- of K for the score waves (the LDS layout is the HBM
     // layout, fragment s is chunk s), of V for the value waves (gathered so that LDS holds fragment (mt, t) as [lane][8 halves]).  Where the block lies in the page and in the
@@ -291,7 +342,12 @@ __global__ __launch_bounds__(512, D == 64 ? 4 : 1) void attn_prefill_kernel(cons
         StepCopies sc;
         const int j = i + (value_wave ? copies_ahead(true) : copies_ahead(false));
         const _Float16 *page = value_wave ? vp : kp;
-        sc.src = reinterpret_cast<const char *>(page + (size_t)page_block(copied_block(j, jb, nb, carry_nb)) * (32 * D)) + (value_wave ? 0 : my_chunk * 1024);
+        int block = copied_block(j, jb, nb, carry_nb);
+        if constexpr (PIECES) {
+            block = walk.block(block);
+            if (block < a.front_blocks) page = (value_wave ? a.v_front : a.k_front) + (size_t)kvh * a.page_elems;
+        }
+        sc.src = reinterpret_cast<const char *>(page + (size_t)page_block(block) * (32 * D)) + (value_wave ? 0 : my_chunk * 1024);
         sc.dst = smem_base + (unsigned)((value_wave ? V_OFF : 0) + in_ring(j + slot_off) * SLOT_BYTES + w4 * CPW * 1024);
         return sc;
     };
@@ -327,10 +383,11 @@ __global__ __launch_bounds__(512, D == 64 ? 4 : 1) void attn_prefill_kernel(cons
         const int window_block = tile_lo >> 5;
         const int last_lo_block = a.window > 0 ? (tile_lo + 31) >> 5 : -1;
         const int end = min(a.kv_valid, a.start + min(a.q_len, tile * 32 + 32));
-        const int nb_tile = (end + 31) >> 5;                   // key blocks this tile needs
+        walk = Walk<PIECES>(a, window_block);
+        const int nb_tile = ((end + 31) >> 5) - walk.skipped;  // key blocks this tile needs
         const int mask_from = (a.start + tile * 32 + 1) >> 5;  // first block in which some row is masked by causality
-        // This workgroup's share of them (all, without key splits); local step i is block jb + i
-        jb = window_block + (a.n_splits > 1 ? split * a.split_blocks : 0);
+        // This workgroup's share of them (all, without key splits); local step i is block jb + i (PIECES: of the walk)
+        jb = (PIECES ? 0 : window_block) + (a.n_splits > 1 ? split * a.split_blocks : 0);
         const int nb = (a.n_splits > 1 ? min(nb_tile, jb + a.split_blocks) : nb_tile) - jb;
         if (nb <= 0) continue;  // nothing of this tile in the range (the same for every wave)
         const int first_masked = min(mask_from, end >> 5);  // ... or cut by the valid length
@@ -395,8 +452,10 @@ __global__ __launch_bounds__(512, D == 64 ? 4 : 1) void attn_prefill_kernel(cons
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 h8 pf[2];
-                const int block = jb + i;
-                const float alpha = softmax_step(s, block >= first_masked || block <= last_lo_block, block << 5, lo, lim, g, a.scale_log2e, m, l, pf);
+                const int block = walk.block(jb + i);
+                const bool below_window = block <= last_lo_block && !(PIECES && (block << 5) + 32 <= a.sinks);
+                const float alpha = softmax_step<PIECES>(s, block >= first_masked || below_window, block << 5, lo, lim, g, a.scale_log2e, m, l, pf,
+                                                 a.sinks);
                 char *pdst = p_mine + (i & 1) * P_STEP;
 #pragma unroll
                 for (int t = 0; t < 2; ++t) *reinterpret_cast<h8 *>(pdst + t * 1024) = pf[t];
@@ -451,6 +510,10 @@ __global__ __launch_bounds__(512, D == 64 ? 4 : 1) void attn_prefill_kernel(cons
                     for (int mt = 0; mt < MT; ++mt) o[mt] *= alpha;
                 }
                 alpha = alpha_mine[(jn & 1) * 128];
+                if constexpr (PIECES) {
+                    const unsigned seen = seen_keys(a, walk.block(jb + i - 2), tile_lo, end);
+                    if (seen != ~0u) drop_unseen(vf, g, seen);
+                }
                 auto multiply = [&](int u, int mt, int t) {  // the u-th: k-step t of 32-dim tile mt
                     const int c = 2 * mt + t;  // the fragment's place in the slot
                     o[mt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[c], pf[t], o[mt], 0, 0, 0);
@@ -559,7 +622,7 @@ __global__ __launch_bounds__(512, D == 64 ? 4 : 1) void attn_prefill_kernel(cons
 // 4,096 rows behind 8,000 keys 729 -> 659 (0.93 -> 1.02 PFLOP/s), from position 0 179 -> 161, 128 rows behind 32,000
 // 97.6 -> 88.  Measured and dropped: both halves in step (2,144 instead of 1,640 cycles by the issue model; 84 us), copies five steps ahead (the same),
 // all of a step's copies in one run or in other places (the same to 1 %), the higher priority for the softmax or for the younger half (0 to -4 %).
-template <int D>
+template <int D, bool PIECES>
 __global__ __launch_bounds__(512, 2) void attn_prefill_halves_kernel(const PrefillArgs a) {
     constexpr int KS = D / 16, MT = D / 32;
     constexpr int BLOCK_BYTES = 32 * D * 2, CHUNKS = BLOCK_BYTES / 1024;
@@ -613,9 +676,10 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_halves_kernel(const Prefi
         const int window_block = tile_lo >> 5;
         const int last_lo_block = a.window > 0 ? (tile_lo + 31) >> 5 : -1;
         const int end = min(a.kv_valid, a.start + min(a.q_len, tile * 32 + 32));
-        const int nb_tile = (end + 31) >> 5;                   // key blocks this tile needs
+        const Walk<PIECES> walk(a, window_block);
+        const int nb_tile = ((end + 31) >> 5) - walk.skipped;  // key blocks this tile needs
         const int mask_from = (a.start + tile * 32 + 1) >> 5;  // first block in which some row is masked by causality
-        const int jb = window_block + (a.n_splits > 1 ? split * a.split_blocks : 0);
+        const int jb = (PIECES ? 0 : window_block) + (a.n_splits > 1 ? split * a.split_blocks : 0);
         const int nb = (a.n_splits > 1 ? min(nb_tile, jb + a.split_blocks) : nb_tile) - jb;
         if (nb <= 0) continue;  // nothing of this tile in the range (the same for every wave)
         const int steps = (nb + 1) / 2, mine = (nb + 1 - half) / 2;  // blocks jb + 2 i + half, i < mine
@@ -628,6 +692,10 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_halves_kernel(const Prefi
             if (a.window > 0) next_first = max(a.start + pair * 32 + 1 - a.window, 0) >> 5;
             next_nb = ((min(a.kv_valid, a.start + min(a.q_len, pair * 32 + 32)) + 31) >> 5) - next_first;
         }
+        const Walk<PIECES> next_walk(a, next_first);
+        if constexpr (PIECES) {
+            if (next_nb > 0) next_nb += next_walk.sink_blocks;
+        }
         // Where the copies stand: sources of the next step's, its place, and how many steps run on in the page before that takes
         // another look (a ring's end, the range's last block, and behind that each one).
         const char *k_src, *v_src;
@@ -636,6 +704,27 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_halves_kernel(const Prefi
         if (carried) copy_off = (copy_off + kHalvesAhead * SLOT_BYTES) & (RING_BYTES - 1);
         auto look = [&]() {
             copy_step += run;
+            if constexpr (PIECES) {
+                // the walk's block, and how many behind it lie one behind the other in the same page
+                const bool here = copy_step < steps || next_nb <= 0;
+                const int walked = halves_block(copy_step, half, jb, nb, 0, next_nb);
+                const int block = here ? walk.block(walked) : next_walk.block(walked);
+                int phys = block, room = 0x40000000;
+                if (walked < walk.sink_blocks) room = walk.sink_blocks - walked;
+                if (block < a.front_blocks) room = min(room, a.front_blocks - block);
+                if (block < a.pinned) room = min(room, a.pinned - block);
+                else if (a.ring_blocks) {
+                    phys = a.pinned + (block - a.pinned) % a.ring_blocks;
+                    room = min(room, a.pinned + a.ring_blocks - phys);
+                }
+                run = copy_step < mine ? min(mine - copy_step, (room + 1) / 2) : 1;
+                left = run;
+                const bool front = block < a.front_blocks;
+                const size_t at = (size_t)(unsigned)phys * BLOCK_BYTES, head_at = (size_t)item.kvh * a.page_elems;
+                k_src = reinterpret_cast<const char *>(front ? a.k_front + head_at : kp) + at;
+                v_src = reinterpret_cast<const char *>(front ? a.v_front + head_at : vp) + at - 1024 * (CPW - 1);
+                return;
+            }
             const int phys = halves_block(copy_step, half, jb, nb, next_first, next_nb) % wrap;
             run = copy_step < mine ? min(mine - copy_step, (wrap - phys + 1) / 2) : 1;
             left = run;
@@ -661,8 +750,10 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_halves_kernel(const Prefi
         }
         unsigned k_read = slot_off, v_read = slot_off;  // where the step lies whose K, V are read next
         // Blocks jb + 2 i + half with plain_from <= i < plain_from + plain need no mask.
-        const int plain_from = last_lo_block < jb + half ? 0 : (last_lo_block - jb - half) / 2 + 1;
-        const unsigned plain = (unsigned)max((first_masked - jb - half + 1) / 2 - plain_from, 0);
+        // (the walk's numbers: real ones from the window's blocks on, whose sinks in front are all masked)
+        const int last_lo_at = last_lo_block - walk.skipped, first_masked_at = first_masked - walk.skipped;
+        const int plain_from = last_lo_at < jb + half ? 0 : (last_lo_at - jb - half) / 2 + 1;
+        const unsigned plain = (unsigned)max((first_masked_at - jb - half + 1) / 2 - plain_from, 0);
         h8 qf[KS];
         const _Float16 *qp = a.q + (long long)(valid ? tok : 0) * a.q_stride + (long long)head * D + 8 * g;
 #pragma unroll
@@ -698,7 +789,13 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_halves_kernel(const Prefi
 #pragma unroll
             for (int t = 0; t < 2 * MT; ++t) vf[t] = *reinterpret_cast<const h8 *>(v_now + t * 1024);
             __builtin_amdgcn_sched_barrier(0);
-            const float alpha = softmax_step(s1, (unsigned)(i - plain_from) >= plain, (jb + 2 * i + half) << 5, lo, lim, g, a.scale_log2e, m, l, pf);
+            const int block = walk.block(jb + 2 * i + half);
+            const float alpha = softmax_step<PIECES>(s1, (unsigned)(i - plain_from) >= plain, block << 5, lo, lim, g, a.scale_log2e, m, l, pf,
+                                             a.sinks);
+            if constexpr (PIECES) {
+                const unsigned seen = seen_keys(a, block, tile_lo, end);
+                if (seen != ~0u) drop_unseen(vf, g, seen);
+            }
             if (__any(alpha != 1.0f)) {
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) rescale_tile(o[mt], alpha);
@@ -869,10 +966,16 @@ static_assert(prefill_lds_bytes(256) <= 160 * 1024 && prefill_halves_lds_bytes(1
 
 int configure_prefill_kernels(tt_hip_ctx *ctx) {
     auto configure = [](const void *kernel, int lds) { return hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds); };
-    hipError_t e = configure(reinterpret_cast<const void *>(attn_prefill_kernel<256>), prefill_lds_bytes(256));
-    if (e == hipSuccess) e = configure(reinterpret_cast<const void *>(attn_prefill_kernel<128>), prefill_lds_bytes(128));
-    if (e == hipSuccess) e = configure(reinterpret_cast<const void *>(attn_prefill_kernel<64>), prefill_lds_bytes(64));
-    if (e == hipSuccess) e = configure(reinterpret_cast<const void *>(attn_prefill_halves_kernel<128>), prefill_halves_lds_bytes(128));
+    auto configure_pieces = [&](auto pieces) {
+        constexpr bool P = decltype(pieces)::value;
+        hipError_t e = configure(reinterpret_cast<const void *>(attn_prefill_kernel<256, P>), prefill_lds_bytes(256));
+        if (e == hipSuccess) e = configure(reinterpret_cast<const void *>(attn_prefill_kernel<128, P>), prefill_lds_bytes(128));
+        if (e == hipSuccess) e = configure(reinterpret_cast<const void *>(attn_prefill_kernel<64, P>), prefill_lds_bytes(64));
+        if (e == hipSuccess) e = configure(reinterpret_cast<const void *>(attn_prefill_halves_kernel<128, P>), prefill_halves_lds_bytes(128));
+        return e;
+    };
+    hipError_t e = configure_pieces(std::false_type{});
+    if (e == hipSuccess) e = configure_pieces(std::true_type{});
     return e == hipSuccess ? TT_HIP_OK : hip_fail(ctx, e, "hipFuncSetAttribute(chunk kernel max dynamic LDS)");
 }
 
@@ -887,7 +990,7 @@ static int launch_chunk(tt_hip_ctx *ctx, F kernel, const PrefillArgs &args, unsi
 int launch_prefill(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int slot, int start, int q_len, int kv_valid,
                    int n_q_heads, const tt_half *q, long long q_stride, const tt_half *gate, long long g_stride,
                    float scale, tt_half *out, long long o_stride, int n_splits, int split_blocks, float *part_o,
-                   float *part_ml, const PageSource *pages, int window, bool single_tiles) {
+                   float *part_ml, const PageSource *pages, int window, bool single_tiles, const ChunkPieces *pieces) {
     PrefillArgs a{};
     a.window = window;
     if (!pages && kv->bits != 16) return TT_HIP_ERR_INVALID_ARGUMENT;  // this kernel reads fp16 pages only
@@ -929,16 +1032,32 @@ int launch_prefill(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int slot, int star
         a.xcd_chunk = (a.per_kvh * a.n_splits + a.xs - 1) / a.xs;
         grid = 8u * (unsigned)a.xcd_chunk;
     }
-    const int walk = a.n_splits > 1 ? std::min(split_blocks, most_tile_blocks(start, q_len, kv_valid, window))
-                                    : most_tile_blocks(start, q_len, kv_valid, window);
-    switch (kv->head_dim) {
-        case 256: return launch_chunk(ctx, attn_prefill_kernel<256>, a, grid, prefill_lds_bytes(256));
-        case 128:
-            if (halves_of_keys(walk, (long long)grid, ctx->n_cus)) return launch_chunk(ctx, attn_prefill_halves_kernel<128>, a, grid, prefill_halves_lds_bytes(128));
-            return launch_chunk(ctx, attn_prefill_kernel<128>, a, grid, prefill_lds_bytes(128));
-        case 64: return launch_chunk(ctx, attn_prefill_kernel<64>, a, grid, prefill_lds_bytes(64));
-        default: return TT_HIP_ERR_SHAPE;
+    if (pieces) {
+        a.sinks = pieces->sinks;
+        if (!pages && kv->ring) {
+            a.pinned = kv->pinned / kBlockTokens;
+            a.ring_blocks = (kv->capacity - kv->pinned) / kBlockTokens;
+        }
+        a.front_blocks = pieces->front_blocks;
+        const size_t front_off = (size_t)pieces->front_slot * kv->n_kv_heads * kv->page_elems();
+        a.k_front = kv->k[layer] + front_off;
+        a.v_front = kv->v[layer] + front_off;
     }
+    const int most = most_tile_blocks(start, q_len, kv_valid, window, a.sinks);
+    const int walk = a.n_splits > 1 ? std::min(split_blocks, most) : most;
+    auto launch = [&](auto of_pieces) -> int {
+        constexpr bool P = decltype(of_pieces)::value;
+        switch (kv->head_dim) {
+            case 256: return launch_chunk(ctx, attn_prefill_kernel<256, P>, a, grid, prefill_lds_bytes(256));
+            case 128:
+                if (halves_of_keys(walk, (long long)grid, ctx->n_cus))
+                    return launch_chunk(ctx, attn_prefill_halves_kernel<128, P>, a, grid, prefill_halves_lds_bytes(128));
+                return launch_chunk(ctx, attn_prefill_kernel<128, P>, a, grid, prefill_lds_bytes(128));
+            case 64: return launch_chunk(ctx, attn_prefill_kernel<64, P>, a, grid, prefill_lds_bytes(64));
+            default: return TT_HIP_ERR_SHAPE;
+        }
+    };
+    return pieces ? launch(std::true_type{}) : launch(std::false_type{});
 }
 
 }  // namespace tt

@@ -363,7 +363,7 @@ template <int D, int NT>
 __device__ __forceinline__ void block_softmax(RowState<D, NT> &st, Scores<D, NT> &sc, Probs<D, NT> &pr,
                                               const Lane<D, NT> &ln, int kbase, int lo, int lim, float scale_log2e,
                                               typename RowState<D, NT>::acc_t *extra = nullptr, unsigned kept = ~0u,
-                                              const unsigned *row_keep = nullptr, unsigned row_bits = ~0u, int sinks = 0) {
+                                              const unsigned *row_keep = nullptr, unsigned row_bits = ~0u, int sinks = kNoSinks) {
     // sinks: keys below it are seen although they lie below `lo`.
     // kept: bit i set = key kbase + i takes part (a sparse selection shared by the tile's rows; all ones without one).
     // row_keep: this lane's own row's 32 selection bytes of the block, as 8 words (a per-query selection).
@@ -510,7 +510,7 @@ template <int D, int NT>
 __device__ __forceinline__ void block_softmax_pv(RowState<D, NT> &st, Scores<D, NT> &sc, VTile<D, NT> &vt,
                                                  const Lane<D, NT> &ln, int kbase, int lo, int lim, float scale_log2e,
                                                  unsigned kept = ~0u, const unsigned *row_keep = nullptr, unsigned row_bits = ~0u,
-                                                 int sinks = 0, unsigned seen = ~0u) {
+                                                 int sinks = kNoSinks, unsigned seen = ~0u) {
     Probs<D, NT> pr;
     block_softmax<D, NT>(st, sc, pr, ln, kbase, lo, lim, scale_log2e, nullptr, kept, row_keep, row_bits, sinks);
     if (seen != ~0u) drop_unseen<D, NT>(vt, ln, seen);
@@ -908,7 +908,7 @@ __device__ __forceinline__ void block_softmax_pv(RowState<D, NT> &st, Scores<D, 
                                                  const Lane<D, NT> &ln, int kbase, int lo, int lim, float scale_log2e,
                                                  typename RowState<D, NT>::acc_t &bias_acc, __amdgpu_buffer_rsrc_t rv,
                                                  unsigned next_bytes, const Voids<D, NT> &vo, unsigned kept = ~0u,
-                                                 const unsigned *row_keep = nullptr, unsigned row_bits = ~0u, int sinks = 0,
+                                                 const unsigned *row_keep = nullptr, unsigned row_bits = ~0u, int sinks = kNoSinks,
                                                  unsigned seen = ~0u) {
     typedef QuantOffsets<D, NT, BITS> O;
     constexpr int GPH = D / 64;
@@ -1342,7 +1342,7 @@ __global__ __launch_bounds__(WAVES * 64, (NT == 16 && (KEEP < 2 || KEEP == kKeep
         }
         return a.ring_blocks ? block % a.ring_blocks : block;
     };
-    const int sinks = SINKS ? a.keep_words : 0;
+    const int sinks = SINKS ? a.keep_words : kNoSinks;
     const int first_lim = min(ti.total, ti.start + ti.t0 + 1), seen_from = a.window > 0 ? max(first_lim - a.window, 0) : 0;
     const int seen_end = ti.tile_end + 32 * ti.skipped;  // (SINKS) keys up to the tile's last row's own
     const bool first_real = b < b_end;
@@ -2007,8 +2007,10 @@ int configure_splitk_kernels(tt_hip_ctx *ctx) {
 // The combine pass on its own: for partials written by another kernel in this kernel's layout.
 int launch_combine(tt_hip_ctx *ctx, const LaunchPlan &plan, int head_dim, int n_seq, const SplitKArgs &args) {
     if (plan.n_tiles > 65535 || n_seq > 65535) return TT_HIP_ERR_SHAPE;
-#define TT_CASE(DD, NN) \
-    if (head_dim == DD && plan.nt == NN) return launch_combine_one<DD, NN, false>(ctx, plan, n_seq, args);
+    const bool sinks = (args.hot.flags & kHotSinks) != 0;
+#define TT_CASE(DD, NN)              \
+    if (head_dim == DD && plan.nt == NN) \
+        return sinks ? launch_combine_one<DD, NN, true>(ctx, plan, n_seq, args) : launch_combine_one<DD, NN, false>(ctx, plan, n_seq, args);
     TT_CASE(256, 16)
     TT_CASE(256, 32)
     TT_CASE(128, 16)

@@ -14,18 +14,19 @@ inline int packed_heads(int group) {
 }
 
 // Key blocks of 32 that the chunk's tile of rows [32 t, 32 t + 32) walks: from the block of the first key its first row sees (a
-// window: the last `window` keys up to the row's own) to the block of its last row's own key.
-inline int chunk_tile_blocks(int start, int q_len, int kv_valid, int window, int t) {
+// window: the last `window` keys up to the row's own) to the block of its last row's own key, and in front of a window the blocks of
+// its sinks.
+inline int chunk_tile_blocks(int start, int q_len, int kv_valid, int window, int t, int sinks = 0) {
     const long long end = std::min<long long>(kv_valid, (long long)start + std::min<long long>(q_len, 32LL * t + 32));
     const long long first = window > 0 && start + 32LL * t + 1 > window ? start + 32LL * t + 1 - window : 0;
-    return (int)((end + 31) / 32 - first / 32);
+    return (int)((end + 31) / 32 - first / 32 + std::min<long long>((sinks + 31LL) / 32, first / 32));
 }
 // The longest of them.  With a window it need be neither the first tile, whose window may still reach over key 0, nor the
 // last, which may end early.
-inline int longest_tile_blocks(int start, int q_len, int kv_valid, int window) {
+inline int longest_tile_blocks(int start, int q_len, int kv_valid, int window, int sinks = 0) {
     if (window <= 0) return chunk_tile_blocks(start, q_len, kv_valid, window, (q_len + 31) / 32 - 1);
     int longest = 0;
-    for (int t = 0; t < (q_len + 31) / 32; ++t) longest = std::max(longest, chunk_tile_blocks(start, q_len, kv_valid, window, t));
+    for (int t = 0; t < (q_len + 31) / 32; ++t) longest = std::max(longest, chunk_tile_blocks(start, q_len, kv_valid, window, t, sinks));
     return longest;
 }
 
@@ -58,9 +59,9 @@ constexpr int halves_block(int step, int half, int first, int nb, int next_first
 inline bool halves_of_keys(int walk, long long workgroups, int n_cus) { return walk >= (workgroups > n_cus ? 4 : 11); }
 
 // At most this many blocks a tile walks: of all keys up to its last row's, those that the windows of 32 rows can touch.
-inline int most_tile_blocks(int start, int q_len, int kv_valid, int window) {
+inline int most_tile_blocks(int start, int q_len, int kv_valid, int window, int sinks = 0) {
     const int all = (int)((std::min<long long>(kv_valid, (long long)start + q_len) + 31) / 32);
-    return window > 0 ? (int)std::min<long long>(all, ((long long)window + 61) / 32 + 1) : all;
+    return window > 0 ? (int)std::min<long long>(all, ((long long)window + 61) / 32 + 1 + (sinks + 31LL) / 32) : all;
 }
 
 // What a chunk costs by the routes that serve it, in us, from timings at 16 q heads / 2 KV heads of 256, 8 / 2 of 256, 32 / 8 of
@@ -139,8 +140,9 @@ inline KeyRanges plan_key_ranges(int n_cus, int D, int n_q_heads, int n_kv_heads
     return r;
 }
 // ... of the keys that a window leaves each tile.
-inline KeyRanges plan_window_ranges(int n_cus, int D, int n_q_heads, int n_kv_heads, int start, int q_len, int kv_valid, int window) {
-    return plan_key_ranges(n_cus, D, n_q_heads, n_kv_heads, q_len, longest_tile_blocks(start, q_len, kv_valid, window));
+inline KeyRanges plan_window_ranges(int n_cus, int D, int n_q_heads, int n_kv_heads, int start, int q_len, int kv_valid, int window,
+                                    int sinks = 0) {
+    return plan_key_ranges(n_cus, D, n_q_heads, n_kv_heads, q_len, longest_tile_blocks(start, q_len, kv_valid, window, sinks));
 }
 
 // Tiles of 32 packed rows that the split-K kernel makes of a chunk, and how many of them run at once.

@@ -298,7 +298,8 @@ struct KeepLists {
 //   kind 1: causal chunk of one sequence.
 //   chunk_splits > 1 (kind 1, one sequence): the chunk kernel over chunk_splits key ranges of
 //   chunk_split_blocks blocks, then the combine pass.
-//   sinks >= 0 (kind 0): the keys [0, sinks) stay visible beside the window; pinned rows of a ring are known.  -1: neither.
+//   sinks >= 0: the keys [0, sinks) stay visible beside the window; pinned rows of a ring are known.  -1: neither.  With chunk_splits > 1
+//   chunk_pieces says so to the chunk kernel.
 //   piece: the pass takes one piece of the rows' keys and leaves its partial results there, for launch_join (at most
 //   kMaxSeqPerLaunch sequences).
 struct KeyPiece {
@@ -314,7 +315,8 @@ static int run_attention(tt_hip_ctx *ctx, tt_hip_kv *kv, int kind, int layer, in
                          long long o_tok_stride, int chunk_splits = 1, int chunk_split_blocks = 0,
                          const PageSource *pages = nullptr, int window = 0, const uint8_t *keep = nullptr,
                          long long keep_seq_stride = 0, long long keep_row_stride = 0, bool static_partials = false,
-                         const KeepLists *lists = nullptr, int sinks = -1, KeyPiece *piece = nullptr) {
+                         const KeepLists *lists = nullptr, int sinks = -1, KeyPiece *piece = nullptr,
+                         const ChunkPieces *chunk_pieces = nullptr) {
     const int D = kv->head_dim;
     hipError_t e = hipSetDevice(ctx->device);
     if (e != hipSuccess) return hip_fail(ctx, e, "hipSetDevice");
@@ -344,7 +346,7 @@ static int run_attention(tt_hip_ctx *ctx, tt_hip_kv *kv, int kind, int layer, in
         if (st != TT_HIP_OK) return st;
         if (chunk_splits > 1) {  // the chunk kernel's geometry: 32-row one-head tiles, its own key ranges
             // (a tile that walked past the launched ranges would lose keys, and the combine pass would count a partial result more)
-            if (longest_tile_blocks(starts[base], rows, totals[base], window) > (long long)chunk_splits * chunk_split_blocks)
+            if (longest_tile_blocks(starts[base], rows, totals[base], window, sinks > 0 ? sinks : 0) > (long long)chunk_splits * chunk_split_blocks)
                 return TT_HIP_ERR_SHAPE;
             plan.split_len = chunk_split_blocks * 32;
             plan.n_splits_max = chunk_splits;
@@ -613,7 +615,8 @@ static int run_attention(tt_hip_ctx *ctx, tt_hip_kv *kv, int kind, int layer, in
         }
         if (chunk_splits > 1) {
             st = launch_prefill(ctx, kv, layer, slots[base], starts[base], rows, totals[base], n_q_heads, q, q_tok_stride, gate,
-                                g_tok_stride, scale, out, o_tok_stride, chunk_splits, chunk_split_blocks, h.part_o, h.part_ml, pages, window);
+                                g_tok_stride, scale, out, o_tok_stride, chunk_splits, chunk_split_blocks, h.part_o, h.part_ml, pages, window, false,
+                                chunk_pieces);
             if (st == TT_HIP_OK && !piece) st = launch_combine(ctx, plan, D, n, a);
         } else {
             st = launch_splitk(ctx, plan, D, n, a, kv_bits);
@@ -1227,206 +1230,6 @@ int tt_hip_attn_prefill(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int slot, int
                                    gate_stride, scale, out, o_stride);
 }
 
-int tt_hip_attn_prefill_sinks(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int slot, int start_pos, int q_len, int kv_valid,
-                              int sliding_window, int sinks, int n_q_heads, const tt_half *q, size_t q_stride, const tt_half *gate,
-                              size_t gate_stride, float scale, tt_half *out, size_t o_stride) {
-    int st = check_common(ctx, kv, layer, n_q_heads, q, out);
-    if (st != TT_HIP_OK) return st;
-    if (slot < 0 || slot >= kv->n_slots || start_pos < 0 || q_len <= 0 || sliding_window < 0 || sinks < 0) return TT_HIP_ERR_INVALID_ARGUMENT;
-    const long long end = (long long)start_pos + q_len;
-    if (!needs_sinks(kv, sliding_window, sinks, end > sliding_window))
-        return tt_hip_attn_prefill_swa(ctx, kv, layer, slot, start_pos, q_len, kv_valid, sliding_window, n_q_heads, q, q_stride, gate,
-                                       gate_stride, scale, out, o_stride);
-    const size_t packed = (size_t)n_q_heads * kv->head_dim;
-    if (q_stride < packed || o_stride < packed || (gate && gate_stride < packed)) return TT_HIP_ERR_SHAPE;
-    if (end > kv_valid) return TT_HIP_ERR_INVALID_ARGUMENT;
-    const long long first = start_pos + 1LL > sliding_window ? start_pos + 1LL - sliding_window : 0;
-    if (!kv->holds_keys_and_sinks((int)std::min<long long>(sinks, std::max(end - sliding_window, 0ll)), first, kv_valid)) return TT_HIP_ERR_CAPACITY;
-    BusyGuard guard(ctx);
-    if (!guard.ok) return TT_HIP_ERR_BUSY;
-    return run_attention(ctx, kv, 0, layer, 1, &slot, &start_pos, &kv_valid, q_len, n_q_heads, q, 0, (long long)q_stride, gate, 0,
-                         (long long)gate_stride, scale, out, 0, (long long)o_stride, 1, 0, nullptr, sliding_window, nullptr, 0, 0, false,
-                         nullptr, std::min(sinks, kv_valid));
-}
-
-int tt_hip_attn_prefill_swa(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int slot, int start_pos, int q_len, int kv_valid,
-                            int sliding_window, int n_q_heads, const tt_half *q, size_t q_stride, const tt_half *gate,
-                            size_t gate_stride, float scale, tt_half *out, size_t o_stride) {
-    if (kv && kv->pinned > 0 && sliding_window > 0)
-        return tt_hip_attn_prefill_sinks(ctx, kv, layer, slot, start_pos, q_len, kv_valid, sliding_window, 0, n_q_heads, q, q_stride, gate,
-                                         gate_stride, scale, out, o_stride);
-    int st = check_common(ctx, kv, layer, n_q_heads, q, out);
-    if (st != TT_HIP_OK) return st;
-    if (slot < 0 || slot >= kv->n_slots || start_pos < 0 || q_len <= 0 || sliding_window < 0) return TT_HIP_ERR_INVALID_ARGUMENT;
-    const size_t packed = (size_t)n_q_heads * kv->head_dim;
-    if (q_stride < packed || o_stride < packed || (gate && gate_stride < packed)) return TT_HIP_ERR_SHAPE;
-    if ((long long)start_pos + q_len > kv_valid) return TT_HIP_ERR_INVALID_ARGUMENT;
-    {
-        const long long first = sliding_window > 0 && start_pos + 1 > sliding_window ? start_pos + 1 - sliding_window : 0;
-        if (!kv->holds_keys(first, kv_valid)) return TT_HIP_ERR_CAPACITY;
-    }
-    BusyGuard guard(ctx);
-    if (!guard.ok) return TT_HIP_ERR_BUSY;
-    const bool aligned = aligned16(q) && aligned16(out) && (!gate || aligned16(gate)) && q_stride % 8 == 0 &&
-                         o_stride % 8 == 0 && (!gate || gate_stride % 8 == 0);
-    // A window that clips no row of the chunk is no window.
-    const int window = sliding_window > 0 && (long long)start_pos + q_len > sliding_window ? sliding_window : 0;
-    // (the chunk kernel takes a row's maximum over the raw scores: a scale that is not positive goes the split-K way)
-    const bool serves = prefill_kernel_serves(n_q_heads, kv->n_kv_heads, kv->head_dim, aligned) && scale > 0.0f;
-    const long long chunk_wgs = (long long)((q_len + 63) / 64) * (n_q_heads / 4);
-    // The chunk kernel as it is -- a workgroup per pair of tiles and 4 heads, all their keys -- where its workgroups
-    // fill half the chip, or a quarter of it with few key blocks each (a long first chunk of a prompt: 1024 rows from
-    // position 0 take 39 us against 41 us through the split-K tiles, 1536 rows 51 against 66).  Fewer workgroups
-    // walking more blocks lose to the other routes at any context: 128 rows behind 1920 keys took 100 us that way,
-    // 25 us through the split-K tiles; behind a 1024-key window 62 us against 20 us.
-    const long long pair_blocks = (2LL * start_pos + q_len) / 32 + 2;  // key blocks a workgroup's pair of tiles walks
-    const bool filled = 2 * chunk_wgs >= ctx->n_cus || (window == 0 && 4 * chunk_wgs >= ctx->n_cus && pair_blocks <= 64);
-    const int first_blocks = chunk_tile_blocks(start_pos, q_len, kv_valid, window, 0);
-    const int last_blocks = chunk_tile_blocks(start_pos, q_len, kv_valid, window, (q_len + 31) / 32 - 1);
-    const ChunkEstimate whole = estimate_chunk(ctx->n_cus, kv->head_dim, n_q_heads, kv->n_kv_heads, q_len, first_blocks, last_blocks);
-    auto whole_tiles = [&](const PageSource *pages) {
-        if (hipSetDevice(ctx->device) != hipSuccess) return (int)TT_HIP_ERR_HIP;
-        return launch_prefill(ctx, kv, layer, slot, start_pos, q_len, kv_valid, n_q_heads, q, (long long)q_stride, gate,
-                              (long long)gate_stride, scale, out, (long long)o_stride, 1, 0, nullptr, nullptr, pages, window,
-                              whole.single_tiles);
-    };
-    const double splitk_us = estimate_splitk_chunk_us(ctx->n_cus, kv->head_dim, n_q_heads, kv->n_kv_heads, q_len, first_blocks, last_blocks);
-    if (window > 0) {
-        // The chunk kernel starts every tile at its window's first block.  It or the split-K kernel (GQA-packed tiles, each
-        // walking only its rows' windows), whichever is estimated faster; quantised pages and head groups the chunk
-        // kernel does not serve go through the latter.  32 / 8 heads of 128 behind a window of 4096 keys: 512 rows 65
-        // against 78 us, 777 rows 105 against 80; 16 / 2 of 256 behind 1024 keys: 512 rows 24 against 34, 777 rows 43
-        // against 34, 1024 rows 47 against 36.
-        // Where the chunk does not fill the chip and the split-K tiles go in whole rounds with the last one part empty, the keys of a
-        // window cut into ranges, as behind a long context (300 rows behind 4096 keys: 24 / 2 heads of 256 113.6 -> 55.3 us, 32 / 8 of
-        // 128 56.7 -> 48.3; 16 / 2 of 256, 600 rows 115.7 -> 66.8, 270 behind 16,384 keys 188.6 -> 92.3), or the chunk kernel as it is.  16 us: the
-        // combine pass and both kernels' starts.  Inside a capture the partial results' store does not grow.
-        if (serves && kv->bits == 16 && !filled && q_len >= 256) {
-            const int longest = longest_tile_blocks(start_pos, q_len, kv_valid, window);
-            const double tiles_us = splitk_rounds_us(ctx->n_cus, n_q_heads, kv->n_kv_heads, q_len, longest, splitk_us);
-            const KeyRanges r = plan_window_ranges(ctx->n_cus, kv->head_dim, n_q_heads, kv->n_kv_heads, start_pos, q_len, kv_valid, window);
-            const size_t part_rows = (size_t)r.n_splits * n_q_heads * ((q_len + 31) / 32) * 32;
-            if (r.n_splits >= 2 && r.us + 16.0 < 0.95 * std::min(whole.us, tiles_us) && (!ctx->capturing || part_rows <= ctx->part_rows))
-                return run_attention(ctx, kv, 1, layer, 1, &slot, &start_pos, &kv_valid, q_len, n_q_heads, q, 0, (long long)q_stride, gate,
-                                     0, (long long)gate_stride, scale, out, 0, (long long)o_stride, r.n_splits, r.split_blocks, nullptr, window);
-            if (whole.us < 0.75 * tiles_us) return whole_tiles(nullptr);
-        }
-        // The estimates do not hold where the split-K tiles are all at work at once, as a few hundred rows of a short window are: 64 / 8
-        // heads of 64, 226 rows behind 96 keys 7.0 us against 10.1, 32 / 8 of 128, 428 behind 128 12.9 / 14.6, 24 / 2 of 256, 247 behind
-        // 33 12.6 / 19.1; one more round the other way (279 rows there 22.5 / 19.1, 560 of 32 / 8 19.1 / 13.8).
-        const bool more_rounds = splitk_tiles(n_q_heads, kv->n_kv_heads, q_len) > splitk_tiles_at_once(ctx->n_cus, kv->head_dim);
-        if (serves && kv->bits == 16 && (filled || (more_rounds && whole.us < splitk_us))) return whole_tiles(nullptr);
-        return run_attention(ctx, kv, 0, layer, 1, &slot, &start_pos, &kv_valid, q_len, n_q_heads, q, 0, (long long)q_stride,
-                             gate, 0, (long long)gate_stride, scale, out, 0, (long long)o_stride, 1, 0, nullptr, window);
-    }
-    // Quantised pages: the split-K kernel reads them as they are (dequantising in registers, once
-    // per 32-row tile -- 269 TFLOP/s on a 4096-row chunk).  A chunk that the MFMA chunk kernel
-    // would take is instead served from fp16 pages of the slot's visible blocks, dequantised once
-    // per call into the context's staging store (4096 rows: one 9 us pass, then the fp16 kernel).
-    PageSource staged{};
-    const PageSource *pages = nullptr;
-    // From this many keys on a chunk that does not fill the chip goes through the chunk kernel over key ranges (below:
-    // through the split-K tiles): 786,432 / rows, i.e. 12k keys at 64 rows, 6k at 128, and at least 4096 (2560 over
-    // quantised pages, whose visible blocks are dequantised once per call first).  The split-K tiles read the keys once
-    // per tile of rows and leave small partial results; the ranges read them once per range and leave rows x heads x D
-    // floats per range.  One box, fp16, split-K / ranges: 64 rows at 8k keys 31.6 / 33.4 us, at 12k 37.2 / 35.3; 96
-    // rows at 4k 28.4 / 32.4, at 12k 47.7 / 42.8; 128 rows at 4k 32.0 / 35.0, at 8k 44.3 / 39.1; 192 rows at 4k 41.8 /
-    // 38.6.  Over 8 bits: 64 rows at 4k 24.4 / 35.4, at 16k 50.1 / 49.2, at 32k 80.7 / 71.9; 128 rows at 4k 34.6 /
-    // 40.2, at 8k 48.9 / 45.0.
-    // Heads that leave rows of a split-K tile empty make more tiles of the same rows, and what that way takes goes by its tiles: there from 393,216 /
-    // (tiles x D / 256) keys on where that is earlier, and from 2,048.  us a layer, split-K / ranges: 24 / 2 heads of 256, 96 rows behind 7,000 keys
-    // 63.8 / 50.0, over 8 bits 81.0 / 55.7, 300 behind 3,000 109.2 / 74.9, 200 behind 1,600 53.0 / 56.0.  Not for other heads, though the ranges would often
-    // be ahead (64 / 8 of 256, 130 rows behind 4,000 keys over 8 bits 173 / 119): not where the tiles share the chip out evenly (64 / 16 of 128, 64
-    // rows behind 7,900 keys 48.1 / 51.3, over 8 bits 58.6 / 77.9, 96 rows behind 5,100 67.8 / 75.8; 32 / 4 of 256, 64 rows 56.9 / 60.7).
-    const bool rows_left_empty = 32 % packed_heads(n_q_heads / kv->n_kv_heads) != 0;
-    const long long by_rows = 786432 / (q_len > 0 ? q_len : 1), others_from = std::max<long long>(by_rows, kv->bits == 16 ? 4096 : 2560);
-    long long ranges_from = others_from;
-    if (rows_left_empty) {
-        const long long tile_widths = splitk_tiles(n_q_heads, kv->n_kv_heads, q_len) * kv->head_dim;
-        ranges_from = std::max<long long>(std::min(393216ll * 256 / (tile_widths > 0 ? tile_widths : 1), by_rows), 2048);
-    }
-    // ... and from this many rows on: 64; at fp16 32 rows deep in a context (32 rows at 32k keys 50 us against 54 us,
-    // 48 rows 62 against 73).  Over quantised pages fewer rows stay with the split-K tiles, which widen a block once per
-    // tile of 16 rows: dequantising the whole context for them costs more than that at any length measured (32 rows
-    // at 64k keys over 8 bits 82 us against 107 us, 12 rows at 32k keys 30 us against 62 us).
-    const int rows_from = kv->bits == 16 ? (kv_valid >= 32768 ? 32 : 64) : 64;
-    if (serves && !filled && (kv->bits == 16 || !kv->ring) && q_len >= rows_from && kv_valid >= ranges_from && kv_valid < others_from) {
-        // (no memory for the ranges' partial results or the dequantised pages, or a capture in which they would have to grow: the split-K way)
-        const int blocks = (kv_valid + 31) / 32;
-        const KeyRanges r = plan_key_ranges(ctx->n_cus, kv->head_dim, n_q_heads, kv->n_kv_heads, q_len, blocks);
-        if (hipSetDevice(ctx->device) != hipSuccess) return TT_HIP_ERR_HIP;
-        st = q_len >= 256 && whole.us < r.us ? TT_HIP_OK : ensure_partials(ctx, (size_t)r.n_splits * n_q_heads * ((q_len + 31) / 32) * 32, kv->head_dim);
-        if (st == TT_HIP_OK && kv->bits != 16) st = ensure_stage(ctx, (size_t)blocks * 32 * kv->head_dim * kv->n_kv_heads);
-        if (st == TT_HIP_ERR_BUSY || st == TT_HIP_ERR_OUT_OF_MEMORY) ranges_from = others_from;
-        else if (st != TT_HIP_OK) return st;
-    }
-    if (kv->bits != 16 && !kv->ring && serves && q_len >= rows_from && (filled || kv_valid >= ranges_from)) {
-        const int n_blocks = (kv_valid + 31) / 32;
-        const size_t page = (size_t)n_blocks * 32 * kv->head_dim;
-        if (hipSetDevice(ctx->device) != hipSuccess) return TT_HIP_ERR_HIP;
-        st = ensure_stage(ctx, page * kv->n_kv_heads);
-        if (st != TT_HIP_OK) return st;
-        st = launch_kvq_dequant_blocks(kv, layer, slot, n_blocks, ctx->stage_k, ctx->stage_v, page);
-        if (st != TT_HIP_OK) return st;
-        staged = PageSource{ctx->stage_k, ctx->stage_v, (long long)page, 0};
-        pages = &staged;
-    }
-    if (serves && (kv->bits == 16 || pages)) {
-        // The chunk kernel gives a workgroup 64 query rows of 4 heads and ALL their keys: one
-        // workgroup per CU at 4096 rows x 16 heads, but a 128-row chunk (the reference's default
-        // prefillChunkTokens) deep into a long context would be 8 workgroups walking 32k keys
-        // each (1318 us at 16q/2kv/256).  Three routes, chosen from timings at that shape:
-        //  * at least half a chip of workgroups, or a quarter with few blocks each: the chunk kernel as it is;
-        //  * 64 rows or more over 4096 keys or more (2560 over quantised pages): the chunk kernel with the keys cut into
-        //    ranges, a workgroup per (tile, 4 heads, range), and the combine pass over the partial
-        //    results (128 rows at 32k keys 98-106 us, 1024 rows 507-538 us; 256 rows at 4k keys 39 us
-        //    against 46 us the split-K way);
-        //  * anything else: the split-K kernel, which packs a KV head's q heads into its tiles
-        //    like a verify pass (64 rows at 16k keys 62 us against 89 us; 512 rows at 2k keys
-        //    59 us against 104 us, where the partial results outweigh the keys).
-        int n_splits = 1, split_blocks = 0;
-        double ranges_us = 0.0;
-        if (!filled && q_len >= rows_from && kv_valid >= ranges_from) {
-            const KeyRanges r = plan_key_ranges(ctx->n_cus, kv->head_dim, n_q_heads, kv->n_kv_heads, q_len, (kv_valid + 31) / 32);
-            n_splits = r.n_splits;
-            split_blocks = r.split_blocks;
-            ranges_us = r.us;
-        }
-        // Unfilled chunks, too, where a workgroup per tile is estimated faster than the ranges (1536 rows behind 8000 keys
-        // 281 -> 237 us) or the split-K tiles (1024 rows behind 2000 keys 84 -> 77 us, 1536 rows 130 -> 92).
-        const bool whole_ahead = q_len >= 256 && whole.us < (n_splits >= 2 ? ranges_us : splitk_us);
-        if (filled || whole_ahead || (pages && n_splits < 2)) return whole_tiles(pages);
-        if (n_splits >= 2)
-            return run_attention(ctx, kv, 1, layer, 1, &slot, &start_pos, &kv_valid, q_len, n_q_heads, q, 0,
-                                 (long long)q_stride, gate, 0, (long long)gate_stride, scale, out, 0, (long long)o_stride,
-                                 n_splits, split_blocks, pages);
-        return run_attention(ctx, kv, 0, layer, 1, &slot, &start_pos, &kv_valid, q_len, n_q_heads, q, 0,
-                             (long long)q_stride, gate, 0, (long long)gate_stride, scale, out, 0, (long long)o_stride);
-    }
-    // What the chunk kernel does not serve (head groups that are no multiple of 4, unaligned rows, quantised pages
-    // that are not staged, a non-positive scale): the split-K kernel over GQA-packed tiles, like a verify pass -- or, where heads that do
-    // not divide a tile's 32 rows leave some of them empty, tiles of 32 rows of ONE head, each walking all its keys, as long as they are
-    // plentiful and the context is short or they are very plentiful (one row at 32k keys over 8 bits took 460 us as 16 one-head tiles
-    // walking 32k keys each).  us a layer over 8 bits, one-head tiles / packed ones, of groups of 4 (32/8 heads of 128): 100 rows behind
-    // 7,000 keys 86.1 / 58.8, 700 behind 2,000 91.8 / 80.1; of 8 (16/2 of 256): 256 rows behind 2,000 64.2 / 52.1, 700 of a prompt 76.6 / 67.5;
-    // of 9 (36/4 of 128): 1,500 rows behind 3,000 256 / 297; of 5 (40/8 of 128): 700 behind 7,000 253 / 262.
-    const long long head_tiles = (long long)((q_len + 31) / 32) * n_q_heads;
-    const bool plentiful = 2 * head_tiles >= ctx->n_cus && (kv_valid <= 8192 || head_tiles >= 2LL * ctx->n_cus);
-    auto in_tiles = [&](int kind) {
-        return run_attention(ctx, kv, kind, layer, 1, &slot, &start_pos, &kv_valid, q_len, n_q_heads, q, 0, (long long)q_stride,
-                             gate, 0, (long long)gate_stride, scale, out, 0, (long long)o_stride);
-    };
-    // (over fp16 pages the two ways mostly take the same -- 116 of 120 chunks of groups of one and two within 5 %, 16/8 heads of 128, 300 rows behind 2,000 keys 37.5 /
-    // 38.6, 1,500 102.4 / 100.4, but 32/16 of 64, 100 rows behind 7,000, 52.9 / 37.8 --: one-head tiles, which need no partial results)
-    if ((rows_left_empty || kv->bits == 16) && plentiful) return in_tiles(1);
-    st = in_tiles(0);
-    // (without memory for the splits' partial results, as inside a capture that would have to grow it: tiles of one head, which have none)
-    if (plentiful && (st == TT_HIP_ERR_BUSY || st == TT_HIP_ERR_OUT_OF_MEMORY)) st = in_tiles(1);
-    return st;
-}
-
-// ---- sequences that share a prefix ------------------------------------------
-
 // Rows of sequences whose keys [0, front) -- whole blocks -- are another slot's rows: a pass over those with the tokens of all
 // sequences as rows of one, a pass over each sequence's own keys from there on, and the join.  The shared keys are then read once per
 // tile of rows, as a chunk's are, and not once per sequence.
@@ -1513,6 +1316,241 @@ static int run_shared_rows(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq,
     return TT_HIP_OK;
 }
 
+// Causal chunk attention, by whichever of the kernels and routes is the fastest.
+//   sinks >= 0: the keys [0, sinks) stay visible beside the window, and pinned rows of a ring are known; -1: neither.
+//   front > 0: the keys [0, front), whole blocks, are those of front_slot.
+static int run_prefill(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int slot, int start_pos, int q_len, int kv_valid, int sliding_window,
+                       int n_q_heads, const tt_half *q, size_t q_stride, const tt_half *gate, size_t gate_stride, float scale, tt_half *out,
+                       size_t o_stride, int sinks = -1, int front_slot = -1, int front = 0) {
+    const bool aligned = aligned16(q) && aligned16(out) && (!gate || aligned16(gate)) && q_stride % 8 == 0 &&
+                         o_stride % 8 == 0 && (!gate || gate_stride % 8 == 0);
+    // Keys in two pieces: the chunk kernel is told of them, except of a front piece that has been staged in front of the slot's own blocks.
+    const ChunkPieces apart{std::max(sinks, 0), std::max(front_slot, 0), front / kBlockTokens}, in_one{std::max(sinks, 0), 0, 0};
+    const bool pieces = sinks >= 0 || front > 0;
+    auto pieces_of = [&](const PageSource *pages) { return !pieces ? nullptr : pages ? &in_one : &apart; };
+    // A window that clips no row of the chunk is no window.
+    const int window = sliding_window > 0 && (long long)start_pos + q_len > sliding_window ? sliding_window : 0;
+    // (the chunk kernel takes a row's maximum over the raw scores: a scale that is not positive goes the split-K way)
+    const bool serves = prefill_kernel_serves(n_q_heads, kv->n_kv_heads, kv->head_dim, aligned) && scale > 0.0f;
+    const long long chunk_wgs = (long long)((q_len + 63) / 64) * (n_q_heads / 4);
+    // The chunk kernel as it is -- a workgroup per pair of tiles and 4 heads, all their keys -- where its workgroups
+    // fill half the chip, or a quarter of it with few key blocks each (a long first chunk of a prompt: 1024 rows from
+    // position 0 take 39 us against 41 us through the split-K tiles, 1536 rows 51 against 66).  Fewer workgroups
+    // walking more blocks lose to the other routes at any context: 128 rows behind 1920 keys took 100 us that way,
+    // 25 us through the split-K tiles; behind a 1024-key window 62 us against 20 us.
+    const long long pair_blocks = (2LL * start_pos + q_len) / 32 + 2;  // key blocks a workgroup's pair of tiles walks
+    const bool filled = 2 * chunk_wgs >= ctx->n_cus || (window == 0 && 4 * chunk_wgs >= ctx->n_cus && pair_blocks <= 64);
+    const int first_blocks = chunk_tile_blocks(start_pos, q_len, kv_valid, window, 0, apart.sinks);
+    const int last_blocks = chunk_tile_blocks(start_pos, q_len, kv_valid, window, (q_len + 31) / 32 - 1, apart.sinks);
+    const ChunkEstimate whole = estimate_chunk(ctx->n_cus, kv->head_dim, n_q_heads, kv->n_kv_heads, q_len, first_blocks, last_blocks);
+    auto whole_tiles = [&](const PageSource *pages) {
+        if (hipSetDevice(ctx->device) != hipSuccess) return (int)TT_HIP_ERR_HIP;
+        return launch_prefill(ctx, kv, layer, slot, start_pos, q_len, kv_valid, n_q_heads, q, (long long)q_stride, gate,
+                              (long long)gate_stride, scale, out, (long long)o_stride, 1, 0, nullptr, nullptr, pages, window,
+                              whole.single_tiles, pieces_of(pages));
+    };
+    const bool halves = kv->bits == 16 || sinks >= 0;  // (quantised pages that a window with sinks may have dequantised)
+    const double splitk_us = estimate_splitk_chunk_us(ctx->n_cus, kv->head_dim, n_q_heads, kv->n_kv_heads, q_len, first_blocks, last_blocks);
+    auto over_ranges = [&](int n_splits, int split_blocks, const PageSource *pages) {
+        return run_attention(ctx, kv, 1, layer, 1, &slot, &start_pos, &kv_valid, q_len, n_q_heads, q, 0, (long long)q_stride, gate, 0,
+                             (long long)gate_stride, scale, out, 0, (long long)o_stride, n_splits, split_blocks, pages, window, nullptr, 0, 0,
+                             false, nullptr, sinks, nullptr, pieces_of(pages));
+    };
+    if (window > 0) {
+        // The chunk kernel starts every tile at its window's first block.  It or the split-K kernel (GQA-packed tiles, each
+        // walking only its rows' windows), whichever is estimated faster; quantised pages and head groups the chunk
+        // kernel does not serve go through the latter.  32 / 8 heads of 128 behind a window of 4096 keys: 512 rows 65
+        // against 78 us, 777 rows 105 against 80; 16 / 2 of 256 behind 1024 keys: 512 rows 24 against 34, 777 rows 43
+        // against 34, 1024 rows 47 against 36.
+        // Where the chunk does not fill the chip and the split-K tiles go in whole rounds with the last one part empty, the keys of a
+        // window cut into ranges, as behind a long context (300 rows behind 4096 keys: 24 / 2 heads of 256 113.6 -> 55.3 us, 32 / 8 of
+        // 128 56.7 -> 48.3; 16 / 2 of 256, 600 rows 115.7 -> 66.8, 270 behind 16,384 keys 188.6 -> 92.3), or the chunk kernel as it is.  16 us: the
+        // combine pass and both kernels' starts.  Inside a capture the partial results' store does not grow.
+        enum { tiles, ranges, chunk } way = tiles;
+        KeyRanges r;
+        if (serves && halves && !filled && q_len >= 256) {
+            const int longest = longest_tile_blocks(start_pos, q_len, kv_valid, window, apart.sinks);
+            const double tiles_us = splitk_rounds_us(ctx->n_cus, n_q_heads, kv->n_kv_heads, q_len, longest, splitk_us);
+            r = plan_window_ranges(ctx->n_cus, kv->head_dim, n_q_heads, kv->n_kv_heads, start_pos, q_len, kv_valid, window, apart.sinks);
+            const size_t part_rows = (size_t)r.n_splits * n_q_heads * ((q_len + 31) / 32) * 32;
+            if (r.n_splits >= 2 && r.us + 16.0 < 0.95 * std::min(whole.us, tiles_us) && (!ctx->capturing || part_rows <= ctx->part_rows)) way = ranges;
+            else if (whole.us < 0.75 * tiles_us) way = chunk;
+        }
+        // The estimates do not hold where the split-K tiles are all at work at once, as a few hundred rows of a short window are: 64 / 8
+        // heads of 64, 226 rows behind 96 keys 7.0 us against 10.1, 32 / 8 of 128, 428 behind 128 12.9 / 14.6, 24 / 2 of 256, 247 behind
+        // 33 12.6 / 19.1; one more round the other way (279 rows there 22.5 / 19.1, 560 of 32 / 8 19.1 / 13.8).
+        const bool more_rounds = splitk_tiles(n_q_heads, kv->n_kv_heads, q_len) > splitk_tiles_at_once(ctx->n_cus, kv->head_dim);
+        if (way == tiles && serves && halves && (filled || (more_rounds && whole.us < splitk_us))) way = chunk;
+        if (way != tiles && kv->bits != 16) {
+            // Sinks over quantised pages, where the chunk kernel is the faster one over fp16 pages: the blocks of the sinks and of the rows'
+            // windows are dequantised once, one behind the other, and the chunk counts its positions from there -- the keys left out in between
+            // are none that a row sees, so that the rows' windows and sinks stay what they are.
+            const int window_block = std::max(start_pos + 1 - window, 0) / kBlockTokens, sink_blocks = std::min((apart.sinks + 31) / 32, window_block);
+            const int skipped = window_block - sink_blocks, end = start_pos + q_len;
+            const int n_blocks = (end + 31) / 32 - skipped;
+            const size_t page = (size_t)n_blocks * 32 * kv->head_dim;
+            if (hipSetDevice(ctx->device) != hipSuccess) return TT_HIP_ERR_HIP;
+            int st = ensure_stage(ctx, page * kv->n_kv_heads);
+            if (st == TT_HIP_OK) {
+                const DequantPieces from{sink_blocks, slot, skipped};
+                st = launch_kvq_dequant_blocks(kv, layer, slot, n_blocks, ctx->stage_k, ctx->stage_v, page, &from);
+                if (st != TT_HIP_OK) return st;
+                const PageSource staged{ctx->stage_k, ctx->stage_v, (long long)page, 0};
+                start_pos -= 32 * skipped;
+                kv_valid = end - 32 * skipped;
+                return way == ranges ? over_ranges(r.n_splits, r.split_blocks, &staged) : whole_tiles(&staged);
+            }
+            if (st != TT_HIP_ERR_BUSY && st != TT_HIP_ERR_OUT_OF_MEMORY) return st;
+            way = tiles;  // (no room for them, or none to be had inside a capture)
+        }
+        if (way == ranges) return over_ranges(r.n_splits, r.split_blocks, nullptr);
+        if (way == chunk) return whole_tiles(nullptr);
+        return run_attention(ctx, kv, 0, layer, 1, &slot, &start_pos, &kv_valid, q_len, n_q_heads, q, 0, (long long)q_stride,
+                             gate, 0, (long long)gate_stride, scale, out, 0, (long long)o_stride, 1, 0, nullptr, window, nullptr, 0, 0, false,
+                             nullptr, sinks);
+    }
+    // Quantised pages: the split-K kernel reads them as they are (dequantising in registers, once
+    // per 32-row tile -- 269 TFLOP/s on a 4096-row chunk).  A chunk that the MFMA chunk kernel
+    // would take is instead served from fp16 pages of the slot's visible blocks, dequantised once
+    // per call into the context's staging store (4096 rows: one 9 us pass, then the fp16 kernel).
+    PageSource staged{};
+    const PageSource *pages = nullptr;
+    auto in_two_passes = [&] {  // (a front piece where the split-K tiles are the faster ones)
+        return run_shared_rows(ctx, kv, layer, 1, &slot, &start_pos, &kv_valid, q_len, front_slot, front, n_q_heads, q, 0, (long long)q_stride,
+                               gate, 0, (long long)gate_stride, scale, out, 0, (long long)o_stride);
+    };
+    int st = TT_HIP_OK;
+    // From this many keys on a chunk that does not fill the chip goes through the chunk kernel over key ranges (below:
+    // through the split-K tiles): 786,432 / rows, i.e. 12k keys at 64 rows, 6k at 128, and at least 4096 (2560 over
+    // quantised pages, whose visible blocks are dequantised once per call first).  The split-K tiles read the keys once
+    // per tile of rows and leave small partial results; the ranges read them once per range and leave rows x heads x D
+    // floats per range.  One box, fp16, split-K / ranges: 64 rows at 8k keys 31.6 / 33.4 us, at 12k 37.2 / 35.3; 96
+    // rows at 4k 28.4 / 32.4, at 12k 47.7 / 42.8; 128 rows at 4k 32.0 / 35.0, at 8k 44.3 / 39.1; 192 rows at 4k 41.8 /
+    // 38.6.  Over 8 bits: 64 rows at 4k 24.4 / 35.4, at 16k 50.1 / 49.2, at 32k 80.7 / 71.9; 128 rows at 4k 34.6 /
+    // 40.2, at 8k 48.9 / 45.0.
+    // Heads that leave rows of a split-K tile empty make more tiles of the same rows, and what that way takes goes by its tiles: there from 393,216 /
+    // (tiles x D / 256) keys on where that is earlier, and from 2,048.  us a layer, split-K / ranges: 24 / 2 heads of 256, 96 rows behind 7,000 keys
+    // 63.8 / 50.0, over 8 bits 81.0 / 55.7, 300 behind 3,000 109.2 / 74.9, 200 behind 1,600 53.0 / 56.0.  Not for other heads, though the ranges would often
+    // be ahead (64 / 8 of 256, 130 rows behind 4,000 keys over 8 bits 173 / 119): not where the tiles share the chip out evenly (64 / 16 of 128, 64
+    // rows behind 7,900 keys 48.1 / 51.3, over 8 bits 58.6 / 77.9, 96 rows behind 5,100 67.8 / 75.8; 32 / 4 of 256, 64 rows 56.9 / 60.7).
+    const bool rows_left_empty = 32 % packed_heads(n_q_heads / kv->n_kv_heads) != 0;
+    const long long by_rows = 786432 / (q_len > 0 ? q_len : 1), others_from = std::max<long long>(by_rows, kv->bits == 16 ? 4096 : 2560);
+    long long ranges_from = others_from;
+    if (rows_left_empty) {
+        const long long tile_widths = splitk_tiles(n_q_heads, kv->n_kv_heads, q_len) * kv->head_dim;
+        ranges_from = std::max<long long>(std::min(393216ll * 256 / (tile_widths > 0 ? tile_widths : 1), by_rows), 2048);
+    }
+    // ... and from this many rows on: 64; at fp16 32 rows deep in a context (32 rows at 32k keys 50 us against 54 us,
+    // 48 rows 62 against 73).  Over quantised pages fewer rows stay with the split-K tiles, which widen a block once per
+    // tile of 16 rows: dequantising the whole context for them costs more than that at any length measured (32 rows
+    // at 64k keys over 8 bits 82 us against 107 us, 12 rows at 32k keys 30 us against 62 us).
+    const int rows_from = kv->bits == 16 ? (kv_valid >= 32768 ? 32 : 64) : 64;
+    if (serves && !filled && (kv->bits == 16 || !kv->ring) && q_len >= rows_from && kv_valid >= ranges_from && kv_valid < others_from) {
+        // (no memory for the ranges' partial results or the dequantised pages, or a capture in which they would have to grow: the split-K way)
+        const int blocks = (kv_valid + 31) / 32;
+        const KeyRanges r = plan_key_ranges(ctx->n_cus, kv->head_dim, n_q_heads, kv->n_kv_heads, q_len, blocks);
+        if (hipSetDevice(ctx->device) != hipSuccess) return TT_HIP_ERR_HIP;
+        st = q_len >= 256 && whole.us < r.us ? TT_HIP_OK : ensure_partials(ctx, (size_t)r.n_splits * n_q_heads * ((q_len + 31) / 32) * 32, kv->head_dim);
+        if (st == TT_HIP_OK && kv->bits != 16) st = ensure_stage(ctx, (size_t)blocks * 32 * kv->head_dim * kv->n_kv_heads);
+        if (st == TT_HIP_ERR_BUSY || st == TT_HIP_ERR_OUT_OF_MEMORY) ranges_from = others_from;
+        else if (st != TT_HIP_OK) return st;
+    }
+    if (kv->bits != 16 && !kv->ring && serves && q_len >= rows_from && (filled || kv_valid >= ranges_from)) {
+        const int n_blocks = (kv_valid + 31) / 32;
+        const size_t page = (size_t)n_blocks * 32 * kv->head_dim;
+        if (hipSetDevice(ctx->device) != hipSuccess) return TT_HIP_ERR_HIP;
+        st = ensure_stage(ctx, page * kv->n_kv_heads);
+        if (st != TT_HIP_OK) return st;
+        const DequantPieces from{apart.front_blocks, apart.front_slot, 0};
+        st = launch_kvq_dequant_blocks(kv, layer, slot, n_blocks, ctx->stage_k, ctx->stage_v, page, &from);
+        if (st != TT_HIP_OK) return st;
+        staged = PageSource{ctx->stage_k, ctx->stage_v, (long long)page, 0};
+        pages = &staged;
+    }
+    if (serves && (kv->bits == 16 || pages)) {
+        // The chunk kernel gives a workgroup 64 query rows of 4 heads and ALL their keys: one
+        // workgroup per CU at 4096 rows x 16 heads, but a 128-row chunk (the reference's default
+        // prefillChunkTokens) deep into a long context would be 8 workgroups walking 32k keys
+        // each (1318 us at 16q/2kv/256).  Three routes, chosen from timings at that shape:
+        //  * at least half a chip of workgroups, or a quarter with few blocks each: the chunk kernel as it is;
+        //  * 64 rows or more over 4096 keys or more (2560 over quantised pages): the chunk kernel with the keys cut into
+        //    ranges, a workgroup per (tile, 4 heads, range), and the combine pass over the partial
+        //    results (128 rows at 32k keys 98-106 us, 1024 rows 507-538 us; 256 rows at 4k keys 39 us
+        //    against 46 us the split-K way);
+        //  * anything else: the split-K kernel, which packs a KV head's q heads into its tiles
+        //    like a verify pass (64 rows at 16k keys 62 us against 89 us; 512 rows at 2k keys
+        //    59 us against 104 us, where the partial results outweigh the keys).
+        int n_splits = 1, split_blocks = 0;
+        double ranges_us = 0.0;
+        if (!filled && q_len >= rows_from && kv_valid >= ranges_from) {
+            const KeyRanges r = plan_key_ranges(ctx->n_cus, kv->head_dim, n_q_heads, kv->n_kv_heads, q_len, (kv_valid + 31) / 32);
+            n_splits = r.n_splits;
+            split_blocks = r.split_blocks;
+            ranges_us = r.us;
+        }
+        // Unfilled chunks, too, where a workgroup per tile is estimated faster than the ranges (1536 rows behind 8000 keys
+        // 281 -> 237 us) or the split-K tiles (1024 rows behind 2000 keys 84 -> 77 us, 1536 rows 130 -> 92).
+        const bool whole_ahead = q_len >= 256 && whole.us < (n_splits >= 2 ? ranges_us : splitk_us);
+        if (filled || whole_ahead || (pages && n_splits < 2)) return whole_tiles(pages);
+        if (n_splits >= 2) return over_ranges(n_splits, split_blocks, pages);
+        if (front > 0) return in_two_passes();
+        return run_attention(ctx, kv, 0, layer, 1, &slot, &start_pos, &kv_valid, q_len, n_q_heads, q, 0,
+                             (long long)q_stride, gate, 0, (long long)gate_stride, scale, out, 0, (long long)o_stride);
+    }
+    if (front > 0) return in_two_passes();
+    // What the chunk kernel does not serve (head groups that are no multiple of 4, unaligned rows, quantised pages
+    // that are not staged, a non-positive scale): the split-K kernel over GQA-packed tiles, like a verify pass -- or, where heads that do
+    // not divide a tile's 32 rows leave some of them empty, tiles of 32 rows of ONE head, each walking all its keys, as long as they are
+    // plentiful and the context is short or they are very plentiful (one row at 32k keys over 8 bits took 460 us as 16 one-head tiles
+    // walking 32k keys each).  us a layer over 8 bits, one-head tiles / packed ones, of groups of 4 (32/8 heads of 128): 100 rows behind
+    // 7,000 keys 86.1 / 58.8, 700 behind 2,000 91.8 / 80.1; of 8 (16/2 of 256): 256 rows behind 2,000 64.2 / 52.1, 700 of a prompt 76.6 / 67.5;
+    // of 9 (36/4 of 128): 1,500 rows behind 3,000 256 / 297; of 5 (40/8 of 128): 700 behind 7,000 253 / 262.
+    const long long head_tiles = (long long)((q_len + 31) / 32) * n_q_heads;
+    const bool plentiful = 2 * head_tiles >= ctx->n_cus && (kv_valid <= 8192 || head_tiles >= 2LL * ctx->n_cus);
+    auto in_tiles = [&](int kind) {
+        return run_attention(ctx, kv, kind, layer, 1, &slot, &start_pos, &kv_valid, q_len, n_q_heads, q, 0, (long long)q_stride,
+                             gate, 0, (long long)gate_stride, scale, out, 0, (long long)o_stride);
+    };
+    // (over fp16 pages the two ways mostly take the same -- 116 of 120 chunks of groups of one and two within 5 %, 16/8 heads of 128, 300 rows behind 2,000 keys 37.5 /
+    // 38.6, 1,500 102.4 / 100.4, but 32/16 of 64, 100 rows behind 7,000, 52.9 / 37.8 --: one-head tiles, which need no partial results)
+    if ((rows_left_empty || kv->bits == 16) && plentiful) return in_tiles(1);
+    st = in_tiles(0);
+    // (without memory for the splits' partial results, as inside a capture that would have to grow it: tiles of one head, which have none)
+    if (plentiful && (st == TT_HIP_ERR_BUSY || st == TT_HIP_ERR_OUT_OF_MEMORY)) st = in_tiles(1);
+    return st;
+}
+
+int tt_hip_attn_prefill_sinks(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int slot, int start_pos, int q_len, int kv_valid,
+                              int sliding_window, int sinks, int n_q_heads, const tt_half *q, size_t q_stride, const tt_half *gate,
+                              size_t gate_stride, float scale, tt_half *out, size_t o_stride) {
+    int st = check_common(ctx, kv, layer, n_q_heads, q, out);
+    if (st != TT_HIP_OK) return st;
+    if (slot < 0 || slot >= kv->n_slots || start_pos < 0 || q_len <= 0 || sliding_window < 0 || sinks < 0) return TT_HIP_ERR_INVALID_ARGUMENT;
+    const size_t packed = (size_t)n_q_heads * kv->head_dim;
+    if (q_stride < packed || o_stride < packed || (gate && gate_stride < packed)) return TT_HIP_ERR_SHAPE;
+    const long long end = (long long)start_pos + q_len;
+    if (end > kv_valid) return TT_HIP_ERR_INVALID_ARGUMENT;
+    const bool clipped = sliding_window > 0 && end > sliding_window;
+    {
+        const long long first = sliding_window > 0 && start_pos + 1LL > sliding_window ? start_pos + 1LL - sliding_window : 0;
+        const int needed = clipped ? (int)std::min<long long>(sinks, end - sliding_window) : 0;
+        if (!kv->holds_keys_and_sinks(needed, first, kv_valid)) return TT_HIP_ERR_CAPACITY;
+    }
+    BusyGuard guard(ctx);
+    if (!guard.ok) return TT_HIP_ERR_BUSY;
+    return run_prefill(ctx, kv, layer, slot, start_pos, q_len, kv_valid, sliding_window, n_q_heads, q, q_stride, gate, gate_stride, scale, out,
+                       o_stride, needs_sinks(kv, sliding_window, sinks, clipped) ? std::min(sinks, kv_valid) : -1);
+}
+
+int tt_hip_attn_prefill_swa(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int slot, int start_pos, int q_len, int kv_valid,
+                            int sliding_window, int n_q_heads, const tt_half *q, size_t q_stride, const tt_half *gate,
+                            size_t gate_stride, float scale, tt_half *out, size_t o_stride) {
+    return tt_hip_attn_prefill_sinks(ctx, kv, layer, slot, start_pos, q_len, kv_valid, sliding_window, 0, n_q_heads, q, q_stride, gate,
+                                     gate_stride, scale, out, o_stride);
+}
+
+// ---- sequences that share a prefix ------------------------------------------
+
 static int check_prefix(const tt_hip_kv *kv, int prefix_slot, int prefix_len) {
     if (prefix_slot < 0 || prefix_slot >= kv->n_slots || prefix_len < 0) return TT_HIP_ERR_INVALID_ARGUMENT;
     if (kv->ring) return TT_HIP_ERR_SHAPE;  // (whose rows the prefix's slot itself overwrites)
@@ -1598,8 +1636,8 @@ int tt_hip_attn_prefill_shared(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int sl
     if (!kv->holds_keys(0, kv_valid)) return TT_HIP_ERR_CAPACITY;
     BusyGuard guard(ctx);
     if (!guard.ok) return TT_HIP_ERR_BUSY;
-    return run_shared_rows(ctx, kv, layer, 1, &slot, &start_pos, &kv_valid, q_len, prefix_slot, front, n_q_heads, q, 0, (long long)q_stride,
-                           gate, 0, (long long)gate_stride, scale, out, 0, (long long)o_stride);
+    return run_prefill(ctx, kv, layer, slot, start_pos, q_len, kv_valid, 0, n_q_heads, q, q_stride, gate, gate_stride, scale, out, o_stride, -1,
+                       prefix_slot, front);
 }
 
 }  // extern "C"

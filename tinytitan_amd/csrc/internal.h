@@ -279,13 +279,20 @@ int plan_launch(const tt_hip_ctx *ctx, int kind, int n_seq, int n_q_heads, int n
 // kv_bits: 16 for fp16 pages, 8 / 4 for quantised ones.
 int launch_splitk(tt_hip_ctx *ctx, const LaunchPlan &plan, int head_dim, int n_seq, const SplitKArgs &args, int kv_bits = 16);
 
+// A chunk whose keys lie in two pieces: sinks beside the window (and the pinned rows of a ring in front of it), or the first front_blocks
+// blocks in another slot's pages of the cache.
+struct ChunkPieces {
+    int sinks, front_slot, front_blocks;
+};
+
 bool prefill_kernel_serves(int n_q_heads, int n_kv_heads, int head_dim, bool aligned);
 // n_splits > 1: every workgroup takes one of n_splits ranges of split_blocks key blocks and leaves
 // unnormalised partials (layout of the split-K kernel at 32-row, one-head tiles) for launch_combine.
 int launch_prefill(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int slot, int start, int q_len, int kv_valid,
                    int n_q_heads, const tt_half *q, long long q_stride, const tt_half *gate, long long g_stride,
                    float scale, tt_half *out, long long o_stride, int n_splits = 1, int split_blocks = 0,
-                   float *part_o = nullptr, float *part_ml = nullptr, const PageSource *pages = nullptr, int window = 0, bool single_tiles = false);
+                   float *part_o = nullptr, float *part_ml = nullptr, const PageSource *pages = nullptr, int window = 0, bool single_tiles = false,
+                   const ChunkPieces *pieces = nullptr);
 int launch_combine(tt_hip_ctx *ctx, const LaunchPlan &plan, int head_dim, int n_seq, const SplitKArgs &args);
 // The rows of n_seq sequences from the partial results of two passes (attn_join.hip).
 int launch_join(tt_hip_ctx *ctx, int head_dim, int n_seq, const JoinArgs &args);
@@ -302,8 +309,12 @@ int launch_kvq_append(tt_hip_kv *kv, int layer, int slot, int position, int n_to
                       size_t stride);
 int launch_kvq_read(tt_hip_kv *kv, int layer, int slot, int position, int n_tokens, tt_half *k, tt_half *v, size_t stride,
                     const int *positions = nullptr, int limit = 0);
+// Which blocks end up one behind the other: [0, front_blocks) of front_slot, then `skipped` further on the slot's own.
+struct DequantPieces {
+    int front_blocks, front_slot, skipped;
+};
 int launch_kvq_dequant_blocks(tt_hip_kv *kv, int layer, int slot, int n_blocks, _Float16 *k_dst, _Float16 *v_dst,
-                              size_t dst_page_elems);
+                              size_t dst_page_elems, const DequantPieces *pieces = nullptr);
 int launch_kvq_rows(tt_hip_kv *kv, int layer, int slot, int position, int n_tokens, uint8_t *k_rows, uint8_t *v_rows,
                     size_t row_stride, bool to_rows);
 

@@ -22,7 +22,9 @@ struct QuantArgs {
     long long page_bytes;
     int slot, n_kv_heads, head_dim, position, n_tokens;
     const int *positions;  // the read kernel only: row t is the row of positions[t]; outside [0, limit) gives zeros
-    int limit, ring_capacity, pinned;  // (the ring goes round behind the pinned rows)
+    int limit, ring_capacity;
+    int pinned;  // the ring goes round behind these rows
+    DequantPieces pieces;  // the dequantising kernel only
 };
 
 __device__ __forceinline__ uint8_t *block_of(const QuantArgs &a, bool is_v, int kvh, int pos, int bits) {
@@ -239,7 +241,11 @@ __global__ __launch_bounds__(256) void kvq_dequant_blocks_kernel(const QuantArgs
     typedef _Float16 h8 __attribute__((ext_vector_type(8)));
     typedef unsigned u2 __attribute__((ext_vector_type(2)));
     const int block = blockIdx.x, kvh = blockIdx.y, D = a.head_dim, gph = D / kQuantGroup;
-    const size_t src = ((size_t)a.slot * a.n_kv_heads + kvh) * (size_t)a.page_bytes + (size_t)block * block_bytes(D, BITS);
+    const bool in_front = block < a.pieces.front_blocks;
+    int from = in_front ? block : block + a.pieces.skipped;
+    if (a.ring_capacity > 0 && from * kBlockTokens >= a.pinned)
+        from = (a.pinned + (from * kBlockTokens - a.pinned) % a.ring_capacity) / kBlockTokens;
+    const size_t src = ((size_t)(in_front ? a.pieces.front_slot : a.slot) * a.n_kv_heads + kvh) * (size_t)a.page_bytes + (size_t)from * block_bytes(D, BITS);
     const uint8_t *kb = a.k_layer + src, *vb = a.v_layer + src;
     const size_t dst = (size_t)kvh * (size_t)dst_page_elems + (size_t)block * (size_t)(kBlockTokens * D);
     const size_t levels = block_level_bytes(D, BITS);
@@ -296,6 +302,7 @@ QuantArgs quant_args(tt_hip_kv *kv, int layer, int slot, int position, int n_tok
     a.limit = 0;
     a.ring_capacity = kv->ring ? kv->capacity - kv->pinned : 0;
     a.pinned = kv->pinned;
+    a.pieces = DequantPieces{0, slot, 0};
     return a;
 }
 
@@ -368,10 +375,12 @@ int launch_kvq_read(tt_hip_kv *kv, int layer, int slot, int position, int n_toke
     return launched(kv, "kvq_read_kernel launch");
 }
 
-// Blocks [0, n_blocks) of `slot`, every kv head, as fp16 pages of dst_page_elems halves each.
+// Blocks [0, n_blocks) of `slot`, every kv head, as fp16 pages of dst_page_elems halves each; with pieces, its first blocks in front and
+// the others, of what lies behind those that are skipped, behind them.
 int launch_kvq_dequant_blocks(tt_hip_kv *kv, int layer, int slot, int n_blocks, _Float16 *k_dst, _Float16 *v_dst,
-                              size_t dst_page_elems) {
-    const QuantArgs a = quant_args(kv, layer, slot, 0, n_blocks * kBlockTokens);
+                              size_t dst_page_elems, const DequantPieces *pieces) {
+    QuantArgs a = quant_args(kv, layer, slot, 0, n_blocks * kBlockTokens);
+    if (pieces) a.pieces = *pieces;
     const dim3 grid((unsigned)n_blocks, (unsigned)kv->n_kv_heads);
     if (kv->bits == 8)
         hipLaunchKernelGGL(kvq_dequant_blocks_kernel<8>, grid, dim3(256), 0, kv->ctx->stream, a, k_dst, v_dst, (long long)dst_page_elems);

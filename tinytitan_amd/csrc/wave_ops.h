@@ -7,6 +7,9 @@
 
 namespace tt {
 
+// A number of sinks that no key is at or past -- the test for it folds away -- where a kernel's rows have none.
+constexpr int kNoSinks = -0x7fffffff - 1;
+
 // The output gate's factor, 1 / (1 + e^-x), rounded as the fp32 division rounds it: the hardware's reciprocal (one unit in the last
 // place) and a Newton step, over a quarter of the denominator (exact) so that no reciprocal is subnormal; an infinite denominator
 // is the fixup's.  Every fp16 gate gives the division's bits (of the factors below 2^-126, which round any fp16 value to zero, all

@@ -1017,6 +1017,8 @@ __device__ __forceinline__ void block_softmax_pv(RowState<D, NT> &st, Scores<D, 
 // KEEP = kKeepSinks: a window whose rows also see the first tokens, the sinks.  A tile walks the sinks' blocks and its window's as
 // one run (TileInfo), so a wavefront goes from one to the other like from block to block -- no pass of its own for a piece that
 // is mostly one block -- and a block's place is looked up from its number in the walk.
+// KEEP = kKeepPieces: the same kernel twice in a launch, over two pieces of the rows' keys with their own arguments (SplitKPair): what sequences
+// share and what is their own.  Neither fills the chip while the other waits for it, and there is one launch less.
 // The hot arguments, this workgroup's sequence entry and where the rows go and their gate beside them, by five scalar loads issued
 // together (the compiler would fetch each field where it is first used: five or six dependent trips to the kernarg segment before
 // the first K/V load can go out, about 0.15 us each, and another ahead of the gate's loads).
@@ -1032,13 +1034,13 @@ struct SplitKOut {
 static_assert(offsetof(SplitKArgs, gate) == 0x480 && offsetof(SplitKArgs, o_tok_stride) == 0x480 + offsetof(SplitKOut, o_tok_stride) &&
                   offsetof(SplitKArgs, out) == 0x480 + offsetof(SplitKOut, out) && sizeof(SplitKOut) == 48,
               "load_args' offsets");
-__device__ __forceinline__ void load_args(SplitKHot &hot, SplitKSeq &sq, SplitKOut &out, int seq) {
+__device__ __forceinline__ void load_args(SplitKHot &hot, SplitKSeq &sq, SplitKOut &out, int seq, unsigned at = 0) {
     typedef int i8v __attribute__((ext_vector_type(8)));
     struct OutWords {
         i8v lo;
         i4 hi;
     };
-    const unsigned long long base = (unsigned long long)__builtin_amdgcn_kernarg_segment_ptr();
+    const unsigned long long base = (unsigned long long)__builtin_amdgcn_kernarg_segment_ptr() + at;
     const unsigned long long entry = base + (unsigned)seq * (unsigned)sizeof(SplitKSeq);
     HotWords w;
     i4 e, t_hi;
@@ -1054,8 +1056,8 @@ __device__ __forceinline__ void load_args(SplitKHot &hot, SplitKSeq &sq, SplitKO
     __builtin_memcpy(&out, &t, sizeof(out));
 }
 typedef __attribute__((address_space(4))) const i4 *seq_entries;  // SplitKSeq: [3] is first_split
-__device__ __forceinline__ seq_entries seq_table() {
-    return (seq_entries)((__attribute__((address_space(4))) const char *)__builtin_amdgcn_kernarg_segment_ptr() + offsetof(SplitKArgs, seq));
+__device__ __forceinline__ seq_entries seq_table(unsigned at = 0) {
+    return (seq_entries)((__attribute__((address_space(4))) const char *)__builtin_amdgcn_kernarg_segment_ptr() + at + offsetof(SplitKArgs, seq));
 }
 static_assert(kMaxSeqPerLaunch == 64 && offsetof(SplitKSeq, first_split) == 12, "a lane per sequence");
 static_assert(offsetof(SplitKArgs, hot) == 0 && offsetof(SplitKArgs, seq) == 0x80, "load_args' offsets");
@@ -1074,7 +1076,9 @@ __device__ __forceinline__ void load_row_words(unsigned (&dst)[8], __amdgpu_buff
 }
 
 template <int D, int NT, int WAVES, int BITS, int KEEP = 0, int STREAM = 0>
-__global__ __launch_bounds__(WAVES * 64, (NT == 16 && (KEEP < 2 || KEEP == kKeepSinks) ? 2 : 1)) void attn_splitk_kernel(const SplitKArgs args) {
+__global__ __launch_bounds__(WAVES * 64, (NT == 16 && (KEEP < 2 || KEEP >= kKeepSinks) ? 2 : 1)) void
+    attn_splitk_kernel(const std::conditional_t<KEEP == kKeepPieces, SplitKPair, SplitKArgs> args) {
+    constexpr bool PAIR = KEEP == kKeepPieces;
     constexpr bool PAIRED = STREAM == 2;
     static_assert(!PAIRED || (D == 256 && NT == 32 && BITS == 16 && KEEP == 0));
     constexpr int AUX = (STREAM ? kStreamed : 0) | (PAIRED ? kPaired : 0);
@@ -1087,28 +1091,41 @@ __global__ __launch_bounds__(WAVES * 64, (NT == 16 && (KEEP < 2 || KEEP == kKeep
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // scalar: block pointers stay in SGPRs
     const Lane<D, NT> ln(lane, PAIRED);
     const int li = ln.li, g = ln.g;
-    int seq = blockIdx.z;
+    int seq = PAIR ? 0 : blockIdx.z;
+    unsigned group = blockIdx.x, args_at = 0;
+    if constexpr (PAIR) {
+        if (group >= (unsigned)args.front_groups) {
+            group -= (unsigned)args.front_groups;
+            args_at = (unsigned)sizeof(SplitKArgs);  // (SplitKPair::own)
+        }
+    }
     SplitKHot a;
     SplitKSeq sq;
     SplitKOut out;
-    load_args(a, sq, out, seq);
-    int split = blockIdx.x, tile = blockIdx.y;
+    load_args(a, sq, out, seq, args_at);
+    int split = (int)group, tile = PAIR ? 0 : blockIdx.y;
+    if constexpr (PAIR) {
+        if (args_at != 0) {  // (tile fastest)
+            split = (int)(group / (unsigned)a.n_tiles);
+            tile = (int)(group - (unsigned)split * (unsigned)a.n_tiles);
+        }
+    }
     if (a.flags & kHotPackedSplits) {
         // Sequences of unlike lengths, their splits one behind the other in x: the entries of all of them in one load (those
         // past the last start beyond every split), and this split's sequence is the last that starts no later.
-        const int first = seq_table()[lane][3];
+        const int first = seq_table(args_at)[lane][3];
         seq = (int)__popcll(__ballot(first <= split)) - 1;
-        sq = __builtin_bit_cast(SplitKSeq, seq_table()[seq]);
+        sq = __builtin_bit_cast(SplitKSeq, seq_table(args_at)[seq]);
         split -= sq.first_split;
     }
     if (a.flags & kHotXcdGrid) {  // many token tiles: the (split, tile) pairs are dealt out XCD by XCD, tile fastest
         const unsigned pairs = (unsigned)a.n_tiles * (unsigned)a.n_splits_max, per_xcd = (pairs + 7u) >> 3;
-        const unsigned pair = (blockIdx.x & 7u) * per_xcd + (blockIdx.x >> 3);
+        const unsigned pair = (group & 7u) * per_xcd + (group >> 3);
         if (pair >= pairs) return;  // the grid is rounded up to a multiple of eight
         split = (int)(pair / (unsigned)a.n_tiles);
         tile = (int)(pair - (unsigned)split * (unsigned)a.n_tiles);
     }
-    constexpr bool SINKS = KEEP == kKeepSinks;
+    constexpr bool SINKS = KEEP >= kKeepSinks;
     const TileInfo ti = tile_info<SINKS>(a, sq, tile);
     const int k_begin = ti.k0 + split * a.split_len;
     if (k_begin >= ti.tile_end && split != 0) return;  // split 0 always runs so that an empty range yields zeros
@@ -1991,6 +2008,7 @@ static hipError_t configure_tile() {
     if constexpr (NT == 32) { TT_CFG(16, 4) }
     if constexpr (lists_fetch_by_key(D, 16)) { TT_CFG(16, 5) }
     TT_CFG(16, kKeepSinks) TT_CFG(8, kKeepSinks) TT_CFG(4, kKeepSinks)
+    TT_CFG(16, kKeepPieces) TT_CFG(8, kKeepPieces) TT_CFG(4, kKeepPieces)
 #undef TT_CFG
     return e;
 }
@@ -2011,6 +2029,28 @@ int launch_combine(tt_hip_ctx *ctx, const LaunchPlan &plan, int head_dim, int n_
 #define TT_CASE(DD, NN)              \
     if (head_dim == DD && plan.nt == NN) \
         return sinks ? launch_combine_one<DD, NN, true>(ctx, plan, n_seq, args) : launch_combine_one<DD, NN, false>(ctx, plan, n_seq, args);
+    TT_CASE(256, 16)
+    TT_CASE(256, 32)
+    TT_CASE(128, 16)
+    TT_CASE(128, 32)
+    TT_CASE(64, 16)
+    TT_CASE(64, 32)
+#undef TT_CASE
+    return TT_HIP_ERR_SHAPE;
+}
+
+int launch_splitk_pair(tt_hip_ctx *ctx, int head_dim, int nt, int kv_bits, unsigned groups, const SplitKPair &args) {
+    auto launch = [&](auto kernel) {
+        launch_profiled(ctx, kernel, dim3(groups), dim3(256), (unsigned)lds_bytes_for(head_dim, nt, 4), args);
+        const hipError_t e = hipGetLastError();
+        return e == hipSuccess ? (int)TT_HIP_OK : hip_fail(ctx, e, "attn_splitk_kernel launch");
+    };
+#define TT_CASE(DD, NN)                                                                  \
+    if (head_dim == DD && nt == NN) {                                                    \
+        if (kv_bits == 16) return launch(attn_splitk_kernel<DD, NN, 4, 16, kKeepPieces>); \
+        if (kv_bits == 8) return launch(attn_splitk_kernel<DD, NN, 4, 8, kKeepPieces>);   \
+        if (kv_bits == 4) return launch(attn_splitk_kernel<DD, NN, 4, 4, kKeepPieces>);   \
+    }
     TT_CASE(256, 16)
     TT_CASE(256, 32)
     TT_CASE(128, 16)

@@ -1230,6 +1230,91 @@ int tt_hip_attn_prefill(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int slot, int
                                    gate_stride, scale, out, o_stride);
 }
 
+// Two passes in one launch: the tokens of all sequences over the keys [0, front) of prefix_slot, every sequence over its own from there on.
+// Both in tiles of the same rows and splits of at most the same length, which is the one that makes the launch's rounds the
+// cheapest: a round costs a split's keys and what a workgroup spends beside them, 5.5 D keys' worth (a pass of 18 rows of 24/2
+// heads of 256 over 12,320 keys in splits of 2,048 / 1,024 / 896 29.4 / 20.1 / 19.6 us, of 20 rows of 32/8 of 128 over 6,000 in 2,048 / 1,024 14.2 / 9.1).
+static int run_pieces(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, const int *slots, const int *starts, const int *totals, int rows,
+                      int prefix_slot, int front, int n_q_heads, const tt_half *q, long long q_seq_stride, long long q_tok_stride, float scale,
+                      PassParts *front_parts, PassParts *own_parts, int *first_split) {
+    const int D = kv->head_dim, tokens = n_seq * rows;
+    LaunchPlan plan{};
+    int st = plan_launch(ctx, 0, 1, n_q_heads, kv->n_kv_heads, D, tokens, front, front, front, &plan, kv->bits, true);
+    if (st != TT_HIP_OK) return st;
+    const int per_token = plan.n_tiles / plan.tok_tiles, own_tok_tiles = (rows + plan.tt - 1) / plan.tt, own_tiles = per_token * own_tok_tiles;
+    auto splits_of = [&](int keys, int len) { return std::max((keys + len - 1) / len, 1); };
+    auto groups_of = [&](int len) {
+        long long own = 0;
+        for (int i = 0; i < n_seq; ++i) own += splits_of(totals[i] - front, len);
+        return (long long)plan.n_tiles * splits_of(front, len) + own * own_tiles;
+    };
+    const long long slots_on_chip = (long long)ctx->n_cus * plan.slots_per_cu;
+    int longest = front, len = 0;
+    for (int i = 0; i < n_seq; ++i) longest = std::max(longest, totals[i] - front);
+    if (ctx->split_override > 0) {
+        len = (ctx->split_override + 31) / 32 * 32;
+    } else {
+        long long best = 0;
+        for (int l = 128; l < longest + 128; l += std::max(128, l / 16 / 128 * 128)) {
+            const long long rounds = (groups_of(l) + slots_on_chip - 1) / slots_on_chip, cost = rounds * (std::min(l, longest) + 11 * D / 2);
+            if (len == 0 || cost < best) {
+                best = cost;
+                len = l;
+            }
+        }
+    }
+    SplitKPair a;
+    std::memset(static_cast<void *>(&a), 0, sizeof(a));
+    auto fill = [&](SplitKArgs &s, int pass_rows, int tok_tiles, int n_tiles, int flags, int n_splits) {
+        SplitKHot &h = s.hot;
+        h.k_layer = kv->k[layer];
+        h.v_layer = kv->v[layer];
+        h.q = reinterpret_cast<const _Float16 *>(q);
+        h.page_elems = (long long)kv->page_elems();
+        h.q_seq_stride = q_seq_stride;
+        h.q_tok_stride = q_tok_stride;
+        h.n_kv_heads = kv->n_kv_heads;
+        h.group = n_q_heads / kv->n_kv_heads;
+        h.rows = pass_rows;
+        h.gh = plan.gh;
+        h.gh_inv = (65536 + plan.gh - 1) / plan.gh;
+        h.tt = plan.tt;
+        h.hsubs = plan.hsubs;
+        h.tok_tiles = tok_tiles;
+        h.n_tiles = n_tiles;
+        h.split_len = len;
+        h.n_splits_max = n_splits;
+        h.flags = flags | kHotSinks;  // (of which there are none)
+        h.scale_log2e = scale * 1.4426950408889634f;
+        for (int i = 0; i < kMaxSeqPerLaunch; ++i) s.seq[i].first_split = 0x7fffffff;
+    };
+    const int front_splits = splits_of(front, len);
+    // (more than one split each as far as the kernel knows: it leaves partial results)
+    fill(a, tokens, plan.tok_tiles, plan.n_tiles, kHotXcdGrid, std::max(front_splits, 2));
+    a.seq[0] = SplitKSeq{prefix_slot, front, front, 0};  // (no row's own position limits what it sees of the shared keys)
+    fill(a.own, rows, own_tok_tiles, own_tiles, kHotPackedSplits, 2);
+    a.own.hot.k_layer += front / kBlockTokens * (kv->block_bytes() / 2);
+    a.own.hot.v_layer += front / kBlockTokens * (kv->block_bytes() / 2);
+    int own_splits = 0;
+    for (int i = 0; i < n_seq; ++i) {
+        first_split[i] = own_splits;
+        a.own.seq[i] = SplitKSeq{slots[i], starts[i] - front, totals[i] - front, own_splits};
+        own_splits += splits_of(totals[i] - front, len);
+    }
+    const size_t front_rows = (size_t)front_splits * plan.n_tiles * plan.nt, own_rows = (size_t)own_splits * own_tiles * plan.nt;
+    st = ensure_partials(ctx, front_rows + own_rows, D);
+    if (st != TT_HIP_OK) return st;
+    a.hot.part_o = ctx->part_o;
+    a.hot.part_ml = ctx->part_ml;
+    a.own.hot.part_o = ctx->part_o + front_rows * D;
+    a.own.hot.part_ml = ctx->part_ml + front_rows * 2;
+    auto parts = [&](const SplitKHot &h) { return PassParts{h.part_o, h.part_ml, plan.nt, plan.gh, plan.tt, plan.hsubs, h.tok_tiles, h.n_tiles, len}; };
+    *front_parts = parts(a.hot);
+    *own_parts = parts(a.own.hot);
+    a.front_groups = (int)(((long long)plan.n_tiles * a.hot.n_splits_max + 7) / 8 * 8);
+    return launch_splitk_pair(ctx, D, plan.nt, kv->bits, (unsigned)(a.front_groups + own_splits * own_tiles), a);
+}
+
 // Rows of sequences whose keys [0, front) -- whole blocks -- are another slot's rows: a pass over those with the tokens of all
 // sequences as rows of one, a pass over each sequence's own keys from there on, and the join.  The shared keys are then read once per
 // tile of rows, as a chunk's are, and not once per sequence.
@@ -1239,13 +1324,11 @@ static int run_shared(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, cons
                       long long o_seq_stride, long long o_tok_stride) {
     if (hipSetDevice(ctx->device) != hipSuccess) return TT_HIP_ERR_HIP;
     const int D = kv->head_dim, tokens = n_seq * rows;
-    const int front_from = front;  // (no row's own position limits what it sees of the shared keys)
     const bool aligned = aligned16(q) && q_tok_stride % 8 == 0;
     const bool serves = prefill_kernel_serves(n_q_heads, kv->n_kv_heads, D, aligned) && scale > 0.0f;
     // The shared keys: as behind a long context, the chunk kernel over ranges of the keys from some rows and keys on, else the split-K tiles.
     const int rows_from = kv->bits == 16 ? (front >= 32768 ? 32 : 64) : 64;
     const long long keys_from = std::max<long long>(786432 / tokens, kv->bits == 16 ? 4096 : 2560);
-    KeyPiece shared{true}, own{false, front / kBlockTokens};
     KeyRanges ranges;
     PageSource staged{};
     const PageSource *pages = nullptr;
@@ -1261,23 +1344,35 @@ static int run_shared(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, cons
         staged = PageSource{ctx->stage_k, ctx->stage_v, (long long)page, 0};
         pages = &staged;
     }
-    const bool by_ranges = ranges.n_splits >= 2;
-    st = run_attention(ctx, kv, by_ranges ? 1 : 0, layer, 1, &prefix_slot, &front_from, &front, tokens, n_q_heads, q, 0, q_tok_stride, nullptr,
-                       0, 0, scale, out, 0, o_tok_stride, by_ranges ? ranges.n_splits : 1, ranges.split_blocks, by_ranges ? pages : nullptr, 0,
-                       nullptr, 0, 0, false, nullptr, -1, &shared);
-    if (st != TT_HIP_OK) return st;
-    IntTable own_starts(n_seq), own_totals(n_seq);
-    for (int i = 0; i < n_seq; ++i) {
-        own_starts[i] = starts[i] - front;
-        own_totals[i] = totals[i] - front;
-    }
-    st = run_attention(ctx, kv, 0, layer, n_seq, slots, own_starts.data(), own_totals.data(), rows, n_q_heads, q, q_seq_stride, q_tok_stride,
-                       nullptr, 0, 0, scale, out, o_seq_stride, o_tok_stride, 1, 0, nullptr, 0, nullptr, 0, 0, false, nullptr, 0, &own);
-    if (st != TT_HIP_OK) return st;
     JoinArgs j{};
-    j.front = shared.parts;
-    j.own = own.parts;
-    j.front_splits = std::max((front + shared.parts.split_len - 1) / shared.parts.split_len, 1);
+    if (ranges.n_splits >= 2) {
+        KeyPiece shared{true}, own{false, front / kBlockTokens};
+        st = run_attention(ctx, kv, 1, layer, 1, &prefix_slot, &front, &front, tokens, n_q_heads, q, 0, q_tok_stride, nullptr, 0, 0, scale, out, 0,
+                           o_tok_stride, ranges.n_splits, ranges.split_blocks, pages, 0, nullptr, 0, 0, false, nullptr, -1, &shared);
+        if (st != TT_HIP_OK) return st;
+        int own_starts[kMaxSeqPerLaunch], own_totals[kMaxSeqPerLaunch];
+        for (int i = 0; i < n_seq; ++i) {
+            own_starts[i] = starts[i] - front;
+            own_totals[i] = totals[i] - front;
+        }
+        st = run_attention(ctx, kv, 0, layer, n_seq, slots, own_starts, own_totals, rows, n_q_heads, q, q_seq_stride, q_tok_stride, nullptr, 0, 0,
+                           scale, out, o_seq_stride, o_tok_stride, 1, 0, nullptr, 0, nullptr, 0, 0, false, nullptr, 0, &own);
+        if (st != TT_HIP_OK) return st;
+        j.front = shared.parts;
+        j.own = own.parts;
+        for (int i = 0; i < n_seq; ++i) j.seq[i].first_split = own.first_split[i];
+    } else {
+        int first_split[kMaxSeqPerLaunch];
+        st = run_pieces(ctx, kv, layer, n_seq, slots, starts, totals, rows, prefix_slot, front, n_q_heads, q, q_seq_stride, q_tok_stride, scale,
+                        &j.front, &j.own, first_split);
+        if (st != TT_HIP_OK) return st;
+        for (int i = 0; i < n_seq; ++i) j.seq[i].first_split = first_split[i];
+    }
+    j.front_splits = std::max((front + j.front.split_len - 1) / j.front.split_len, 1);
+    for (int i = 0; i < n_seq; ++i) {
+        j.seq[i].start = starts[i] - front;
+        j.seq[i].total = totals[i] - front;
+    }
     j.rows = rows;
     j.heads = n_q_heads;
     j.group = n_q_heads / kv->n_kv_heads;
@@ -1288,7 +1383,6 @@ static int run_shared(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, cons
     j.o_seq_stride = o_seq_stride;
     j.o_tok_stride = o_tok_stride;
     j.aligned = aligned16(out) && o_seq_stride % 8 == 0 && o_tok_stride % 8 == 0;
-    for (int i = 0; i < n_seq; ++i) j.seq[i] = JoinSeq{own_starts[i], own_totals[i], own.first_split[i]};
     return launch_join(ctx, D, n_seq, j);
 }
 

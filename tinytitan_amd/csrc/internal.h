@@ -38,6 +38,7 @@ constexpr int kHotPackedSplits = 4;
 // blocks at the page's front that its ring leaves alone.
 constexpr int kHotSinks = 8, kHotPinnedShift = 8;
 constexpr int kKeepSinks = 6;  // that kernel's KEEP (attn_splitk.hip)
+constexpr int kKeepPieces = 7;  // ... and of two passes in one launch, over the keys that sequences share and over their own
 struct SplitKHot {                         // dword
     const _Float16 *k_layer;               //  0
     const _Float16 *v_layer;               //  2
@@ -120,6 +121,14 @@ struct LaunchPlan {
     int packed_splits;  // > 0: launch with kHotPackedSplits over this many splits
     bool partials_only;  // the partial results are somebody else's to combine (PassParts)
 };
+
+// Two passes in one launch (kKeepPieces): workgroups [0, front_groups) are those of the base's, a chunk's token tiles dealt out XCD by XCD
+// (kHotXcdGrid), the others, tile fastest, the packed splits of `own` (kHotPackedSplits).
+struct alignas(64) SplitKPair : SplitKArgs {
+    SplitKArgs own;
+    int front_groups;
+};
+static_assert(sizeof(SplitKPair) == 2 * sizeof(SplitKArgs) + 64, "`own` right behind the base, where the kernel looks for it");
 
 // Where a pass over one piece of the keys has left its partial results: row n of a tile's split lies at
 // ((first_split(sequence) + split) * n_tiles + tile) * nt + n, D floats of `o` and a (maximum, sum) pair of `ml`.
@@ -275,6 +284,9 @@ struct PageSource {
 // of the chunk kernel, whose callers fix the tile themselves).
 int plan_launch(const tt_hip_ctx *ctx, int kind, int n_seq, int n_q_heads, int n_kv_heads, int head_dim, int rows,
                 long long total_keys, int min_keys, int max_keys, LaunchPlan *plan, int kv_bits = 16, bool small_tiles_ok = false);
+
+// A launch of a pair (nt: its tiles' rows, groups: its workgroups in all).
+int launch_splitk_pair(tt_hip_ctx *ctx, int head_dim, int nt, int kv_bits, unsigned groups, const SplitKPair &args);
 
 // kv_bits: 16 for fp16 pages, 8 / 4 for quantised ones.
 int launch_splitk(tt_hip_ctx *ctx, const LaunchPlan &plan, int head_dim, int n_seq, const SplitKArgs &args, int kv_bits = 16);

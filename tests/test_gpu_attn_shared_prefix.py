@@ -84,7 +84,7 @@ def test_decode(gpu_ctx, H, KH, D, bits, prefix):
 
 
 @pytest.mark.parametrize("H,KH,D,bits,prefix,n", [(16, 2, 256, 16, 9000, 70), (32, 8, 128, 8, 5000, 64), (16, 4, 64, 16, 12321, 66),
-                                                  (16, 2, 256, 4, 33000, 40), (8, 2, 256, 8, 6000, 100)])
+                                                  (16, 2, 256, 4, 33000, 40), (8, 2, 256, 8, 6000, 100), (16, 2, 256, 8, 20011, 64)])
 def test_a_large_batch(gpu_ctx, H, KH, D, bits, prefix, n):
     # more sequences than one launch takes, and enough rows for the chunk kernel over the shared keys
     lengths = [prefix + 1 + (i * i * 7) % 300 for i in range(n)]
@@ -97,6 +97,20 @@ def test_a_large_batch(gpu_ctx, H, KH, D, bits, prefix, n):
     pick = [5, 3, 3, 0]
     got = _decode(gpu_ctx, f, q[pick], D ** -0.5, g[pick], [lengths[i] for i in pick], [f.slots[i] for i in pick])
     check(got, [f.row(i, q[i], lengths[i] - 1, D ** -0.5, g[i]) for i in pick], "picked")
+    f.kv.close()
+
+
+@pytest.mark.parametrize("H,KH,D", [(16, 2, 256), (24, 2, 256), (32, 8, 128), (40, 8, 128), (16, 4, 64), (32, 1, 64)])
+@pytest.mark.parametrize("bits", [16, 8, 4])
+@pytest.mark.parametrize("prefix,n", [(900, 3), (4500, 7), (10007, 18)])
+def test_few_rows_behind_a_long_prefix(gpu_ctx, H, KH, D, bits, prefix, n):
+    # tiles that the tokens of several sequences share, whole and ragged, over any number of splits; own keys of one split and of several
+    lengths = [prefix + 1 + (i * 37) % 90 + (1500 if i == n - 1 else 0) for i in range(n)]
+    f = Family(gpu_ctx, KH, D, prefix, lengths, bits, home=n)
+    q, g = _rows(13, n, H, D), _rows(14, n, H, D)
+    got = _decode(gpu_ctx, f, q, D ** -0.5, g)
+    some = sorted({0, n // 2, n - 1})
+    check(got[some], [f.row(i, q[i], lengths[i] - 1, D ** -0.5, g[i]) for i in some], "rows")
     f.kv.close()
 
 

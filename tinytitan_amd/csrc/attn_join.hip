@@ -5,8 +5,11 @@
 // and the same over any number of splits of either piece, so the splits of both are added up in one go; then the gate, in fp32, and one
 // rounding.  A row that sees nothing gives zeros.
 //
-// What it takes is a trip to memory for the arguments and one for the partial rows: a workgroup is one (token, head), its threads own
-// four dims of every G-th split each, and ask for kBatch of those at once.
+// What it takes is its trips to memory, one for the arguments and as few as may be for the partial rows: a workgroup is one (token, head) and
+// DIMS dims of it, its threads own four dims of every G-th split, G = 1024 / DIMS, and ask for BATCH of those at once.  Rows of many splits
+// go by 64 dims (sixteen splits side by side, up to 128 in one trip), rows of few in one workgroup, of which there are then fewer.
+#include <algorithm>
+
 #include "internal.h"
 #include "wave_ops.h"
 
@@ -18,7 +21,6 @@ typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f2 __attribute__((ext_vector_type(2)));
 constexpr float kNegBig = -1.0e30f;
-constexpr int kBatch = 4;
 
 // Row n of tile `tile` in split 0 of a pass, for token `tok` of a sequence and q head `head`.
 __device__ __forceinline__ size_t part_row(const PassParts &p, int group, int tok, int head) {
@@ -28,55 +30,56 @@ __device__ __forceinline__ size_t part_row(const PassParts &p, int group, int to
     return (size_t)tile * p.nt + (tok - tok_tile * p.tt) * p.gh + (in_group - hsub * p.gh);
 }
 
-template <int D>
+template <int D, int DIMS, int BATCH>
 __global__ __launch_bounds__(256) void attn_join_kernel(const JoinArgs a) {
-    constexpr int D4 = D / 4, G = 256 / D4;
-    __shared__ f4 sums[G][D4];
+    constexpr int LANES = DIMS / 4, G = 256 / LANES, PARTS = D / DIMS;
+    __shared__ f4 sums[G][LANES];
     __shared__ f2 stats[G];
-    const int head = blockIdx.x, row = blockIdx.y, seq = blockIdx.z;
-    const int d = (threadIdx.x % D4) * 4, g = threadIdx.x / D4;
+    const int head = blockIdx.x / PARTS, row = blockIdx.y, seq = blockIdx.z;
+    const int lane = threadIdx.x % LANES, g = threadIdx.x / LANES, d = (blockIdx.x - head * PARTS) * DIMS + lane * 4;
     const JoinSeq sq = a.seq[seq];
-    const _Float16 *gate_at = a.gate + seq * a.g_seq_stride + row * a.g_tok_stride + (long long)head * D + d;
     _Float16 gate[4] = {};
     if (a.gate && g == 0) {
+        const _Float16 *at = a.gate + seq * a.g_seq_stride + row * a.g_tok_stride + (long long)head * D + d;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) gate[i] = gate_at[i];
+        for (int i = 0; i < 4; ++i) gate[i] = at[i];
     }
+    // The splits of both pieces in one count: where split s lies is `base + s * stride` of its piece.
+    const size_t front_stride = (size_t)a.front.n_tiles * a.front.nt, own_stride = (size_t)a.own.n_tiles * a.own.nt;
     const size_t front_row = part_row(a.front, a.group, seq * a.rows + row, head);
-    const size_t own_row = part_row(a.own, a.group, row, head) + (size_t)sq.first_split * a.own.n_tiles * a.own.nt;
+    const size_t own_row = part_row(a.own, a.group, row, head) + (size_t)sq.first_split * own_stride;
     const int tile_end = min(sq.total, sq.start + min((row / a.own.tt + 1) * a.own.tt, a.rows));
     const int n = a.front_splits + max((max(tile_end, 0) + a.own.split_len - 1) / a.own.split_len, 1);
     float m = kNegBig, l = 0.0f;
     f4 acc = (f4)0.0f;
-    for (int first = g; first < n; first += G * kBatch) {
-        f4 o[kBatch];
-        f2 ml[kBatch];
+    for (int first = g; first < n; first += G * BATCH) {
+        f4 o[BATCH];
+        f2 ml[BATCH];
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
+        for (int i = 0; i < BATCH; ++i) {
             const int s = min(first + i * G, n - 1);
             const bool front = s < a.front_splits;
-            const PassParts &p = front ? a.front : a.own;
-            const size_t at = (front ? front_row : own_row) + (size_t)(front ? s : s - a.front_splits) * p.n_tiles * p.nt;
-            ml[i] = *reinterpret_cast<const f2 *>(p.ml + at * 2);
-            o[i] = *reinterpret_cast<const f4 *>(p.o + at * D + d);
+            const size_t at = front ? front_row + s * front_stride : own_row + (s - a.front_splits) * own_stride;
+            ml[i] = *reinterpret_cast<const f2 *>((front ? a.front.ml : a.own.ml) + at * 2);
+            o[i] = *reinterpret_cast<const f4 *>((front ? a.front.o : a.own.o) + at * D + d);
         }
         float top = m;
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) top = fmaxf(top, ml[i][0]);
+        for (int i = 0; i < BATCH; ++i) top = fmaxf(top, ml[i][0]);
         const float keep = __builtin_amdgcn_exp2f(m - top);
         l *= keep;
         acc *= keep;
         m = top;
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
+        for (int i = 0; i < BATCH; ++i) {
             if (first + i * G >= n) break;  // (not a factor of zero, which an infinite value makes NaN of)
             const float f = __builtin_amdgcn_exp2f(ml[i][0] - m);
             l += f * ml[i][1];
             acc += f * o[i];
         }
     }
-    sums[g][threadIdx.x % D4] = acc;
-    if (threadIdx.x % D4 == 0) stats[g] = f2{m, l};
+    sums[g][lane] = acc;
+    if (lane == 0) stats[g] = f2{m, l};
     __syncthreads();
     if (g != 0) return;
 #pragma unroll
@@ -87,7 +90,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const JoinArgs a) {
     for (int i = 0; i < G; ++i) {
         const float f = __builtin_amdgcn_exp2f(stats[i][0] - m);
         total += f * stats[i][1];
-        out += f * sums[i][threadIdx.x];
+        out += f * sums[i][lane];
     }
     out *= total > 0.0f ? 1.0f / total : 0.0f;
     if (a.gate) {
@@ -104,15 +107,27 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const JoinArgs a) {
     }
 }
 
+template <int D>
+void launch_join_of(tt_hip_ctx *ctx, int n_seq, const JoinArgs &args) {
+    int most = 0;  // splits of a row
+    for (int i = 0; i < n_seq; ++i) most = std::max(most, args.seq[i].total);
+    most = args.front_splits + std::max((most + args.own.split_len - 1) / args.own.split_len, 1);
+    auto launch = [&](auto kernel, int parts) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(args.heads * parts), (unsigned)args.rows, (unsigned)n_seq), dim3(256), 0, ctx->stream, args);
+    };
+    if (most <= 4 * 1024 / D) launch(attn_join_kernel<D, D, 4>, 1);
+    else if (most <= 64) launch(attn_join_kernel<D, 64, 4>, D / 64);
+    else launch(attn_join_kernel<D, 64, 8>, D / 64);
+}
+
 }  // namespace
 
 int launch_join(tt_hip_ctx *ctx, int head_dim, int n_seq, const JoinArgs &args) {
     if (n_seq > kMaxSeqPerLaunch || args.rows > 65535) return TT_HIP_ERR_SHAPE;
-    const dim3 grid((unsigned)args.heads, (unsigned)args.rows, (unsigned)n_seq);
     switch (head_dim) {
-        case 256: hipLaunchKernelGGL(attn_join_kernel<256>, grid, dim3(256), 0, ctx->stream, args); break;
-        case 128: hipLaunchKernelGGL(attn_join_kernel<128>, grid, dim3(256), 0, ctx->stream, args); break;
-        case 64: hipLaunchKernelGGL(attn_join_kernel<64>, grid, dim3(256), 0, ctx->stream, args); break;
+        case 256: launch_join_of<256>(ctx, n_seq, args); break;
+        case 128: launch_join_of<128>(ctx, n_seq, args); break;
+        case 64: launch_join_of<64>(ctx, n_seq, args); break;
         default: return TT_HIP_ERR_SHAPE;
     }
     const hipError_t e = hipGetLastError();

@@ -1135,6 +1135,14 @@ __global__ __launch_bounds__(WAVES * 64, (NT == 16 && (KEEP < 2 || KEEP >= kKeep
     const size_t page = ((size_t)sq.slot * a.n_kv_heads + ti.kvh) * (size_t)a.page_elems;
     const __amdgpu_buffer_rsrc_t rk = make_rsrc(a.k_layer + page, (unsigned)(a.page_elems * 2));
     const __amdgpu_buffer_rsrc_t rv = make_rsrc(a.v_layer + page, (unsigned)(a.page_elems * 2));
+    // (a prefix in another slot: its blocks come out of that slot's page)
+    constexpr bool FRONT = KEEP == kKeepSinks;
+    const int front_blocks = FRONT && (a.flags & kHotFront) ? a.flags >> kHotPinnedShift : 0;
+    const size_t front_page = FRONT && front_blocks > 0 ? ((size_t)a.keep_words * a.n_kv_heads + ti.kvh) * (size_t)a.page_elems : page;
+    auto page_of = [&](const _Float16 *layer, const __amdgpu_buffer_rsrc_t &own, int block) {
+        if constexpr (FRONT) return make_rsrc(layer + (block < front_blocks ? front_page : page), (unsigned)(a.page_elems * 2));
+        return own;
+    };
 
     // This lane's query row.
     const int t_local = (li * a.gh_inv) >> 16;  // li / gh
@@ -1354,12 +1362,12 @@ __global__ __launch_bounds__(WAVES * 64, (NT == 16 && (KEEP < 2 || KEEP >= kKeep
     auto page_block = [&](int i) {
         const int block = walked_block(i);
         if constexpr (SINKS) {
-            const int pinned = a.flags >> kHotPinnedShift;
+            const int pinned = a.flags >> kHotPinnedShift;  // (with a ring only)
             return a.ring_blocks && block >= pinned ? pinned + (block - pinned) % a.ring_blocks : block;
         }
         return a.ring_blocks ? block % a.ring_blocks : block;
     };
-    const int sinks = SINKS ? a.keep_words : kNoSinks;
+    const int sinks = SINKS ? (a.flags & kHotFront ? 0 : a.keep_words) : kNoSinks;
     const int first_lim = min(ti.total, ti.start + ti.t0 + 1), seen_from = a.window > 0 ? max(first_lim - a.window, 0) : 0;
     const int seen_end = ti.tile_end + 32 * ti.skipped;  // (SINKS) keys up to the tile's last row's own
     const bool first_real = b < b_end;
@@ -1376,7 +1384,7 @@ __global__ __launch_bounds__(WAVES * 64, (NT == 16 && (KEEP < 2 || KEEP >= kKeep
             load_k_groups<D>(kt, rk, at_next);
         }
     } else {
-        load_k<AUX>(kt, rk, first_bytes, ln, first_void);
+        load_k<AUX>(kt, page_of(a.k_layer, rk, b), first_bytes, ln, first_void);
     }
     __builtin_amdgcn_sched_barrier(0);  // the first block's K loads are issued HERE, before the query is waited for
     if constexpr (KEEP == 2) {
@@ -1424,7 +1432,7 @@ __global__ __launch_bounds__(WAVES * 64, (NT == 16 && (KEEP < 2 || KEEP >= kKeep
     if constexpr (KEEP == 4) {
         if (run_end > 0) load_v_groups<D>(vt, rv, at_next);
     } else {
-        load_v<AUX>(vt, rv, first_bytes, ln, first_void);
+        load_v<AUX>(vt, page_of(a.v_layer, rv, b), first_bytes, ln, first_void);
     }
     __builtin_amdgcn_sched_barrier(0);
 
@@ -1493,6 +1501,7 @@ __global__ __launch_bounds__(WAVES * 64, (NT == 16 && (KEEP < 2 || KEEP >= kKeep
         const bool real = nb < b_end && next_kept;
         const unsigned next = real ? (unsigned)page_block(nb) * BLK_BYTES : 0u;
         const int kbase = walked_block(b) << 5;
+        const __amdgpu_buffer_rsrc_t next_k = page_of(a.k_layer, rk, nb), next_v = page_of(a.v_layer, rv, nb);
         unsigned seen = ~0u;  // the block's keys that some row of the tile sees
         if constexpr (SINKS) {
             auto below = [](int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; };
@@ -1501,16 +1510,16 @@ __global__ __launch_bounds__(WAVES * 64, (NT == 16 && (KEEP < 2 || KEEP >= kKeep
         Voids<D, NT> vo(real ? 0u : kVoidLoad);
         if constexpr (BY_KEY) vo = Voids<D, NT>(real ? 0u : kVoidLoad, next_keys, ln);
         if constexpr (BITS == 16 && NT == 32) {
-            block_scores_refill<AUX, D>(sc, kt, qf, rk, next, ln, vo);
-            block_softmax_pv_refill<AUX, D>(st, sc, vt, ln, kbase, lo, lim, a.scale_log2e, rv, next, vo, kept, row_keep, row_bits, sinks, seen);
+            block_scores_refill<AUX, D>(sc, kt, qf, next_k, next, ln, vo);
+            block_softmax_pv_refill<AUX, D>(st, sc, vt, ln, kbase, lo, lim, a.scale_log2e, next_v, next, vo, kept, row_keep, row_bits, sinks, seen);
         } else if constexpr (BITS == 16) {
             block_scores(sc, kt, qf, qlds, lane);
-            load_k<AUX>(kt, rk, next, ln, vo);
+            load_k<AUX>(kt, next_k, next, ln, vo);
             block_softmax_pv<D, NT>(st, sc, vt, ln, kbase, lo, lim, a.scale_log2e, kept, row_keep, row_bits, sinks, seen);
-            load_v<AUX>(vt, rv, next, ln, vo);
+            load_v<AUX>(vt, next_v, next, ln, vo);
         } else {  // the phases refill their tiles as they go
-            block_scores<AUX, D, NT, BITS>(sc, kt, qf, qlds, lane, rk, next, ln, vo);
-            block_softmax_pv<AUX, D, NT, BITS>(st, sc, vt, ln, kbase, lo, lim, a.scale_log2e, bias_acc, rv, next, vo, kept,
+            block_scores<AUX, D, NT, BITS>(sc, kt, qf, qlds, lane, next_k, next, ln, vo);
+            block_softmax_pv<AUX, D, NT, BITS>(st, sc, vt, ln, kbase, lo, lim, a.scale_log2e, bias_acc, next_v, next, vo, kept,
                                           row_keep, row_bits, sinks, seen);
         }
         if constexpr (KEEP == 1) {

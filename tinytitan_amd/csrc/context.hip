@@ -299,7 +299,7 @@ struct KeepLists {
 //   chunk_splits > 1 (kind 1, one sequence): the chunk kernel over chunk_splits key ranges of
 //   chunk_split_blocks blocks, then the combine pass.
 //   sinks >= 0: the keys [0, sinks) stay visible beside the window; pinned rows of a ring are known.  -1: neither.  With chunk_splits > 1
-//   chunk_pieces says so to the chunk kernel.
+//   chunk_pieces says so to the chunk kernel; its front piece (sinks 0, no window) is also the split-K kernel's.
 //   piece: the pass takes one piece of the rows' keys and leaves its partial results there, for launch_join (at most
 //   kMaxSeqPerLaunch sequences).
 struct KeyPiece {
@@ -576,6 +576,10 @@ static int run_attention(tt_hip_ctx *ctx, tt_hip_kv *kv, int kind, int layer, in
         h.keep_words = a.keep && (uintptr_t)a.keep % 4 == 0 && (n == 1 || keep_seq_stride % 4 == 0) &&
                        plan.split_len >= listed_blocks * plan.waves * 32;
         if (sinks >= 0) h.keep_words = sinks;
+        if (chunk_pieces && chunk_pieces->front_blocks > 0) {
+            h.keep_words = chunk_pieces->front_slot;
+            h.flags |= kHotFront | chunk_pieces->front_blocks << kHotPinnedShift;
+        }
         for (int i = 0; i < n; ++i) {
             a.seq[i].slot = walks_pages ? 0 : slots[base + i];
             a.seq[i].start = starts[base + i];
@@ -1230,39 +1234,66 @@ int tt_hip_attn_prefill(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int slot, int
                                    gate_stride, scale, out, o_stride);
 }
 
+// What 128 keys of a tile's walk (a block for each of its workgroup's wavefronts) take of a CU, us: their way out of L2, mostly, whatever their
+// bits, which over fewer of them is their widening.  And what partial results cost that are written and read back.
+static double turn_us(int D) { return 0.2 + 0.0057 * D; }
+static double partials_us(double rows, int D) { return rows * D * 8.0 / 2.5e6; }
+
 // Two passes in one launch: the tokens of all sequences over the keys [0, front) of prefix_slot, every sequence over its own from there on.
 // Both in tiles of the same rows and splits of at most the same length, which is the one that makes the launch's rounds the
-// cheapest: a round costs a split's keys and what a workgroup spends beside them, 5.5 D keys' worth (a pass of 18 rows of 24/2
-// heads of 256 over 12,320 keys in splits of 2,048 / 1,024 / 896 29.4 / 20.1 / 19.6 us, of 20 rows of 32/8 of 128 over 6,000 in 2,048 / 1,024 14.2 / 9.1).
-static int run_pieces(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, const int *slots, const int *starts, const int *totals, int rows,
-                      int prefix_slot, int front, int n_q_heads, const tt_half *q, long long q_seq_stride, long long q_tok_stride, float scale,
-                      PassParts *front_parts, PassParts *own_parts, int *first_split) {
+// cheapest (a pass of 18 rows of 24/2 heads of 256 over 12,320 keys in splits of 2,048 / 1,024 / 896 / 512 29.4 / 20.1 / 19.6 / 27.0 us, of 20 rows of
+// 32/8 of 128 over 6,000 in 2,048 / 1,024 / 512 14.2 / 9.1 / 10.2).
+struct PairPlan {
+    LaunchPlan tiles;
+    int own_tok_tiles, own_tiles, len;
+    double us;  // with the join behind it
+};
+static int splits_in(int keys, int len) { return std::max((keys + len - 1) / len, 1); }
+static int plan_pieces(const tt_hip_ctx *ctx, const tt_hip_kv *kv, int n_seq, const int *totals, int rows, int front, int n_q_heads, PairPlan *p) {
     const int D = kv->head_dim, tokens = n_seq * rows;
-    LaunchPlan plan{};
-    int st = plan_launch(ctx, 0, 1, n_q_heads, kv->n_kv_heads, D, tokens, front, front, front, &plan, kv->bits, true);
+    const int st = plan_launch(ctx, 0, 1, n_q_heads, kv->n_kv_heads, D, tokens, front, front, front, &p->tiles, kv->bits, true);
     if (st != TT_HIP_OK) return st;
-    const int per_token = plan.n_tiles / plan.tok_tiles, own_tok_tiles = (rows + plan.tt - 1) / plan.tt, own_tiles = per_token * own_tok_tiles;
-    auto splits_of = [&](int keys, int len) { return std::max((keys + len - 1) / len, 1); };
-    auto groups_of = [&](int len) {
+    const LaunchPlan &plan = p->tiles;
+    p->own_tok_tiles = (rows + plan.tt - 1) / plan.tt;
+    p->own_tiles = plan.n_tiles / plan.tok_tiles * p->own_tok_tiles;
+    // A workgroup beside its walk; over quantised pages a tile of 32 rows has registers for one workgroup a SIMD only, which then widens or multiplies.
+    const int slots_on_chip = ctx->n_cus * (plan.nt == 32 ? 256 / D : D == 256 ? 2 : 4);
+    const double fixed = plan.nt == 32 ? 1.5 + 0.0215 * D : 2.0 + 0.0098 * D;
+    const double turn = 1.1 * turn_us(D) * (kv->bits == 16 || plan.nt == 16 ? 1.0 : D == 256 ? 1.6 : 1.15), alone = plan.nt == 32 && D == 256 ? 1.0 : 0.6;
+    int longest = front;
+    double turns = (double)plan.n_tiles * ((front + 127) / 128);
+    for (int i = 0; i < n_seq; ++i) {
+        longest = std::max(longest, totals[i] - front);
+        turns += (double)p->own_tiles * ((totals[i] - front + 127) / 128);
+    }
+    auto us_of = [&](int len) {
         long long own = 0;
-        for (int i = 0; i < n_seq; ++i) own += splits_of(totals[i] - front, len);
-        return (long long)plan.n_tiles * splits_of(front, len) + own * own_tiles;
+        for (int i = 0; i < n_seq; ++i) own += splits_in(totals[i] - front, len);
+        const long long groups = (long long)plan.n_tiles * splits_in(front, len) + own * p->own_tiles, rounds = (groups + slots_on_chip - 1) / slots_on_chip;
+        const double part_rows = ((double)tokens * splits_in(front, len) + (double)rows * own) * n_q_heads;
+        return fixed * (1.0 + 0.7 * (rounds - 1)) + std::max(turns * turn / ctx->n_cus, (std::min(len, longest) + 127) / 128 * turn * alone) +
+               partials_us(part_rows, D) + 4.5;
     };
-    const long long slots_on_chip = (long long)ctx->n_cus * plan.slots_per_cu;
-    int longest = front, len = 0;
-    for (int i = 0; i < n_seq; ++i) longest = std::max(longest, totals[i] - front);
     if (ctx->split_override > 0) {
-        len = (ctx->split_override + 31) / 32 * 32;
-    } else {
-        long long best = 0;
-        for (int l = 128; l < longest + 128; l += std::max(128, l / 16 / 128 * 128)) {
-            const long long rounds = (groups_of(l) + slots_on_chip - 1) / slots_on_chip, cost = rounds * (std::min(l, longest) + 11 * D / 2);
-            if (len == 0 || cost < best) {
-                best = cost;
-                len = l;
-            }
+        p->len = (ctx->split_override + 31) / 32 * 32;
+        p->us = us_of(p->len);
+        return TT_HIP_OK;
+    }
+    p->len = 0;
+    for (int len = 128; len < longest + 128; len += std::max(128, len / 6 / 128 * 128)) {
+        const double us = us_of(len);
+        if (p->len == 0 || us < p->us) {
+            p->us = us;
+            p->len = len;
         }
     }
+    return TT_HIP_OK;
+}
+static int run_pieces(tt_hip_ctx *ctx, tt_hip_kv *kv, const PairPlan &pair, int layer, int n_seq, const int *slots, const int *starts,
+                      const int *totals, int rows, int prefix_slot, int front, int n_q_heads, const tt_half *q, long long q_seq_stride,
+                      long long q_tok_stride, float scale, PassParts *front_parts, PassParts *own_parts, JoinSeq *seqs) {
+    const LaunchPlan &plan = pair.tiles;
+    const int D = kv->head_dim, tokens = n_seq * rows, len = pair.len, own_tok_tiles = pair.own_tok_tiles, own_tiles = pair.own_tiles;
     SplitKPair a;
     std::memset(static_cast<void *>(&a), 0, sizeof(a));
     auto fill = [&](SplitKArgs &s, int pass_rows, int tok_tiles, int n_tiles, int flags, int n_splits) {
@@ -1288,7 +1319,7 @@ static int run_pieces(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, cons
         h.scale_log2e = scale * 1.4426950408889634f;
         for (int i = 0; i < kMaxSeqPerLaunch; ++i) s.seq[i].first_split = 0x7fffffff;
     };
-    const int front_splits = splits_of(front, len);
+    const int front_splits = splits_in(front, len);
     // (more than one split each as far as the kernel knows: it leaves partial results)
     fill(a, tokens, plan.tok_tiles, plan.n_tiles, kHotXcdGrid, std::max(front_splits, 2));
     a.seq[0] = SplitKSeq{prefix_slot, front, front, 0};  // (no row's own position limits what it sees of the shared keys)
@@ -1297,12 +1328,12 @@ static int run_pieces(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, cons
     a.own.hot.v_layer += front / kBlockTokens * (kv->block_bytes() / 2);
     int own_splits = 0;
     for (int i = 0; i < n_seq; ++i) {
-        first_split[i] = own_splits;
+        seqs[i].first_split = own_splits;
         a.own.seq[i] = SplitKSeq{slots[i], starts[i] - front, totals[i] - front, own_splits};
-        own_splits += splits_of(totals[i] - front, len);
+        own_splits += splits_in(totals[i] - front, len);
     }
     const size_t front_rows = (size_t)front_splits * plan.n_tiles * plan.nt, own_rows = (size_t)own_splits * own_tiles * plan.nt;
-    st = ensure_partials(ctx, front_rows + own_rows, D);
+    const int st = ensure_partials(ctx, front_rows + own_rows, D);
     if (st != TT_HIP_OK) return st;
     a.hot.part_o = ctx->part_o;
     a.hot.part_ml = ctx->part_ml;
@@ -1315,37 +1346,74 @@ static int run_pieces(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, cons
     return launch_splitk_pair(ctx, D, plan.nt, kv->bits, (unsigned)(a.front_groups + own_splits * own_tiles), a);
 }
 
-// Rows of sequences whose keys [0, front) -- whole blocks -- are another slot's rows: a pass over those with the tokens of all
-// sequences as rows of one, a pass over each sequence's own keys from there on, and the join.  The shared keys are then read once per
-// tile of rows, as a chunk's are, and not once per sequence.
+// Rows of sequences whose keys [0, front) -- whole blocks -- are another slot's, by the cheapest of three ways:
+//  * one pass: every sequence walks the shared keys like its own, out of the other slot's page; they are read once per sequence, mostly from L2;
+//  * two passes in one launch and a join: the shared keys are read once per tile of the tokens of ALL sequences, which fill tiles that
+//    one sequence's rows leave mostly empty;
+//  * the chunk kernel over ranges of the shared keys, whose copies in LDS four tiles read, a pass over the own keys, and the join.
+// At most kMaxSeqPerLaunch sequences.  One pass / two / ranges, us, one row a sequence of 16/2 heads of 256: 2 behind 200 keys 7.7 / 10.1 / 10.0, 2
+// behind 2,000 9.6 / 11.2 / 24, 20 behind 6,000 21.7 / 18.7 / 29.6, 64 behind 20,000 136 / 56.4 / 48.7; four rows a sequence, whose
+// own tiles are full: 64 behind 2,000 28.1 / 48.3 / 46.1, behind 20,000 140 / 147 / 104; 32/8 of 128 over 8 bits, 20 behind 6,000 57.4 / 19.1 / 32.4.
+// Over 480 such calls the estimates' choices take 7 % more than the best of the three would.
 static int run_shared(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, const int *slots, const int *starts, const int *totals, int rows,
                       int prefix_slot, int front, int n_q_heads, const tt_half *q, long long q_seq_stride, long long q_tok_stride,
                       const tt_half *gate, long long g_seq_stride, long long g_tok_stride, float scale, tt_half *out,
                       long long o_seq_stride, long long o_tok_stride) {
     if (hipSetDevice(ctx->device) != hipSuccess) return TT_HIP_ERR_HIP;
     const int D = kv->head_dim, tokens = n_seq * rows;
+    long long keys = 0;
+    int longest = 0;
+    for (int i = 0; i < n_seq; ++i) {
+        keys += totals[i];
+        longest = std::max(longest, totals[i]);
+    }
+    auto one_pass = [&] {
+        const ChunkPieces pieces{0, prefix_slot, front / kBlockTokens};
+        return run_attention(ctx, kv, 0, layer, n_seq, slots, starts, totals, rows, n_q_heads, q, q_seq_stride, q_tok_stride, gate, g_seq_stride,
+                             g_tok_stride, scale, out, o_seq_stride, o_tok_stride, 1, 0, nullptr, 0, nullptr, 0, 0, false, nullptr, 0, nullptr,
+                             &pieces);
+    };
+    if (n_seq == 1 || longest <= 384) return one_pass();  // (nobody to share with; one launch that ends in the final rows)
+    LaunchPlan alone{};
+    int st = plan_launch(ctx, 0, n_seq, n_q_heads, kv->n_kv_heads, D, rows, keys, longest, longest, &alone, kv->bits, true);
+    if (st != TT_HIP_OK) return st;
+    PairPlan pair{};
+    st = plan_pieces(ctx, kv, n_seq, totals, rows, front, n_q_heads, &pair);
+    if (st != TT_HIP_OK) return st;
+    // (one sequence's tiles walk apart from the others', but of a few rows; full tiles of 32 over heads of 256 wait for what they do not share)
+    const double key_us = (alone.nt == 32 && D == 256 ? 1.4 : 0.88) * turn_us(D) / ctx->n_cus / 128.0;  // of a tile
+    // (splits of equal length: as many a tile as one round of workgroups holds, which may leave CUs idle)
+    const long long tiles = (long long)n_seq * alone.n_tiles;
+    const double idle = keys == (long long)n_seq * longest && tiles <= ctx->n_cus ? (double)ctx->n_cus / (double)(ctx->n_cus / tiles * tiles) : 1.0;
+    const double alone_us = 7.5 + 0.006 * D + key_us * alone.n_tiles * (double)keys * idle;
     const bool aligned = aligned16(q) && q_tok_stride % 8 == 0;
-    const bool serves = prefill_kernel_serves(n_q_heads, kv->n_kv_heads, D, aligned) && scale > 0.0f;
-    // The shared keys: as behind a long context, the chunk kernel over ranges of the keys from some rows and keys on, else the split-K tiles.
-    const int rows_from = kv->bits == 16 ? (front >= 32768 ? 32 : 64) : 64;
-    const long long keys_from = std::max<long long>(786432 / tokens, kv->bits == 16 ? 4096 : 2560);
     KeyRanges ranges;
+    double ranges_us = 0.0;
+    if (prefill_kernel_serves(n_q_heads, kv->n_kv_heads, D, aligned) && scale > 0.0f) {
+        ranges = plan_key_ranges(ctx->n_cus, D, n_q_heads, kv->n_kv_heads, tokens, front / kBlockTokens);
+        ranges_us = ranges.us + 4.0 + 4.0 + key_us * alone.n_tiles * (double)(keys - (long long)n_seq * front) + 3.0;
+        // (quantised pages are dequantised once per call in front of the chunk kernel)
+        if (kv->bits != 16) ranges_us += 4.0 + (double)front * kv->n_kv_heads * D * (2.0 + kv->bits / 8.0) * 2.0 / 6.0e6;
+    }
+    if (alone_us <= pair.us && (ranges.n_splits < 2 || alone_us <= ranges_us)) return one_pass();
+    bool by_ranges = ranges.n_splits >= 2 && ranges_us < pair.us;
     PageSource staged{};
     const PageSource *pages = nullptr;
-    int st = TT_HIP_OK;
-    if (serves && tokens >= rows_from && front >= keys_from)
-        ranges = plan_key_ranges(ctx->n_cus, D, n_q_heads, kv->n_kv_heads, tokens, front / kBlockTokens);
-    if (ranges.n_splits >= 2 && kv->bits != 16) {
+    if (by_ranges && kv->bits != 16) {
         const size_t page = (size_t)front * D;
         st = ensure_stage(ctx, page * kv->n_kv_heads);
-        if (st == TT_HIP_OK) st = launch_kvq_dequant_blocks(kv, layer, prefix_slot, front / kBlockTokens, ctx->stage_k, ctx->stage_v, page);
-        else if (st == TT_HIP_ERR_BUSY || st == TT_HIP_ERR_OUT_OF_MEMORY) ranges.n_splits = 1, st = TT_HIP_OK;  // (the pages as they are)
+        if (st == TT_HIP_OK) {
+            st = launch_kvq_dequant_blocks(kv, layer, prefix_slot, front / kBlockTokens, ctx->stage_k, ctx->stage_v, page);
+            staged = PageSource{ctx->stage_k, ctx->stage_v, (long long)page, 0};
+            pages = &staged;
+        } else if (st == TT_HIP_ERR_BUSY || st == TT_HIP_ERR_OUT_OF_MEMORY) {
+            by_ranges = false;  // (no room for them, or none to be had inside a capture: the pages as they are)
+            st = TT_HIP_OK;
+        }
         if (st != TT_HIP_OK) return st;
-        staged = PageSource{ctx->stage_k, ctx->stage_v, (long long)page, 0};
-        pages = &staged;
     }
     JoinArgs j{};
-    if (ranges.n_splits >= 2) {
+    if (by_ranges) {
         KeyPiece shared{true}, own{false, front / kBlockTokens};
         st = run_attention(ctx, kv, 1, layer, 1, &prefix_slot, &front, &front, tokens, n_q_heads, q, 0, q_tok_stride, nullptr, 0, 0, scale, out, 0,
                            o_tok_stride, ranges.n_splits, ranges.split_blocks, pages, 0, nullptr, 0, 0, false, nullptr, -1, &shared);
@@ -1357,17 +1425,14 @@ static int run_shared(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, cons
         }
         st = run_attention(ctx, kv, 0, layer, n_seq, slots, own_starts, own_totals, rows, n_q_heads, q, q_seq_stride, q_tok_stride, nullptr, 0, 0,
                            scale, out, o_seq_stride, o_tok_stride, 1, 0, nullptr, 0, nullptr, 0, 0, false, nullptr, 0, &own);
-        if (st != TT_HIP_OK) return st;
         j.front = shared.parts;
         j.own = own.parts;
         for (int i = 0; i < n_seq; ++i) j.seq[i].first_split = own.first_split[i];
     } else {
-        int first_split[kMaxSeqPerLaunch];
-        st = run_pieces(ctx, kv, layer, n_seq, slots, starts, totals, rows, prefix_slot, front, n_q_heads, q, q_seq_stride, q_tok_stride, scale,
-                        &j.front, &j.own, first_split);
-        if (st != TT_HIP_OK) return st;
-        for (int i = 0; i < n_seq; ++i) j.seq[i].first_split = first_split[i];
+        st = run_pieces(ctx, kv, pair, layer, n_seq, slots, starts, totals, rows, prefix_slot, front, n_q_heads, q, q_seq_stride, q_tok_stride, scale,
+                        &j.front, &j.own, j.seq);
     }
+    if (st != TT_HIP_OK) return st;
     j.front_splits = std::max((front + j.front.split_len - 1) / j.front.split_len, 1);
     for (int i = 0; i < n_seq; ++i) {
         j.seq[i].start = starts[i] - front;

@@ -37,6 +37,8 @@ constexpr int kHotPackedSplits = 4;
 // A window with sinks: keep_words is the number of first tokens that stay visible, and from kHotPinnedShift on the flags hold the
 // blocks at the page's front that its ring leaves alone.
 constexpr int kHotSinks = 8, kHotPinnedShift = 8;
+// The same kernel for a prefix in another slot: keep_words is that slot, and from kHotPinnedShift on the flags hold the prefix's blocks.
+constexpr int kHotFront = 16;
 constexpr int kKeepSinks = 6;  // that kernel's KEEP (attn_splitk.hip)
 constexpr int kKeepPieces = 7;  // ... and of two passes in one launch, over the keys that sequences share and over their own
 struct SplitKHot {                         // dword
@@ -58,7 +60,7 @@ struct SplitKHot {                         // dword
     float scale_log2e;                     // 22
     int n_splits_max;                      // 23
     int n_tiles;                           // 24  n_kv_heads * hsubs * tok_tiles
-    int flags;                             // 25  kHotAligned | kHotXcdGrid | kHotPackedSplits | kHotSinks
+    int flags;                             // 25  kHotAligned | kHotXcdGrid | kHotPackedSplits | kHotSinks | kHotFront
     int keep_words;   // 26  (kHotSinks: the sinks) per-sequence masks start on 4-byte boundaries: a wavefront may read its blocks' bytes as words
     int gh_inv;       // 27  ceil(65536 / gh): (i * gh_inv) >> 16 == i / gh for 0 <= i < 64, gh <= 32
     float *part_o;    // 28  [first_split(seq) + split][tile][NT][D]

@@ -25,6 +25,10 @@ constexpr float kNegBig = -1.0e30f;
 // Row n of tile `tile` in split 0 of a pass, for token `tok` of a sequence and q head `head`.
 __device__ __forceinline__ size_t part_row(const PassParts &p, int group, int tok, int head) {
     const int kvh = head / group, in_group = head - kvh * group;
+    if (p.gh == 0) {
+        const int row = tok * group + in_group;
+        return (size_t)(kvh * p.tok_tiles + row / p.nt) * p.nt + row % p.nt;
+    }
     const int hsub = in_group / p.gh, tok_tile = tok / p.tt;
     const int tile = (kvh * p.hsubs + hsub) * p.tok_tiles + tok_tile;
     return (size_t)tile * p.nt + (tok - tok_tile * p.tt) * p.gh + (in_group - hsub * p.gh);

@@ -16,7 +16,9 @@
 // (sources/TinyTitanCore/Metal/Attention/attention.metal:162-269, :395-437) and,
 // for multi-row tiles, attention_prefill_causal_q8
 // (sources/TinyTitanCore/Metal/Prefill/prefill.metal:1172-1313).
+#include <algorithm>
 #include <type_traits>
+#include <utility>
 
 #include "chunk_plan.h"
 #include "internal.h"
@@ -1019,6 +1021,7 @@ __device__ __forceinline__ void block_softmax_pv(RowState<D, NT> &st, Scores<D, 
 // is mostly one block -- and a block's place is looked up from its number in the walk.
 // KEEP = kKeepPieces: the same kernel twice in a launch, over two pieces of the rows' keys with their own arguments (SplitKPair): what sequences
 // share and what is their own.  Neither fills the chip while the other waits for it, and there is one launch less.
+// KEEP = kKeepRows: the shared keys by front_rows, their own like that.
 // The hot arguments, this workgroup's sequence entry and where the rows go and their gate beside them, by five scalar loads issued
 // together (the compiler would fetch each field where it is first used: five or six dependent trips to the kernarg segment before
 // the first K/V load can go out, about 0.15 us each, and another ahead of the gate's loads).
@@ -1075,10 +1078,242 @@ __device__ __forceinline__ void load_row_words(unsigned (&dst)[8], __amdgpu_buff
     }
 }
 
+// ---------------------------------------------------------------------------
+// The keys that sequences share, over tiles of kFrontRows rows packed token by token (row r: token r / group, head r % group of
+// the KV head): every row sees every key, so nothing is masked and no tile has an order.
+//
+// Where the split-K tiles give a workgroup's four wavefronts four blocks of keys and the same 32 rows, here they have 32 rows each and one block:
+// it comes out of L2 once for 128 rows instead of four times, and a quantised one is widened once, into LDS, instead of in
+// each tile that walks it, which is what those tiles wait for (18 tokens of 24/2 heads of 256 over 12,320 keys over 4 bits 36 us, here 27).
+//
+// What bounds it: a block is 4 D / 32 MFMAs of 32 cycles a wavefront, and as many KiB that each of the four reads out of LDS at 128 bytes a
+// cycle between them, as long; the CU has one such workgroup with heads of 256 and nothing else to cover a wait.  So a block's scores are due one
+// block ahead, beside the softmax of the block before; operands are four products ahead of their use, the next block's stores and
+// widening lie between the products, and its loads are two blocks ahead, in registers.  LDS holds K of two blocks and V of two.  A block of
+// 128 rows of 256 takes 0.84 us (read, wait, multiply in turn 1.35; with the softmax between the products 0.91), over 4 bits 1.13 (1.67),
+// of 128 over fp16 / 8 bits 0.57 / 0.67.
+// ---------------------------------------------------------------------------
+template <int D, int BITS>
+struct FrontBlock {  // a thread's share of a block of K and V, as loaded
+    static constexpr int N = BITS == 16 ? D / 32 : D / 64;  // fp16 pieces of 16 bytes, or units of 16 values: K's, then V's
+    h8 piece[BITS == 16 ? N : 1];
+    unsigned levels[BITS == 16 ? 1 : N][BITS == 16 ? 1 : BITS / 2];
+    unsigned k_params[BITS == 16 ? 1 : N];
+    unsigned v_scale[BITS == 16 ? 1 : N][4], v_bias[BITS == 16 ? 1 : N][4];
+};
+// Unit i of this thread is one of V's (the same for a whole wavefront), and its number among K's or V's.
+template <int D, int BITS>
+__device__ __forceinline__ bool front_unit(int i, int wave, unsigned &u) {
+    constexpr unsigned HALF = BITS == 16 ? 4 * D : 2 * D;  // units of K, and of V
+    u = (unsigned)i * 256u + threadIdx.x;
+    bool is_v;
+    if constexpr (HALF >= 256) is_v = (unsigned)i * 256u >= HALF;
+    else is_v = wave >= (int)(HALF / 64);
+    if (is_v) u -= HALF;
+    return is_v;
+}
+template <int D, int BITS>
+__device__ __forceinline__ void front_load(FrontBlock<D, BITS> &f, __amdgpu_buffer_rsrc_t rk, __amdgpu_buffer_rsrc_t rv, int wave, unsigned k_block,
+                                           unsigned v_block) {
+    constexpr unsigned LEVELS = 32u * D * BITS / 8, GPH = D / 64;
+#pragma unroll
+    for (int i = 0; i < FrontBlock<D, BITS>::N; ++i) {
+        unsigned u;
+        const bool is_v = front_unit<D, BITS>(i, wave, u);
+        if constexpr (BITS == 16) {
+            f.piece[i] = buf_load_h8<0>(is_v ? rv : rk, u * 16u, is_v ? v_block : k_block);
+        } else {
+            buf_load_words<0>(f.levels[i], is_v ? rv : rk, u * (2u * BITS), is_v ? v_block : k_block);
+            if (is_v) {
+                const unsigned at = (u >> 7) * 64u + (u & 3u) * 16u;
+                buf_load_words<0>(f.v_scale[i], rv, at, v_block + LEVELS);
+                buf_load_words<0>(f.v_bias[i], rv, at, v_block + LEVELS + GPH * 64u);
+            } else {
+                f.k_params[i] = __builtin_amdgcn_raw_buffer_load_b32(rk, ((u & 31u) * GPH + (u >> 7)) * 4u, k_block + LEVELS, 0);
+            }
+        }
+    }
+}
+// ... into LDS, pieces or units FROM to TO of it: K fragment t of a score step at t KiB, V fragment (mt, t) at 2 mt + t KiB, each
+// [lane][8 halves].
+template <int D, int BITS, int FROM, int TO>
+__device__ __forceinline__ void front_store(const FrontBlock<D, BITS> &f, char *k_to, char *v_to, int wave) {
+    auto v_at = [&](unsigned d, unsigned chunk) { return v_to + (((d >> 5) * 2 + (chunk >> 1)) * 64 + (chunk & 1) * 32 + (d & 31)) * 16; };
+#pragma unroll
+    for (int i = FROM; i < TO; ++i) {
+        unsigned u;
+        const bool is_v = front_unit<D, BITS>(i, wave, u);
+        if constexpr (BITS == 16) {
+            if (is_v) {
+                const unsigned d = D == 256 ? (u >> 6) * 16 + (u & 15) : u >> 2, chunk = D == 256 ? (u >> 4) & 3 : u & 3;
+                *reinterpret_cast<h8 *>(v_at(d, chunk)) = f.piece[i];
+            } else {
+                *reinterpret_cast<h8 *>(k_to + u * 16) = f.piece[i];
+            }
+        } else if (is_v) {
+            h8 lo, hi;
+            v_run_operands<BITS>(f.levels[i], lo, hi);
+            const h8 scale = words_as_h8(f.v_scale[i]), bias = words_as_h8(f.v_bias[i]);
+            const unsigned d = (u >> 7) * 64 + ((u >> 2) & 31), chunk = u & 3;
+            *reinterpret_cast<h8 *>(v_at(d, chunk)) = lo * scale + bias;  // (a level and its product are exact in the multiply-add: one rounding)
+            *reinterpret_cast<h8 *>(v_at(d + 32, chunk)) = hi * scale + bias;
+        } else {
+            const unsigned key = u & 31, unit = u >> 5;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                *reinterpret_cast<h8 *>(k_to + ((2 * unit + h) * 32 + key) * 16) = k_unit_operand<BITS>(f.levels[i], h, f.k_params[i]);
+        }
+    }
+}
+
+// The order of a phase of MFMAS matrix products with an operand each out of LDS: FIRST reads, a read behind every product, of MFMAS + EXTRA in all, and of
+// the next block's way into LDS a little beside each.
+template <int FIRST, int MFMAS, int EXTRA, int BITS>
+__device__ __forceinline__ void reads_ahead() {
+    constexpr int BEHIND = MFMAS + EXTRA - FIRST;
+    __builtin_amdgcn_sched_group_barrier(0x100, FIRST, 0);
+    [&]<int... I>(std::integer_sequence<int, I...>) {
+        ((__builtin_amdgcn_sched_group_barrier(0x008, 1, 0), I < BEHIND ? __builtin_amdgcn_sched_group_barrier(0x100, 1, 0) : (void)0,
+          BITS == 16 ? (void)0 : __builtin_amdgcn_sched_group_barrier(0x002, 6, 0), __builtin_amdgcn_sched_group_barrier(0x200, 1, 0)),
+         ...);
+    }(std::make_integer_sequence<int, MFMAS>{});
+}
+
+constexpr int kFrontPitch = 36;  // floats of a row of 32 dims on its way out
+static constexpr size_t front_lds_bytes(int D) { return std::max<size_t>(2 * 128 * (size_t)D, 4 * 32 * kFrontPitch * sizeof(float)); }
+
+template <int D, int BITS>
+__device__ __forceinline__ void front_rows(const SplitKHot &a, const SplitKSeq &sq, unsigned group_id, char *smem) {
+    constexpr int KS = D / 16, MT = D / 32, N = FrontBlock<D, BITS>::N;
+    constexpr int HALF_BLOCK = 64 * D;  // bytes of a block of K or V as halves
+    constexpr int AHEAD = 4;            // operands on their way out of LDS
+    constexpr unsigned BLK_BYTES = BITS == 16 ? 32 * D * 2 : 32 * D * BITS / 8 + 32 * (D / 64) * 4;
+    // (range, tile) pairs XCD by XCD, tile fastest: tiles that walk the same keys meet in one L2
+    const unsigned pairs = (unsigned)a.n_tiles * (unsigned)a.n_splits_max, per_xcd = (pairs + 7u) >> 3;
+    const unsigned pair = (group_id & 7u) * per_xcd + (group_id >> 3);
+    if (pair >= pairs) return;
+    const int split = (int)(pair / (unsigned)a.n_tiles), tile = (int)(pair - (unsigned)split * (unsigned)a.n_tiles);
+    const int kvh = tile / a.tok_tiles, row0 = (tile - kvh * a.tok_tiles) * kFrontRows;
+    const int first = split * (a.split_len >> 5), nb = min(a.split_len >> 5, (sq.total >> 5) - first);
+    if (nb <= 0) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int li = lane & 31, g = lane >> 5;
+    const size_t page = ((size_t)sq.slot * a.n_kv_heads + kvh) * (size_t)a.page_elems;
+    const __amdgpu_buffer_rsrc_t rk = make_rsrc(a.k_layer + page, (unsigned)(a.page_elems * 2));
+    const __amdgpu_buffer_rsrc_t rv = make_rsrc(a.v_layer + page, (unsigned)(a.page_elems * 2));
+    const int n_rows = a.rows * a.group, row = row0 + wave * 32 + li;
+    const bool valid = row < n_rows;  // (a wavefront whose rows all are not multiplies zeros: a branch around its products would move its accumulators)
+    const int tok = (valid ? row : 0) / a.group, head = kvh * a.group + (valid ? row : 0) - tok * a.group;
+    const global_halves qp = (global_halves)(a.q + tok * a.q_tok_stride + (long long)head * D);
+    auto block_bytes = [&](int i) { return (unsigned)(first + min(max(i, 0), nb - 1)) * BLK_BYTES; };  // (past the range's last the last again)
+    // Frame i: V of block i and K of the next, whose scores are due while block i's softmax is worked out.
+    FrontBlock<D, BITS> even, odd;
+    auto load = [&](FrontBlock<D, BITS> &f, int i) { front_load<D, BITS>(f, rk, rv, wave, block_bytes(i + 1), block_bytes(i)); };
+    char *const k_lds = smem, *const v_lds = smem + 2 * HALF_BLOCK;
+    load(odd, -1);
+    load(even, 0);
+    h8 qf[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+        const h8 x = load_h8(qp + 16 * s + 8 * g);
+        qf[s] = valid ? x : (h8)(_Float16)0;
+    }
+    RowState<D, 32> st;
+    st.init();
+    front_store<D, BITS, 0, N>(odd, k_lds, v_lds + HALF_BLOCK, wave);
+    load(odd, 1);
+    front_store<D, BITS, 0, N>(even, k_lds + HALF_BLOCK, v_lds, wave);
+    __syncthreads();
+    f16v s = (f16v)0.0f;
+#pragma unroll
+    for (int t = 0; t < KS; ++t) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const h8 *>(k_lds + t * 1024 + lane * 16), qf[t], s, 0, 0, 0);
+    __syncthreads();
+    // Block i, with its scores in s: its softmax beside the next block's scores, then its values; and the next frame's way into LDS beside both.
+    auto step = [&](int here, const FrontBlock<D, BITS> &next) {
+        const char *const k_at = k_lds + (here ^ 1) * HALF_BLOCK + lane * 16, *const v_at = v_lds + here * HALF_BLOCK + lane * 16;
+        char *const k_to = k_lds + here * HALF_BLOCK, *const v_to = v_lds + (here ^ 1) * HALF_BLOCK;
+        f16v s_next = (f16v)0.0f;
+        h8 kf[KS], vf[2 * MT];  // (AHEAD of them in registers at a time)
+        Probs<D, 32> pr;
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int t = 0; t < KS; ++t) kf[t] = *reinterpret_cast<const h8 *>(k_at + t * 1024);
+#pragma unroll
+        for (int t = 0; t < AHEAD; ++t) vf[t] = *reinterpret_cast<const h8 *>(v_at + t * 1024);
+        front_store<D, BITS, 0, N / 2>(next, k_to, v_to, wave);
+#pragma unroll
+        for (int t = 0; t < KS; ++t) s_next = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[t], qf[t], s_next, 0, 0, 0);
+        float mx = kNegBig;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+            s[v] *= a.scale_log2e;
+            mx = fmaxf(mx, s[v]);
+        }
+        mx = max_across_halves(mx);
+        const float m_new = mx > st.m + kLazyRescaleHalfPages ? mx : st.m, alpha = fast_exp2(st.m - m_new);
+        float psum = 0.0f;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+            const float p = fast_exp2(s[v] - m_new);
+            psum += p;
+            pr.pf[v >> 3][v & 7] = (_Float16)p;
+        }
+        st.l = st.l * alpha + psum;
+        st.m = m_new;
+        reads_ahead<AHEAD, KS, AHEAD, BITS>();
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("" : "+v"(pr.pf[0]), "+v"(pr.pf[1]));  // (the compiler would work them out behind the branch, where no product covers it)
+        if (!__all(alpha == 1.0f)) {
+            rescale_settle();
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) rescale_tile(st.o[mt], alpha);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int t = AHEAD; t < 2 * MT; ++t) vf[t] = *reinterpret_cast<const h8 *>(v_at + t * 1024);
+        front_store<D, BITS, N / 2, N>(next, k_to, v_to, wave);
+#pragma unroll
+        for (int t = 0; t < 2 * MT; ++t) st.o[t / 2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[t], pr.pf[t & 1], st.o[t / 2], 0, 0, 0);
+        reads_ahead<0, 2 * MT, -AHEAD, BITS>();
+        __builtin_amdgcn_sched_barrier(0);
+        s = s_next;
+    };
+    for (int i = 0; i < nb; i += 2) {
+        load(even, i + 2);
+        step(0, odd);
+        __syncthreads();
+        if (i + 1 >= nb) break;
+        load(odd, i + 3);
+        step(1, even);
+        __syncthreads();
+    }
+    if (row0 + wave * 32 >= n_rows) return;
+    // The rows' states: 32 dims of 32 rows at a time through LDS (nobody reads a block any more), so that a store writes whole lines.
+    const float l = sum_across_halves(st.l);
+    const size_t out_row = ((size_t)split * a.n_tiles + tile) * kFrontRows + wave * 32;
+    if (valid && g == 0) {
+        a.part_ml[(out_row + li) * 2] = st.m;
+        a.part_ml[(out_row + li) * 2 + 1] = l;
+    }
+    float *const stage = reinterpret_cast<float *>(smem) + wave * (32 * kFrontPitch);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+        for (int vq = 0; vq < 4; ++vq)
+            *reinterpret_cast<f4 *>(stage + li * kFrontPitch + 8 * vq + 4 * g) = f4{st.o[mt][4 * vq], st.o[mt][4 * vq + 1], st.o[mt][4 * vq + 2], st.o[mt][4 * vq + 3]};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int r = 8 * k + (lane >> 3), d = (lane & 7) * 4;
+            const f4 x = *reinterpret_cast<const f4 *>(stage + r * kFrontPitch + d);
+            if (row0 + wave * 32 + r < n_rows) *reinterpret_cast<f4 *>(a.part_o + (out_row + r) * D + 32 * mt + d) = x;
+        }
+    }
+}
+
 template <int D, int NT, int WAVES, int BITS, int KEEP = 0, int STREAM = 0>
-__global__ __launch_bounds__(WAVES * 64, (NT == 16 && (KEEP < 2 || KEEP >= kKeepSinks) ? 2 : 1)) void
-    attn_splitk_kernel(const std::conditional_t<KEEP == kKeepPieces, SplitKPair, SplitKArgs> args) {
-    constexpr bool PAIR = KEEP == kKeepPieces;
+__global__ __launch_bounds__(WAVES * 64, ((NT == 16 && (KEEP < 2 || KEEP == kKeepSinks || KEEP == kKeepPieces)) || (KEEP == kKeepRows && D < 256) ? 2 : 1)) void
+    attn_splitk_kernel(const std::conditional_t<KEEP >= kKeepPieces, SplitKPair, SplitKArgs> args) {
+    constexpr bool PAIR = KEEP >= kKeepPieces;
     constexpr bool PAIRED = STREAM == 2;
     static_assert(!PAIRED || (D == 256 && NT == 32 && BITS == 16 && KEEP == 0));
     constexpr int AUX = (STREAM ? kStreamed : 0) | (PAIRED ? kPaired : 0);
@@ -1103,6 +1338,12 @@ __global__ __launch_bounds__(WAVES * 64, (NT == 16 && (KEEP < 2 || KEEP >= kKeep
     SplitKSeq sq;
     SplitKOut out;
     load_args(a, sq, out, seq, args_at);
+    if constexpr (KEEP == kKeepRows) {
+        if (args_at == 0) {
+            front_rows<D, BITS>(a, sq, group, reinterpret_cast<char *>(lds));
+            return;
+        }
+    }
     int split = (int)group, tile = PAIR ? 0 : blockIdx.y;
     if constexpr (PAIR) {
         if (args_at != 0) {  // (tile fastest)
@@ -1991,7 +2232,8 @@ static int launch_one(tt_hip_ctx *ctx, const LaunchPlan &plan, int n_seq, const 
 template <int D, int NT, int BITS, int KEEP>
 static hipError_t configure_one() {
     hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(attn_splitk_kernel<D, NT, 4, BITS, KEEP, 0>),
-                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)(lds_bytes_for(D, NT, 4) + keep_list_bytes(KEEP, 4)));
+                                       hipFuncAttributeMaxDynamicSharedMemorySize,
+                                       (int)std::max(lds_bytes_for(D, NT, 4) + keep_list_bytes(KEEP, 4), KEEP == kKeepRows ? front_lds_bytes(D) : 0));
     if constexpr (D == 256 && NT == 32 && BITS == 16 && KEEP == 0) {
         if (e == hipSuccess)
             e = hipFuncSetAttribute(reinterpret_cast<const void *>(attn_splitk_kernel<D, NT, 4, BITS, KEEP, 2>),
@@ -2018,6 +2260,7 @@ static hipError_t configure_tile() {
     if constexpr (lists_fetch_by_key(D, 16)) { TT_CFG(16, 5) }
     TT_CFG(16, kKeepSinks) TT_CFG(8, kKeepSinks) TT_CFG(4, kKeepSinks)
     TT_CFG(16, kKeepPieces) TT_CFG(8, kKeepPieces) TT_CFG(4, kKeepPieces)
+    TT_CFG(16, kKeepRows) TT_CFG(8, kKeepRows) TT_CFG(4, kKeepRows)
 #undef TT_CFG
     return e;
 }
@@ -2048,13 +2291,19 @@ int launch_combine(tt_hip_ctx *ctx, const LaunchPlan &plan, int head_dim, int n_
     return TT_HIP_ERR_SHAPE;
 }
 
-int launch_splitk_pair(tt_hip_ctx *ctx, int head_dim, int nt, int kv_bits, unsigned groups, const SplitKPair &args) {
+int launch_splitk_pair(tt_hip_ctx *ctx, int head_dim, int nt, int kv_bits, bool packed_rows, unsigned groups, const SplitKPair &args) {
     auto launch = [&](auto kernel) {
-        launch_profiled(ctx, kernel, dim3(groups), dim3(256), (unsigned)lds_bytes_for(head_dim, nt, 4), args);
+        const size_t lds = std::max(lds_bytes_for(head_dim, nt, 4), packed_rows ? front_lds_bytes(head_dim) : 0);
+        launch_profiled(ctx, kernel, dim3(groups), dim3(256), (unsigned)lds, args);
         const hipError_t e = hipGetLastError();
         return e == hipSuccess ? (int)TT_HIP_OK : hip_fail(ctx, e, "attn_splitk_kernel launch");
     };
 #define TT_CASE(DD, NN)                                                                  \
+    if (head_dim == DD && nt == NN && packed_rows) {                                     \
+        if (kv_bits == 16) return launch(attn_splitk_kernel<DD, NN, 4, 16, kKeepRows>);  \
+        if (kv_bits == 8) return launch(attn_splitk_kernel<DD, NN, 4, 8, kKeepRows>);    \
+        if (kv_bits == 4) return launch(attn_splitk_kernel<DD, NN, 4, 4, kKeepRows>);    \
+    }                                                                                    \
     if (head_dim == DD && nt == NN) {                                                    \
         if (kv_bits == 16) return launch(attn_splitk_kernel<DD, NN, 4, 16, kKeepPieces>); \
         if (kv_bits == 8) return launch(attn_splitk_kernel<DD, NN, 4, 8, kKeepPieces>);   \

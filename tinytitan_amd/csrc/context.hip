@@ -466,13 +466,16 @@ static int run_attention(tt_hip_ctx *ctx, tt_hip_kv *kv, int kind, int layer, in
         // A chunk's token tiles over several key ranges: workgroups that share an XCD share the K/V blocks of a range.  Over index lists also with
         // one range: a KV head's tiles, one behind the other on the XCDs, were in all of their L2s (32/8 heads of 128, 256 rows behind 100k keys
         // 644 -> 418 us a sparse layer's step, behind 60k 400 -> 328; 16/2 of 256, 500 rows 418 -> 301 and 291 -> 252).
-        plan.xcd_grid = ctx->xcd_grid && chunk_splits <= 1 && plan.tok_tiles > 1 && (plan.n_splits_max > 1 || lists) && !ragged;
+        // (not where several sequences walk one prefix and pairs are left over: their XCDs are the same for every sequence)
+        const bool shared_front = chunk_pieces && chunk_pieces->front_blocks > 0 && n > 1;
+        plan.xcd_grid = ctx->xcd_grid && chunk_splits <= 1 && plan.tok_tiles > 1 && (plan.n_splits_max > 1 || lists) && !ragged &&
+                        !(shared_front && (long long)plan.n_splits_max * plan.n_tiles % 8 != 0);
         // Pages that the launch reads once -- one tile per KV head, as in a decode step or a verify pass of a few
         // rows -- are loaded non-temporal once there are enough of them that they would not survive in the
         // 256 MiB memory-side cache until the same layer's next step anyway (16 MiB a launch: sixteen layers of it).
         {
             const long long kv_bytes = total_keys * (long long)kv->n_kv_heads * (long long)(kv->block_bytes() / kBlockTokens) * 2;
-            plan.stream = plan.tok_tiles == 1 && plan.hsubs == 1 && chunk_splits <= 1 && keep_row_stride == 0 &&
+            plan.stream = plan.tok_tiles == 1 && plan.hsubs == 1 && chunk_splits <= 1 && keep_row_stride == 0 && !shared_front &&
                           (ctx->stream_override < 0 ? kv_bytes >= (16ll << 20) : ctx->stream_override != 0);
             // V operands in pairs where every CU has a workgroup of its own for the whole of a long launch, which is then what the memory
             // gives (8 sequences x 4 rows of 16/2 heads behind 64k keys, 1 GiB, 179.0 -> 173.8 us a step; behind 45,678, 0.7 GiB,
@@ -1234,45 +1237,75 @@ int tt_hip_attn_prefill(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int slot, int
                                    gate_stride, scale, out, o_stride);
 }
 
-// What 128 keys of a tile's walk (a block for each of its workgroup's wavefronts) take of a CU, us: their way out of L2, mostly, whatever their
-// bits, which over fewer of them is their widening.  And what partial results cost that are written and read back.
-static double turn_us(int D) { return 0.2 + 0.0057 * D; }
+// What the ways of a shared-prefix call are estimated to take, in us: fitted to calls of 2 .. 64 sequences of 1 and 4 rows behind 700 .. 20,000
+// keys, of 16/4 heads of 64, 32/8 of 128, 16/2 and 24/2 of 256 over 16, 8 and 4 bits, where what they choose takes 3 % more than the best way.
+// 128 keys of a tile's walk (a block for each of its workgroup's wavefronts): their way out of L2, mostly, whatever their
+// bits, and over fewer of them the 32-row tiles' widening.
+static double turn_us(int D, int nt, int bits) {
+    return (0.2 + 0.0057 * D) * (bits == 16 || nt == 16 ? 1.0 : D == 256 ? 1.6 : 1.15);
+}
+// A workgroup beside its walk, and how many of them a CU holds.
+static double start_us(int D, int nt) { return nt == 32 ? 1.5 + 0.0215 * D : 2.0 + 0.0098 * D; }
+static int groups_per_cu(int D, int nt) { return nt == 32 ? 256 / D : D == 256 ? 2 : 4; }
+// Partial results that are written and read back.
 static double partials_us(double rows, int D) { return rows * D * 8.0 / 2.5e6; }
 
 // Two passes in one launch: the tokens of all sequences over the keys [0, front) of prefix_slot, every sequence over its own from there on.
-// Both in tiles of the same rows and splits of at most the same length, which is the one that makes the launch's rounds the
-// cheapest (a pass of 18 rows of 24/2 heads of 256 over 12,320 keys in splits of 2,048 / 1,024 / 896 / 512 29.4 / 20.1 / 19.6 / 27.0 us, of 20 rows of
-// 32/8 of 128 over 6,000 in 2,048 / 1,024 / 512 14.2 / 9.1 / 10.2).
+// The shared keys in the split-K tiles of 16 or 32 rows or in tiles of 128 packed ones, the own keys in split-K tiles, both in splits of at
+// most the same length, the one that makes the launch the cheapest (64 rows of 16/2 heads of 256 over 30,011 keys and 50 .. 2,000 of their
+// own, packed, in splits of 256 / 512 / 960 / 1,536 / 2,048 113 / 84 / 79 / 67 / 74 us, with the join; 20 of 32/8 of 128 over 6,000 over 8 bits, not
+// packed, in 128 / 512 / 1,024 / 2,048 26 / 17.6 / 17.4 / 23.6).
 struct PairPlan {
     LaunchPlan tiles;
+    bool packed_rows;  // the shared keys by tiles of kFrontRows packed rows (attn_splitk.hip); tiles.nt and .tt are those of the own keys' tiles
     int own_tok_tiles, own_tiles, len;
     double us;  // with the join behind it
 };
 static int splits_in(int keys, int len) { return std::max((keys + len - 1) / len, 1); }
-static int plan_pieces(const tt_hip_ctx *ctx, const tt_hip_kv *kv, int n_seq, const int *totals, int rows, int front, int n_q_heads, PairPlan *p) {
+static int plan_pieces(const tt_hip_ctx *ctx, const tt_hip_kv *kv, int n_seq, const int *totals, int rows, int front, int n_q_heads,
+                       bool packed_rows, PairPlan *p) {
     const int D = kv->head_dim, tokens = n_seq * rows;
-    const int st = plan_launch(ctx, 0, 1, n_q_heads, kv->n_kv_heads, D, tokens, front, front, front, &p->tiles, kv->bits, true);
+    const int st = plan_launch(ctx, 0, 1, n_q_heads, kv->n_kv_heads, D, packed_rows ? rows : tokens, front, front, front, &p->tiles, kv->bits, true);
     if (st != TT_HIP_OK) return st;
-    const LaunchPlan &plan = p->tiles;
+    LaunchPlan &plan = p->tiles;
+    p->packed_rows = packed_rows;
     p->own_tok_tiles = (rows + plan.tt - 1) / plan.tt;
     p->own_tiles = plan.n_tiles / plan.tok_tiles * p->own_tok_tiles;
-    // A workgroup beside its walk; over quantised pages a tile of 32 rows has registers for one workgroup a SIMD only, which then widens or multiplies.
-    const int slots_on_chip = ctx->n_cus * (plan.nt == 32 ? 256 / D : D == 256 ? 2 : 4);
-    const double fixed = plan.nt == 32 ? 1.5 + 0.0215 * D : 2.0 + 0.0098 * D;
-    const double turn = 1.1 * turn_us(D) * (kv->bits == 16 || plan.nt == 16 ? 1.0 : D == 256 ? 1.6 : 1.15), alone = plan.nt == 32 && D == 256 ? 1.0 : 0.6;
-    int longest = front;
-    double turns = (double)plan.n_tiles * ((front + 127) / 128);
-    for (int i = 0; i < n_seq; ++i) {
-        longest = std::max(longest, totals[i] - front);
-        turns += (double)p->own_tiles * ((totals[i] - front + 127) / 128);
+    if (packed_rows) {
+        plan.tok_tiles = (tokens * (n_q_heads / kv->n_kv_heads) + kFrontRows - 1) / kFrontRows;
+        plan.n_tiles = plan.tok_tiles * kv->n_kv_heads;
     }
+    const int slots_on_chip = ctx->n_cus * groups_per_cu(D, packed_rows ? 32 : plan.nt);
+    const double fixed = start_us(D, packed_rows ? 32 : plan.nt), turn = turn_us(D, plan.nt, kv->bits);
+    long long own_keys = 0, own_turns = 0;
+    int longest_own = 0;
+    for (int i = 0; i < n_seq; ++i) {
+        const int own = totals[i] - front;
+        longest_own = std::max(longest_own, own);
+        own_keys += own;
+        own_turns += (own + 127) / 128;
+    }
+    // (packed rows: a block of keys a step; the workgroups of a CU hide some of each other's)
+    const int per_cu = groups_per_cu(D, 32);
+    const double step = (0.3 + 0.0021 * D) * (kv->bits == 16 ? 1.0 : 1.0 + 0.0013 * D);
+    const double shared_step = step * (per_cu == 1 ? 1.0 : per_cu == 2 ? 1.2 : 1.8);
+    const double walk_us = 1.36 * ((double)plan.n_tiles * ((front + 127) / 128) + (double)own_turns * p->own_tiles) * turn / ctx->n_cus;
+    const double turn_alone = 0.36 + 0.005 * D;
+    const int longest = std::max(front, longest_own);
     auto us_of = [&](int len) {
-        long long own = 0;
-        for (int i = 0; i < n_seq; ++i) own += splits_in(totals[i] - front, len);
-        const long long groups = (long long)plan.n_tiles * splits_in(front, len) + own * p->own_tiles, rounds = (groups + slots_on_chip - 1) / slots_on_chip;
-        const double part_rows = ((double)tokens * splits_in(front, len) + (double)rows * own) * n_q_heads;
-        return fixed * (1.0 + 0.7 * (rounds - 1)) + std::max(turns * turn / ctx->n_cus, (std::min(len, longest) + 127) / 128 * turn * alone) +
-               partials_us(part_rows, D) + 4.5;
+        const double own = n_seq + (longest_own > len ? (double)(own_keys / len) : 0.0);  // (splits of own keys, or a few more)
+        const double front_groups = (double)plan.n_tiles * splits_in(front, len), groups = front_groups + own * p->own_tiles;
+        const double rounds = std::ceil(groups / slots_on_chip), part_rows = ((double)tokens * splits_in(front, len) + rows * own) * n_q_heads;
+        if (packed_rows) {
+            // The workgroups over shared keys start first, those over own keys take the places that they leave.
+            const int steps = std::min(len, front) / 32;
+            const double own_group = 0.35 * fixed + (0.13 + 0.0023 * D) * ((std::min(len, longest_own) + 127) / 128);
+            const double busy = (front_groups * (0.57 * fixed + steps * shared_step) + own * p->own_tiles * own_group) / slots_on_chip;
+            const double walk = std::max(std::ceil(front_groups / slots_on_chip) * (0.57 * fixed + steps * step), busy + 1.8 * own_group);
+            return 7.5 + 0.0016 * tokens * n_q_heads + walk + 0.48 * partials_us(part_rows, D);
+        }
+        return 6.6 + fixed * (0.16 + 0.84 * rounds) + std::max(walk_us, (std::min(len, longest) + 127) / 128 * turn_alone) +
+               0.2 * partials_us(part_rows, D);
     };
     if (ctx->split_override > 0) {
         p->len = (ctx->split_override + 31) / 32 * 32;
@@ -1280,7 +1313,8 @@ static int plan_pieces(const tt_hip_ctx *ctx, const tt_hip_kv *kv, int n_seq, co
         return TT_HIP_OK;
     }
     p->len = 0;
-    for (int len = 128; len < longest + 128; len += std::max(128, len / 6 / 128 * 128)) {
+    const int finest = packed_rows ? 32 : 128;
+    for (int len = 128; len < longest + finest; len += std::max(finest, len / 8 / finest * finest)) {
         const double us = us_of(len);
         if (p->len == 0 || us < p->us) {
             p->us = us;
@@ -1296,6 +1330,7 @@ static int run_pieces(tt_hip_ctx *ctx, tt_hip_kv *kv, const PairPlan &pair, int 
     const int D = kv->head_dim, tokens = n_seq * rows, len = pair.len, own_tok_tiles = pair.own_tok_tiles, own_tiles = pair.own_tiles;
     SplitKPair a;
     std::memset(static_cast<void *>(&a), 0, sizeof(a));
+    const int front_nt = pair.packed_rows ? kFrontRows : plan.nt;
     auto fill = [&](SplitKArgs &s, int pass_rows, int tok_tiles, int n_tiles, int flags, int n_splits) {
         SplitKHot &h = s.hot;
         h.k_layer = kv->k[layer];
@@ -1332,7 +1367,7 @@ static int run_pieces(tt_hip_ctx *ctx, tt_hip_kv *kv, const PairPlan &pair, int 
         a.own.seq[i] = SplitKSeq{slots[i], starts[i] - front, totals[i] - front, own_splits};
         own_splits += splits_in(totals[i] - front, len);
     }
-    const size_t front_rows = (size_t)front_splits * plan.n_tiles * plan.nt, own_rows = (size_t)own_splits * own_tiles * plan.nt;
+    const size_t front_rows = (size_t)front_splits * plan.n_tiles * front_nt, own_rows = (size_t)own_splits * own_tiles * plan.nt;
     const int st = ensure_partials(ctx, front_rows + own_rows, D);
     if (st != TT_HIP_OK) return st;
     a.hot.part_o = ctx->part_o;
@@ -1341,20 +1376,25 @@ static int run_pieces(tt_hip_ctx *ctx, tt_hip_kv *kv, const PairPlan &pair, int 
     a.own.hot.part_ml = ctx->part_ml + front_rows * 2;
     auto parts = [&](const SplitKHot &h) { return PassParts{h.part_o, h.part_ml, plan.nt, plan.gh, plan.tt, plan.hsubs, h.tok_tiles, h.n_tiles, len}; };
     *front_parts = parts(a.hot);
+    if (pair.packed_rows) {
+        front_parts->nt = kFrontRows;
+        front_parts->gh = 0;
+    }
     *own_parts = parts(a.own.hot);
     a.front_groups = (int)(((long long)plan.n_tiles * a.hot.n_splits_max + 7) / 8 * 8);
-    return launch_splitk_pair(ctx, D, plan.nt, kv->bits, (unsigned)(a.front_groups + own_splits * own_tiles), a);
+    return launch_splitk_pair(ctx, D, plan.nt, kv->bits, pair.packed_rows, (unsigned)(a.front_groups + own_splits * own_tiles), a);
 }
 
-// Rows of sequences whose keys [0, front) -- whole blocks -- are another slot's, by the cheapest of three ways:
+// Rows of sequences whose keys [0, front) -- whole blocks -- are another slot's, by the cheapest of four ways:
 //  * one pass: every sequence walks the shared keys like its own, out of the other slot's page; they are read once per sequence, mostly from L2;
-//  * two passes in one launch and a join: the shared keys are read once per tile of the tokens of ALL sequences, which fill tiles that
-//    one sequence's rows leave mostly empty;
-//  * the chunk kernel over ranges of the shared keys, whose copies in LDS four tiles read, a pass over the own keys, and the join.
-// At most kMaxSeqPerLaunch sequences.  One pass / two / ranges, us, one row a sequence of 16/2 heads of 256: 2 behind 200 keys 7.7 / 10.1 / 10.0, 2
-// behind 2,000 9.6 / 11.2 / 24, 20 behind 6,000 21.7 / 18.7 / 29.6, 64 behind 20,000 136 / 56.4 / 48.7; four rows a sequence, whose
-// own tiles are full: 64 behind 2,000 28.1 / 48.3 / 46.1, behind 20,000 140 / 147 / 104; 32/8 of 128 over 8 bits, 20 behind 6,000 57.4 / 19.1 / 32.4.
-// Over 480 such calls the estimates' choices take 7 % more than the best of the three would.
+//  * two passes in one launch and a join, the shared keys by split-K tiles, which the tokens of ALL sequences fill that one
+//    sequence's rows leave mostly empty;
+//  * the same, the shared keys by tiles of 128 packed rows: for more rows than a split-K tile has;
+//  * the chunk kernel over ranges of the shared keys, its scores and values on wavefronts of their own, a pass over the own keys, and the join.
+// At most kMaxSeqPerLaunch sequences.  One pass / two / two with packed rows / ranges, us, 100 own keys: one row a sequence of 16/2 heads of
+// 256, 2 behind 2,000 9.1 / 11.0 / 13.3 / 24, 20 behind 6,000 18.3 / 16.3 / 23.5 / 29.5, 64 behind 20,000 92.8 / 44.9 / 44.0 / 47.7; 24/2 heads over 4
+// bits, 20 behind 20,000 60 / 80 / 39 / 51; 32/8 of 128 over 8 bits, 20 behind 6,000 56 / 18.9 / 20.1 / 32.6, behind 20,000 177 / 44.5 / 33.2 / 57.7; four
+// rows a sequence, 64 of 24/2 of 256 behind 2,000 39.4 / 91.6 / 50.4 / 56.6, behind 20,000 267 / 290 / 160 / 153.
 static int run_shared(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, const int *slots, const int *starts, const int *totals, int rows,
                       int prefix_slot, int front, int n_q_heads, const tt_half *q, long long q_seq_stride, long long q_tok_stride,
                       const tt_half *gate, long long g_seq_stride, long long g_tok_stride, float scale, tt_half *out,
@@ -1377,21 +1417,25 @@ static int run_shared(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, cons
     LaunchPlan alone{};
     int st = plan_launch(ctx, 0, n_seq, n_q_heads, kv->n_kv_heads, D, rows, keys, longest, longest, &alone, kv->bits, true);
     if (st != TT_HIP_OK) return st;
-    PairPlan pair{};
-    st = plan_pieces(ctx, kv, n_seq, totals, rows, front, n_q_heads, &pair);
+    PairPlan pair{}, packed{};
+    st = plan_pieces(ctx, kv, n_seq, totals, rows, front, n_q_heads, false, &pair);
+    if (st == TT_HIP_OK) st = plan_pieces(ctx, kv, n_seq, totals, rows, front, n_q_heads, true, &packed);
     if (st != TT_HIP_OK) return st;
-    // (one sequence's tiles walk apart from the others', but of a few rows; full tiles of 32 over heads of 256 wait for what they do not share)
-    const double key_us = (alone.nt == 32 && D == 256 ? 1.4 : 0.88) * turn_us(D) / ctx->n_cus / 128.0;  // of a tile
-    // (splits of equal length: as many a tile as one round of workgroups holds, which may leave CUs idle)
-    const long long tiles = (long long)n_seq * alone.n_tiles;
-    const double idle = keys == (long long)n_seq * longest && tiles <= ctx->n_cus ? (double)ctx->n_cus / (double)(ctx->n_cus / tiles * tiles) : 1.0;
-    const double alone_us = 7.5 + 0.006 * D + key_us * alone.n_tiles * (double)keys * idle;
+    if (packed.us < pair.us) pair = packed;
+    const double turn = turn_us(D, alone.nt, kv->bits), key_us = 0.9 * turn / ctx->n_cus / 128.0;  // of a tile
+    long long splits = 0;
+    for (int i = 0; i < n_seq; ++i) splits += splits_in(totals[i], alone.split_len);
+    const bool joined = longest > alone.split_len;
+    const double rounds = std::ceil((double)splits * alone.n_tiles / (ctx->n_cus * groups_per_cu(D, alone.nt)));
+    const double alone_us = 2.9 + start_us(D, alone.nt) * (0.45 + 0.5 * rounds) +
+                            std::max(key_us * alone.n_tiles * (double)keys, (std::min(alone.split_len, longest) + 127) / 128 * 0.8 * turn) +
+                            (joined ? 1.6 + 0.75 * partials_us((double)splits * rows * n_q_heads, D) : 0.0);
     const bool aligned = aligned16(q) && q_tok_stride % 8 == 0;
     KeyRanges ranges;
     double ranges_us = 0.0;
     if (prefill_kernel_serves(n_q_heads, kv->n_kv_heads, D, aligned) && scale > 0.0f) {
         ranges = plan_key_ranges(ctx->n_cus, D, n_q_heads, kv->n_kv_heads, tokens, front / kBlockTokens);
-        ranges_us = ranges.us + 4.0 + 4.0 + key_us * alone.n_tiles * (double)(keys - (long long)n_seq * front) + 3.0;
+        ranges_us = ranges.us + 4.0 + 4.0 + key_us * alone.n_tiles * (double)(keys - (long long)n_seq * front) + 7.0;
         // (quantised pages are dequantised once per call in front of the chunk kernel)
         if (kv->bits != 16) ranges_us += 4.0 + (double)front * kv->n_kv_heads * D * (2.0 + kv->bits / 8.0) * 2.0 / 6.0e6;
     }

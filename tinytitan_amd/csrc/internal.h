@@ -41,6 +41,8 @@ constexpr int kHotSinks = 8, kHotPinnedShift = 8;
 constexpr int kHotFront = 16;
 constexpr int kKeepSinks = 6;  // that kernel's KEEP (attn_splitk.hip)
 constexpr int kKeepPieces = 7;  // ... and of two passes in one launch, over the keys that sequences share and over their own
+constexpr int kKeepRows = 8;    // ... with the first of them over tiles of kFrontRows packed rows, whose wavefronts share a block of keys in LDS
+constexpr int kFrontRows = 128;
 struct SplitKHot {                         // dword
     const _Float16 *k_layer;               //  0
     const _Float16 *v_layer;               //  2
@@ -124,7 +126,7 @@ struct LaunchPlan {
     bool partials_only;  // the partial results are somebody else's to combine (PassParts)
 };
 
-// Two passes in one launch (kKeepPieces): workgroups [0, front_groups) are those of the base's, a chunk's token tiles dealt out XCD by XCD
+// Two passes in one launch (kKeepPieces, kKeepRows): workgroups [0, front_groups) are those of the base's, a chunk's token tiles dealt out XCD by XCD
 // (kHotXcdGrid), the others, tile fastest, the packed splits of `own` (kHotPackedSplits).
 struct alignas(64) SplitKPair : SplitKArgs {
     SplitKArgs own;
@@ -136,7 +138,7 @@ static_assert(sizeof(SplitKPair) == 2 * sizeof(SplitKArgs) + 64, "`own` right be
 // ((first_split(sequence) + split) * n_tiles + tile) * nt + n, D floats of `o` and a (maximum, sum) pair of `ml`.
 struct PassParts {
     const float *o, *ml;
-    int nt, gh, tt, hsubs, tok_tiles, n_tiles;
+    int nt, gh, tt, hsubs, tok_tiles, n_tiles;  // gh 0: tiles of nt packed rows, token by token the heads that share a KV head, tok_tiles of them a KV head
     int split_len;  // keys of a split; a tile of a sequence has as many splits as its last row's keys need, one at least
 };
 // A sequence of a join: its own piece of the keys as the pass over that saw it.
@@ -287,8 +289,8 @@ struct PageSource {
 int plan_launch(const tt_hip_ctx *ctx, int kind, int n_seq, int n_q_heads, int n_kv_heads, int head_dim, int rows,
                 long long total_keys, int min_keys, int max_keys, LaunchPlan *plan, int kv_bits = 16, bool small_tiles_ok = false);
 
-// A launch of a pair (nt: its tiles' rows, groups: its workgroups in all).
-int launch_splitk_pair(tt_hip_ctx *ctx, int head_dim, int nt, int kv_bits, unsigned groups, const SplitKPair &args);
+// A launch of a pair (nt: the rows of its tiles, or of those of `own` where the shared keys go by packed rows; groups: its workgroups in all).
+int launch_splitk_pair(tt_hip_ctx *ctx, int head_dim, int nt, int kv_bits, bool packed_rows, unsigned groups, const SplitKPair &args);
 
 // kv_bits: 16 for fp16 pages, 8 / 4 for quantised ones.
 int launch_splitk(tt_hip_ctx *ctx, const LaunchPlan &plan, int head_dim, int n_seq, const SplitKArgs &args, int kv_bits = 16);

@@ -246,7 +246,8 @@ TT_HIP_API tt_hip_kv *tt_hip_kv_create_ring(tt_hip_ctx *ctx, int n_layers, int n
  *   rows      a range may not cross the place where the ring comes round;
  *   keys      the windowed calls (_swa, _sinks; window + rows + 30 <= R serves every position) know where the rows lie; the calls
  *             without a window and those over key selections serve such a cache while the sequence fits the capacity, else
- *             TT_HIP_ERR_CAPACITY.
+ *             TT_HIP_ERR_CAPACITY;
+ *   snapshots restore into a cache made with the same ring and sinks.
  * sink_tokens 0 is tt_hip_kv_create_ring. */
 TT_HIP_API tt_hip_kv *tt_hip_kv_create_ring_sinks(tt_hip_ctx *ctx, int n_layers, int n_kv_heads, int head_dim, int n_slots,
                                                   int ring_capacity_tokens, int sink_tokens, int max_context_tokens, int bits,

@@ -3,7 +3,7 @@ the keys, tiles whose last rows are few, the same sequence twice, another stream
 import numpy as np
 import pytest
 
-from tests.exact_attention import attend, check, dequantise, stored_rows
+from tests.exact_attention import check, dequantise, stored_rows
 from tests.test_gpu_attn_shared_prefix import Family, _decode, _fill
 from tests.test_gpu_attn_sinks import _dev, _rows
 

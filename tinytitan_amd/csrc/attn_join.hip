@@ -7,7 +7,9 @@
 //
 // What it takes is its trips to memory, one for the arguments and as few as may be for the partial rows: a workgroup is one (token, head) and
 // DIMS dims of it, its threads own four dims of every G-th split, G = 1024 / DIMS, and ask for BATCH of those at once.  Rows of many splits
-// go by 64 dims (sixteen splits side by side, up to 128 in one trip), rows of few in one workgroup, of which there are then fewer.
+// go by 64 dims (sixteen splits side by side, up to 128 in one trip), rows of few in one workgroup, of which there are then fewer, and so do
+// as many rows as fill the chip, whose splits are then read in longer runs (64 tokens of 16 heads of 256, 33 MB of partial
+// results, by 64 dims / by 128 / whole 10.8 / 8.9 / 8.4 us; 18 of 24, 6.0 / 5.7 / 5.9; 20 of 32 heads of 128, 4.9 / 4.3 / 4.3).
 #include <algorithm>
 
 #include "internal.h"
@@ -119,7 +121,7 @@ void launch_join_of(tt_hip_ctx *ctx, int n_seq, const JoinArgs &args) {
     auto launch = [&](auto kernel, int parts) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)(args.heads * parts), (unsigned)args.rows, (unsigned)n_seq), dim3(256), 0, ctx->stream, args);
     };
-    if (most <= 4 * 1024 / D) launch(attn_join_kernel<D, D, 4>, 1);
+    if (most <= 4 * 1024 / D || (long long)args.heads * args.rows * n_seq >= 2 * ctx->n_cus) launch(attn_join_kernel<D, D, 4>, 1);
     else if (most <= 64) launch(attn_join_kernel<D, 64, 4>, D / 64);
     else launch(attn_join_kernel<D, 64, 8>, D / 64);
 }

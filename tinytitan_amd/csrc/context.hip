@@ -1299,7 +1299,7 @@ static int plan_pieces(const tt_hip_ctx *ctx, const tt_hip_kv *kv, int n_seq, co
         if (packed_rows) {
             // The workgroups over shared keys start first, those over own keys take the places that they leave.
             const int steps = std::min(len, front) / 32;
-            const double own_group = 0.35 * fixed + (0.13 + 0.0023 * D) * ((std::min(len, longest_own) + 127) / 128);
+            const double own_group = 0.35 * fixed + (0.13 + 0.0023 * D) * std::ceil(std::min<double>(len, own_keys / own) / 128.0);
             const double busy = (front_groups * (0.57 * fixed + steps * shared_step) + own * p->own_tiles * own_group) / slots_on_chip;
             const double walk = std::max(std::ceil(front_groups / slots_on_chip) * (0.57 * fixed + steps * step), busy + 1.8 * own_group);
             return 7.5 + 0.0016 * tokens * n_q_heads + walk + 0.48 * partials_us(part_rows, D);

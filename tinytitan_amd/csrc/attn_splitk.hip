@@ -1,7 +1,7 @@
 // Split-K flash attention over the swizzled KV pages (fp16 values, or 8 / 4-bit levels
 // dequantised in registers; linear pages or a ring): GQA decode, multi-row verify and causal
 // prefill for the shapes the chunk kernel does not take, each with an optional sliding
-// window, on gfx950 MFMA.
+// window (and sinks beside it) or a prefix in another slot's pages, on gfx950 MFMA.
 //
 // Formulation (everything transposed so that per-query-row state is per-lane):
 //   S^T[key][row]  = K[key][:] . Q[row][:]        A = K fragment,  B = Q^T fragment

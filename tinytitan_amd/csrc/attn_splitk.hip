@@ -1168,15 +1168,16 @@ __device__ __forceinline__ void front_store(const FrontBlock<D, BITS> &f, char *
 
 // The order of a phase of MFMAS matrix products with an operand each out of LDS: FIRST reads, a read behind every product, of MFMAS + EXTRA in all, and of
 // the next block's way into LDS a little beside each.
+template <int BITS, int BEHIND, int... I>
+__device__ __forceinline__ void reads_behind(std::integer_sequence<int, I...>) {
+    ((__builtin_amdgcn_sched_group_barrier(0x008, 1, 0), I < BEHIND ? __builtin_amdgcn_sched_group_barrier(0x100, 1, 0) : (void)0,
+      BITS == 16 ? (void)0 : __builtin_amdgcn_sched_group_barrier(0x002, 6, 0), __builtin_amdgcn_sched_group_barrier(0x200, 1, 0)),
+     ...);
+}
 template <int FIRST, int MFMAS, int EXTRA, int BITS>
 __device__ __forceinline__ void reads_ahead() {
-    constexpr int BEHIND = MFMAS + EXTRA - FIRST;
     __builtin_amdgcn_sched_group_barrier(0x100, FIRST, 0);
-    [&]<int... I>(std::integer_sequence<int, I...>) {
-        ((__builtin_amdgcn_sched_group_barrier(0x008, 1, 0), I < BEHIND ? __builtin_amdgcn_sched_group_barrier(0x100, 1, 0) : (void)0,
-          BITS == 16 ? (void)0 : __builtin_amdgcn_sched_group_barrier(0x002, 6, 0), __builtin_amdgcn_sched_group_barrier(0x200, 1, 0)),
-         ...);
-    }(std::make_integer_sequence<int, MFMAS>{});
+    reads_behind<BITS, MFMAS + EXTRA - FIRST>(std::make_integer_sequence<int, MFMAS>{});
 }
 
 constexpr int kFrontPitch = 36;  // floats of a row of 32 dims on its way out

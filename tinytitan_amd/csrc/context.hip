@@ -1314,7 +1314,7 @@ static int plan_pieces(const tt_hip_ctx *ctx, const tt_hip_kv *kv, int n_seq, co
     }
     p->len = 0;
     const int finest = packed_rows ? 32 : 128;
-    for (int len = 128; len < longest + finest; len += std::max(finest, len / 8 / finest * finest)) {
+    for (int len = 128; p->len == 0 || len < longest + finest; len += std::max(finest, len / 8 / finest * finest)) {
         const double us = us_of(len);
         if (p->len == 0 || us < p->us) {
             p->us = us;

@@ -1265,7 +1265,17 @@ static int splits_in(int keys, int len) { return std::max((keys + len - 1) / len
 static int plan_pieces(const tt_hip_ctx *ctx, const tt_hip_kv *kv, int n_seq, const int *totals, int rows, int front, int n_q_heads,
                        bool packed_rows, PairPlan *p) {
     const int D = kv->head_dim, tokens = n_seq * rows;
-    const int st = plan_launch(ctx, 0, 1, n_q_heads, kv->n_kv_heads, D, packed_rows ? rows : tokens, front, front, front, &p->tiles, kv->bits, true);
+    long long own_keys = 0, own_turns = 0;
+    int longest_own = 0;
+    for (int i = 0; i < n_seq; ++i) {
+        const int own = totals[i] - front;
+        longest_own = std::max(longest_own, own);
+        own_keys += own;
+        own_turns += (own + 127) / 128;
+    }
+    // (tiles of 16 or 32 rows: by the shared keys, which both passes then take in the same ones, or by the own keys alone)
+    const int st = packed_rows ? plan_launch(ctx, 0, n_seq, n_q_heads, kv->n_kv_heads, D, rows, own_keys, 0, longest_own, &p->tiles, kv->bits, true)
+                               : plan_launch(ctx, 0, 1, n_q_heads, kv->n_kv_heads, D, tokens, front, front, front, &p->tiles, kv->bits, true);
     if (st != TT_HIP_OK) return st;
     LaunchPlan &plan = p->tiles;
     p->packed_rows = packed_rows;
@@ -1277,14 +1287,6 @@ static int plan_pieces(const tt_hip_ctx *ctx, const tt_hip_kv *kv, int n_seq, co
     }
     const int slots_on_chip = ctx->n_cus * groups_per_cu(D, packed_rows ? 32 : plan.nt);
     const double fixed = start_us(D, packed_rows ? 32 : plan.nt), turn = turn_us(D, plan.nt, kv->bits);
-    long long own_keys = 0, own_turns = 0;
-    int longest_own = 0;
-    for (int i = 0; i < n_seq; ++i) {
-        const int own = totals[i] - front;
-        longest_own = std::max(longest_own, own);
-        own_keys += own;
-        own_turns += (own + 127) / 128;
-    }
     // (packed rows: a block of keys a step; the workgroups of a CU hide some of each other's)
     const int per_cu = groups_per_cu(D, 32);
     const double step = (0.3 + 0.0021 * D) * (kv->bits == 16 ? 1.0 : 1.0 + 0.0013 * D);

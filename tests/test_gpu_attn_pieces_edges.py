@@ -3,7 +3,7 @@ sequences than a launch takes, other writers and readers of a ring that keeps it
 import numpy as np
 import pytest
 
-from tests.exact_attention import check
+from tests.exact_attention import attend, check, dequantise
 from tests.test_gpu_attn_shared_prefix import Family
 from tests.test_gpu_attn_sinks import Session, _cache, _decode, _dev, _rows
 
@@ -120,3 +120,41 @@ def test_long_verify_passes_behind_a_prefix(gpu_ctx, H, KH, D, bits, prefix, row
             check(got[i][some], [f.row(i, q[i, r], starts[i] + r, D ** -0.5) for r in some], f"sequence {i} of {n}")
         assert np.isnan(got[n:]).all()
     f.kv.close()
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_slots_that_lie_past_four_gibibytes(gpu_ctx, bits):
+    import torch
+    from tinytitan_amd.engine import Attention, KVCacheManager, SharedPrefix
+    H, KH, D, prefix, slots = 16, 2, 256, 5005, 9
+    capacity = 640_000 if bits == 16 else 1_200_000
+    kv = KVCacheManager(gpu_ctx, 1, KH, D, slots=slots, max_context=capacity, initial_capacity=capacity, precision_bits=bits)
+    assert kv.token_stride_bytes * capacity * 8 > 2 ** 32
+    lengths = {0: prefix + 3, 1: prefix + 40, 6: prefix + 1, 7: prefix + 333}
+    home = Session(kv, 8, prefix, 1, bits)
+    kv.advance(8, prefix)
+    kv.share_prefix(8, prefix, list(lengths))
+    own = {}
+    for slot, length in lengths.items():
+        new = [_dev(part) for part in _rows(slot + 2, 2, length - prefix, KH * D)]
+        torch.cuda.synchronize()
+        kv.append(0, slot, prefix, *new)
+        k, v = kv.export_rows(0, slot, prefix, length - prefix)
+        gpu_ctx.synchronize()
+        own[slot] = [dequantise(t.cpu().numpy(), KH * D, bits) for t in (k, v)]
+    for copies in (1, 16):  # (few rows and many: every way over the shared keys)
+        table = list(lengths) * copies
+        q = _rows(50 + copies, len(table), H, D)
+        qd = _dev(q)
+        out = torch.full_like(qd, float("nan"))
+        torch.cuda.synchronize()
+        Attention(gpu_ctx).encode_full(kv, 0, qd, out, H, [lengths[s] for s in table], 0.0625, slot=table, prefix=SharedPrefix(8, prefix))
+        gpu_ctx.synchronize()
+        got = out.cpu().numpy()
+        for i in range(4):
+            k, v = ([np.concatenate(p) for p in zip(front, mine)] for front, mine in zip((home.k64, home.v64), own[table[i]]))
+            check(got[i:i + 1], [attend(q[i], k, v, np.arange(len(k[0])) >= 0, 0.0625, None, bits)], f"{copies} copies, sequence {i}")
+    q = _rows(60, 1, H, D)
+    got = _decode(gpu_ctx, kv, q, [prefix], 300, 7, 0.0625, slots=[8])
+    check(got, [home.row(q[0], prefix - 1, 300, 7, 0.0625, None, bits)], "sinks in the last slot")
+    kv.close()

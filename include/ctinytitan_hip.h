@@ -328,8 +328,11 @@ TT_HIP_API int tt_hip_kv_expect_position(const tt_hip_kv *kv, int slot, int posi
  * below prefix_len & ~31 are read by the _shared attention calls only, from prefix_slot, whose first prefix_len rows have to stay as they
  * are; other readers of such a slot (plain attention calls, tt_hip_kv_read, snapshots) find what its own pages hold there.
  * The rows from prefix_len on are the slot's own, at their own positions: append, epilogue, advance and rewind as ever.
+ * A slot that started so is no prefix_slot itself, here or in a _shared call (TT_HIP_ERR_CURSOR): a conversation that forks from it
+ * is shared from the slot that holds the prefix.  Nor is it served behind a shorter prefix than it started from, but for one that it
+ * has been rewound to.  tt_hip_kv_reset, a rewind to 0 and a restored snapshot end this: the rows are the slot's own then.
  * TT_HIP_ERR_INVALID_ARGUMENT: a slot out of range, or prefix_slot itself among the slots; TT_HIP_ERR_CURSOR: prefix_slot has fewer
- * rows; TT_HIP_ERR_SHAPE: a ring. */
+ * rows, or starts from another's; TT_HIP_ERR_SHAPE: a ring. */
 TT_HIP_API int tt_hip_kv_share_prefix(tt_hip_kv *kv, int prefix_slot, int prefix_len, int n_slots, const int *slots);
 
 /* Element offsets (in halves, within one [slot][kv_head] page) of key/value

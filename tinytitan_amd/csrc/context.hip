@@ -1762,6 +1762,14 @@ static int check_prefix(const tt_hip_kv *kv, int prefix_slot, int prefix_len) {
     return prefix_len <= kv->capacity ? TT_HIP_OK : TT_HIP_ERR_CAPACITY;
 }
 
+// ... and that the pages of a call hold what it reads of them: the prefix's slot the prefix, a sequence's own the rows behind its whole blocks.
+static int check_rows_held(const tt_hip_kv *kv, int prefix_slot, int prefix_len, int n_slots, const int *slots) {
+    if (prefix_len > 0 && kv->borrowed[prefix_slot] > 0) return TT_HIP_ERR_CURSOR;
+    for (int i = 0; i < n_slots; ++i)
+        if (kv->borrowed[slots[i]] > prefix_len / kBlockTokens * kBlockTokens) return TT_HIP_ERR_CURSOR;
+    return TT_HIP_OK;
+}
+
 int tt_hip_kv_share_prefix(tt_hip_kv *kv, int prefix_slot, int prefix_len, int n_slots, const int *slots) {
     if (!kv || n_slots <= 0 || !slots) return TT_HIP_ERR_INVALID_ARGUMENT;
     int st = check_prefix(kv, prefix_slot, prefix_len);
@@ -1769,6 +1777,7 @@ int tt_hip_kv_share_prefix(tt_hip_kv *kv, int prefix_slot, int prefix_len, int n
     for (int i = 0; i < n_slots; ++i)
         if (slots[i] < 0 || slots[i] >= kv->n_slots || slots[i] == prefix_slot) return TT_HIP_ERR_INVALID_ARGUMENT;
     if (kv->positions[prefix_slot] < prefix_len) return TT_HIP_ERR_CURSOR;
+    if (prefix_len > 0 && kv->borrowed[prefix_slot] > 0) return TT_HIP_ERR_CURSOR;  // (its pages do not hold the prefix)
     BusyGuard guard(kv->ctx);
     if (!guard.ok) return TT_HIP_ERR_BUSY;
     if (prefix_len % kBlockTokens != 0) {
@@ -1776,7 +1785,10 @@ int tt_hip_kv_share_prefix(tt_hip_kv *kv, int prefix_slot, int prefix_len, int n
         st = launch_kv_copy_block(kv, prefix_slot, prefix_len / kBlockTokens, n_slots, slots);
         if (st != TT_HIP_OK) return st;
     }
-    for (int i = 0; i < n_slots; ++i) kv->positions[slots[i]] = prefix_len;
+    for (int i = 0; i < n_slots; ++i) {
+        kv->positions[slots[i]] = prefix_len;
+        kv->borrowed[slots[i]] = prefix_len / kBlockTokens * kBlockTokens;
+    }
     return TT_HIP_OK;
 }
 
@@ -1794,6 +1806,8 @@ int tt_hip_attn_verify_shared(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_s
         if (!kv->holds_keys(0, (long long)start_positions[i] + rows)) return TT_HIP_ERR_CAPACITY;
         totals[i] = start_positions[i] + rows;
     }
+    st = check_rows_held(kv, prefix_slot, prefix_len, n_seq, slots);
+    if (st != TT_HIP_OK) return st;
     const int front = prefix_len / kBlockTokens * kBlockTokens;
     if (front == 0) return tt_hip_attn_verify(ctx, kv, layer, n_seq, slots, start_positions, rows, n_q_heads, q, gate, scale, out);
     BusyGuard guard(ctx);
@@ -1812,7 +1826,9 @@ int tt_hip_attn_decode_shared(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_s
     if (st != TT_HIP_OK) return st;
     if (prefix_len < kBlockTokens) {  // (a sequence without keys is the plain call's to serve)
         for (int i = 0; i < n_seq; ++i)
-            if (seq_lens[i] < prefix_len) return TT_HIP_ERR_INVALID_ARGUMENT;
+            if (slots[i] < 0 || slots[i] >= kv->n_slots || seq_lens[i] < prefix_len) return TT_HIP_ERR_INVALID_ARGUMENT;
+        st = check_rows_held(kv, prefix_slot, prefix_len, n_seq, slots);
+        if (st != TT_HIP_OK) return st;
         return tt_hip_attn_decode(ctx, kv, layer, n_seq, slots, seq_lens, n_q_heads, q, gate, scale, out);
     }
     IntTable starts(n_seq);
@@ -1831,6 +1847,8 @@ int tt_hip_attn_prefill_shared(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int sl
     st = check_prefix(kv, prefix_slot, prefix_len);
     if (st != TT_HIP_OK) return st;
     if (slot < 0 || slot >= kv->n_slots || start_pos < 0 || q_len <= 0 || start_pos + 1LL < prefix_len) return TT_HIP_ERR_INVALID_ARGUMENT;
+    st = check_rows_held(kv, prefix_slot, prefix_len, 1, &slot);
+    if (st != TT_HIP_OK) return st;
     const int front = prefix_len / kBlockTokens * kBlockTokens;
     if (front == 0 || slot == prefix_slot)
         return tt_hip_attn_prefill(ctx, kv, layer, slot, start_pos, q_len, kv_valid, n_q_heads, q, q_stride, gate, gate_stride, scale, out,

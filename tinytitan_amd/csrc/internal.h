@@ -226,6 +226,7 @@ struct tt_hip_kv {
     uint64_t generation = 0;       // bumped when the stores are reallocated
     std::vector<_Float16 *> k, v;  // one K and one V store per layer (bytes at 8 / 4 bits)
     std::vector<int> positions;
+    std::vector<int> borrowed;  // a slot's first rows that are another slot's (tt_hip_kv_share_prefix): its own pages do not hold them
     size_t block_bytes() const { return tt::block_bytes(head_dim, bits); }
     size_t page_bytes() const { return (size_t)(capacity / tt::kBlockTokens) * block_bytes(); }
     size_t layer_bytes() const { return (size_t)n_slots * n_kv_heads * page_bytes(); }

@@ -356,6 +356,7 @@ tt_hip_kv *tt_hip_kv_create_quantized(tt_hip_ctx *ctx, int n_layers, int n_kv_he
     if (capacity > kv->max_context) capacity = kv->max_context;
     kv->capacity = capacity;
     kv->positions.assign(n_slots, 0);
+    kv->borrowed.assign(n_slots, 0);
     int st = alloc_layers(kv, capacity, &kv->k, &kv->v);
     if (st != TT_HIP_OK) {
         delete kv;
@@ -508,6 +509,7 @@ int tt_hip_kv_rewind(tt_hip_kv *kv, int slot, int position) {
     if (!kv || slot < 0 || slot >= kv->n_slots) return TT_HIP_ERR_INVALID_ARGUMENT;
     if (position < 0 || position > kv->positions[slot]) return TT_HIP_ERR_CURSOR;
     kv->positions[slot] = position;
+    kv->borrowed[slot] = std::min(kv->borrowed[slot], position);  // (rows from here on will be its own)
     return TT_HIP_OK;
 }
 
@@ -515,8 +517,10 @@ int tt_hip_kv_reset(tt_hip_kv *kv, int slot) {
     if (!kv || slot < -1 || slot >= kv->n_slots) return TT_HIP_ERR_INVALID_ARGUMENT;
     if (slot == -1) {
         for (auto &p : kv->positions) p = 0;
+        for (auto &b : kv->borrowed) b = 0;
     } else {
         kv->positions[slot] = 0;
+        kv->borrowed[slot] = 0;
     }
     return TT_HIP_OK;
 }
@@ -659,6 +663,7 @@ int tt_hip_kv_snapshot_restore(tt_hip_kv *kv, int position, const size_t *length
     if (!guard.ok || kv->ctx->capturing) return TT_HIP_ERR_BUSY;
     if (hipSetDevice(kv->ctx->device) != hipSuccess) return TT_HIP_ERR_HIP;
     for (auto &p : kv->positions) p = 0;  // reset() (:88)
+    for (auto &b : kv->borrowed) b = 0;
     const size_t stride = tt_hip_kv_token_stride_bytes(kv);
     const int stored = position < kv->capacity ? position : kv->capacity;
     const size_t seg = (size_t)stored * stride;

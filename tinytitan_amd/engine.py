@@ -248,7 +248,8 @@ class KVCacheManager:
 
     def share_prefix(self, prefix_slot: int, length: int, slots: Sequence[int]) -> None:
         """The listed slots start from rows ``[0, length)`` of ``prefix_slot``: nothing is copied but the last part block, and the
-        slots' cursors are set to ``length``.  Attention calls then take ``prefix=SharedPrefix(prefix_slot, length)``."""
+        slots' cursors are set to ``length``.  Attention calls then take ``prefix=SharedPrefix(prefix_slot, length)``.  A slot that starts
+        from another's rows is no ``prefix_slot`` itself until it is reset."""
         table = capi.int_array(slots)
         self.ctx._check(self._lib.tt_hip_kv_share_prefix(self.handle, prefix_slot, length, len(table), table), "tt_hip_kv_share_prefix")
 

@@ -324,7 +324,8 @@ TT_HIP_API int tt_hip_kv_expect_position(const tt_hip_kv *kv, int slot, int posi
 
 /* Slots that start from one prefix: rows [0, prefix_len) of prefix_slot -- written, its cursor at prefix_len or beyond -- become the
  * first rows of the listed slots without being copied: only the last block of 32 is, where the prefix ends inside one (one launch for
- * all layers and slots), and the slots' cursors are set to prefix_len, whatever they held before.  From then on a listed slot's rows
+ * all layers and slots; values of V behind the prefix in that block that are not finite as zeros, since the slots' sequences do not
+ * see them), and the slots' cursors are set to prefix_len, whatever they held before.  From then on a listed slot's rows
  * below prefix_len & ~31 are read by the _shared attention calls only, from prefix_slot, whose first prefix_len rows have to stay as they
  * are; other readers of such a slot (plain attention calls, tt_hip_kv_read, snapshots) find what its own pages hold there.
  * The rows from prefix_len on are the slot's own, at their own positions: append, epilogue, advance and rewind as ever.

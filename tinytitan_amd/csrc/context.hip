@@ -1782,7 +1782,7 @@ int tt_hip_kv_share_prefix(tt_hip_kv *kv, int prefix_slot, int prefix_len, int n
     if (!guard.ok) return TT_HIP_ERR_BUSY;
     if (prefix_len % kBlockTokens != 0) {
         if (hipSetDevice(kv->ctx->device) != hipSuccess) return TT_HIP_ERR_HIP;
-        st = launch_kv_copy_block(kv, prefix_slot, prefix_len / kBlockTokens, n_slots, slots);
+        st = launch_kv_copy_block(kv, prefix_slot, prefix_len / kBlockTokens, prefix_len % kBlockTokens, n_slots, slots);
         if (st != TT_HIP_OK) return st;
     }
     for (int i = 0; i < n_slots; ++i) {

@@ -314,8 +314,9 @@ int launch_combine(tt_hip_ctx *ctx, const LaunchPlan &plan, int head_dim, int n_
 // The rows of n_seq sequences from the partial results of two passes (attn_join.hip).
 int launch_join(tt_hip_ctx *ctx, int head_dim, int n_seq, const JoinArgs &args);
 
-// A prefix that slots share: block `block` of `slot`'s pages, every layer, into the same place of `n_slots` others.
-int launch_kv_copy_block(tt_hip_kv *kv, int slot, int block, int n_slots, const int *slots);
+// A prefix that slots share: block `block` of `slot`'s pages, of which `rows` are the prefix's, every layer, into the same place of
+// `n_slots` others.
+int launch_kv_copy_block(tt_hip_kv *kv, int slot, int block, int rows, int n_slots, const int *slots);
 
 int launch_kv_append(tt_hip_kv *kv, int layer, int slot, int position, int n_tokens, const tt_half *k, const tt_half *v,
                      size_t stride);

@@ -219,11 +219,14 @@ static int round_up_block(long long tokens) {
 }
 
 // One block of a slot's pages into other slots' pages, as it is stored, whatever that is: (slot, kv head, K or V of a layer) a workgroup.
+// But of V's rows from `rows` on, which the slot copied from may have gone on to write, nothing that is not finite: no sequence of the slots
+// copied to sees them before it has written its own, and a probability of zero would make NaN of an infinity.
 constexpr int kCopyLayers = 64;
 struct CopyBlockArgs {
     uint8_t *store[kCopyLayers][2];
     long long page_bytes, block_at;
     int block_bytes, n_kv_heads, from;
+    int rows, head_dim, bits;
     uint8_t to[TT_HIP_MAX_SLOTS];
 };
 static_assert(TT_HIP_MAX_SLOTS <= 256, "a slot is a byte");
@@ -232,16 +235,32 @@ __global__ __launch_bounds__(256) void kv_copy_block_kernel(const CopyBlockArgs 
     uint8_t *const store = a.store[blockIdx.z >> 1][blockIdx.z & 1];
     const u4 *src = reinterpret_cast<const u4 *>(store + ((long long)a.from * a.n_kv_heads + blockIdx.y) * a.page_bytes + a.block_at);
     u4 *dst = reinterpret_cast<u4 *>(store + ((long long)a.to[blockIdx.x] * a.n_kv_heads + blockIdx.y) * a.page_bytes + a.block_at);
-    for (int i = threadIdx.x; i < a.block_bytes / 16; i += 256) dst[i] = src[i];
+    // V's halves -- values, or behind the levels scales and biases -- lie in pieces of eight keys, the piece's chunk of the block in its number.
+    const int halves = a.bits == 16 ? 0 : (int)block_level_bytes(a.head_dim, a.bits) / 16, shift = a.bits == 16 && a.head_dim == 256 ? 4 : 0;
+    for (int i = threadIdx.x; i < a.block_bytes / 16; i += 256) {
+        u4 x = src[i];
+        if ((blockIdx.z & 1) && i >= halves) {
+            const int chunk = ((i - halves) >> shift) & 3;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const unsigned infinite = 0x7c00u << (16 * (e & 1));
+                if (v_key_at(chunk, e) >= a.rows && (x[e >> 1] & infinite) == infinite) x[e >> 1] &= ~(0xffffu << (16 * (e & 1)));
+            }
+        }
+        dst[i] = x;
+    }
 }
 
-int launch_kv_copy_block(tt_hip_kv *kv, int slot, int block, int n_slots, const int *slots) {
+int launch_kv_copy_block(tt_hip_kv *kv, int slot, int block, int rows, int n_slots, const int *slots) {
     CopyBlockArgs a;
     a.page_bytes = (long long)kv->page_bytes();
     a.block_bytes = (int)kv->block_bytes();
     a.block_at = (long long)block * a.block_bytes;
     a.n_kv_heads = kv->n_kv_heads;
     a.from = slot;
+    a.rows = rows;
+    a.head_dim = kv->head_dim;
+    a.bits = kv->bits;
     for (int first = 0; first < n_slots; first += TT_HIP_MAX_SLOTS) {
         const int n = std::min(n_slots - first, TT_HIP_MAX_SLOTS);
         for (int i = 0; i < n; ++i) a.to[i] = (uint8_t)slots[first + i];

@@ -1387,6 +1387,27 @@ static int run_pieces(tt_hip_ctx *ctx, tt_hip_kv *kv, const PairPlan &pair, int 
     return launch_splitk_pair(ctx, D, plan.nt, kv->bits, pair.packed_rows, (unsigned)(a.front_groups + own_splits * own_tiles), a);
 }
 
+// Rows of any number of sequences whose keys [0, front) -- whole blocks -- are another slot's, in one pass: every sequence walks them like its
+// own, out of the other slot's page, in split-K tiles (kind 0) or in tiles of one head (kind 1), as run_attention takes them.
+// In one launch, but for more rows than a launch has tiles for (of 16 rows of one head: a tile has as many at least, packed or not).
+static int run_one_pass(tt_hip_ctx *ctx, tt_hip_kv *kv, int kind, int layer, int n_seq, const int *slots, const int *starts, const int *totals,
+                        int rows, int prefix_slot, int front, int n_q_heads, const tt_half *q, long long q_seq_stride, long long q_tok_stride,
+                        const tt_half *gate, long long g_seq_stride, long long g_tok_stride, float scale, tt_half *out, long long o_seq_stride,
+                        long long o_tok_stride) {
+    const ChunkPieces pieces{0, prefix_slot, front / kBlockTokens};
+    const int rows_at_once = std::max(65535 / n_q_heads - 1, 1) * 16;
+    IntTable first(n_seq);
+    for (int r = 0; r < rows; r += rows_at_once) {
+        for (int i = 0; i < n_seq; ++i) first[i] = starts[i] + r;
+        const int st = run_attention(ctx, kv, kind, layer, n_seq, slots, first.data(), totals, std::min(rows - r, rows_at_once), n_q_heads,
+                                     q + r * q_tok_stride, q_seq_stride, q_tok_stride, gate ? gate + r * g_tok_stride : nullptr, g_seq_stride,
+                                     g_tok_stride, scale, out + r * o_tok_stride, o_seq_stride, o_tok_stride, 1, 0, nullptr, 0, nullptr, 0, 0, false,
+                                     nullptr, 0, nullptr, &pieces);
+        if (st != TT_HIP_OK) return st;
+    }
+    return TT_HIP_OK;
+}
+
 // Rows of sequences whose keys [0, front) -- whole blocks -- are another slot's, by the cheapest of four ways:
 //  * one pass: every sequence walks the shared keys like its own, out of the other slot's page; they are read once per sequence, mostly from L2;
 //  * two passes in one launch and a join, the shared keys by split-K tiles, which the tokens of ALL sequences fill that one
@@ -1410,10 +1431,8 @@ static int run_shared(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, cons
         longest = std::max(longest, totals[i]);
     }
     auto one_pass = [&] {
-        const ChunkPieces pieces{0, prefix_slot, front / kBlockTokens};
-        return run_attention(ctx, kv, 0, layer, n_seq, slots, starts, totals, rows, n_q_heads, q, q_seq_stride, q_tok_stride, gate, g_seq_stride,
-                             g_tok_stride, scale, out, o_seq_stride, o_tok_stride, 1, 0, nullptr, 0, nullptr, 0, 0, false, nullptr, 0, nullptr,
-                             &pieces);
+        return run_one_pass(ctx, kv, 0, layer, n_seq, slots, starts, totals, rows, prefix_slot, front, n_q_heads, q, q_seq_stride, q_tok_stride, gate,
+                            g_seq_stride, g_tok_stride, scale, out, o_seq_stride, o_tok_stride);
     };
     if (n_seq == 1 || longest <= 384) return one_pass();  // (nobody to share with; one launch that ends in the final rows)
     LaunchPlan alone{};
@@ -1498,25 +1517,23 @@ static int run_shared(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, cons
 }
 
 // ... of any number of sequences and rows, in pieces of at most kMaxSeqPerLaunch sequences and kSharedTokens rows of all together, so that
-// the partial results stay small.  (Several sequences in a piece come with all of their rows: these then lie one behind the other, as
-// the pass over the shared keys takes them.)
+// the partial results stay small.  (A piece's sequences come with all of their rows, which lie one behind the other, as the pass over the
+// shared keys takes them.)  Where a piece has room for one sequence only there is nobody to share with: one pass.
 constexpr int kSharedTokens = 1024;
 static int run_shared_rows(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, const int *slots, const int *starts, const int *totals,
                            int rows, int prefix_slot, int front, int n_q_heads, const tt_half *q, long long q_seq_stride,
                            long long q_tok_stride, const tt_half *gate, long long g_seq_stride, long long g_tok_stride, float scale,
                            tt_half *out, long long o_seq_stride, long long o_tok_stride) {
-    const int seqs_at_once = std::min(std::max(kSharedTokens / rows, 1), kMaxSeqPerLaunch), rows_at_once = std::min(rows, kSharedTokens);
+    const int seqs_at_once = std::min(kSharedTokens / rows, kMaxSeqPerLaunch);
+    if (n_seq == 1 || seqs_at_once <= 1)
+        return run_one_pass(ctx, kv, 0, layer, n_seq, slots, starts, totals, rows, prefix_slot, front, n_q_heads, q, q_seq_stride, q_tok_stride, gate,
+                            g_seq_stride, g_tok_stride, scale, out, o_seq_stride, o_tok_stride);
     for (int base = 0; base < n_seq; base += seqs_at_once) {
-        const int n = std::min(n_seq - base, seqs_at_once);
-        for (int r = 0; r < rows; r += rows_at_once) {
-            int first[kMaxSeqPerLaunch];
-            for (int i = 0; i < n; ++i) first[i] = starts[base + i] + r;
-            const int st = run_shared(ctx, kv, layer, n, slots + base, first, totals + base, std::min(rows - r, rows_at_once), prefix_slot, front,
-                                      n_q_heads, q + base * q_seq_stride + r * q_tok_stride, q_seq_stride, q_tok_stride,
-                                      gate ? gate + base * g_seq_stride + r * g_tok_stride : nullptr, g_seq_stride, g_tok_stride, scale,
-                                      out + base * o_seq_stride + r * o_tok_stride, o_seq_stride, o_tok_stride);
-            if (st != TT_HIP_OK) return st;
-        }
+        const int st = run_shared(ctx, kv, layer, std::min(n_seq - base, seqs_at_once), slots + base, starts + base, totals + base, rows, prefix_slot,
+                                  front, n_q_heads, q + base * q_seq_stride, q_seq_stride, q_tok_stride,
+                                  gate ? gate + base * g_seq_stride : nullptr, g_seq_stride, g_tok_stride, scale, out + base * o_seq_stride,
+                                  o_seq_stride, o_tok_stride);
+        if (st != TT_HIP_OK) return st;
     }
     return TT_HIP_OK;
 }
@@ -1620,9 +1637,12 @@ static int run_prefill(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int slot, int 
     // per call into the context's staging store (4096 rows: one 9 us pass, then the fp16 kernel).
     PageSource staged{};
     const PageSource *pages = nullptr;
-    auto in_two_passes = [&] {  // (a front piece where the split-K tiles are the faster ones)
-        return run_shared_rows(ctx, kv, layer, 1, &slot, &start_pos, &kv_valid, q_len, front_slot, front, n_q_heads, q, 0, (long long)q_stride,
-                               gate, 0, (long long)gate_stride, scale, out, 0, (long long)o_stride);
+    auto in_tiles = [&](int kind) {  // the split-K kernel: packed tiles (0) or tiles of one head (1)
+        if (front > 0)
+            return run_one_pass(ctx, kv, kind, layer, 1, &slot, &start_pos, &kv_valid, q_len, front_slot, front, n_q_heads, q, 0, (long long)q_stride,
+                                gate, 0, (long long)gate_stride, scale, out, 0, (long long)o_stride);
+        return run_attention(ctx, kv, kind, layer, 1, &slot, &start_pos, &kv_valid, q_len, n_q_heads, q, 0, (long long)q_stride,
+                             gate, 0, (long long)gate_stride, scale, out, 0, (long long)o_stride);
     };
     int st = TT_HIP_OK;
     // From this many keys on a chunk that does not fill the chip goes through the chunk kernel over key ranges (below:
@@ -1698,11 +1718,8 @@ static int run_prefill(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int slot, int 
         const bool whole_ahead = q_len >= 256 && whole.us < (n_splits >= 2 ? ranges_us : splitk_us);
         if (filled || whole_ahead || (pages && n_splits < 2)) return whole_tiles(pages);
         if (n_splits >= 2) return over_ranges(n_splits, split_blocks, pages);
-        if (front > 0) return in_two_passes();
-        return run_attention(ctx, kv, 0, layer, 1, &slot, &start_pos, &kv_valid, q_len, n_q_heads, q, 0,
-                             (long long)q_stride, gate, 0, (long long)gate_stride, scale, out, 0, (long long)o_stride);
+        return in_tiles(0);
     }
-    if (front > 0) return in_two_passes();
     // What the chunk kernel does not serve (head groups that are no multiple of 4, unaligned rows, quantised pages
     // that are not staged, a non-positive scale): the split-K kernel over GQA-packed tiles, like a verify pass -- or, where heads that do
     // not divide a tile's 32 rows leave some of them empty, tiles of 32 rows of ONE head, each walking all its keys, as long as they are
@@ -1712,13 +1729,11 @@ static int run_prefill(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int slot, int 
     // of 9 (36/4 of 128): 1,500 rows behind 3,000 256 / 297; of 5 (40/8 of 128): 700 behind 7,000 253 / 262.
     const long long head_tiles = (long long)((q_len + 31) / 32) * n_q_heads;
     const bool plentiful = 2 * head_tiles >= ctx->n_cus && (kv_valid <= 8192 || head_tiles >= 2LL * ctx->n_cus);
-    auto in_tiles = [&](int kind) {
-        return run_attention(ctx, kv, kind, layer, 1, &slot, &start_pos, &kv_valid, q_len, n_q_heads, q, 0, (long long)q_stride,
-                             gate, 0, (long long)gate_stride, scale, out, 0, (long long)o_stride);
-    };
     // (over fp16 pages the two ways mostly take the same -- 116 of 120 chunks of groups of one and two within 5 %, 16/8 heads of 128, 300 rows behind 2,000 keys 37.5 /
     // 38.6, 1,500 102.4 / 100.4, but 32/16 of 64, 100 rows behind 7,000, 52.9 / 37.8 --: one-head tiles, which need no partial results)
-    if ((rows_left_empty || kv->bits == 16) && plentiful) return in_tiles(1);
+    // (Not behind a front piece, whose blocks cost their look-up in each tile: 4/2 heads of 64, 1,000 rows behind 2,048 shared keys one-head
+    // 29.8, packed 19.9; 16/2 of 256, 3,000 unaligned behind 4,096 443 / 394.)
+    if ((rows_left_empty || (kv->bits == 16 && front == 0)) && plentiful) return in_tiles(1);
     st = in_tiles(0);
     // (without memory for the splits' partial results, as inside a capture that would have to grow it: tiles of one head, which have none)
     if (plentiful && (st == TT_HIP_ERR_BUSY || st == TT_HIP_ERR_OUT_OF_MEMORY)) st = in_tiles(1);

@@ -1237,94 +1237,6 @@ int tt_hip_attn_prefill(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int slot, int
                                    gate_stride, scale, out, o_stride);
 }
 
-// What the ways of a shared-prefix call are estimated to take, in us: fitted to calls of 2 .. 64 sequences of 1 and 4 rows behind 700 .. 20,000
-// keys, of 16/4 heads of 64, 32/8 of 128, 16/2 and 24/2 of 256 over 16, 8 and 4 bits, where what they choose takes 3 % more than the best way.
-// 128 keys of a tile's walk (a block for each of its workgroup's wavefronts): their way out of L2, mostly, whatever their
-// bits, and over fewer of them the 32-row tiles' widening.
-static double turn_us(int D, int nt, int bits) {
-    return (0.2 + 0.0057 * D) * (bits == 16 || nt == 16 ? 1.0 : D == 256 ? 1.6 : 1.15);
-}
-// A workgroup beside its walk, and how many of them a CU holds.
-static double start_us(int D, int nt) { return nt == 32 ? 1.5 + 0.0215 * D : 2.0 + 0.0098 * D; }
-static int groups_per_cu(int D, int nt) { return nt == 32 ? 256 / D : D == 256 ? 2 : 4; }
-// Partial results that are written and read back.
-static double partials_us(double rows, int D) { return rows * D * 8.0 / 2.5e6; }
-
-// Two passes in one launch: the tokens of all sequences over the keys [0, front) of prefix_slot, every sequence over its own from there on.
-// The shared keys in the split-K tiles of 16 or 32 rows or in tiles of 128 packed ones, the own keys in split-K tiles, both in splits of at
-// most the same length, the one that makes the launch the cheapest (64 rows of 16/2 heads of 256 over 30,011 keys and 50 .. 2,000 of their
-// own, packed, in splits of 256 / 512 / 960 / 1,536 / 2,048 113 / 84 / 79 / 67 / 74 us, with the join; 20 of 32/8 of 128 over 6,000 over 8 bits, not
-// packed, in 128 / 512 / 1,024 / 2,048 26 / 17.6 / 17.4 / 23.6).
-struct PairPlan {
-    LaunchPlan tiles;
-    bool packed_rows;  // the shared keys by tiles of kFrontRows packed rows (attn_splitk.hip); tiles.nt and .tt are those of the own keys' tiles
-    int own_tok_tiles, own_tiles, len;
-    double us;  // with the join behind it
-};
-static int splits_in(int keys, int len) { return std::max((keys + len - 1) / len, 1); }
-static int plan_pieces(const tt_hip_ctx *ctx, const tt_hip_kv *kv, int n_seq, const int *totals, int rows, int front, int n_q_heads,
-                       bool packed_rows, PairPlan *p) {
-    const int D = kv->head_dim, tokens = n_seq * rows;
-    long long own_keys = 0, own_turns = 0;
-    int longest_own = 0;
-    for (int i = 0; i < n_seq; ++i) {
-        const int own = totals[i] - front;
-        longest_own = std::max(longest_own, own);
-        own_keys += own;
-        own_turns += (own + 127) / 128;
-    }
-    // (tiles of 16 or 32 rows: by the shared keys, which both passes then take in the same ones, or by the own keys alone)
-    const int st = packed_rows ? plan_launch(ctx, 0, n_seq, n_q_heads, kv->n_kv_heads, D, rows, own_keys, 0, longest_own, &p->tiles, kv->bits, true)
-                               : plan_launch(ctx, 0, 1, n_q_heads, kv->n_kv_heads, D, tokens, front, front, front, &p->tiles, kv->bits, true);
-    if (st != TT_HIP_OK) return st;
-    LaunchPlan &plan = p->tiles;
-    p->packed_rows = packed_rows;
-    p->own_tok_tiles = (rows + plan.tt - 1) / plan.tt;
-    p->own_tiles = plan.n_tiles / plan.tok_tiles * p->own_tok_tiles;
-    if (packed_rows) {
-        plan.tok_tiles = (tokens * (n_q_heads / kv->n_kv_heads) + kFrontRows - 1) / kFrontRows;
-        plan.n_tiles = plan.tok_tiles * kv->n_kv_heads;
-    }
-    const int slots_on_chip = ctx->n_cus * groups_per_cu(D, packed_rows ? 32 : plan.nt);
-    const double fixed = start_us(D, packed_rows ? 32 : plan.nt), turn = turn_us(D, plan.nt, kv->bits);
-    // (packed rows: a block of keys a step; the workgroups of a CU hide some of each other's)
-    const int per_cu = groups_per_cu(D, 32);
-    const double step = (0.3 + 0.0021 * D) * (kv->bits == 16 ? 1.0 : 1.0 + 0.0013 * D);
-    const double shared_step = step * (per_cu == 1 ? 1.0 : per_cu == 2 ? 1.2 : 1.8);
-    const double walk_us = 1.36 * ((double)plan.n_tiles * ((front + 127) / 128) + (double)own_turns * p->own_tiles) * turn / ctx->n_cus;
-    const double turn_alone = 0.36 + 0.005 * D;
-    const int longest = std::max(front, longest_own);
-    auto us_of = [&](int len) {
-        const double own = n_seq + (longest_own > len ? (double)(own_keys / len) : 0.0);  // (splits of own keys, or a few more)
-        const double front_groups = (double)plan.n_tiles * splits_in(front, len), groups = front_groups + own * p->own_tiles;
-        const double rounds = std::ceil(groups / slots_on_chip), part_rows = ((double)tokens * splits_in(front, len) + rows * own) * n_q_heads;
-        if (packed_rows) {
-            // The workgroups over shared keys start first, those over own keys take the places that they leave.
-            const int steps = std::min(len, front) / 32;
-            const double own_group = 0.35 * fixed + (0.13 + 0.0023 * D) * std::ceil(std::min<double>(len, own_keys / own) / 128.0);
-            const double busy = (front_groups * (0.57 * fixed + steps * shared_step) + own * p->own_tiles * own_group) / slots_on_chip;
-            const double walk = std::max(std::ceil(front_groups / slots_on_chip) * (0.57 * fixed + steps * step), busy + 1.8 * own_group);
-            return 7.5 + 0.0016 * tokens * n_q_heads + walk + 0.48 * partials_us(part_rows, D);
-        }
-        return 6.6 + fixed * (0.16 + 0.84 * rounds) + std::max(walk_us, (std::min(len, longest) + 127) / 128 * turn_alone) +
-               0.2 * partials_us(part_rows, D);
-    };
-    if (ctx->split_override > 0) {
-        p->len = (ctx->split_override + 31) / 32 * 32;
-        p->us = us_of(p->len);
-        return TT_HIP_OK;
-    }
-    p->len = 0;
-    const int finest = packed_rows ? 32 : 128;
-    for (int len = 128; p->len == 0 || len < longest + finest; len += std::max(finest, len / 8 / finest * finest)) {
-        const double us = us_of(len);
-        if (p->len == 0 || us < p->us) {
-            p->us = us;
-            p->len = len;
-        }
-    }
-    return TT_HIP_OK;
-}
 static int run_pieces(tt_hip_ctx *ctx, tt_hip_kv *kv, const PairPlan &pair, int layer, int n_seq, const int *slots, const int *starts,
                       const int *totals, int rows, int prefix_slot, int front, int n_q_heads, const tt_half *q, long long q_seq_stride,
                       long long q_tok_stride, float scale, PassParts *front_parts, PassParts *own_parts, JoinSeq *seqs) {
@@ -1408,63 +1320,21 @@ static int run_one_pass(tt_hip_ctx *ctx, tt_hip_kv *kv, int kind, int layer, int
     return TT_HIP_OK;
 }
 
-// Rows of sequences whose keys [0, front) -- whole blocks -- are another slot's, by the cheapest of four ways:
-//  * one pass: every sequence walks the shared keys like its own, out of the other slot's page; they are read once per sequence, mostly from L2;
-//  * two passes in one launch and a join, the shared keys by split-K tiles, which the tokens of ALL sequences fill that one
-//    sequence's rows leave mostly empty;
-//  * the same, the shared keys by tiles of 128 packed rows: for more rows than a split-K tile has;
-//  * the chunk kernel over ranges of the shared keys, its scores and values on wavefronts of their own, a pass over the own keys, and the join.
-// At most kMaxSeqPerLaunch sequences.  One pass / two / two with packed rows / ranges, us, 100 own keys: one row a sequence of 16/2 heads of
-// 256, 2 behind 2,000 9.1 / 11.0 / 13.3 / 24, 20 behind 6,000 18.3 / 16.3 / 23.5 / 29.5, 64 behind 20,000 92.8 / 44.9 / 44.0 / 47.7; 24/2 heads over 4
-// bits, 20 behind 20,000 60 / 80 / 39 / 51; 32/8 of 128 over 8 bits, 20 behind 6,000 56 / 18.9 / 20.1 / 32.6, behind 20,000 177 / 44.5 / 33.2 / 57.7; four
-// rows a sequence, 64 of 24/2 of 256 behind 2,000 39.4 / 91.6 / 50.4 / 56.6, behind 20,000 267 / 290 / 160 / 153.
+// Rows of sequences whose keys [0, front) -- whole blocks -- are another slot's, by the cheapest of four ways (plan_shared).  At most
+// kMaxSeqPerLaunch sequences.
 static int run_shared(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, const int *slots, const int *starts, const int *totals, int rows,
                       int prefix_slot, int front, int n_q_heads, const tt_half *q, long long q_seq_stride, long long q_tok_stride,
                       const tt_half *gate, long long g_seq_stride, long long g_tok_stride, float scale, tt_half *out,
                       long long o_seq_stride, long long o_tok_stride) {
     if (hipSetDevice(ctx->device) != hipSuccess) return TT_HIP_ERR_HIP;
     const int D = kv->head_dim, tokens = n_seq * rows;
-    long long keys = 0;
-    int longest = 0;
-    for (int i = 0; i < n_seq; ++i) {
-        keys += totals[i];
-        longest = std::max(longest, totals[i]);
-    }
-    auto one_pass = [&] {
-        return run_one_pass(ctx, kv, 0, layer, n_seq, slots, starts, totals, rows, prefix_slot, front, n_q_heads, q, q_seq_stride, q_tok_stride, gate,
-                            g_seq_stride, g_tok_stride, scale, out, o_seq_stride, o_tok_stride);
-    };
-    if (n_seq == 1 || longest <= 384) return one_pass();  // (nobody to share with; one launch that ends in the final rows)
-    LaunchPlan alone{};
-    int st = plan_launch(ctx, 0, n_seq, n_q_heads, kv->n_kv_heads, D, rows, keys, longest, longest, &alone, kv->bits, true);
+    const bool chunk_kernel = prefill_kernel_serves(n_q_heads, kv->n_kv_heads, D, aligned16(q) && q_tok_stride % 8 == 0) && scale > 0.0f;
+    SharedPlan plan{};
+    int st = plan_shared({ctx->n_cus, ctx->split_override, n_seq, totals, rows, front, n_q_heads, kv->n_kv_heads, D, kv->bits, chunk_kernel}, &plan);
     if (st != TT_HIP_OK) return st;
-    PairPlan pair{}, packed{};
-    st = plan_pieces(ctx, kv, n_seq, totals, rows, front, n_q_heads, false, &pair);
-    if (st == TT_HIP_OK) st = plan_pieces(ctx, kv, n_seq, totals, rows, front, n_q_heads, true, &packed);
-    if (st != TT_HIP_OK) return st;
-    if (packed.us < pair.us) pair = packed;
-    const double turn = turn_us(D, alone.nt, kv->bits), key_us = 0.9 * turn / ctx->n_cus / 128.0;  // of a tile
-    long long splits = 0;
-    for (int i = 0; i < n_seq; ++i) splits += splits_in(totals[i], alone.split_len);
-    const bool joined = longest > alone.split_len;
-    const double rounds = std::ceil((double)splits * alone.n_tiles / (ctx->n_cus * groups_per_cu(D, alone.nt)));
-    const double alone_us = 2.9 + start_us(D, alone.nt) * (0.45 + 0.5 * rounds) +
-                            std::max(key_us * alone.n_tiles * (double)keys, (std::min(alone.split_len, longest) + 127) / 128 * 0.8 * turn) +
-                            (joined ? 1.6 + 0.75 * partials_us((double)splits * rows * n_q_heads, D) : 0.0);
-    const bool aligned = aligned16(q) && q_tok_stride % 8 == 0;
-    KeyRanges ranges;
-    double ranges_us = 0.0;
-    if (prefill_kernel_serves(n_q_heads, kv->n_kv_heads, D, aligned) && scale > 0.0f) {
-        ranges = plan_key_ranges(ctx->n_cus, D, n_q_heads, kv->n_kv_heads, tokens, front / kBlockTokens);
-        ranges_us = ranges.us + 4.0 + 4.0 + key_us * alone.n_tiles * (double)(keys - (long long)n_seq * front) + 7.0;
-        // (quantised pages are dequantised once per call in front of the chunk kernel)
-        if (kv->bits != 16) ranges_us += 4.0 + (double)front * kv->n_kv_heads * D * (2.0 + kv->bits / 8.0) * 2.0 / 6.0e6;
-    }
-    if (alone_us <= pair.us && (ranges.n_splits < 2 || alone_us <= ranges_us)) return one_pass();
-    bool by_ranges = ranges.n_splits >= 2 && ranges_us < pair.us;
     PageSource staged{};
     const PageSource *pages = nullptr;
-    if (by_ranges && kv->bits != 16) {
+    if (plan.way == SharedWay::ranges && kv->bits != 16) {
         const size_t page = (size_t)front * D;
         st = ensure_stage(ctx, page * kv->n_kv_heads);
         if (st == TT_HIP_OK) {
@@ -1472,16 +1342,19 @@ static int run_shared(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, cons
             staged = PageSource{ctx->stage_k, ctx->stage_v, (long long)page, 0};
             pages = &staged;
         } else if (st == TT_HIP_ERR_BUSY || st == TT_HIP_ERR_OUT_OF_MEMORY) {
-            by_ranges = false;  // (no room for them, or none to be had inside a capture: the pages as they are)
+            plan.way = plan.without_ranges;  // (no room for them, or none to be had inside a capture: the pages as they are)
             st = TT_HIP_OK;
         }
         if (st != TT_HIP_OK) return st;
     }
+    if (plan.way == SharedWay::one_pass)
+        return run_one_pass(ctx, kv, 0, layer, n_seq, slots, starts, totals, rows, prefix_slot, front, n_q_heads, q, q_seq_stride, q_tok_stride, gate,
+                            g_seq_stride, g_tok_stride, scale, out, o_seq_stride, o_tok_stride);
     JoinArgs j{};
-    if (by_ranges) {
+    if (plan.way == SharedWay::ranges) {
         KeyPiece shared{true}, own{false, front / kBlockTokens};
         st = run_attention(ctx, kv, 1, layer, 1, &prefix_slot, &front, &front, tokens, n_q_heads, q, 0, q_tok_stride, nullptr, 0, 0, scale, out, 0,
-                           o_tok_stride, ranges.n_splits, ranges.split_blocks, pages, 0, nullptr, 0, 0, false, nullptr, -1, &shared);
+                           o_tok_stride, plan.ranges.n_splits, plan.ranges.split_blocks, pages, 0, nullptr, 0, 0, false, nullptr, -1, &shared);
         if (st != TT_HIP_OK) return st;
         int own_starts[kMaxSeqPerLaunch], own_totals[kMaxSeqPerLaunch];
         for (int i = 0; i < n_seq; ++i) {
@@ -1494,7 +1367,7 @@ static int run_shared(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, cons
         j.own = own.parts;
         for (int i = 0; i < n_seq; ++i) j.seq[i].first_split = own.first_split[i];
     } else {
-        st = run_pieces(ctx, kv, pair, layer, n_seq, slots, starts, totals, rows, prefix_slot, front, n_q_heads, q, q_seq_stride, q_tok_stride, scale,
+        st = run_pieces(ctx, kv, plan.pair, layer, n_seq, slots, starts, totals, rows, prefix_slot, front, n_q_heads, q, q_seq_stride, q_tok_stride, scale,
                         &j.front, &j.own, j.seq);
     }
     if (st != TT_HIP_OK) return st;
@@ -1519,13 +1392,12 @@ static int run_shared(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, cons
 // ... of any number of sequences and rows, in pieces of at most kMaxSeqPerLaunch sequences and kSharedTokens rows of all together, so that
 // the partial results stay small.  (A piece's sequences come with all of their rows, which lie one behind the other, as the pass over the
 // shared keys takes them.)  Where a piece has room for one sequence only there is nobody to share with: one pass.
-constexpr int kSharedTokens = 1024;
 static int run_shared_rows(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, const int *slots, const int *starts, const int *totals,
                            int rows, int prefix_slot, int front, int n_q_heads, const tt_half *q, long long q_seq_stride,
                            long long q_tok_stride, const tt_half *gate, long long g_seq_stride, long long g_tok_stride, float scale,
                            tt_half *out, long long o_seq_stride, long long o_tok_stride) {
-    const int seqs_at_once = std::min(kSharedTokens / rows, kMaxSeqPerLaunch);
-    if (n_seq == 1 || seqs_at_once <= 1)
+    const int seqs_at_once = shared_seqs_at_once(n_seq, rows);
+    if (seqs_at_once == 1)
         return run_one_pass(ctx, kv, 0, layer, n_seq, slots, starts, totals, rows, prefix_slot, front, n_q_heads, q, q_seq_stride, q_tok_stride, gate,
                             g_seq_stride, g_tok_stride, scale, out, o_seq_stride, o_tok_stride);
     for (int base = 0; base < n_seq; base += seqs_at_once) {

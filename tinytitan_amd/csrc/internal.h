@@ -9,10 +9,10 @@
 
 #include "../../include/ctinytitan_hip.h"
 #include "kv_layout.h"
+#include "shared_plan.h"
 
 namespace tt {
 
-constexpr int kMaxSeqPerLaunch = 64;
 // A wavefront of the split-K kernel lists the blocks that a per-query selection touches, over up to this many
 // 64-block windows of its split: a split of such a launch is at most kKeepWindows * 64 blocks per wavefront.
 constexpr int kKeepWindows = 8;
@@ -42,7 +42,6 @@ constexpr int kHotFront = 16;
 constexpr int kKeepSinks = 6;  // that kernel's KEEP (attn_splitk.hip)
 constexpr int kKeepPieces = 7;  // ... and of two passes in one launch, over the keys that sequences share and over their own
 constexpr int kKeepRows = 8;    // ... with the first of them over tiles of kFrontRows packed rows, whose wavefronts share a block of keys in LDS
-constexpr int kFrontRows = 128;
 struct SplitKHot {                         // dword
     const _Float16 *k_layer;               //  0
     const _Float16 *v_layer;               //  2
@@ -110,21 +109,6 @@ constexpr bool lists_fetch_by_key(int head_dim, int kv_bits) { return head_dim >
 inline bool launch_fetches_by_key(int head_dim, int kv_bits, long long n_tiles, long long entries, int keys, int n_cus) {
     return lists_fetch_by_key(head_dim, kv_bits) && (head_dim == 256 || (4 * n_tiles >= 3ll * n_cus && entries < keys));
 }
-
-struct LaunchPlan {
-    int nt;  // 16 or 32 query rows per tile
-    int gh, tt, hsubs, tok_tiles, n_tiles;
-    int waves;
-    int split_len, n_splits_max;
-    long long workgroups;
-    size_t lds_bytes;
-    bool stream;  // every K/V byte is read once by the launch, and there are many of them: non-temporal loads
-    bool paired;  // ... and V operands in pairs, over heads of 256 in tiles of 32 rows
-    bool xcd_grid;  // launch with kHotXcdGrid
-    int slots_per_cu;  // workgroups that the planner's rule for unlike lengths counts on
-    int packed_splits;  // > 0: launch with kHotPackedSplits over this many splits
-    bool partials_only;  // the partial results are somebody else's to combine (PassParts)
-};
 
 // Two passes in one launch (kKeepPieces, kKeepRows): workgroups [0, front_groups) are those of the base's, a chunk's token tiles dealt out XCD by XCD
 // (kHotXcdGrid), the others, tile fastest, the packed splits of `own` (kHotPackedSplits).

@@ -1334,18 +1334,19 @@ static int run_shared(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, cons
     if (st != TT_HIP_OK) return st;
     PageSource staged{};
     const PageSource *pages = nullptr;
+    if (plan.way == SharedWay::ranges) {
+        st = ensure_partials(ctx, (size_t)plan.ranges.n_splits * n_q_heads * ((tokens + 31) / 32) * 32, D, true);
+        if (st == TT_HIP_OK && kv->bits != 16) st = ensure_stage(ctx, (size_t)front * D * kv->n_kv_heads);
+        // (no room for their results or the dequantised pages, or none to be had inside a capture: a way that needs neither)
+        if (st == TT_HIP_ERR_BUSY || st == TT_HIP_ERR_OUT_OF_MEMORY) plan.way = plan.without_ranges;
+        else if (st != TT_HIP_OK) return st;
+    }
     if (plan.way == SharedWay::ranges && kv->bits != 16) {
         const size_t page = (size_t)front * D;
-        st = ensure_stage(ctx, page * kv->n_kv_heads);
-        if (st == TT_HIP_OK) {
-            st = launch_kvq_dequant_blocks(kv, layer, prefix_slot, front / kBlockTokens, ctx->stage_k, ctx->stage_v, page);
-            staged = PageSource{ctx->stage_k, ctx->stage_v, (long long)page, 0};
-            pages = &staged;
-        } else if (st == TT_HIP_ERR_BUSY || st == TT_HIP_ERR_OUT_OF_MEMORY) {
-            plan.way = plan.without_ranges;  // (no room for them, or none to be had inside a capture: the pages as they are)
-            st = TT_HIP_OK;
-        }
+        st = launch_kvq_dequant_blocks(kv, layer, prefix_slot, front / kBlockTokens, ctx->stage_k, ctx->stage_v, page);
         if (st != TT_HIP_OK) return st;
+        staged = PageSource{ctx->stage_k, ctx->stage_v, (long long)page, 0};
+        pages = &staged;
     }
     if (plan.way == SharedWay::one_pass)
         return run_one_pass(ctx, kv, 0, layer, n_seq, slots, starts, totals, rows, prefix_slot, front, n_q_heads, q, q_seq_stride, q_tok_stride, gate,

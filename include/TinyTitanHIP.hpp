@@ -219,7 +219,7 @@ public:
                                  numQHeads, q, gate, scale, out),
               "Attention.encodeBatch");
     }
-    // The same for slots that share a prefix, which is read once for all of them.
+    // The same for slots that share a prefix, which is stored once for all of them (see tt_hip_attn_decode_shared for how often it is read).
     void encodeBatch(KVCacheManager &kv, int layer, const std::vector<int> &slots, const std::vector<int> &seqLens, SharedPrefix prefix,
                      const tt_half *q, tt_half *out, int numQHeads, float scale, const tt_half *gate = nullptr) {
         if (slots.size() != seqLens.size()) throw Error(TT_HIP_ERR_INVALID_ARGUMENT, "Attention.encodeBatch");

@@ -332,6 +332,8 @@ TT_HIP_API int tt_hip_kv_expect_position(const tt_hip_kv *kv, int slot, int posi
  * A slot that started so is no prefix_slot itself, here or in a _shared call (TT_HIP_ERR_CURSOR): a conversation that forks from it
  * is shared from the slot that holds the prefix.  Nor is it served behind a shorter prefix than it started from, but for one that it
  * has been rewound to.  tt_hip_kv_reset, a rewind to 0 and a restored snapshot end this: the rows are the slot's own then.
+ * What is shared is written and read, not room: pages are n_slots x capacity rows whatever they hold, so a listed slot's rows below
+ * prefix_len & ~31 stay reserved, unused.
  * TT_HIP_ERR_INVALID_ARGUMENT: a slot out of range, or prefix_slot itself among the slots; TT_HIP_ERR_CURSOR: prefix_slot has fewer
  * rows, or starts from another's; TT_HIP_ERR_SHAPE: a ring. */
 TT_HIP_API int tt_hip_kv_share_prefix(tt_hip_kv *kv, int prefix_slot, int prefix_len, int n_slots, const int *slots);
@@ -499,14 +501,17 @@ TT_HIP_API int tt_hip_attn_prefill_sinks(tt_hip_ctx *ctx, tt_hip_kv *kv, int lay
                                          size_t o_stride);
 
 /* Sequences that share a prefix (tt_hip_kv_share_prefix): tt_hip_attn_decode, _verify and _prefill with the keys of positions
- * [0, prefix_len) taken from prefix_slot, which the call reads once for all of its rows -- as it reads a chunk's keys -- and not
- * once per sequence: many samples of one prompt, many users behind one system prompt, and a session's own first chunk behind it.
+ * [0, prefix_len) taken from prefix_slot, where they are stored once for all: many samples of one prompt, many users behind one system
+ * prompt, and a session's own first chunk behind it.  They are read once for all rows of a call, as a chunk's keys are, or once per sequence,
+ * whichever is estimated to take less time; at most 64 sequences and 1,024 rows of all together are served at a time, and sequences of more
+ * than 512 rows each read them for themselves.
  * The rest of a row's keys are its own slot's.  Every sequence of a call starts from the same prefix (one call per prefix); a
  * sequence has prefix_len keys at least (seq_lens[i] >= prefix_len, start positions + 1 >= prefix_len), else
  * TT_HIP_ERR_INVALID_ARGUMENT.  prefix_slot may be one of the slots; prefix_len below 32 is the plain call.  Results are those of the
- * plain call over slots that hold the prefix's rows themselves, up to the order of the additions.  Not over a ring (TT_HIP_ERR_SHAPE).
- * The partial results of the pass over the prefix live in a store the context owns (grown on demand: TT_HIP_ERR_BUSY inside a
- * graph capture if it has to grow).  No counterpart in the reference, whose slots each hold their prompt. */
+ * plain call over slots that hold the prefix's rows themselves, up to the order of the additions.  Not over a ring (TT_HIP_ERR_SHAPE);
+ * TT_HIP_ERR_CURSOR where a slot does not hold what the call takes from it (tt_hip_kv_share_prefix).
+ * The partial results of the passes over the pieces live in stores the context owns (grown on demand: TT_HIP_ERR_BUSY inside a
+ * graph capture if they have to grow and no other way of the call does without).  No counterpart in the reference, whose slots each hold their prompt. */
 TT_HIP_API int tt_hip_attn_decode_shared(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, const int *slots,
                                          const int *seq_lens, int prefix_slot, int prefix_len, int n_q_heads, const tt_half *q,
                                          const tt_half *gate, float scale, tt_half *out);

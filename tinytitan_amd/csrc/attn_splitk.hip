@@ -1087,8 +1087,10 @@ __device__ __forceinline__ void load_row_words(unsigned (&dst)[8], __amdgpu_buff
 // each tile that walks it, which is what those tiles wait for (18 tokens of 24/2 heads of 256 over 12,320 keys over 4 bits 36 us, here 27).
 //
 // What bounds it: a block is 4 D / 32 MFMAs of 32 cycles a wavefront, and as many KiB that each of the four reads out of LDS at 128 bytes a
-// cycle between them, as long; the CU has one such workgroup with heads of 256 and nothing else to cover a wait.  So a block's scores are due one
-// block ahead, beside the softmax of the block before; operands are four products ahead of their use, the next block's stores and
+// cycle between them, as long; the CU has one such workgroup with heads of 256 and nothing else to cover a wait.  (Counted over a launch of
+// 64 tokens of 16/2 heads of 256, 30,011 shared keys and their own: products 36 % of the wavefronts' time, the issue of vector instructions 28,
+// waits 28, that for LDS instructions among them 7: no unit is full, a lone wavefront a SIMD does its parts one after the other.)  So a block's
+// scores are due one block ahead, beside the softmax of the block before; operands are four products ahead of their use, the next block's stores and
 // widening lie between the products, and its loads are two blocks ahead, in registers.  LDS holds K of two blocks and V of two.  A block of
 // 128 rows of 256 takes 0.84 us (read, wait, multiply in turn 1.35; with the softmax between the products 0.91), over 4 bits 1.13 (1.67),
 // of 128 over fp16 / 8 bits 0.57 / 0.67.

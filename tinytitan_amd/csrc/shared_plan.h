@@ -120,10 +120,13 @@ inline int plan_pieces(const SharedCall &c, bool packed_rows, PairPlan *p) {
 //    sequence's rows leave mostly empty;
 //  * the same, the shared keys by tiles of 128 packed rows: for more rows than a split-K tile has;
 //  * the chunk kernel over ranges of the shared keys, its scores and values on wavefronts of their own, a pass over the own keys, and the join.
-// One pass / two / two with packed rows / ranges, us, 100 own keys: one row a sequence of 16/2 heads of
-// 256, 2 behind 2,000 9.1 / 11.0 / 13.3 / 24, 20 behind 6,000 18.3 / 16.3 / 23.5 / 29.5, 64 behind 20,000 92.8 / 44.9 / 44.0 / 47.7; 24/2 heads over 4
+// One pass / two / two with packed rows / ranges, us, 100 own keys: one row a sequence of 16/2 heads of 256, 2 behind 2,000 9.1 / 11.0 / 13.3 / 24, 20 behind 6,000 18.3 / 16.3 / 23.5 / 29.5, 64 behind 20,000 92.8 / 44.9 / 44.0 / 47.7; 24/2 heads over 4
 // bits, 20 behind 20,000 60 / 80 / 39 / 51; 32/8 of 128 over 8 bits, 20 behind 6,000 56 / 18.9 / 20.1 / 32.6, behind 20,000 177 / 44.5 / 33.2 / 57.7; four
 // rows a sequence, 64 of 24/2 of 256 behind 2,000 39.4 / 91.6 / 50.4 / 56.6, behind 20,000 267 / 290 / 160 / 153.
+// Between ranges and the rest the estimates are the coarsest.  Ranges / what the call takes without them, of calls that are sent to ranges: heads of
+// 256, 16/2, 64 x 16 rows behind 4,096 140 / 166, 5 x 200 158 / 224, over 8 bits 64 x 4 behind 20,011 121 / 134; 24/2, 3 x 100 behind 4,100 78 / 185, over
+// 8 bits 8 x 100 behind 1,055 204 / 363, over 4 bits 64 x 2 behind 32,768 142 / 166, but 5 x 200 behind 2,080 over 16 bits 260 / 186; heads of 128, 32/8,
+// 64 x 4 rows behind 4,096 57.8 / 51.8, over 8 bits 64 x 16 168 / 147, 32/4, 32 x 32 161 / 127.
 enum class SharedWay { one_pass, tiles, packed_rows, ranges };
 struct SharedPlan {
     SharedWay way;

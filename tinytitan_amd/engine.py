@@ -249,7 +249,7 @@ class KVCacheManager:
     def share_prefix(self, prefix_slot: int, length: int, slots: Sequence[int]) -> None:
         """The listed slots start from rows ``[0, length)`` of ``prefix_slot``: nothing is copied but the last part block, and the
         slots' cursors are set to ``length``.  Attention calls then take ``prefix=SharedPrefix(prefix_slot, length)``.  A slot that starts
-        from another's rows is no ``prefix_slot`` itself until it is reset."""
+        from another's rows is no ``prefix_slot`` itself until it is reset.  Room is not saved: the slots' pages keep theirs."""
         table = capi.int_array(slots)
         self.ctx._check(self._lib.tt_hip_kv_share_prefix(self.handle, prefix_slot, length, len(table), table), "tt_hip_kv_share_prefix")
 
@@ -369,7 +369,7 @@ class Attention:
                     prefix: Optional[SharedPrefix] = None) -> None:
         """``seq_len`` is the exclusive key count (position + 1).  ``slot``/``seq_len`` may be
         lists for the batched form (one query token per sequence).  With ``prefix`` the keys of its positions are its slot's, read
-        once for all sequences."""
+        once for all sequences or once for each, whichever is estimated to be faster."""
         if prefix is not None:
             status = self._calls.attn_decode_shared(self.ctx.handle, kv.handle, layer, slot, seq_len, prefix.slot, prefix.length, num_q_heads,
                                                     q, gate, scale, out)

@@ -50,7 +50,7 @@ inline int plan_splitk(int n_cus, int split_override, int kind, int n_seq, int n
         //    pages the 32-row tile is dearer still (4 rows at 64k keys over 8 bits 28.6 -> 24.6 us).
         //  * A short chunk behind a short context (more tiles, which re-read the same keys from L2), as long as the
         //    tiles are one round of workgroups: 32 rows from position 0 11.0 -> 6.5 us, 128 rows behind 1024 keys
-        //    18.7 -> 15.0, 256 rows behind 1024 keys 22.8 -> 17.4; 128 rows behind 3072 keys 26.4 against 29.2 the
+        //    18.7 -> 15.0, 256 rows behind 1024 keys 22.8 -> 17.4; 128 rows behind 3k keys 26.4 against 29.2 the
         //    other way, and 512 rows from position 0 were 17.0 against 19.7.
         // With 8 KV heads of 128 the same counts hold per KV head four times earlier (4 sequences x 16 rows at 4k keys:
         // 22.2 us in tiles of 32, 27.2 in tiles of 16; 8 rows at 8k keys 15.1 against 13.9), with 4 of 64 twice.

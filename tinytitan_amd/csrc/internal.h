@@ -39,7 +39,7 @@ constexpr int kHotPackedSplits = 4;
 constexpr int kHotSinks = 8, kHotPinnedShift = 8;
 // The same kernel for a prefix in another slot: keep_words is that slot, and from kHotPinnedShift on the flags hold the prefix's blocks.
 constexpr int kHotFront = 16;
-constexpr int kKeepSinks = 6;  // that kernel's KEEP (attn_splitk.hip)
+constexpr int kKeepSinks = 6;  // that kernel's KEEP (splitk_kernel.h)
 constexpr int kKeepPieces = 7;  // ... and of two passes in one launch, over the keys that sequences share and over their own
 constexpr int kKeepRows = 8;    // ... with the first of them over tiles of kFrontRows packed rows, whose wavefronts share a block of keys in LDS
 struct SplitKHot {                         // dword
@@ -97,7 +97,7 @@ struct alignas(64) SplitKArgs {
     int plan_cap;                 // entries a tile's list has room for
 };
 
-// Whether a chunk's lists, walked block by block, may fetch a touched block's kept keys only (Voids in attn_splitk.hip), or
+// Whether a chunk's lists, walked block by block, may fetch a touched block's kept keys only (Voids in splitk_kernel.h), or
 // always the block whole: the offsets by key cost a block's turn the same whatever its bytes.  By key / whole: 16/4 of 64, 300
 // rows behind 25,000 88.5 / 85.2 us; 8 bits, 8/2 of 256, 489 rows behind 257,507 789 / 755.
 constexpr bool lists_fetch_by_key(int head_dim, int kv_bits) { return head_dim >= 128 && kv_bits == 16; }

@@ -9,7 +9,7 @@
 
 namespace tt {
 
-constexpr int kFrontRows = 128;      // rows of a tile that packs the rows of all sequences (attn_splitk.hip)
+constexpr int kFrontRows = 128;      // rows of a tile that packs the rows of all sequences (splitk_kernel.h)
 constexpr int kSharedTokens = 1024;  // rows of all sequences together that are served at a time, so that the partial results stay small
 // Sequences that are served at a time: 1 where there is nobody to share with.
 inline int shared_seqs_at_once(int n_seq, int rows) { return std::max(std::min({n_seq, kMaxSeqPerLaunch, kSharedTokens / rows}), 1); }
@@ -43,7 +43,7 @@ inline double partials_us(double rows, int D) { return rows * D * 8.0 / 2.5e6; }
 // packed, in 128 / 512 / 1,024 / 2,048 26 / 17.6 / 17.4 / 23.6).
 struct PairPlan {
     LaunchPlan tiles;
-    bool packed_rows;  // the shared keys by tiles of kFrontRows packed rows (attn_splitk.hip); tiles.nt and .tt are those of the own keys' tiles
+    bool packed_rows;  // the shared keys by tiles of kFrontRows packed rows (splitk_kernel.h); tiles.nt and .tt are those of the own keys' tiles
     int own_tok_tiles, own_tiles, len;
     double us;  // with the join behind it
 };

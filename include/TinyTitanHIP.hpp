@@ -342,6 +342,84 @@ private:
     Context &context_;
 };
 
+// Attention whose weights are the difference of two softmax maps (no counterpart in the reference): a q head's row is two queries, its
+// KV head's key row two keys of half the head's dims.  lambdas: fp32 factors, one per q head, or a row of them per token
+// (lambdaStride floats apart; 0: one row for all tokens).
+struct DifferentialHeads {
+    const float *lambdas = nullptr;
+    size_t lambdaStride = 0;
+    const uint16_t *normWeightBF16 = nullptr;  // [headDim], of the norm over a head's values; null: no norm
+    float eps = 1e-5f;
+    float outScale = 1.0f;
+};
+
+class DifferentialAttention {
+public:
+    explicit DifferentialAttention(Context &context) : context_(context) {}
+    // lambdas[h] = exp(q1[h] . k1[h]) - exp(q2[h] . k2[h]) + lambdaInit over vectors of `dims` floats, vectorStride apart (0: one for all heads).
+    void encodeLambda(const float *q1, const float *k1, const float *q2, const float *k2, size_t vectorStride, int heads, int dims,
+                      float lambdaInit, float *lambdas) {
+        check(tt_hip_diff_lambda(context_.handle(), q1, k1, q2, k2, vectorStride, heads, dims, lambdaInit, lambdas),
+              "DifferentialAttention.encodeLambda");
+    }
+    void encodeBatch(KVCacheManager &kv, int layer, const std::vector<int> &slots, const std::vector<int> &seqLens, const tt_half *q,
+                     tt_half *out, int numQHeads, float scale, const DifferentialHeads &heads, const tt_half *gate = nullptr,
+                     int window = 0) {
+        if (slots.size() != seqLens.size()) throw Error(TT_HIP_ERR_INVALID_ARGUMENT, "DifferentialAttention.encodeBatch");
+        check(tt_hip_attn_decode_diff(context_.handle(), kv.handle(), layer, (int)slots.size(), slots.data(), seqLens.data(), window,
+                                      numQHeads, q, gate, scale, heads.lambdas, heads.lambdaStride, heads.normWeightBF16, heads.eps,
+                                      heads.outScale, out),
+              "DifferentialAttention.encodeBatch");
+    }
+    void encodeVerifyRows(KVCacheManager &kv, int layer, const std::vector<int> &slots, const std::vector<int> &startPositions, int rows,
+                          const tt_half *q, tt_half *out, int numQHeads, float scale, const DifferentialHeads &heads,
+                          const tt_half *gate = nullptr, int window = 0) {
+        if (slots.size() != startPositions.size()) throw Error(TT_HIP_ERR_INVALID_ARGUMENT, "DifferentialAttention.encodeVerifyRows");
+        check(tt_hip_attn_verify_diff(context_.handle(), kv.handle(), layer, (int)slots.size(), slots.data(), startPositions.data(), rows,
+                                      window, numQHeads, q, gate, scale, heads.lambdas, heads.lambdaStride, heads.normWeightBF16, heads.eps,
+                                      heads.outScale, out),
+              "DifferentialAttention.encodeVerifyRows");
+    }
+    void encodeCausal(KVCacheManager &kv, int layer, int slot, const tt_half *q, tt_half *out, const PrefillAttentionParams &p,
+                      const DifferentialHeads &heads, const tt_half *gate = nullptr) {
+        if (p.sinks) throw Error(TT_HIP_ERR_INVALID_ARGUMENT, "DifferentialAttention.encodeCausal");
+        check(tt_hip_attn_prefill_diff(context_.handle(), kv.handle(), layer, slot, p.startPosition, p.queryCount, p.kvValidCount,
+                                       p.slidingWindow, p.numQHeads, q, p.qStride, gate, p.gateStride ? p.gateStride : p.qStride, p.scale,
+                                       heads.lambdas, heads.lambdaStride, heads.normWeightBF16, heads.eps, heads.outScale, out, p.oStride),
+              "DifferentialAttention.encodeCausal");
+    }
+
+private:
+    Context &context_;
+};
+
+// Products of 8-bit integers with a scale for each token and each output channel (no counterpart in the reference, whose 8-bit weights are
+// affine): strides in elements, 0 = packed.
+class Int8Projection {
+public:
+    explicit Int8Projection(Context &context) : context_(context) {}
+    void encode(const int8_t *weights, const float *weightScales, const tt_half *x, tt_half *y, int rows, int columns, int tokenCount,
+                size_t xStride = 0, size_t yStride = 0) {
+        check(tt_hip_int8_projection(context_.handle(), weights, weightScales, x, xStride ? xStride : (size_t)columns, y, rows, columns,
+                                     tokenCount, yStride ? yStride : (size_t)rows),
+              "Int8Projection.encode");
+    }
+    void quantise(const tt_half *x, int8_t *levels, float *scales, int columns, int tokenCount, size_t xStride = 0, size_t levelsStride = 0) {
+        check(tt_hip_int8_quantise_rows(context_.handle(), x, xStride ? xStride : (size_t)columns, tokenCount, columns, levels,
+                                        levelsStride ? levelsStride : (size_t)columns, scales),
+              "Int8Projection.quantise");
+    }
+    void encodeLevels(const int8_t *weights, const float *weightScales, const int8_t *levels, const float *scales, tt_half *y, int rows,
+                      int columns, int tokenCount, size_t levelsStride = 0, size_t yStride = 0) {
+        check(tt_hip_int8_projection_levels(context_.handle(), weights, weightScales, levels, levelsStride ? levelsStride : (size_t)columns,
+                                            scales, y, rows, columns, tokenCount, yStride ? yStride : (size_t)rows),
+              "Int8Projection.encodeLevels");
+    }
+
+private:
+    Context &context_;
+};
+
 // encodeAffineProjection for o_proj (RealForwardRunner+PrefillProjection.swift:53-66) and the decode
 // GEMVs behind the gate (DequantInt4GEMV.swift:72-143): strides in elements, 0 = packed.
 class AffineProjection {

@@ -523,6 +523,41 @@ TT_HIP_API int tt_hip_attn_prefill_shared(tt_hip_ctx *ctx, tt_hip_kv *kv, int la
                                           size_t q_stride, const tt_half *gate, size_t gate_stride, float scale, tt_half *out,
                                           size_t o_stride);
 
+/* Differential attention: a head's weights are the difference of two softmax maps.  A q head's row is two queries of head_dim / 2 one
+ * behind the other, its KV head's key row two keys, its value row one value of head_dim:
+ *   a   = sum_j softmax_j(scale q1 . k1_j) v_j - lambda sum_j softmax_j(scale q2 . k2_j) v_j        (scale: (head_dim / 2)^-1/2, usually)
+ *   out = sigmoid(gate) * out_scale * norm_weight * a / sqrt(mean(a^2) + eps)
+ * The cache is the one of the other calls, whose rows the caller writes as they come (tt_hip_kv_append; positions' rotations on
+ * either half by itself), of every precision, linear or a ring.  Which keys a row sees, the shapes and the strides are those of
+ * tt_hip_attn_decode_swa, _verify_swa and _prefill_swa; window 0 is every key up to the row's own.
+ *   lambda         fp32, one factor per q head: row t of the call (sequence by sequence) takes lambda[t * lambda_stride + head]; a stride
+ *                  of 0 is one row for all tokens (factors that come from a token's own projection have one of n_q_heads or more).
+ *                  tt_hip_diff_lambda makes a layer's row from its learned vectors.
+ *   norm_weight_bf16, eps   the norm over a head's values, its weight [head_dim] bfloat16; NULL: no norm.  out_scale belongs to either
+ *                  (1 - lambda_init, as such models have it; 1 otherwise).
+ *   gate           the sigmoid gate behind that, or NULL.
+ * Softmax statistics, sums, difference and norm are in fp32, with one rounding to fp16.  A row without a visible key (a sequence of
+ * length 0) gives zeros.  Values of keys that no row of a call sees do not reach it, whatever the cache holds there.
+ * Both maps come from one pass over the cache.  No counterpart in the reference.
+ * TT_HIP_ERR_INVALID_ARGUMENT: a NULL lambda, an eps below zero or NaN; TT_HIP_ERR_SHAPE: a lambda_stride between 0 and n_q_heads;
+ * TT_HIP_ERR_CURSOR: a slot that starts from another slot's prefix (tt_hip_kv_share_prefix); TT_HIP_ERR_CAPACITY as for the _swa calls, and
+ * for a ring that keeps sinks as soon as a sequence has outgrown it. */
+TT_HIP_API int tt_hip_attn_decode_diff(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, const int *slots, const int *seq_lens,
+                                       int window, int n_q_heads, const tt_half *q, const tt_half *gate, float scale, const float *lambda,
+                                       size_t lambda_stride, const uint16_t *norm_weight_bf16, float eps, float out_scale, tt_half *out);
+TT_HIP_API int tt_hip_attn_verify_diff(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, const int *slots, const int *start_positions,
+                                       int rows, int window, int n_q_heads, const tt_half *q, const tt_half *gate, float scale,
+                                       const float *lambda, size_t lambda_stride, const uint16_t *norm_weight_bf16, float eps,
+                                       float out_scale, tt_half *out);
+TT_HIP_API int tt_hip_attn_prefill_diff(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int slot, int start_pos, int q_len, int kv_valid,
+                                        int window, int n_q_heads, const tt_half *q, size_t q_stride, const tt_half *gate,
+                                        size_t gate_stride, float scale, const float *lambda, size_t lambda_stride,
+                                        const uint16_t *norm_weight_bf16, float eps, float out_scale, tt_half *out, size_t o_stride);
+/* lambda[h] = exp(q1[h] . k1[h]) - exp(q2[h] . k2[h]) + lambda_init, fp32, for the learned vectors of `dims` values that lie
+ * vector_stride floats apart from head to head (0: the same ones for all heads).  Once per layer, when a model is loaded. */
+TT_HIP_API int tt_hip_diff_lambda(tt_hip_ctx *ctx, const float *q1, const float *k1, const float *q2, const float *k2,
+                                  size_t vector_stride, int n_heads, int dims, float lambda_init, float *lambda);
+
 /* Multi-row verify (MTP pair / wide verify): replaces
  * encodeFullAttentionDecodeOrderRows (RealForwardRunner+VerifyDecodeOrderAttention.swift:52-110)
  * and verifyGreedyPair's 2-token prefill (RealForwardRunner+MTPVerify.swift:57-103).
@@ -626,6 +661,30 @@ TT_HIP_API int tt_hip_affine_projection(tt_hip_ctx *ctx, int weight_bits, const 
                                         const uint16_t *scales_bf16, const uint16_t *biases_bf16, const tt_half *x,
                                         tt_half *y, int rows, int columns, int token_count, size_t x_stride,
                                         size_t y_stride);
+
+/* Products of 8-bit integers with a scale for each token and each output channel, as models are served whose weights and activations
+ * are both held in 8 bits: y[t][r] = scales[t] * weight_scales[r] * sum_k weights[r][k] * levels[t][k], the sum exact in 32-bit
+ * integers, the scaling in fp32 with one rounding to fp16.
+ *   weights        int8 [rows][columns], row-major; weight_scales fp32 [rows]
+ *   x              fp16 [token][columns], token stride x_stride elements; a token is quantised on the way:
+ *                  scales[t] = max |x[t]| / 127, levels[t] = round(x[t] / scales[t]), both divisions and the rounding (ties to even)
+ *                  as fp32 has them.  A token of zeros has zeros; of one with an infinite or NaN element every output is NaN (its scale
+ *                  is NaN, its levels zero), and no other token's.
+ *   y              fp16 [token][rows], token stride y_stride elements, written, not accumulated.
+ * tt_hip_int8_projection takes fp16 tokens; where several projections share their input, tt_hip_int8_quantise_rows does that part
+ * once (levels int8 [token][columns], levels_stride bytes apart; scales fp32 [token]) and tt_hip_int8_projection_levels the rest, with the
+ * same results bit for bit.  The tokens that a call quantises itself go to a store that the context owns (grown on demand:
+ * TT_HIP_ERR_BUSY inside a graph capture if it has to grow).  No counterpart in the reference, whose 8-bit weights are affine
+ * (tt_hip_affine_projection).
+ * TT_HIP_ERR_SHAPE: columns not a multiple of 16 or 131,072 and more (whose sums could leave 32 bits), strides below the row widths, x,
+ * levels or weights not 16-byte aligned, x_stride not a multiple of 8, levels_stride not one of 16. */
+TT_HIP_API int tt_hip_int8_projection(tt_hip_ctx *ctx, const int8_t *weights, const float *weight_scales, const tt_half *x, size_t x_stride,
+                                      tt_half *y, int rows, int columns, int token_count, size_t y_stride);
+TT_HIP_API int tt_hip_int8_quantise_rows(tt_hip_ctx *ctx, const tt_half *x, size_t x_stride, int token_count, int columns, int8_t *levels,
+                                         size_t levels_stride, float *scales);
+TT_HIP_API int tt_hip_int8_projection_levels(tt_hip_ctx *ctx, const int8_t *weights, const float *weight_scales, const int8_t *levels,
+                                             size_t levels_stride, const float *scales, tt_half *y, int rows, int columns, int token_count,
+                                             size_t y_stride);
 
 /* ---- The sparse-attention block indexer: what produces the selections that
  * tt_hip_attn_decode_keep / tt_hip_attn_prefill_keep / tt_hip_kv_gather take.  Buffers are the

@@ -103,6 +103,16 @@ _SIGNATURES = {
     "tt_hip_attn_decode_shared": (_i, [_vp, _vp, _i, _i, _c_int_p, _c_int_p, _i, _i, _i, _vp, _vp, ctypes.c_float, _vp]),
     "tt_hip_attn_verify_shared": (_i, [_vp, _vp, _i, _i, _c_int_p, _c_int_p, _i, _i, _i, _i, _vp, _vp, ctypes.c_float, _vp]),
     "tt_hip_attn_prefill_shared": (_i, [_vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _sz, _vp, _sz, ctypes.c_float, _vp, _sz]),
+    "tt_hip_attn_decode_diff": (_i, [_vp, _vp, _i, _i, _c_int_p, _c_int_p, _i, _i, _vp, _vp, ctypes.c_float, _vp, _sz, _vp, ctypes.c_float,
+                                     ctypes.c_float, _vp]),
+    "tt_hip_attn_verify_diff": (_i, [_vp, _vp, _i, _i, _c_int_p, _c_int_p, _i, _i, _i, _vp, _vp, ctypes.c_float, _vp, _sz, _vp, ctypes.c_float,
+                                     ctypes.c_float, _vp]),
+    "tt_hip_attn_prefill_diff": (_i, [_vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _sz, _vp, _sz, ctypes.c_float, _vp, _sz, _vp, ctypes.c_float,
+                                      ctypes.c_float, _vp, _sz]),
+    "tt_hip_diff_lambda": (_i, [_vp, _vp, _vp, _vp, _vp, _sz, _i, _i, ctypes.c_float, _vp]),
+    "tt_hip_int8_projection": (_i, [_vp, _vp, _vp, _vp, _sz, _vp, _i, _i, _i, _sz]),
+    "tt_hip_int8_quantise_rows": (_i, [_vp, _vp, _sz, _i, _i, _vp, _sz, _vp]),
+    "tt_hip_int8_projection_levels": (_i, [_vp, _vp, _vp, _vp, _sz, _vp, _vp, _i, _i, _i, _sz]),
     "tt_hip_attn_verify": (_i, [_vp, _vp, _i, _i, _c_int_p, _c_int_p, _i, _i, _vp, _vp, ctypes.c_float, _vp]),
     "tt_hip_kv_snapshot_segment_count": (_i, [_vp]),
     "tt_hip_kv_snapshot_segment_lengths": (_i, [_vp, _i, ctypes.POINTER(ctypes.c_size_t), _i]),

@@ -1,0 +1,254 @@
+// Differential attention: a head's weights are the difference of two softmax maps over the cache.
+//
+//   a   = softmax(scale K1 q1) V - lambda softmax(scale K2 q2) V       q1, q2: the halves of the head's query row, K1, K2 those of
+//   out = gate * out_scale * weight * a / rms(a)                        the KV head's key rows; lambda per head, or per token and head
+//
+// The passes over K and V are those of plain attention with two rows a head: the split-K kernel's kKeepMaps, whose tiles take the maps of
+// the heads that share a KV head together, so that the cache is read once for both.  Here are its launches and the pass
+// behind it, which adds up the splits' partial results of both maps (as attn_join.hip does: the rows' o and l about a common
+// maximum), subtracts, and applies norm and gate in fp32 with one rounding.  A row that sees no key gives zeros.
+#include <algorithm>
+
+#include "splitk_kernel.h"
+
+namespace tt {
+
+namespace {
+
+typedef float f2 __attribute__((ext_vector_type(2)));
+
+// Row n of tile `tile` in split 0 of the pass, for token `tok` of a sequence and row `row` of the heads' maps.
+__device__ __forceinline__ size_t part_row(const PassParts &p, int group, int tok, int row) {
+    const int kvh = row / group, in_group = row - kvh * group;
+    const int hsub = in_group / p.gh, tok_tile = tok / p.tt;
+    const int tile = (kvh * p.hsubs + hsub) * p.tok_tiles + tok_tile;
+    return (size_t)tile * p.nt + (tok - tok_tile * p.tt) * p.gh + (in_group - hsub * p.gh);
+}
+
+// a1 - lambda a2 of the maps' sums and what they are divided by.  Either map's result is rounded before the difference, no product is
+// fused into it: maps that are the same then cancel to zero, and not to a rounding that the norm behind makes a row of.
+__device__ __forceinline__ f4 difference(f4 o1, float inv1, f4 o2, float inv2, float lambda) {
+#pragma clang fp contract(off)
+    const f4 a1 = o1 * inv1, a2 = o2 * inv2;
+    return a1 - lambda * a2;
+}
+
+// A (token, head) item is D / 4 threads of four dims each, and G of those that share its splits; a workgroup is ITEMS of them.
+template <int D, int G>
+__global__ __launch_bounds__(G * D / 4 > 256 ? G * D / 4 : 256) void attn_maps_join_kernel(const MapsJoinArgs a) {
+    constexpr int LANES = D / 4, THREADS = G * LANES > 256 ? G * LANES : 256, ITEMS = THREADS / (G * LANES), BATCH = 4;
+    __shared__ f4 sums[G > 1 ? 2 : 1][G][G > 1 ? ITEMS * LANES : 1];
+    __shared__ f2 stats[G > 1 ? 2 : 1][G][ITEMS];
+    const int lane = threadIdx.x % LANES, in_group = threadIdx.x / LANES, item = in_group % ITEMS, g = in_group / ITEMS;
+    const int d = lane * 4, seq = blockIdx.y;
+    const long long at_item = (long long)blockIdx.x * ITEMS + item;
+    const bool real = at_item < (long long)a.rows * a.heads;
+    const int row = real ? (int)(at_item / a.heads) : 0, head = real ? (int)(at_item - (long long)row * a.heads) : 0;
+    const JoinSeq sq = a.seq[seq];
+    // (asked for here, in front of the partial results)
+    const float lambda = a.maps.lambda[seq * a.lambda_seq_stride + row * a.maps.lambda_stride + head];
+    h4 gate = (h4)(_Float16)0.0f;
+    if (a.gate) {
+        gate = *(const __attribute__((address_space(1))) h4_unaligned *)(global_halves)(a.gate + seq * a.g_seq_stride + row * a.g_tok_stride + (long long)head * D + d);
+    }
+    f4 weight = (f4)1.0f;
+    if (a.maps.norm) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) weight[i] = __builtin_bit_cast(float, (unsigned)a.maps.norm[d + i] << 16);
+    }
+    // The tile's splits, as the pass counted them.
+    const PassParts &p = a.parts;
+    const int t0 = row / p.tt * p.tt, tile_end = max(0, min(sq.total, sq.start + min(t0 + p.tt, a.rows)));
+    const int first_lim = min(sq.total, sq.start + t0 + 1);
+    const int k0 = a.window > 0 && first_lim > a.window ? (first_lim - a.window) & ~31 : 0;
+    const int n = (int)((unsigned)(max(tile_end - k0, 1) + p.split_len - 1) / (unsigned)p.split_len);
+    const size_t stride = (size_t)p.n_tiles * p.nt;
+    f4 acc[2];
+    float m[2], l[2];
+#pragma unroll
+    for (int map = 0; map < 2; ++map) {
+        acc[map] = (f4)0.0f;
+        m[map] = kNegBig;
+        l[map] = 0.0f;
+    }
+    const size_t at[2] = {part_row(p, a.group2, row, 2 * head) + (size_t)sq.first_split * stride,
+                          part_row(p, a.group2, row, 2 * head + 1) + (size_t)sq.first_split * stride};
+    for (int first = g; first < n; first += G * BATCH) {
+        f4 o[2][BATCH];
+        f2 ml[2][BATCH];
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+            const size_t s = (size_t)min(first + i * G, n - 1) * stride;
+#pragma unroll
+            for (int map = 0; map < 2; ++map) {
+                ml[map][i] = *reinterpret_cast<const f2 *>(p.ml + (at[map] + s) * 2);
+                o[map][i] = *reinterpret_cast<const f4 *>(p.o + (at[map] + s) * D + d);
+            }
+        }
+#pragma unroll
+        for (int map = 0; map < 2; ++map) {
+            float top = m[map];
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) top = fmaxf(top, ml[map][i][0]);
+            const float keep = fast_exp2(m[map] - top);
+            l[map] *= keep;
+            acc[map] *= keep;
+            m[map] = top;
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) {
+                if (first + i * G >= n) break;  // (not a factor of zero, which an infinite value makes NaN of)
+                const float f = fast_exp2(ml[map][i][0] - top);
+                l[map] += f * ml[map][i][1];
+                acc[map] += f * o[map][i];
+            }
+        }
+    }
+    if constexpr (G > 1) {
+#pragma unroll
+        for (int map = 0; map < 2; ++map) {
+            sums[map][g][item * LANES + lane] = acc[map];
+            if (lane == 0) stats[map][g][item] = f2{m[map], l[map]};
+        }
+        __syncthreads();
+        if (g != 0) return;
+#pragma unroll
+        for (int map = 0; map < 2; ++map) {
+            float top = kNegBig;
+#pragma unroll 4
+            for (int i = 0; i < G; ++i) top = fmaxf(top, stats[map][i][item][0]);
+            acc[map] = (f4)0.0f;
+            l[map] = 0.0f;
+#pragma unroll 4
+            for (int i = 0; i < G; ++i) {
+                const float f = fast_exp2(stats[map][i][item][0] - top);
+                l[map] += f * stats[map][i][item][1];
+                acc[map] += f * sums[map][i][item * LANES + lane];
+            }
+        }
+    }
+    f4 out = difference(acc[0], l[0] > 0.0f ? 1.0f / l[0] : 0.0f, acc[1], l[1] > 0.0f ? 1.0f / l[1] : 0.0f, lambda);
+    float scale = a.maps.out_scale;
+    if (a.maps.norm) {
+        float squares = out[0] * out[0] + out[1] * out[1] + out[2] * out[2] + out[3] * out[3];
+#pragma unroll
+        for (int step = 1; step < LANES; step *= 2) squares += __shfl_xor(squares, step);
+        // (a row of zeros stays one, whatever eps is)
+        scale *= squares == 0.0f ? 0.0f : 1.0f / sqrtf(squares * (1.0f / D) + a.maps.eps);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        out[i] *= scale * weight[i];
+        if (a.gate) out[i] *= sigmoid((float)gate[i]);
+    }
+    if (!real) return;
+    _Float16 *const to = a.out + seq * a.o_seq_stride + row * a.o_tok_stride + (long long)head * D + d;
+    const h4 r = {(_Float16)out[0], (_Float16)out[1], (_Float16)out[2], (_Float16)out[3]};
+    if (a.aligned) {
+        *reinterpret_cast<h4 *>(to) = r;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) to[i] = r[i];
+    }
+}
+
+// A wavefront per head: lambda = exp(q1 . k1) - exp(q2 . k2) + init.
+__global__ __launch_bounds__(64) void diff_lambda_kernel(const float *q1, const float *k1, const float *q2, const float *k2, long long stride, int dims,
+                                                         float init, float *lambda) {
+    const long long at = blockIdx.x * stride;
+    float first = 0.0f, second = 0.0f;
+    for (int i = threadIdx.x; i < dims; i += 64) {
+        first += q1[at + i] * k1[at + i];
+        second += q2[at + i] * k2[at + i];
+    }
+#pragma unroll
+    for (int step = 32; step > 0; step /= 2) {
+        first += __shfl_xor(first, step);
+        second += __shfl_xor(second, step);
+    }
+    if (threadIdx.x == 0) lambda[blockIdx.x] = expf(first) - expf(second) + init;
+}
+
+template <int D, int G>
+void launch_join_of(tt_hip_ctx *ctx, int n_seq, const MapsJoinArgs &args) {
+    constexpr int THREADS = G * D / 4 > 256 ? G * D / 4 : 256, ITEMS = THREADS * 4 / (G * D);
+    const long long items = (long long)args.rows * args.heads;
+    hipLaunchKernelGGL((attn_maps_join_kernel<D, G>), dim3((unsigned)((items + ITEMS - 1) / ITEMS), (unsigned)n_seq), dim3(THREADS), 0, ctx->stream, args);
+}
+template <int D>
+void launch_join_by_splits(tt_hip_ctx *ctx, int n_seq, const MapsJoinArgs &args, int most_splits) {
+    if (most_splits <= 4) launch_join_of<D, 1>(ctx, n_seq, args);
+    else if (most_splits <= 16 || (long long)args.rows * args.heads * n_seq >= 4 * ctx->n_cus) launch_join_of<D, 4>(ctx, n_seq, args);
+    else launch_join_of<D, 16>(ctx, n_seq, args);
+}
+
+template <int D, int NT, int BITS, int STREAM>
+int launch_pass(tt_hip_ctx *ctx, const LaunchPlan &plan, int n_seq, const SplitKArgs &args) {
+    auto kernel = attn_splitk_kernel<D, NT, 4, BITS, kKeepMaps, STREAM>;
+    dim3 grid((unsigned)plan.n_splits_max, (unsigned)plan.n_tiles, (unsigned)n_seq);
+    if (plan.packed_splits > 0) grid = dim3((unsigned)plan.packed_splits, (unsigned)plan.n_tiles);
+    if (plan.xcd_grid) grid = dim3((unsigned)(((long long)plan.n_splits_max * plan.n_tiles + 7) / 8 * 8), 1u, (unsigned)n_seq);
+    launch_profiled(ctx, kernel, grid, dim3(256), (unsigned)plan.lds_bytes, args);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? TT_HIP_OK : hip_fail(ctx, e, "attn_splitk_kernel launch");
+}
+
+}  // namespace
+
+int configure_maps_kernels(tt_hip_ctx *ctx) {
+    hipError_t e = hipSuccess;
+#define TT_CFG(DD, NN, BB, SS) \
+    if (e == hipSuccess) e = hipFuncSetAttribute(reinterpret_cast<const void *>(attn_splitk_kernel<DD, NN, 4, BB, kKeepMaps, SS>), \
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_bytes_for(DD, NN, 4));
+#define TT_CFG_BITS(DD, NN) \
+    TT_CFG(DD, NN, 16, 0) TT_CFG(DD, NN, 16, 1) TT_CFG(DD, NN, 8, 0) TT_CFG(DD, NN, 8, 1) TT_CFG(DD, NN, 4, 0) TT_CFG(DD, NN, 4, 1)
+    TT_CFG_BITS(256, 16) TT_CFG_BITS(256, 32) TT_CFG_BITS(128, 16) TT_CFG_BITS(128, 32) TT_CFG_BITS(64, 16) TT_CFG_BITS(64, 32)
+#undef TT_CFG_BITS
+#undef TT_CFG
+    return e == hipSuccess ? TT_HIP_OK : hip_fail(ctx, e, "hipFuncSetAttribute(split-K max dynamic LDS)");
+}
+
+int launch_splitk_maps(tt_hip_ctx *ctx, const LaunchPlan &plan, int head_dim, int n_seq, const SplitKArgs &args, int kv_bits) {
+#define TT_CASE(DD, NN)                                                                                        \
+    if (head_dim == DD && plan.nt == NN) {                                                                     \
+        if (kv_bits == 16) return plan.stream ? launch_pass<DD, NN, 16, 1>(ctx, plan, n_seq, args) : launch_pass<DD, NN, 16, 0>(ctx, plan, n_seq, args); \
+        if (kv_bits == 8) return plan.stream ? launch_pass<DD, NN, 8, 1>(ctx, plan, n_seq, args) : launch_pass<DD, NN, 8, 0>(ctx, plan, n_seq, args);    \
+        if (kv_bits == 4) return plan.stream ? launch_pass<DD, NN, 4, 1>(ctx, plan, n_seq, args) : launch_pass<DD, NN, 4, 0>(ctx, plan, n_seq, args);    \
+    }
+    TT_CASE(256, 16)
+    TT_CASE(256, 32)
+    TT_CASE(128, 16)
+    TT_CASE(128, 32)
+    TT_CASE(64, 16)
+    TT_CASE(64, 32)
+#undef TT_CASE
+    return TT_HIP_ERR_SHAPE;
+}
+
+int launch_maps_join(tt_hip_ctx *ctx, int head_dim, int n_seq, const MapsJoinArgs &args, int most_splits) {
+    if (n_seq > kMaxSeqPerLaunch || (long long)args.rows * args.heads > 0x7fffffffll) return TT_HIP_ERR_SHAPE;
+    switch (head_dim) {
+        case 256: launch_join_by_splits<256>(ctx, n_seq, args, most_splits); break;
+        case 128: launch_join_by_splits<128>(ctx, n_seq, args, most_splits); break;
+        case 64: launch_join_by_splits<64>(ctx, n_seq, args, most_splits); break;
+        default: return TT_HIP_ERR_SHAPE;
+    }
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? TT_HIP_OK : hip_fail(ctx, e, "attn_maps_join_kernel launch");
+}
+
+}  // namespace tt
+
+using namespace tt;
+
+extern "C" int tt_hip_diff_lambda(tt_hip_ctx *ctx, const float *q1, const float *k1, const float *q2, const float *k2, size_t vector_stride, int n_heads,
+                                  int dims, float lambda_init, float *lambda) {
+    if (!ctx || !q1 || !k1 || !q2 || !k2 || !lambda || n_heads <= 0 || dims <= 0) return TT_HIP_ERR_INVALID_ARGUMENT;
+    if (vector_stride != 0 && vector_stride < (size_t)dims) return TT_HIP_ERR_SHAPE;
+    BusyGuard guard(ctx);
+    if (!guard.ok) return TT_HIP_ERR_BUSY;
+    if (hipSetDevice(ctx->device) != hipSuccess) return TT_HIP_ERR_HIP;
+    hipLaunchKernelGGL(diff_lambda_kernel, dim3((unsigned)n_heads), dim3(64), 0, ctx->stream, q1, k1, q2, k2, (long long)vector_stride, dims, lambda_init,
+                       lambda);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? TT_HIP_OK : hip_fail(ctx, e, "diff_lambda_kernel launch");
+}

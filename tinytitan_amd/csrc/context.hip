@@ -307,6 +307,7 @@ struct KeyPiece {
     int first_block = 0;  // the pages' blocks in front of the piece: starts and totals count from here
     PassParts parts{};
     int first_split[kMaxSeqPerLaunch] = {};
+    bool maps = false;  // the rows are those of two maps a head: n_q_heads counts both, q's rows are the heads'
 };
 static int run_attention(tt_hip_ctx *ctx, tt_hip_kv *kv, int kind, int layer, int n_seq, const int *slots,
                          const int *starts, const int *totals, int rows, int n_q_heads, const tt_half *q,
@@ -555,6 +556,7 @@ static int run_attention(tt_hip_ctx *ctx, tt_hip_kv *kv, int kind, int layer, in
                              q_tok_stride % 8 == 0 && g_seq_stride % 8 == 0 && g_tok_stride % 8 == 0 && o_seq_stride % 8 == 0 &&
                              o_tok_stride % 8 == 0;
         h.flags = (aligned ? kHotAligned : 0) | (plan.xcd_grid ? kHotXcdGrid : 0) | (plan.packed_splits > 0 ? kHotPackedSplits : 0);
+        if (piece && piece->maps) h.flags |= kHotMaps;
         h.scale_log2e = scale * 1.4426950408889634f;
         h.window = window;
         h.ring_blocks = walks_pages ? pages->ring_blocks : kv->ring_blocks();
@@ -705,6 +707,7 @@ tt_hip_ctx *tt_hip_ctx_create(int device, int *out_err) {
             int st = configure_splitk_kernels(ctx);
             if (st == TT_HIP_OK) st = configure_prefill_kernels(ctx);
             if (st == TT_HIP_OK) st = configure_affine_kernels(ctx);
+            if (st == TT_HIP_OK) st = configure_maps_kernels(ctx);
             if (st != TT_HIP_OK) {
                 tt_hip_ctx_destroy(ctx);
                 return fail(st);
@@ -728,6 +731,7 @@ void tt_hip_ctx_destroy(tt_hip_ctx *ctx) {
     if (ctx->stage_v) (void)hipFree(ctx->stage_v);
     if (ctx->select_ws) (void)hipFree(ctx->select_ws);
     if (ctx->keep_rows) (void)hipFree(ctx->keep_rows);
+    if (ctx->levels) (void)hipFree(ctx->levels);
     for (hipEvent_t ev : ctx->prof_events) (void)hipEventDestroy(ev);
     if (ctx->ev_begin) (void)hipEventDestroy(ctx->ev_begin);
     if (ctx->ev_end) (void)hipEventDestroy(ctx->ev_end);
@@ -1640,6 +1644,136 @@ int tt_hip_attn_prefill_swa(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int slot,
                             size_t gate_stride, float scale, tt_half *out, size_t o_stride) {
     return tt_hip_attn_prefill_sinks(ctx, kv, layer, slot, start_pos, q_len, kv_valid, sliding_window, 0, n_q_heads, q, q_stride, gate,
                                      gate_stride, scale, out, o_stride);
+}
+
+// ---- differential attention --------------------------------------------------
+
+// What a call reads of its sequences' slots: the keys [first, end), rows of the slot's own.
+static int check_maps_keys(const tt_hip_kv *kv, int slot, int window, long long start, long long end) {
+    if (slot < 0 || slot >= kv->n_slots) return TT_HIP_ERR_INVALID_ARGUMENT;
+    if (kv->borrowed[slot] > 0) return TT_HIP_ERR_CURSOR;
+    const long long first = window > 0 && start + 1 > window ? start + 1 - window : 0;
+    if (!kv->holds_keys(first, end) || (kv->pinned > 0 && end > kv->capacity)) return TT_HIP_ERR_CAPACITY;
+    return TT_HIP_OK;
+}
+static int check_maps(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_q_heads, const void *q, const void *out, int window, const MapHeads &maps) {
+    const int st = check_common(ctx, kv, layer, n_q_heads, q, out);
+    if (st != TT_HIP_OK) return st;
+    if (!maps.lambda || window < 0 || (maps.norm && !(maps.eps >= 0.0f))) return TT_HIP_ERR_INVALID_ARGUMENT;
+    if (maps.lambda_stride != 0 && maps.lambda_stride < n_q_heads) return TT_HIP_ERR_SHAPE;
+    return TT_HIP_OK;
+}
+
+// `rows` tokens of each sequence over the split-K tiles: the pass over both maps' rows, some rows at a time where their partial results
+// would be many, and the join.
+static int run_maps_tiles(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, const int *slots, const int *starts, const int *totals, int rows,
+                          int n_q_heads, const tt_half *q, long long q_seq_stride, long long q_tok_stride, const tt_half *gate,
+                          long long g_seq_stride, long long g_tok_stride, float scale, int window, const MapHeads &maps, tt_half *out,
+                          long long o_seq_stride, long long o_tok_stride) {
+    const int rows_at_once = std::max(kMapsRowsAtOnce / (2 * n_q_heads), 16);
+    for (int base = 0; base < n_seq; base += kMaxSeqPerLaunch) {
+        const int n = std::min(n_seq - base, kMaxSeqPerLaunch);
+        for (int r = 0; r < rows; r += rows_at_once) {
+            int first[kMaxSeqPerLaunch];
+            for (int i = 0; i < n; ++i) first[i] = starts[base + i] + r;
+            const int some = std::min(rows - r, rows_at_once);
+            const long long q_at = base * q_seq_stride + r * q_tok_stride, o_at = base * o_seq_stride + r * o_tok_stride;
+            KeyPiece piece{};
+            piece.maps = true;
+            const int st = run_attention(ctx, kv, 0, layer, n, slots + base, first, totals + base, some, 2 * n_q_heads, q + q_at, q_seq_stride,
+                                         q_tok_stride, nullptr, 0, 0, scale, out + o_at, o_seq_stride, o_tok_stride, 1, 0, nullptr, window, nullptr,
+                                         0, 0, false, nullptr, -1, &piece);
+            if (st != TT_HIP_OK) return st;
+            MapsJoinArgs a;
+            std::memset(static_cast<void *>(&a), 0, sizeof(a));
+            a.parts = piece.parts;
+            a.window = window;
+            a.rows = some;
+            a.heads = n_q_heads;
+            a.group2 = 2 * (n_q_heads / kv->n_kv_heads);
+            a.maps = maps;
+            a.maps.lambda += ((long long)base * rows + r) * maps.lambda_stride;
+            a.lambda_seq_stride = rows * maps.lambda_stride;
+            a.gate = gate ? reinterpret_cast<const _Float16 *>(gate) + base * g_seq_stride + r * g_tok_stride : nullptr;
+            a.out = reinterpret_cast<_Float16 *>(out) + o_at;
+            a.g_seq_stride = g_seq_stride;
+            a.g_tok_stride = g_tok_stride;
+            a.o_seq_stride = o_seq_stride;
+            a.o_tok_stride = o_tok_stride;
+            a.aligned = aligned16(a.out) && o_seq_stride % 8 == 0 && o_tok_stride % 8 == 0;
+            int most = 1;
+            for (int i = 0; i < n; ++i) {
+                a.seq[i] = JoinSeq{first[i], totals[base + i], piece.first_split[i]};
+                const long long keys = std::min<long long>(totals[base + i], window > 0 ? window + some + 32ll : totals[base + i]);
+                most = std::max(most, (int)((keys + piece.parts.split_len - 1) / piece.parts.split_len));
+            }
+            const int joined = launch_maps_join(ctx, kv->head_dim, n, a, most);
+            if (joined != TT_HIP_OK) return joined;
+        }
+    }
+    return TT_HIP_OK;
+}
+
+int tt_hip_attn_verify_diff(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, const int *slots, const int *start_positions, int rows,
+                            int window, int n_q_heads, const tt_half *q, const tt_half *gate, float scale, const float *lambda,
+                            size_t lambda_stride, const uint16_t *norm_weight_bf16, float eps, float out_scale, tt_half *out) {
+    const MapHeads maps{lambda, (long long)lambda_stride, norm_weight_bf16, eps, out_scale};
+    int st = check_maps(ctx, kv, layer, n_q_heads, q, out, window, maps);
+    if (st != TT_HIP_OK) return st;
+    if (n_seq <= 0 || rows <= 0 || !slots || !start_positions) return TT_HIP_ERR_INVALID_ARGUMENT;
+    IntTable totals(n_seq);
+    for (int i = 0; i < n_seq; ++i) {
+        if (start_positions[i] < 0) return TT_HIP_ERR_INVALID_ARGUMENT;
+        const long long end = (long long)start_positions[i] + rows;
+        st = check_maps_keys(kv, slots[i], window, start_positions[i], end);
+        if (st != TT_HIP_OK) return st;
+        totals[i] = (int)end;
+    }
+    BusyGuard guard(ctx);
+    if (!guard.ok) return TT_HIP_ERR_BUSY;
+    const long long tok = (long long)n_q_heads * kv->head_dim, seq = tok * rows;
+    return run_maps_tiles(ctx, kv, layer, n_seq, slots, start_positions, totals.data(), rows, n_q_heads, q, seq, tok, gate, seq, tok, scale, window,
+                          maps, out, seq, tok);
+}
+
+int tt_hip_attn_decode_diff(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, const int *slots, const int *seq_lens, int window,
+                            int n_q_heads, const tt_half *q, const tt_half *gate, float scale, const float *lambda, size_t lambda_stride,
+                            const uint16_t *norm_weight_bf16, float eps, float out_scale, tt_half *out) {
+    const MapHeads maps{lambda, (long long)lambda_stride, norm_weight_bf16, eps, out_scale};
+    int st = check_maps(ctx, kv, layer, n_q_heads, q, out, window, maps);
+    if (st != TT_HIP_OK) return st;
+    if (n_seq <= 0 || !slots || !seq_lens) return TT_HIP_ERR_INVALID_ARGUMENT;
+    IntTable starts(n_seq);
+    for (int i = 0; i < n_seq; ++i) {
+        if (seq_lens[i] < 0) return TT_HIP_ERR_INVALID_ARGUMENT;
+        st = check_maps_keys(kv, slots[i], window, seq_lens[i] - 1LL, seq_lens[i]);
+        if (st != TT_HIP_OK) return st;
+        starts[i] = seq_lens[i] - 1;
+    }
+    BusyGuard guard(ctx);
+    if (!guard.ok) return TT_HIP_ERR_BUSY;
+    const long long row = (long long)n_q_heads * kv->head_dim;
+    return run_maps_tiles(ctx, kv, layer, n_seq, slots, starts.data(), seq_lens, 1, n_q_heads, q, row, row, gate, row, row, scale, window, maps,
+                          out, row, row);
+}
+
+int tt_hip_attn_prefill_diff(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int slot, int start_pos, int q_len, int kv_valid, int window,
+                             int n_q_heads, const tt_half *q, size_t q_stride, const tt_half *gate, size_t gate_stride, float scale,
+                             const float *lambda, size_t lambda_stride, const uint16_t *norm_weight_bf16, float eps, float out_scale,
+                             tt_half *out, size_t o_stride) {
+    const MapHeads maps{lambda, (long long)lambda_stride, norm_weight_bf16, eps, out_scale};
+    int st = check_maps(ctx, kv, layer, n_q_heads, q, out, window, maps);
+    if (st != TT_HIP_OK) return st;
+    if (start_pos < 0 || q_len <= 0) return TT_HIP_ERR_INVALID_ARGUMENT;
+    const size_t packed = (size_t)n_q_heads * kv->head_dim;
+    if (q_stride < packed || o_stride < packed || (gate && gate_stride < packed)) return TT_HIP_ERR_SHAPE;
+    if ((long long)start_pos + q_len > kv_valid) return TT_HIP_ERR_INVALID_ARGUMENT;
+    st = check_maps_keys(kv, slot, window, start_pos, kv_valid);
+    if (st != TT_HIP_OK) return st;
+    BusyGuard guard(ctx);
+    if (!guard.ok) return TT_HIP_ERR_BUSY;
+    return run_maps_tiles(ctx, kv, layer, 1, &slot, &start_pos, &kv_valid, q_len, n_q_heads, q, 0, (long long)q_stride, gate, 0,
+                          (long long)gate_stride, scale, window, maps, out, 0, (long long)o_stride);
 }
 
 // ---- sequences that share a prefix ------------------------------------------

@@ -39,8 +39,11 @@ constexpr int kHotPackedSplits = 4;
 constexpr int kHotSinks = 8, kHotPinnedShift = 8;
 // The same kernel for a prefix in another slot: keep_words is that slot, and from kHotPinnedShift on the flags hold the prefix's blocks.
 constexpr int kHotFront = 16;
+// Two softmax maps a head (kKeepMaps).
+constexpr int kHotMaps = 32;
 constexpr int kKeepSinks = 6;  // that kernel's KEEP (splitk_kernel.h)
 constexpr int kKeepPieces = 7;  // ... and of two passes in one launch, over the keys that sequences share and over their own
+constexpr int kKeepMaps = 9;    // ... of two softmax maps a head: `group` counts two rows a head
 constexpr int kKeepRows = 8;    // ... with the first of them over tiles of kFrontRows packed rows, whose wavefronts share a block of keys in LDS
 struct SplitKHot {                         // dword
     const _Float16 *k_layer;               //  0
@@ -118,6 +121,15 @@ struct alignas(64) SplitKPair : SplitKArgs {
 };
 static_assert(sizeof(SplitKPair) == 2 * sizeof(SplitKArgs) + 64, "`own` right behind the base, where the kernel looks for it");
 
+// The heads of differential attention: a token's row of factors, one a head, the norm over a head's values (nullptr: none) and what
+// it is scaled by behind it.
+struct MapHeads {
+    const float *lambda;
+    long long lambda_stride;  // floats from a token's row to the next token's; 0: one row for all
+    const uint16_t *norm;     // bfloat16 [D]
+    float eps, out_scale;
+};
+
 // Where a pass over one piece of the keys has left its partial results: row n of a tile's split lies at
 // ((first_split(sequence) + split) * n_tiles + tile) * nt + n, D floats of `o` and a (maximum, sum) pair of `ml`.
 struct PassParts {
@@ -161,13 +173,15 @@ struct tt_hip_ctx {
     void *select_ws = nullptr;  // the multi-workgroup key selection's sorted chunks and their tables
     uint8_t *keep_rows = nullptr;  // selection bytes written out from a chunk's index lists (tt_hip_attn_prefill_keep_indices)
     size_t keep_rows_bytes = 0;
+    int8_t *levels = nullptr;  // tokens that an 8-bit projection has quantised itself, and their scales
+    size_t levels_bytes = 0;
     int split_override = 0;
     bool xcd_grid = true;  // chunks through the split-K kernel launch XCD-major (TT_HIP_OPT_XCD_GRID)
     bool pass_only = false;  // measurement control (TT_HIP_OPT_MEASURE_PASS_ONLY): split-K launches go without their combine pass
     int stream_override = -1;  // -1: automatic; 0 / 1: never / always mark single-read K/V loads non-temporal
     bool capturing = false;
     // Bumped whenever device memory that a captured graph may have baked into its kernel arguments is released:
-    // the split-K scratch, the staging pages, the selection workspace, a cache's stores (growth, destruction).
+    // the split-K scratch, the staging pages, the selection workspace, the quantised tokens, a cache's stores (growth, destruction).
     // A graph remembers the value it was captured at and refuses to replay once it has moved.
     uint64_t generation = 0;
     // per-launch timing of the dominant kernel
@@ -297,6 +311,23 @@ int launch_prefill(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int slot, int star
 int launch_combine(tt_hip_ctx *ctx, const LaunchPlan &plan, int head_dim, int n_seq, const SplitKArgs &args);
 // The rows of n_seq sequences from the partial results of two passes (attn_join.hip).
 int launch_join(tt_hip_ctx *ctx, int head_dim, int n_seq, const JoinArgs &args);
+
+// Differential attention (attn_maps.hip): the split-K pass over both maps' rows, and the heads' rows from its partial results.
+struct MapsJoinArgs {
+    PassParts parts;  // tiles whose rows are the maps', two a head
+    long long lambda_seq_stride;  // floats from a sequence's first row of factors to the next one's
+    int window, rows, heads, group2, aligned;  // group2: rows that share a KV head, two a q head
+    MapHeads maps;
+    const _Float16 *gate;
+    _Float16 *out;
+    long long g_seq_stride, g_tok_stride, o_seq_stride, o_tok_stride;
+    JoinSeq seq[kMaxSeqPerLaunch];
+};
+// Rows of maps whose partial results of a split are kept at a time (128 MiB with heads of 256).
+constexpr int kMapsRowsAtOnce = 131072;
+int configure_maps_kernels(tt_hip_ctx *ctx);
+int launch_splitk_maps(tt_hip_ctx *ctx, const LaunchPlan &plan, int head_dim, int n_seq, const SplitKArgs &args, int kv_bits);
+int launch_maps_join(tt_hip_ctx *ctx, int head_dim, int n_seq, const MapsJoinArgs &args, int most_splits);
 
 // A prefix that slots share: block `block` of `slot`'s pages, of which `rows` are the prefix's, every layer, into the same place of
 // `n_slots` others.

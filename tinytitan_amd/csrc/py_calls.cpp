@@ -29,6 +29,12 @@ namespace {
     F(tt_hip_attn_decode_shared)                                                                                         \
     F(tt_hip_attn_verify_shared)                                                                                         \
     F(tt_hip_attn_prefill_shared)                                                                                        \
+    F(tt_hip_attn_decode_diff)                                                                                           \
+    F(tt_hip_attn_verify_diff)                                                                                           \
+    F(tt_hip_attn_prefill_diff)                                                                                          \
+    F(tt_hip_int8_projection)                                                                                            \
+    F(tt_hip_int8_quantise_rows)                                                                                         \
+    F(tt_hip_int8_projection_levels)                                                                                     \
     F(tt_hip_attn_prefill)                                                                                               \
     F(tt_hip_attn_prefill_swa)                                                                                           \
     F(tt_hip_attn_prefill_keep)                                                                                          \
@@ -99,6 +105,10 @@ struct Args {
         if (!t->is_cuda() || t->element_size() != 2) return fail<uint16_t>("expected a device tensor of 16-bit elements");
         return static_cast<uint16_t *>(address_of(*t));
     }
+    // an fp32 device tensor whose last dimension is contiguous, or None
+    float *floats() { return static_cast<float *>(typed(at::kFloat, "expected an fp32 device tensor with a contiguous last dimension")); }
+    // an int8 device tensor of that kind, or None
+    int8_t *levels() { return static_cast<int8_t *>(typed(at::kChar, "expected an int8 device tensor with a contiguous last dimension")); }
     // a contiguous device tensor of any type, or None
     void *raw() {
         const at::Tensor *t = tensor();
@@ -171,6 +181,19 @@ private:
         const unsigned long long v = bits_of(whole);
         Py_DECREF(whole);
         return v;
+    }
+    void *typed(at::ScalarType type, const char *what) {
+        const at::Tensor *t = tensor();
+        if (!t) return nullptr;
+        if (!t->is_cuda() || t->scalar_type() != type) return fail<void>(what);
+        try {
+            if (t->dim() > 0 && t->size(-1) > 1 && t->stride(-1) != 1) return fail<void>(what);
+        } catch (const std::exception &e) {
+            ok = false;
+            PyErr_SetString(PyExc_RuntimeError, e.what());
+            return nullptr;
+        }
+        return address_of(*t);
     }
     // Throws nothing: a tensor without memory of its own (a traced or fake one) is a Python exception.
     void *address_of(const at::Tensor &t, bool raw = false) {
@@ -637,6 +660,128 @@ TT_CALL(qsa_select) {
     });
 }
 
+// (ctx, kv, layer, slots, lengths, window, heads, q, gate, scale, lambda, lambda_stride, norm, eps, out_scale, out)
+TT_CALL(attn_decode_diff) {
+    Args a(args, n, 16);
+    if (!a.ok) return nullptr;
+    auto *ctx = a.handle<tt_hip_ctx>();
+    auto *kv = a.handle<tt_hip_kv>();
+    const int layer = a.i();
+    Ints slots, lens;
+    slots.take(a);
+    lens.take(a);
+    const int window = a.i(), heads = a.i();
+    const tt_half *q = a.half(), *gate = a.half();
+    const float scale = a.real();
+    const float *lambda = a.floats();
+    const size_t lambda_stride = a.size();
+    const uint16_t *norm = a.bits16();
+    const float eps = a.real(), out_scale = a.real();
+    tt_half *out = a.half();
+    return finish(a, [&] {
+        if (slots.count != lens.count) return (int)TT_HIP_ERR_INVALID_ARGUMENT;
+        return lib.tt_hip_attn_decode_diff(ctx, kv, layer, slots.count, slots.values, lens.values, window, heads, q, gate, scale, lambda,
+                                           lambda_stride, norm, eps, out_scale, out);
+    });
+}
+
+// (ctx, kv, layer, slots, start_positions, rows, window, heads, q, gate, scale, lambda, lambda_stride, norm, eps, out_scale, out)
+TT_CALL(attn_verify_diff) {
+    Args a(args, n, 17);
+    if (!a.ok) return nullptr;
+    auto *ctx = a.handle<tt_hip_ctx>();
+    auto *kv = a.handle<tt_hip_kv>();
+    const int layer = a.i();
+    Ints slots, starts;
+    slots.take(a, true);
+    starts.take(a, true);
+    const int rows = a.i(), window = a.i(), heads = a.i();
+    const tt_half *q = a.half(), *gate = a.half();
+    const float scale = a.real();
+    const float *lambda = a.floats();
+    const size_t lambda_stride = a.size();
+    const uint16_t *norm = a.bits16();
+    const float eps = a.real(), out_scale = a.real();
+    tt_half *out = a.half();
+    return finish(a, [&] {
+        if (slots.count != starts.count) return (int)TT_HIP_ERR_INVALID_ARGUMENT;
+        return lib.tt_hip_attn_verify_diff(ctx, kv, layer, slots.count, slots.values, starts.values, rows, window, heads, q, gate, scale, lambda,
+                                           lambda_stride, norm, eps, out_scale, out);
+    });
+}
+
+// (ctx, kv, layer, slot, start_pos, q_len, kv_valid, window, heads, q, q_stride, gate, gate_stride, scale, lambda, lambda_stride, norm, eps,
+//  out_scale, out, o_stride)
+TT_CALL(attn_prefill_diff) {
+    Args a(args, n, 21);
+    if (!a.ok) return nullptr;
+    auto *ctx = a.handle<tt_hip_ctx>();
+    auto *kv = a.handle<tt_hip_kv>();
+    const int layer = a.i(), slot = a.i(), start = a.i(), rows = a.i(), valid = a.i(), window = a.i(), heads = a.i();
+    const tt_half *q = a.half();
+    const size_t q_stride = a.size();
+    const tt_half *gate = a.half();
+    const size_t gate_stride = a.size();
+    const float scale = a.real();
+    const float *lambda = a.floats();
+    const size_t lambda_stride = a.size();
+    const uint16_t *norm = a.bits16();
+    const float eps = a.real(), out_scale = a.real();
+    tt_half *out = a.half();
+    const size_t o_stride = a.size();
+    return finish(a, [&] {
+        return lib.tt_hip_attn_prefill_diff(ctx, kv, layer, slot, start, rows, valid, window, heads, q, q_stride, gate, gate_stride, scale, lambda,
+                                            lambda_stride, norm, eps, out_scale, out, o_stride);
+    });
+}
+
+// (ctx, weights, weight_scales, x, x_stride, y, rows, columns, tokens, y_stride)
+TT_CALL(int8_projection) {
+    Args a(args, n, 10);
+    if (!a.ok) return nullptr;
+    auto *ctx = a.handle<tt_hip_ctx>();
+    const int8_t *weights = a.levels();
+    const float *weight_scales = a.floats();
+    const tt_half *x = a.half();
+    const size_t x_stride = a.size();
+    tt_half *y = a.half();
+    const int rows = a.i(), columns = a.i(), tokens = a.i();
+    const size_t y_stride = a.size();
+    return finish(a, [&] { return lib.tt_hip_int8_projection(ctx, weights, weight_scales, x, x_stride, y, rows, columns, tokens, y_stride); });
+}
+
+// (ctx, x, x_stride, tokens, columns, levels, levels_stride, scales)
+TT_CALL(int8_quantise_rows) {
+    Args a(args, n, 8);
+    if (!a.ok) return nullptr;
+    auto *ctx = a.handle<tt_hip_ctx>();
+    const tt_half *x = a.half();
+    const size_t x_stride = a.size();
+    const int tokens = a.i(), columns = a.i();
+    int8_t *levels = a.levels();
+    const size_t levels_stride = a.size();
+    float *scales = a.floats();
+    return finish(a, [&] { return lib.tt_hip_int8_quantise_rows(ctx, x, x_stride, tokens, columns, levels, levels_stride, scales); });
+}
+
+// (ctx, weights, weight_scales, levels, levels_stride, scales, y, rows, columns, tokens, y_stride)
+TT_CALL(int8_projection_levels) {
+    Args a(args, n, 11);
+    if (!a.ok) return nullptr;
+    auto *ctx = a.handle<tt_hip_ctx>();
+    const int8_t *weights = a.levels();
+    const float *weight_scales = a.floats();
+    const int8_t *levels = a.levels();
+    const size_t levels_stride = a.size();
+    const float *scales = a.floats();
+    tt_half *y = a.half();
+    const int rows = a.i(), columns = a.i(), tokens = a.i();
+    const size_t y_stride = a.size();
+    return finish(a, [&] {
+        return lib.tt_hip_int8_projection_levels(ctx, weights, weight_scales, levels, levels_stride, scales, y, rows, columns, tokens, y_stride);
+    });
+}
+
 // bind(path): takes the functions' addresses from the library at `path`, which the process has loaded already.
 PyObject *bind(PyObject *, PyObject *arg) {
     const char *path = PyUnicode_AsUTF8(arg);
@@ -658,6 +803,8 @@ PyMethodDef methods[] = {
     TT_METHOD(attn_decode) TT_METHOD(attn_decode_swa) TT_METHOD(attn_decode_keep) TT_METHOD(attn_decode_keep_indices)
     TT_METHOD(attn_verify_swa) TT_METHOD(attn_decode_sinks) TT_METHOD(attn_verify_sinks) TT_METHOD(attn_prefill_sinks)
     TT_METHOD(attn_decode_shared) TT_METHOD(attn_verify_shared) TT_METHOD(attn_prefill_shared)
+    TT_METHOD(attn_decode_diff) TT_METHOD(attn_verify_diff) TT_METHOD(attn_prefill_diff)
+    TT_METHOD(int8_projection) TT_METHOD(int8_quantise_rows) TT_METHOD(int8_projection_levels)
     TT_METHOD(attn_prefill) TT_METHOD(attn_prefill_keep) TT_METHOD(attn_prefill_keep_indices)
     TT_METHOD(kv_append) TT_METHOD(qkv_epilogue_append) TT_METHOD(affine_projection) TT_METHOD(qsa_pool_blocks)
     TT_METHOD(qsa_norm_rope_rows) TT_METHOD(qsa_block_scores) TT_METHOD(qsa_decode_scores) TT_METHOD(qsa_select)

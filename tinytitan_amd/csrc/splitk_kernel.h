@@ -490,6 +490,11 @@ __device__ __forceinline__ h8 only_seen(h8 x, const unsigned (&mask)[4]) {
     const words m = {mask[0], mask[1], mask[2], mask[3]};
     return __builtin_bit_cast(h8, __builtin_bit_cast(words, x) & m);
 }
+// Keys [from, to) of a block of 32 (either may lie outside it), bit by bit.
+__device__ __forceinline__ unsigned keys_between(int from, int to) {
+    auto below = [](int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; };
+    return below(to) & ~below(from);
+}
 template <int D, int NT>
 __device__ __forceinline__ void drop_unseen(VTile<D, NT> &vt, const Lane<D, NT> &ln, unsigned seen) {
     if constexpr (NT == 32) {
@@ -1023,6 +1028,11 @@ __device__ __forceinline__ void block_softmax_pv(RowState<D, NT> &st, Scores<D, 
 // KEEP = kKeepPieces: the same kernel twice in a launch, over two pieces of the rows' keys with their own arguments (SplitKPair): what sequences
 // share and what is their own.  Neither fills the chip while the other waits for it, and there is one launch less.
 // KEEP = kKeepRows: the shared keys by front_rows, their own like that.
+// KEEP = kKeepMaps: two softmax maps a head.  A head's query row holds two queries of D / 2, a key row two keys, and the tile has a
+// row for either of a head's maps whose other half of the query is zeros: the contraction over D is then the map's own over D / 2, at the
+// price of half of the score MFMAs multiplying zeros, which a pass that waits for K and V does not notice.  `group` counts the
+// rows, two a head; the partial results of both are joined by attn_maps.hip.  (Values of keys that no row of a tile sees
+// are dropped, as with sinks.)
 // The hot arguments, this workgroup's sequence entry and where the rows go and their gate beside them, by five scalar loads issued
 // together (the compiler would fetch each field where it is first used: five or six dependent trips to the kernarg segment before
 // the first K/V load can go out, about 0.15 us each, and another ahead of the gate's loads).
@@ -1315,9 +1325,10 @@ __device__ __forceinline__ void front_rows(const SplitKHot &a, const SplitKSeq &
 }
 
 template <int D, int NT, int WAVES, int BITS, int KEEP = 0, int STREAM = 0>
-__global__ __launch_bounds__(WAVES * 64, ((NT == 16 && (KEEP < 2 || KEEP == kKeepSinks || KEEP == kKeepPieces)) || (KEEP == kKeepRows && D < 256) ? 2 : 1)) void
-    attn_splitk_kernel(const std::conditional_t<KEEP >= kKeepPieces, SplitKPair, SplitKArgs> args) {
-    constexpr bool PAIR = KEEP >= kKeepPieces;
+__global__ __launch_bounds__(WAVES * 64, ((NT == 16 && (KEEP < 2 || KEEP == kKeepSinks || KEEP == kKeepPieces || KEEP == kKeepMaps)) || (KEEP == kKeepRows && D < 256) ? 2 : 1)) void
+    attn_splitk_kernel(const std::conditional_t<KEEP == kKeepPieces || KEEP == kKeepRows, SplitKPair, SplitKArgs> args) {
+    constexpr bool PAIR = KEEP == kKeepPieces || KEEP == kKeepRows;
+    constexpr bool MAPS = KEEP == kKeepMaps;
     constexpr bool PAIRED = STREAM == 2;
     static_assert(!PAIRED || (D == 256 && NT == 32 && BITS == 16 && KEEP == 0));
     constexpr int AUX = (STREAM ? kStreamed : 0) | (PAIRED ? kPaired : 0);
@@ -1370,7 +1381,7 @@ __global__ __launch_bounds__(WAVES * 64, ((NT == 16 && (KEEP < 2 || KEEP == kKee
         split = (int)(pair / (unsigned)a.n_tiles);
         tile = (int)(pair - (unsigned)split * (unsigned)a.n_tiles);
     }
-    constexpr bool SINKS = KEEP >= kKeepSinks;
+    constexpr bool SINKS = KEEP == kKeepSinks || PAIR;
     const TileInfo ti = tile_info<SINKS>(a, sq, tile);
     const int k_begin = ti.k0 + split * a.split_len;
     if (k_begin >= ti.tile_end && split != 0) return;  // split 0 always runs so that an empty range yields zeros
@@ -1394,7 +1405,9 @@ __global__ __launch_bounds__(WAVES * 64, ((NT == 16 && (KEEP < 2 || KEEP == kKee
     const int hg = li - t_local * a.gh;
     const bool valid = t_local < ti.tile_rows;
     const int tok = ti.t0 + (valid ? t_local : 0);  // clamped so that the address is always in range
-    const int head = ti.kvh * a.group + ti.hsub * a.gh + hg;
+    // (MAPS: rows 2 h and 2 h + 1 of a token are the two maps of its head h)
+    const int head = MAPS ? ti.kvh * (a.group >> 1) + ((ti.hsub * a.gh + hg) >> 1) : ti.kvh * a.group + ti.hsub * a.gh + hg;
+    [[maybe_unused]] const bool second_map = (ti.hsub * a.gh + hg) & 1;
     const int lim = valid ? min(ti.total, ti.start + tok + 1) : 0;  // keys [lo, lim) are visible
     const int lo = (a.window > 0 && lim > a.window) ? lim - a.window : 0;  // sliding window: the last `window` keys
     const global_halves qp = (global_halves)(a.q + seq * a.q_seq_stride + tok * a.q_tok_stride + (long long)head * D);
@@ -1670,7 +1683,9 @@ __global__ __launch_bounds__(WAVES * 64, ((NT == 16 && (KEEP < 2 || KEEP == kKee
     }
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-        qf[s] = valid ? qf[s] : (h8)(_Float16)0;
+        bool mine = valid;
+        if constexpr (MAPS) mine = valid && ((BITS == 16 ? QSTEP * s + 8 * g : q_dim_of_step<NT>(s, g)) >= D / 2) == second_map;
+        qf[s] = mine ? qf[s] : (h8)(_Float16)0;
         if constexpr (Q_IN_LDS) qlds[s * 64 + lane] = qf[s];  // read back by this wave only: no barrier
     }
     __builtin_amdgcn_sched_barrier(0);
@@ -1752,6 +1767,7 @@ __global__ __launch_bounds__(WAVES * 64, ((NT == 16 && (KEEP < 2 || KEEP == kKee
             auto below = [](int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; };
             seen = below(seen_end - kbase) & (below(sinks - kbase) | ~below(seen_from - kbase));
         }
+        if constexpr (MAPS) seen = keys_between(seen_from - kbase, ti.tile_end - kbase);
         Voids<D, NT> vo(real ? 0u : kVoidLoad);
         if constexpr (BY_KEY) vo = Voids<D, NT>(real ? 0u : kVoidLoad, next_keys, ln);
         if constexpr (BITS == 16 && NT == 32) {

@@ -520,6 +520,95 @@ class PrefillAttention:
             self.ctx._check(status, "tt_hip_attn_prefill_swa" if p.sliding_window else "tt_hip_attn_prefill")
 
 
+@dataclass
+class DifferentialHeads:
+    """What a differential attention layer knows of its heads: ``lambdas``, fp32, one factor per q head (``[heads]``) or per token and
+    head (``[tokens, heads]``, rows of any stride); ``norm_weight``, bfloat16 ``[head_dim]``, of the norm over a head's values (None:
+    no norm) with its ``eps``; ``out_scale``, by which the heads' rows are multiplied (1 - lambda_init, as such models have it)."""
+    lambdas: torch.Tensor
+    norm_weight: Optional[torch.Tensor] = None
+    eps: float = 1e-5
+    out_scale: float = 1.0
+
+    def stride(self, heads: int, tokens: int) -> int:
+        """Floats from one token's factors to the next one's: 0 where all tokens share them."""
+        shape = tuple(self.lambdas.shape)
+        if shape == (heads,):
+            return 0
+        if shape != (tokens, heads) or (tokens > 1 and self.lambdas.stride(0) < heads):
+            raise TinyTitanHIPError(capi.ERR_SHAPE, "DifferentialHeads")
+        return self.lambdas.stride(0) if tokens > 1 else heads
+
+    def check(self, head_dim: int) -> None:
+        w = self.norm_weight
+        if w is not None and (w.numel() != head_dim or not w.is_contiguous()):
+            raise TinyTitanHIPError(capi.ERR_SHAPE, "DifferentialHeads")
+
+
+class DifferentialAttention:
+    """Attention whose weights are the difference of two softmax maps (no counterpart in the reference).  A q head's row is two
+    queries of ``head_dim / 2``, one behind the other, its KV head's key row two keys, its value row one value of ``head_dim``; the
+    cache is the one the other attention classes read, and slots, lengths, windows and strides are as in ``Attention`` and
+    ``PrefillAttention``:
+
+        a   = softmax(scale q1 K1) V - lambda softmax(scale q2 K2) V
+        out = sigmoid(gate) * out_scale * norm_weight * a / sqrt(mean(a^2) + eps)"""
+
+    def __init__(self, ctx: HIPContext):
+        self.ctx = ctx
+        self._calls = ctx._calls
+
+    def encode_lambda(self, q1: torch.Tensor, k1: torch.Tensor, q2: torch.Tensor, k2: torch.Tensor, lambda_init: float,
+                      lambdas: torch.Tensor) -> None:
+        """``lambdas[h] = exp(q1[h] . k1[h]) - exp(q2[h] . k2[h]) + lambda_init`` for learned vectors ``[heads, dims]``, or one
+        ``[dims]`` for all heads; fp32, contiguous.  Once per layer, when a model is loaded."""
+        vectors = (q1, k1, q2, k2)
+        if any(t.dtype != torch.float32 or not t.is_cuda or not t.is_contiguous() for t in vectors + (lambdas,)):
+            raise TypeError("expected contiguous fp32 device tensors")
+        if any(t.shape != q1.shape for t in vectors) or q1.dim() not in (1, 2) or (q1.dim() == 2 and q1.shape[0] != lambdas.numel()):
+            raise TinyTitanHIPError(capi.ERR_SHAPE, "DifferentialAttention.encode_lambda")
+        dims = q1.shape[-1]
+        self.ctx._check(self.ctx._lib.tt_hip_diff_lambda(self.ctx.handle, q1.data_ptr(), k1.data_ptr(), q2.data_ptr(), k2.data_ptr(),
+                                                         dims if q1.dim() == 2 else 0, lambdas.numel(), dims, lambda_init,
+                                                         lambdas.data_ptr()), "tt_hip_diff_lambda")
+
+    def encode_full(self, kv: KVCacheManager, layer: int, q: torch.Tensor, out: torch.Tensor, num_q_heads: int, seq_len, scale: float,
+                    heads: DifferentialHeads, slot=0, gate: Optional[torch.Tensor] = None, window: int = 0) -> None:
+        """One query token per sequence over its first ``seq_len`` keys, or the last ``window`` of them; ``slot`` / ``seq_len`` may be
+        lists."""
+        heads.check(kv.head_dim)
+        stride = heads.stride(num_q_heads, len(seq_len) if isinstance(seq_len, (list, tuple)) else 1)
+        status = self._calls.attn_decode_diff(self.ctx.handle, kv.handle, layer, slot, seq_len, window, num_q_heads, q, gate, scale,
+                                              heads.lambdas, stride, heads.norm_weight, heads.eps, heads.out_scale, out)
+        if status:
+            self.ctx._check(status, "tt_hip_attn_decode_diff")
+
+    def encode_verify_rows(self, kv: KVCacheManager, layer: int, q: torch.Tensor, out: torch.Tensor, num_q_heads: int,
+                           start_positions: Sequence[int], rows: int, scale: float, heads: DifferentialHeads, slots: Sequence[int],
+                           gate: Optional[torch.Tensor] = None, window: int = 0) -> None:
+        """Row r of sequence i attends like a decode at ``start_positions[i] + r``."""
+        heads.check(kv.head_dim)
+        status = self._calls.attn_verify_diff(self.ctx.handle, kv.handle, layer, slots, start_positions, rows, window, num_q_heads, q, gate,
+                                              scale, heads.lambdas, heads.stride(num_q_heads, len(slots) * rows), heads.norm_weight,
+                                              heads.eps, heads.out_scale, out)
+        if status:
+            self.ctx._check(status, "tt_hip_attn_verify_diff")
+
+    def encode_causal(self, kv: KVCacheManager, layer: int, slot: int, q: torch.Tensor, out: torch.Tensor, params: PrefillAttentionParams,
+                      heads: DifferentialHeads, gate: Optional[torch.Tensor] = None) -> None:
+        """A causal chunk of one sequence (``params.sliding_window`` 0: every key up to the row's own)."""
+        p = params
+        if p.sinks:
+            raise TinyTitanHIPError(capi.ERR_INVALID_ARGUMENT, "DifferentialAttention.encode_causal")
+        heads.check(kv.head_dim)
+        status = self._calls.attn_prefill_diff(self.ctx.handle, kv.handle, layer, slot, p.start_position, p.query_count, p.kv_valid_count,
+                                               p.sliding_window, p.num_q_heads, q, p.q_stride, gate, p.gate_stride or p.q_stride, p.scale,
+                                               heads.lambdas, heads.stride(p.num_q_heads, p.query_count), heads.norm_weight, heads.eps,
+                                               heads.out_scale, out, p.o_stride)
+        if status:
+            self.ctx._check(status, "tt_hip_attn_prefill_diff")
+
+
 class QKVEpilogue:
     """Split [query ; gate], per-head q/k RMS norms, NeoX sub-dim RoPE and the K/V cache write in one
     launch: ``encodeGatedFullPostProjection`` (RealForwardRunner+DecodeFullAttention.swift:123-185)
@@ -566,6 +655,41 @@ class AffineProjection:
                                                token_count, x_stride or columns, y_stride or rows)
         if status:
             self.ctx._check(status, "tt_hip_affine_projection")
+
+
+class Int8Projection:
+    """``y[t] = W x[t]`` in 8-bit integers, with a scale for each token and each output channel (no counterpart in the reference, whose
+    8-bit weights are affine: ``AffineProjection``).  ``weights`` is an int8 device tensor ``[rows][columns]``, ``weight_scales`` fp32
+    ``[rows]``; a token's scale is ``max |x| / 127``, its levels ``round(x / scale)``, their sum of products exact in integers."""
+
+    def __init__(self, ctx: HIPContext):
+        self.ctx = ctx
+        self._calls = ctx._calls
+
+    def encode(self, weights: torch.Tensor, weight_scales: torch.Tensor, x: torch.Tensor, y: torch.Tensor, rows: int, columns: int,
+               token_count: int, x_stride: Optional[int] = None, y_stride: Optional[int] = None) -> None:
+        """From fp16 tokens, which the call quantises."""
+        status = self._calls.int8_projection(self.ctx.handle, weights, weight_scales, x, x_stride or columns, y, rows, columns, token_count,
+                                             y_stride or rows)
+        if status:
+            self.ctx._check(status, "tt_hip_int8_projection")
+
+    def quantise(self, x: torch.Tensor, levels: torch.Tensor, scales: torch.Tensor, columns: int, token_count: int,
+                 x_stride: Optional[int] = None, levels_stride: Optional[int] = None) -> None:
+        """fp16 tokens into ``levels`` (int8) and ``scales`` (fp32), once for all projections of the same input."""
+        status = self._calls.int8_quantise_rows(self.ctx.handle, x, x_stride or columns, token_count, columns, levels,
+                                                levels_stride or columns, scales)
+        if status:
+            self.ctx._check(status, "tt_hip_int8_quantise_rows")
+
+    def encode_levels(self, weights: torch.Tensor, weight_scales: torch.Tensor, levels: torch.Tensor, scales: torch.Tensor, y: torch.Tensor,
+                      rows: int, columns: int, token_count: int, levels_stride: Optional[int] = None,
+                      y_stride: Optional[int] = None) -> None:
+        """From tokens that ``quantise`` has made; the same results as ``encode``."""
+        status = self._calls.int8_projection_levels(self.ctx.handle, weights, weight_scales, levels, levels_stride or columns, scales, y, rows,
+                                                    columns, token_count, y_stride or rows)
+        if status:
+            self.ctx._check(status, "tt_hip_int8_projection_levels")
 
 
 @dataclass(frozen=True)

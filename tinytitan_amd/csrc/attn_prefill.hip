@@ -38,6 +38,7 @@
 // PrefillAttention.encodeCausal (sources/TinyTitan/Kernels/Attention/PrefillAttention.swift:165-258).
 #include "chunk_plan.h"
 #include "internal.h"
+#include "lds_copy.h"
 #include "wave_ops.h"
 
 namespace tt {
@@ -89,24 +90,6 @@ __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_ex
 typedef __attribute__((address_space(3))) void *lds_ptr_t;
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 
-// 16 bytes per lane, global -> LDS without passing through registers: lane l's 16 bytes land at
-// lds_addr + 16 l.  Issued as inline assembly on purpose: the compiler, when it sees an LDS DMA,
-// guards every later LDS read with a full vmcnt(0) wait (it cannot tell the stages apart),
-// which would turn a multi-stage prefetch into none.  Completion is tracked by hand instead:
-// TT_WAIT_VMCNT before the barrier that publishes a stage.
-__device__ __forceinline__ void copy16_global_to_lds(const void *base, unsigned lane_offset, unsigned lds_addr) {
-    // base and lds_addr are wave-uniform by construction; say so, in case the compiler lost track
-    const unsigned long long b = (unsigned long long)base;
-    const unsigned b_hi = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(b >> 32));
-    const unsigned b_lo = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)b);  // (the builtin returns a signed int)
-    base = (const void *)(((unsigned long long)b_hi << 32) | (unsigned long long)b_lo);
-    lds_addr = (unsigned)__builtin_amdgcn_readfirstlane((int)lds_addr);
-    // m0 carries the LDS address of the copy.  The compiler owns m0 (it is a reserved register: naming it as a clobber is not honoured), but has
-    // no use for it in the kernels that copy by this (tests/test_wait_states.py looks), so it is not put back.  Between a scalar write of m0 and a
-    // copy into LDS belongs one wait state, which is nobody's to add but the block's own.
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %0" : : "s"(base), "v"(lane_offset), "s"(lds_addr) : "memory");
-}
-
 // N pieces of 1 KiB that lie one behind the other in both places (an instruction's offset counts for both).
 template <int N>
 __device__ __forceinline__ void copies_global_to_lds(const void *base, unsigned first, unsigned second, unsigned lds_addr) {
@@ -138,9 +121,6 @@ __device__ __forceinline__ void rescale_tile(f16v &o, float alpha) {
         o[j + 3] = a3;
     }
 }
-
-// vmcnt(n) only: leaves the LDS/scalar and export counters alone.
-#define TT_WAIT_VMCNT(n) __builtin_amdgcn_s_waitcnt(((n) & 0xF) | (((n) >> 4) << 14) | (0x7 << 4) | (0xF << 8))
 
 // One online-softmax step of the score wave on a block's scores: mask, move the row's reference
 // max where the block max exceeds it by more than the threshold, and produce the

@@ -708,6 +708,7 @@ tt_hip_ctx *tt_hip_ctx_create(int device, int *out_err) {
             if (st == TT_HIP_OK) st = configure_prefill_kernels(ctx);
             if (st == TT_HIP_OK) st = configure_affine_kernels(ctx);
             if (st == TT_HIP_OK) st = configure_maps_kernels(ctx);
+            if (st == TT_HIP_OK) st = configure_int8_kernels(ctx);
             if (st != TT_HIP_OK) {
                 tt_hip_ctx_destroy(ctx);
                 return fail(st);

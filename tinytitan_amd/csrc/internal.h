@@ -271,6 +271,7 @@ struct BusyGuard {
 int configure_splitk_kernels(tt_hip_ctx *ctx);
 int configure_prefill_kernels(tt_hip_ctx *ctx);
 int configure_affine_kernels(tt_hip_ctx *ctx);
+int configure_int8_kernels(tt_hip_ctx *ctx);
 
 int ensure_partials(tt_hip_ctx *ctx, size_t rows, int head_dim, bool front = false);
 int ensure_stage(tt_hip_ctx *ctx, size_t elems);

@@ -11,7 +11,7 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 LIB_DIR = os.path.join(PKG, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libctinytitan_hip.so")
-SOURCES = ["context.hip", "kv_cache.hip", "kv_quant.hip", "attn_splitk.hip", "attn_prefill.hip", "attn_join.hip", "attn_maps.hip",
+SOURCES = ["context.hip", "kv_cache.hip", "kv_quant.hip", "attn_splitk.hip", "attn_prefill.hip", "attn_join.hip", "attn_maps.hip", "attn_maps_chunk.hip",
            "qkv_epilogue.hip", "affine_proj.hip", "int8_proj.hip", "qsa_indexer.hip"]
 
 CALLS_SOURCE = "py_calls.cpp"

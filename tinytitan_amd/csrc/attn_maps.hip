@@ -25,14 +25,6 @@ __device__ __forceinline__ size_t part_row(const PassParts &p, int group, int to
     return (size_t)tile * p.nt + (tok - tok_tile * p.tt) * p.gh + (in_group - hsub * p.gh);
 }
 
-// a1 - lambda a2 of the maps' sums and what they are divided by.  Either map's result is rounded before the difference, no product is
-// fused into it: maps that are the same then cancel to zero, and not to a rounding that the norm behind makes a row of.
-__device__ __forceinline__ f4 difference(f4 o1, float inv1, f4 o2, float inv2, float lambda) {
-#pragma clang fp contract(off)
-    const f4 a1 = o1 * inv1, a2 = o2 * inv2;
-    return a1 - lambda * a2;
-}
-
 // A (token, head) item is D / 4 threads of four dims each, and G of those that share its splits; a workgroup is ITEMS of them.
 template <int D, int G>
 __global__ __launch_bounds__(G * D / 4 > 256 ? G * D / 4 : 256) void attn_maps_join_kernel(const MapsJoinArgs a) {
@@ -126,7 +118,10 @@ __global__ __launch_bounds__(G * D / 4 > 256 ? G * D / 4 : 256) void attn_maps_j
             }
         }
     }
-    f4 out = difference(acc[0], l[0] > 0.0f ? 1.0f / l[0] : 0.0f, acc[1], l[1] > 0.0f ? 1.0f / l[1] : 0.0f, lambda);
+    const f4 a1 = acc[0] * (l[0] > 0.0f ? 1.0f / l[0] : 0.0f), a2 = acc[1] * (l[1] > 0.0f ? 1.0f / l[1] : 0.0f);
+    f4 out;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = map_difference(a1[i], a2[i], lambda);
     float scale = a.maps.out_scale;
     if (a.maps.norm) {
         float squares = out[0] * out[0] + out[1] * out[1] + out[2] * out[2] + out[3] * out[3];

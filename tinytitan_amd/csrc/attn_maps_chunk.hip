@@ -1,0 +1,537 @@
+// Differential attention of a causal chunk on gfx950 MFMA (attn_maps.hip tells the operator).
+//
+// Transposed as the other attention kernels are, a lane owns a query row:
+//   S^T[key][row] = K_m . Q_m^T      A = K fragment, of map m's half of the dims,  B = Q^T fragment, both in registers
+//   O^T[d][row]  += V^T . P^T        A = V^T fragment out of LDS,                  B = P^T as it left S^T's registers
+// with v_mfma_f32_32x32x16_f16.  A workgroup is four wavefronts over 128 rows, four tiles of 32 (heads that share a KV head, of one or more tiles
+// of tokens): wavefront 2 p + m takes map m of tiles 2 p and 2 p + 1, all dims of both.  The maps of a tile meet at the end.
+//
+// What shapes it: LDS hands out 64 bytes a cycle and CU, half of what a matrix product wants whose operand comes from there each time.  So an
+// operand of V is used for two tiles, and K, whose blocks lie in memory as the operands are, comes straight into registers, a block ahead.
+// Of heads of 256 a block of keys is 48 products a wavefront, 1,536 cycles, beside 80 KiB of LDS traffic a CU, 1,280, and 48 KiB through the
+// vector memory path, 768.  One wavefront a SIMD has all 512 registers (256 of them sums over V), so nothing but its own order hides one kind of work
+// behind another: the softmax of block i is cut into pieces of a few instructions each, one between any two of the products of block i's
+// scores and block i - 1's values.
+#include <algorithm>
+
+#include "lds_copy.h"
+#include "splitk_kernel.h"
+
+namespace tt {
+
+namespace {
+
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+constexpr float kChunkRescale = 8.0f;
+constexpr int kVRing = 4;  // blocks of V in LDS: the one in hand, the next two, and the one that every wavefront is done with
+
+struct MapsChunkArgs {
+    const _Float16 *k_slot, *v_slot;  // page of KV head 0 of the slot
+    const _Float16 *q, *gate;
+    _Float16 *out;
+    long long page_elems, q_stride, g_stride, o_stride;
+    MapHeads maps;
+    int n_kv_heads, group, hs, sets;  // hs: heads of a workgroup (4, 2 or 1), of which a KV head has `sets`
+    int tok_tiles;                    // of 128 / hs tokens
+    int xs, per_kvh;                  // XCDs of a KV head (0: dealt out as they come), workgroups of one
+    int start, q_len, kv_valid, window, ring_blocks;
+    float scale_log2e;
+    int n_splits, split_blocks;  // n_splits > 1: ranges of this many blocks, partial results
+    float *part_o, *part_ml;     // [split][(row of maps) * tok_tiles + tile][token of the tile]
+    int aligned;
+};
+
+template <int D>
+struct ChunkShape {
+    static constexpr int KS = D / 32, MT = D / 32, VF = 2 * MT, CPW = VF / 4;  // score steps of a map, tiles of dims, V fragments of a block, copies a wavefront
+    static constexpr int V_BYTES = 64 * D, RING_BYTES = kVRing * V_BYTES;
+    static constexpr int X_BYTES = 128 * D;               // a tile's sums on their way to the other map's wavefront
+    static constexpr int STAGE_PITCH = 64 + 16, STAGE_BYTES = 32 * STAGE_PITCH;
+    static constexpr int STAGE_OFF = std::max(RING_BYTES, 4 * X_BYTES);
+    static constexpr int LDS = STAGE_OFF + 4 * STAGE_BYTES;
+};
+
+// The products of the scores, in vector registers: the compiler gives every matrix instruction of a kernel with 512 registers accumulation registers,
+// and those are the sums over V alone.  What the compiler does about an instruction's wait states it does not do for these:
+//   a product reads the sum of the one before it as it comes (the same registers), and the first takes a zero for it, not one that was just written;
+//   a vector instruction that reads a sum wants 19 cycles of four clocks behind the last of its products.  Every product of this size holds the
+//   matrix pipe for eight of those cycles, so that two more products issued in between are room enough.
+__device__ __forceinline__ void first_score(f16v &s, h8 k, h8 q) { asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, 0" : "=&v"(s) : "v"(k), "v"(q)); }
+__device__ __forceinline__ void next_score(f16v &s, h8 k, h8 q) { asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(s) : "v"(k), "v"(q)); }
+// ... where no two products follow.
+__device__ __forceinline__ void settle(f16v &s) { asm volatile("s_nop 15\n\ts_nop 7" : "+v"(s)); }
+
+// A sum over V stays in accumulation registers, wherever control flow comes from: told so behind everything that writes it, or the compiler moves
+// the sums to vector registers and back around every block.
+__device__ __forceinline__ void keep_sum(f16v &o) { asm volatile("" : "+a"(o)); }
+
+template <typename F, int... I>
+__device__ __forceinline__ void unrolled_over(std::integer_sequence<int, I...>, F f) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void unrolled(F f) {
+    unrolled_over(std::make_integer_sequence<int, N>{}, f);
+}
+// `pieces` pieces of work over the slots [from, slots): the first one of slot `slot`.
+constexpr int piece_of_slot(int slot, int from, int slots, int pieces) {
+    return slot <= from ? 0 : ((slot - from) * pieces + slots - from - 1) / (slots - from);
+}
+
+template <int D>
+__global__ __launch_bounds__(256, D == 64 ? 2 : 1) void attn_maps_chunk_kernel(const MapsChunkArgs a) {
+    typedef ChunkShape<D> C;
+    constexpr int KS = C::KS, MT = C::MT, VF = C::VF, CPW = C::CPW, BLOCK = 64 * D;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 31, g = lane >> 5;
+    const int map = wave & 1, pair = wave >> 1;
+
+    // Workgroup -> (KV head, range, tile of tokens, set of heads); the longest tiles first, a KV head's on its own XCDs.
+    int kvh, r;
+    if (a.xs > 0) {
+        const int x = blockIdx.x & 7;
+        kvh = x / a.xs;
+        r = (int)(blockIdx.x >> 3) * a.xs + (x - kvh * a.xs);
+    } else {
+        kvh = blockIdx.x / a.per_kvh;
+        r = blockIdx.x - kvh * a.per_kvh;
+    }
+    if (r >= a.per_kvh) return;
+    const int per_split = a.tok_tiles * a.sets, split = r / per_split, in_split = r - split * per_split;
+    const int tile = a.tok_tiles - 1 - in_split / a.sets, set = in_split % a.sets;
+    const int span = 128 / a.hs, t0 = tile * span;  // tokens of the workgroup
+
+    // The blocks it walks: from the one of the first key that its first row sees to the one of its last row's last key.
+    const int end = min(a.kv_valid, a.start + min(a.q_len, t0 + span));
+    const int first_key = a.window > 0 && a.start + t0 + 1 > a.window ? a.start + t0 + 1 - a.window : 0;
+    const int jb = (first_key >> 5) + split * a.split_blocks, nb_all = ((end + 31) >> 5) - jb;
+    const int nb = a.n_splits > 1 ? min(nb_all, a.split_blocks) : nb_all;
+    if (nb <= 0) return;
+
+    // This wavefront's rows: two tiles, 2 pair and 2 pair + 1.
+    int head[2], tok[2], lim[2], lo[2];
+    bool valid[2];
+#pragma unroll
+    for (int rt = 0; rt < 2; ++rt) {
+        const int u = 2 * pair + rt;
+        head[rt] = kvh * a.group + set * a.hs + u % a.hs;
+        tok[rt] = t0 + 32 * (u / a.hs) + li;
+        valid[rt] = tok[rt] < a.q_len;
+        // (a row that is not there sees everything: no block is masked for it, and nobody looks at it)
+        lim[rt] = valid[rt] ? min(a.kv_valid, a.start + tok[rt] + 1) : 0x7fffffff;
+        lo[rt] = valid[rt] && a.window > 0 && a.start + tok[rt] + 1 > a.window ? a.start + tok[rt] + 1 - a.window : 0;
+    }
+    // Blocks from first_masked on, and with a window those up to last_below, hide keys from some row of the wavefront.
+    const int wave_t0 = t0 + 32 * (2 * pair / a.hs), wave_t1 = t0 + 32 * ((2 * pair + 1) / a.hs) + 31;
+    const int first_masked = min(a.start + wave_t0 + 1, a.kv_valid) >> 5;
+    const int last_below = a.window > 0 && a.start + wave_t1 + 1 > a.window ? (a.start + wave_t1 - a.window) >> 5 : -1;
+
+    const __amdgpu_buffer_rsrc_t rk = make_rsrc(a.k_slot + (size_t)kvh * a.page_elems, (unsigned)(a.page_elems * 2));
+    const _Float16 *const v_page = a.v_slot + (size_t)kvh * a.page_elems;
+    // Where a block of the walk lies in the page, in bytes, from block to block; past the last one that again.
+    struct Place {
+        unsigned at, wrap;
+        int left;
+        __device__ __forceinline__ void next() {
+            const unsigned on = at + (unsigned)BLOCK;
+            at = left > 0 ? (on == wrap ? 0u : on) : at;
+            --left;
+        }
+    };
+    Place k_at{(unsigned)(a.ring_blocks ? jb % a.ring_blocks : jb) * (unsigned)BLOCK, a.ring_blocks ? (unsigned)a.ring_blocks * (unsigned)BLOCK : 0xffffffffu, nb - 1};
+    Place v_at = k_at;
+    const unsigned k_lane = (unsigned)(map * (BLOCK / 2) + lane * 16);
+    const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) void *)smem;
+    unsigned v_from[CPW];
+#pragma unroll
+    for (int c = 0; c < CPW; ++c) {
+        const int f = wave * CPW + c;
+        v_from[c] = 2u * (unsigned)(v_piece(D, li, g) + v_piece(D, 32 * (f >> 1), 2 * (f & 1)));
+    }
+    auto copy_v = [&](int i, int c) {  // of block i, which lies at v_at
+        copy16_global_to_lds(reinterpret_cast<const char *>(v_page) + v_at.at, v_from[c], lds0 + (unsigned)((i % kVRing) * C::V_BYTES + (wave * CPW + c) * 1024));
+    };
+
+    h8 q[2][KS], kf[KS];
+#pragma unroll
+    for (int rt = 0; rt < 2; ++rt) {
+        const global_halves row = (global_halves)(a.q + (long long)(valid[rt] ? tok[rt] : 0) * a.q_stride + (long long)head[rt] * D + map * (D / 2) + 8 * g);
+#pragma unroll
+        for (int t = 0; t < KS; ++t) q[rt][t] = load_h8(row + 16 * t);
+    }
+#pragma unroll
+    for (int t = 0; t < KS; ++t) kf[t] = buf_load_h8<0>(rk, k_lane, k_at.at + t * 1024);
+    k_at.next();
+#pragma unroll
+    for (int i = 0; i < kVRing - 1; ++i) {
+#pragma unroll
+        for (int c = 0; c < CPW; ++c) copy_v(i, c);
+        v_at.next();
+    }
+#pragma unroll
+    for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+        for (int t = 0; t < KS; ++t) q[rt][t] = valid[rt] ? q[rt][t] : (h8)(_Float16)0;
+
+    f16v o[2][MT], s[2];
+    float m[2], l[2], l_odd[2], mx[2], alpha[2];
+    h8 p_now[2][2], p_next[2][2];
+#pragma unroll
+    for (int rt = 0; rt < 2; ++rt) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            o[rt][mt] = (f16v)0.0f;
+            keep_sum(o[rt][mt]);
+        }
+        m[rt] = kNegBig;
+        l[rt] = l_odd[rt] = 0.0f;
+    }
+    // The softmax of a tile's block in PIECES pieces: four of the maximum, one of the reference, one a key of the lane's.
+    constexpr int PIECES = 4 + 1 + 16;
+    auto soften = [&](auto rt_c, auto piece_c) __attribute__((always_inline)) {
+        constexpr int rt = decltype(rt_c)::value, piece = decltype(piece_c)::value;
+        if constexpr (piece < 4) {
+            const float x = fmaxf(fmaxf(s[rt][4 * piece], s[rt][4 * piece + 1]), fmaxf(s[rt][4 * piece + 2], s[rt][4 * piece + 3]));
+            mx[rt] = piece == 0 ? x : fmaxf(mx[rt], x);
+        } else if constexpr (piece == 4) {
+            const float top = max_across_halves(mx[rt]) * a.scale_log2e;
+            const bool move = top > m[rt] + kChunkRescale;  // (a row's first visible block always moves)
+            const float moved = move ? top : m[rt];
+            alpha[rt] = move ? fast_exp2(m[rt] - moved) : 1.0f;
+            l[rt] *= alpha[rt];
+            l_odd[rt] *= alpha[rt];
+            m[rt] = moved;
+        } else {
+            constexpr int v = piece - 5;
+            s[rt][v] = fast_exp2(__builtin_fmaf(s[rt][v], a.scale_log2e, -m[rt]));
+            if constexpr (v & 1) {
+                // (the sum over the rounded weights, those that the products with V see)
+                const h2 w = {(_Float16)s[rt][v - 1], (_Float16)s[rt][v]};
+                asm("v_fma_mix_f32 %0, %1, 1.0, %0 op_sel_hi:[1,0,0]" : "+v"(l[rt]) : "v"(w));
+                asm("v_fma_mix_f32 %0, %1, 1.0, %0 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "+v"(l_odd[rt]) : "v"(w));
+                p_next[rt][v >> 3][(v & 7) - 1] = w[0];
+                p_next[rt][v >> 3][v & 7] = w[1];
+            }
+        }
+    };
+    auto hide = [&](int rt, int block) __attribute__((always_inline)) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+            const int key = (block << 5) + 8 * (v >> 2) + 4 * g + (v & 3);
+            if (key >= lim[rt] || key < lo[rt]) s[rt][v] = -INFINITY;
+        }
+    };
+    auto masked = [&](int i) { return jb + i >= first_masked || jb + i <= last_below; };
+    // Keys of block i that some row of the workgroup sees, bit by bit.
+    auto seen_of = [&](int i) { return keys_between(first_key - ((jb + i) << 5), end - ((jb + i) << 5)); };
+    // Values of keys that no row sees, whatever the cache holds there, as zeros: a weight of zero would make NaN of an infinite one.  Every wavefront
+    // those of its own copies, which have landed; they are in the walk's first block and in the sequence's last one.
+    auto drop_unseen_of = [&](int i) __attribute__((always_inline)) {
+        const unsigned seen = seen_of(i);
+        if (seen == ~0u) return;
+#pragma unroll
+        for (int c = 0; c < CPW; ++c) {
+            h8 *const at = reinterpret_cast<h8 *>(smem + (i % kVRing) * C::V_BYTES + (wave * CPW + c) * 1024 + lane * 16);
+            unsigned mask[4];
+            seen_words(mask, 2 * ((wave * CPW + c) & 1) + g, seen);
+            *at = only_seen(*at, mask);
+        }
+    };
+    auto read_v = [&](int i, int f) { return *reinterpret_cast<const h8 *>(smem + (i % kVRing) * C::V_BYTES + f * 1024 + lane * 16); };
+    auto take_weights = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) p_now[rt][t] = p_next[rt][t];
+    };
+    constexpr int AHEAD = 4;  // V fragments on their way out of LDS
+    // Step i: the scores of block i, and between their products and those of block i - 1's values the softmax of block i.
+    auto step = [&](int i) __attribute__((always_inline)) {
+        constexpr int SLOTS = KS + 2 * VF, FROM = 2;  // (a tile's scores are read behind the third product after their last)
+        // V of block i - 1 has landed (K and V of the two blocks since may be on their way), and every wavefront is done with the block whose place
+        // the copies of this step take.
+        TT_WAIT_VMCNT(2 * (KS + CPW));
+        __syncthreads();
+        const unsigned next_k = k_at.at;
+        const bool hidden = masked(i);
+        h8 vf[AHEAD];
+#pragma unroll
+        for (int t = 0; t < KS; ++t) {
+            if (t == 0) first_score(s[0], kf[0], q[0][0]);
+            else next_score(s[0], kf[t], q[0][t]);
+            if (t < AHEAD) vf[t] = read_v(i - 1, t);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int t = KS; t < AHEAD; ++t) vf[t] = read_v(i - 1, t);
+        if (hidden) {
+            settle(s[0]);
+            hide(0, jb + i);
+        }
+        unrolled<SLOTS>([&](auto slot_c) __attribute__((always_inline)) {
+            constexpr int slot = decltype(slot_c)::value;
+            if constexpr (slot < KS) {
+                if constexpr (slot == 0) first_score(s[1], kf[0], q[1][0]);
+                else next_score(s[1], kf[slot], q[1][slot]);
+                kf[slot] = buf_load_h8<0>(rk, k_lane, next_k + slot * 1024);
+            } else {
+                constexpr int u = slot - KS, f = u >> 1, rt = u & 1;
+                if constexpr (u == 0) {
+                    if (hidden) {
+                        settle(s[1]);
+                        hide(1, jb + i);
+                    }
+                }
+                o[rt][f >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[f % AHEAD], p_now[rt][f & 1], o[rt][f >> 1], 0, 0, 0);
+                keep_sum(o[rt][f >> 1]);
+                if constexpr (rt == 1 && f + AHEAD < VF) vf[f % AHEAD] = read_v(i - 1, f + AHEAD);
+                constexpr int EVERY = 2 * VF / CPW;
+                if constexpr (u % EVERY == 2) copy_v(i + 2, u / EVERY);
+            }
+            constexpr int first = piece_of_slot(slot, FROM, SLOTS, 2 * PIECES), behind = piece_of_slot(slot + 1, FROM, SLOTS, 2 * PIECES);
+            if constexpr (first < behind && first <= PIECES && behind > PIECES) static_assert(slot >= KS + 2, "the other tile's scores");
+            unrolled<behind - first>([&](auto at) __attribute__((always_inline)) {
+                constexpr int piece = first + decltype(at)::value;
+                if constexpr (piece % PIECES == 0) asm volatile("" : "+v"(s[piece / PIECES]));  // (not read before here)
+                soften(std::integral_constant<int, piece / PIECES>{}, std::integral_constant<int, piece % PIECES>{});
+            });
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        k_at.next();
+        v_at.next();
+        take_weights();
+    };
+
+    // Block 0's scores and softmax.
+#pragma unroll
+    for (int t = 0; t < KS; ++t) {
+        if (t == 0) {
+            first_score(s[0], kf[0], q[0][0]);
+            first_score(s[1], kf[0], q[1][0]);
+        } else {
+            next_score(s[0], kf[t], q[0][t]);
+            next_score(s[1], kf[t], q[1][t]);
+        }
+        kf[t] = buf_load_h8<0>(rk, k_lane, k_at.at + t * 1024);
+    }
+    k_at.next();
+    settle(s[0]);
+    settle(s[1]);
+#pragma unroll
+    for (int rt = 0; rt < 2; ++rt) {
+        if (masked(0)) hide(rt, jb);
+    }
+    unrolled<2 * PIECES>([&](auto piece) __attribute__((always_inline)) {
+        soften(std::integral_constant<int, decltype(piece)::value / PIECES>{}, std::integral_constant<int, decltype(piece)::value % PIECES>{});
+    });
+    take_weights();  // (no sums yet that a moved reference would mean)
+    const int last = nb - 1;
+    if (last > 0 && seen_of(0) != ~0u) {
+        TT_WAIT_VMCNT(0);
+        asm volatile("" ::: "memory");
+        drop_unseen_of(0);
+    }
+    // A run of steps is a loop of its own, left where a row's reference moves: with the rare scaling of the sums inside it the compiler moved them
+    // about in every step.
+    for (int i = 1; i <= last;) {
+        bool scale_sums;
+#pragma nounroll
+        do {
+            step(i);
+            ++i;
+            scale_sums = __any(alpha[0] != 1.0f || alpha[1] != 1.0f);
+        } while (!scale_sums && i <= last);
+        if (scale_sums) {
+#pragma unroll
+            for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    keep_sum(o[rt][mt]);
+                    o[rt][mt] *= alpha[rt];
+                    keep_sum(o[rt][mt]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+        }
+    }
+    // The last block's values.
+    TT_WAIT_VMCNT(0);
+    asm volatile("" ::: "memory");
+    drop_unseen_of(last);
+    __syncthreads();
+#pragma unroll
+    for (int f = 0; f < VF; ++f) {
+        const h8 x = read_v(last, f);
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt) {
+            o[rt][f >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, p_now[rt][f & 1], o[rt][f >> 1], 0, 0, 0);
+            keep_sum(o[rt][f >> 1]);
+        }
+    }
+#pragma unroll
+    for (int rt = 0; rt < 2; ++rt) l[rt] = sum_across_halves(l[rt] + l_odd[rt]);
+
+    // Lane (li, g), register v of tile mt holds dim 32 mt + 8 (v / 4) + 4 g + v % 4 of row li.
+    if (a.n_splits > 1) {
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt) {
+            if (!valid[rt]) continue;
+            const size_t row = (((size_t)split * (2 * a.group * a.n_kv_heads) + 2 * head[rt] + map) * a.tok_tiles + tile) * span + (tok[rt] - t0);
+            float *const po = a.part_o + row * D + 4 * g;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int vq = 0; vq < 4; ++vq) {
+                    const f4 x = {o[rt][mt][4 * vq], o[rt][mt][4 * vq + 1], o[rt][mt][4 * vq + 2], o[rt][mt][4 * vq + 3]};
+                    *reinterpret_cast<f4 *>(po + 32 * mt + 8 * vq) = x;
+                }
+            if (g == 0) {
+                a.part_ml[row * 2] = m[rt];
+                a.part_ml[row * 2 + 1] = l[rt];
+            }
+        }
+        return;
+    }
+
+    // The maps of a tile meet: wavefront (pair, map) takes the pair's tile `map` and hands the other one over.  Written out per tile of
+    // 32 dims, so that no register is indexed by what is not known here.
+    __syncthreads();  // (the ring's place is the sums')
+    f4 *const to_partner = reinterpret_cast<f4 *>(smem + wave * C::X_BYTES) + lane;
+    const f4 *const from_partner = reinterpret_cast<const f4 *>(smem + (wave ^ 1) * C::X_BYTES) + lane;
+    const float inv[2] = {l[0] > 0.0f ? 1.0f / l[0] : 0.0f, l[1] > 0.0f ? 1.0f / l[1] : 0.0f};
+    const float inv_mine = map ? inv[1] : inv[0], inv_theirs = map ? inv[0] : inv[1];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+        for (int vq = 0; vq < 4; ++vq) {
+            f4 x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = (map ? o[0][mt][4 * vq + e] : o[1][mt][4 * vq + e]) * inv_theirs;
+            to_partner[(mt * 4 + vq) * 64] = x;
+        }
+    }
+    const int my_tok = map ? tok[1] : tok[0], my_head = map ? head[1] : head[0];
+    const bool my_valid = map ? valid[1] : valid[0];
+    const float lambda = a.maps.lambda[(long long)(my_valid ? my_tok : 0) * a.maps.lambda_stride + my_head];
+    __syncthreads();
+    float squares = 0.0f;
+    f16v mine[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int vq = 0; vq < 4; ++vq) {
+            const f4 theirs = from_partner[(mt * 4 + vq) * 64];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float x = (map ? o[1][mt][4 * vq + e] : o[0][mt][4 * vq + e]) * inv_mine;
+                const float d = map_difference(map ? theirs[e] : x, map ? x : theirs[e], lambda);
+                squares += d * d;
+                mine[mt][4 * vq + e] = d;
+            }
+        }
+    float scale = a.maps.out_scale;
+    if (a.maps.norm) {
+        squares = sum_across_halves(squares);
+        scale *= squares == 0.0f ? 0.0f : 1.0f / sqrtf(squares * (1.0f / D) + a.maps.eps);
+    }
+    // Norm weight and gate, and the rows out through LDS, 32 dims at a time: a store writes 64 bytes of 16 rows.
+    char *const stage = smem + C::STAGE_OFF + wave * C::STAGE_BYTES;
+    const int out_row = lane >> 2, out_piece = lane & 3, tile_tok = my_tok - li;
+    const global_halves gate_row = (global_halves)(a.gate + (long long)(my_valid ? my_tok : 0) * a.g_stride + (long long)my_head * D + 4 * g);
+    h4 gate[2][4];
+    auto load_gate = [&](int mt) {
+#pragma unroll
+        for (int vq = 0; vq < 4; ++vq) gate[mt & 1][vq] = *(const __attribute__((address_space(1))) h4_unaligned *)(gate_row + 32 * mt + 8 * vq);
+    };
+    if (a.gate) load_gate(0);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        if (a.gate && mt + 1 < MT) load_gate(mt + 1);
+#pragma unroll
+        for (int vq = 0; vq < 4; ++vq) {
+            h4 x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int d = 32 * mt + 8 * vq + 4 * g + e;
+                float y = mine[mt][4 * vq + e] * scale;
+                if (a.maps.norm) y *= __builtin_bit_cast(float, (unsigned)a.maps.norm[d] << 16);
+                if (a.gate) y *= sigmoid((float)gate[mt & 1][vq][e]);
+                x[e] = (_Float16)y;
+            }
+            *reinterpret_cast<h4 *>(stage + li * C::STAGE_PITCH + (8 * vq + 4 * g) * 2) = x;
+        }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int row = 16 * half + out_row, t = tile_tok + row;
+            const h8 x = *reinterpret_cast<const h8 *>(stage + row * C::STAGE_PITCH + out_piece * 16);
+            if (t < a.q_len) {
+                _Float16 *const to = a.out + (long long)t * a.o_stride + (long long)my_head * D + 32 * mt + out_piece * 8;
+                if (a.aligned) {
+                    *reinterpret_cast<h8 *>(to) = x;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) to[e] = x[e];
+                }
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+template <int D>
+hipError_t configure_chunk() {
+    return hipFuncSetAttribute(reinterpret_cast<const void *>(attn_maps_chunk_kernel<D>), hipFuncAttributeMaxDynamicSharedMemorySize, ChunkShape<D>::LDS);
+}
+
+}  // namespace
+
+int configure_maps_chunk_kernels(tt_hip_ctx *ctx) {
+    hipError_t e = configure_chunk<256>();
+    if (e == hipSuccess) e = configure_chunk<128>();
+    if (e == hipSuccess) e = configure_chunk<64>();
+    return e == hipSuccess ? TT_HIP_OK : hip_fail(ctx, e, "hipFuncSetAttribute(two-map chunk max dynamic LDS)");
+}
+
+int launch_maps_chunk(tt_hip_ctx *ctx, int head_dim, int n_kv_heads, const MapsChunk &c) {
+    MapsChunkArgs a{};
+    a.k_slot = c.pages.k;
+    a.v_slot = c.pages.v;
+    a.page_elems = c.pages.page_elems;
+    a.ring_blocks = c.pages.ring_blocks;
+    a.q = c.q;
+    a.gate = c.gate;
+    a.out = c.out;
+    a.q_stride = c.q_stride;
+    a.g_stride = c.g_stride;
+    a.o_stride = c.o_stride;
+    a.maps = c.maps;
+    a.n_kv_heads = n_kv_heads;
+    a.group = c.n_q_heads / n_kv_heads;
+    a.hs = maps_chunk_heads(a.group);
+    a.sets = a.group / a.hs;
+    const int span = 128 / a.hs;
+    a.tok_tiles = (c.q_len + span - 1) / span;
+    a.start = c.start;
+    a.q_len = c.q_len;
+    a.kv_valid = c.kv_valid;
+    a.window = c.window;
+    a.scale_log2e = c.scale * 1.4426950408889634f;
+    a.n_splits = c.n_splits;
+    a.split_blocks = c.split_blocks;
+    a.part_o = c.part_o;
+    a.part_ml = c.part_ml;
+    a.aligned = c.aligned;
+    a.per_kvh = a.sets * a.tok_tiles * a.n_splits;
+    a.xs = n_kv_heads <= 8 && 8 % n_kv_heads == 0 ? 8 / n_kv_heads : 0;
+    const unsigned grid = a.xs > 0 ? 8u * (unsigned)((a.per_kvh + a.xs - 1) / a.xs) : (unsigned)(a.per_kvh * n_kv_heads);
+    switch (head_dim) {
+        case 256: launch_profiled(ctx, attn_maps_chunk_kernel<256>, dim3(grid), dim3(256), (unsigned)ChunkShape<256>::LDS, a); break;
+        case 128: launch_profiled(ctx, attn_maps_chunk_kernel<128>, dim3(grid), dim3(256), (unsigned)ChunkShape<128>::LDS, a); break;
+        case 64: launch_profiled(ctx, attn_maps_chunk_kernel<64>, dim3(grid), dim3(256), (unsigned)ChunkShape<64>::LDS, a); break;
+        default: return TT_HIP_ERR_SHAPE;
+    }
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? TT_HIP_OK : hip_fail(ctx, e, "attn_maps_chunk_kernel launch");
+}
+
+}  // namespace tt

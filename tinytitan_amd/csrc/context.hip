@@ -708,6 +708,7 @@ tt_hip_ctx *tt_hip_ctx_create(int device, int *out_err) {
             if (st == TT_HIP_OK) st = configure_prefill_kernels(ctx);
             if (st == TT_HIP_OK) st = configure_affine_kernels(ctx);
             if (st == TT_HIP_OK) st = configure_maps_kernels(ctx);
+            if (st == TT_HIP_OK) st = configure_maps_chunk_kernels(ctx);
             if (st == TT_HIP_OK) st = configure_int8_kernels(ctx);
             if (st != TT_HIP_OK) {
                 tt_hip_ctx_destroy(ctx);
@@ -1773,6 +1774,28 @@ int tt_hip_attn_prefill_diff(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int slot
     if (st != TT_HIP_OK) return st;
     BusyGuard guard(ctx);
     if (!guard.ok) return TT_HIP_ERR_BUSY;
+    if (scale > 0.0f && kv->bits == 16 && !getenv("TT_TILES")) {
+        if (hipSetDevice(ctx->device) != hipSuccess) return TT_HIP_ERR_HIP;
+        MapsChunk c{};
+        const size_t slot_elems = (size_t)slot * kv->n_kv_heads * kv->page_elems();
+        c.pages = PageSource{kv->k[layer] + slot_elems, kv->v[layer] + slot_elems, (long long)kv->page_elems(), kv->ring_blocks()};
+        c.q = reinterpret_cast<const _Float16 *>(q);
+        c.gate = reinterpret_cast<const _Float16 *>(gate);
+        c.out = reinterpret_cast<_Float16 *>(out);
+        c.q_stride = (long long)q_stride;
+        c.g_stride = (long long)gate_stride;
+        c.o_stride = (long long)o_stride;
+        c.aligned = aligned16(out) && o_stride % 8 == 0;
+        c.maps = maps;
+        c.n_q_heads = n_q_heads;
+        c.start = start_pos;
+        c.q_len = q_len;
+        c.kv_valid = kv_valid;
+        c.window = window;
+        c.scale = scale;
+        c.n_splits = 1;
+        return launch_maps_chunk(ctx, kv->head_dim, kv->n_kv_heads, c);
+    }
     return run_maps_tiles(ctx, kv, layer, 1, &slot, &start_pos, &kv_valid, q_len, n_q_heads, q, 0, (long long)q_stride, gate, 0,
                           (long long)gate_stride, scale, window, maps, out, 0, (long long)o_stride);
 }

@@ -330,6 +330,25 @@ int configure_maps_kernels(tt_hip_ctx *ctx);
 int launch_splitk_maps(tt_hip_ctx *ctx, const LaunchPlan &plan, int head_dim, int n_seq, const SplitKArgs &args, int kv_bits);
 int launch_maps_join(tt_hip_ctx *ctx, int head_dim, int n_seq, const MapsJoinArgs &args, int most_splits);
 
+// A chunk of one sequence by the kernel of attn_maps_chunk.hip, over fp16 pages; with n_splits > 1 each workgroup takes a range of split_blocks
+// key blocks and leaves partial results for launch_maps_join (maps_chunk_parts).
+struct MapsChunk {
+    PageSource pages;
+    const _Float16 *q, *gate;
+    _Float16 *out;
+    long long q_stride, g_stride, o_stride;
+    int aligned;  // out's rows are 16-byte aligned
+    MapHeads maps;
+    int n_q_heads, start, q_len, kv_valid, window;
+    float scale;  // above zero: a row's maximum is taken over the raw scores
+    int n_splits, split_blocks;
+    float *part_o, *part_ml;
+};
+// Heads whose rows share a workgroup, of those that share a KV head.
+inline int maps_chunk_heads(int group) { return group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1; }
+int configure_maps_chunk_kernels(tt_hip_ctx *ctx);
+int launch_maps_chunk(tt_hip_ctx *ctx, int head_dim, int n_kv_heads, const MapsChunk &chunk);
+
 // A prefix that slots share: block `block` of `slot`'s pages, of which `rows` are the prefix's, every layer, into the same place of
 // `n_slots` others.
 int launch_kv_copy_block(tt_hip_kv *kv, int slot, int block, int rows, int n_slots, const int *slots);

@@ -1890,6 +1890,14 @@ __global__ __launch_bounds__(WAVES * 64, ((NT == 16 && (KEEP < 2 || KEEP == kKee
     }
 }
 
+// a1 - lambda a2 of two maps' results.  Either is rounded before the difference, no product is fused into it: maps that are the same then cancel
+// to zero, and not to a rounding that a norm behind makes a row of.
+__device__ __forceinline__ float map_difference(float a1, float a2, float lambda) {
+    asm("" : "+v"(a1));
+    asm("" : "+v"(a2));
+    return __builtin_fmaf(-lambda, a2, a1);
+}
+
 constexpr size_t keep_list_bytes(int keep, int waves) { return keep == 2 ? (size_t)waves * kKeepWindows * (64 + 1) * sizeof(int) : 0; }
 
 inline size_t lds_bytes_for(int D, int NT, int waves) {

@@ -61,6 +61,11 @@ __device__ __forceinline__ void next_score(f16v &s, h8 k, h8 q) { asm volatile("
 // ... where no two products follow.
 __device__ __forceinline__ void settle(f16v &s) { asm volatile("s_nop 15\n\ts_nop 7" : "+v"(s)); }
 
+__device__ __forceinline__ float max3(float x, float y, float z) {  // (written as a maximum of maxima, each operand is first made canonical)
+    float most;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(most) : "v"(x), "v"(y), "v"(z));
+    return most;
+}
 // A sum over V stays in accumulation registers, wherever control flow comes from: told so behind everything that writes it, or the compiler moves
 // the sums to vector registers and back around every block.
 __device__ __forceinline__ void keep_sum(f16v &o) { asm volatile("" : "+a"(o)); }
@@ -175,7 +180,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void attn_maps_chunk_kernel(c
 
     f16v o[2][MT], s[2];
     float m[2], l[2], l_odd[2], mx[2], alpha[2];
-    h8 p_now[2][2], p_next[2][2];
+    h8 p[2][2];  // weights of the block whose values are next
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt) {
 #pragma unroll
@@ -186,42 +191,50 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void attn_maps_chunk_kernel(c
         m[rt] = kNegBig;
         l[rt] = l_odd[rt] = 0.0f;
     }
-    // The softmax of a tile's block in PIECES pieces: four of the maximum, one of the reference, one a key of the lane's.
-    constexpr int PIECES = 4 + 1 + 16;
-    auto soften = [&](auto rt_c, auto piece_c) __attribute__((always_inline)) {
+    // The softmax of a tile's block in PIECES pieces: two of the maximum, two of the reference, and of each of the lane's eight pairs of keys two, so
+    // that no piece reads an exponential of its own.
+    constexpr int PIECES = 2 + 2 + 2 * 8;
+    auto soften = [&](auto rt_c, auto piece_c, h8 (&p_next)[2][2]) __attribute__((always_inline)) {
         constexpr int rt = decltype(rt_c)::value, piece = decltype(piece_c)::value;
-        if constexpr (piece < 4) {
-            const float x = fmaxf(fmaxf(s[rt][4 * piece], s[rt][4 * piece + 1]), fmaxf(s[rt][4 * piece + 2], s[rt][4 * piece + 3]));
-            mx[rt] = piece == 0 ? x : fmaxf(mx[rt], x);
-        } else if constexpr (piece == 4) {
-            const float top = max_across_halves(mx[rt]) * a.scale_log2e;
-            const bool move = top > m[rt] + kChunkRescale;  // (a row's first visible block always moves)
-            const float moved = move ? top : m[rt];
-            alpha[rt] = move ? fast_exp2(m[rt] - moved) : 1.0f;
+        if constexpr (piece < 2) {
+            constexpr int v = 8 * piece;
+            float x = max3(s[rt][v], s[rt][v + 1], s[rt][v + 2]);
+            x = max3(x, s[rt][v + 3], s[rt][v + 4]);
+            x = max3(x, s[rt][v + 5], s[rt][v + 6]);
+            mx[rt] = piece == 0 ? max3(x, s[rt][v + 7], s[rt][v + 7]) : max3(x, s[rt][v + 7], mx[rt]);
+        } else if constexpr (piece == 2) {
+            mx[rt] = max_across_halves(mx[rt]) * a.scale_log2e;
+        } else if constexpr (piece == 3) {
+            const bool move = mx[rt] > m[rt] + kChunkRescale;  // (a row's first visible block always moves)
+            const float moved = move ? mx[rt] : m[rt];
+            alpha[rt] = fast_exp2(m[rt] - moved);  // (1 where it stays)
             l[rt] *= alpha[rt];
             l_odd[rt] *= alpha[rt];
             m[rt] = moved;
         } else {
-            constexpr int v = piece - 5;
-            s[rt][v] = fast_exp2(__builtin_fmaf(s[rt][v], a.scale_log2e, -m[rt]));
-            if constexpr (v & 1) {
+            constexpr int v = (piece - 4) / 2 * 2;
+            if constexpr (piece % 2 == 0) {
+                s[rt][v] = fast_exp2(__builtin_fmaf(s[rt][v], a.scale_log2e, -m[rt]));
+                s[rt][v + 1] = fast_exp2(__builtin_fmaf(s[rt][v + 1], a.scale_log2e, -m[rt]));
+            } else {
                 // (the sum over the rounded weights, those that the products with V see)
-                const h2 w = {(_Float16)s[rt][v - 1], (_Float16)s[rt][v]};
+                const h2 w = {(_Float16)s[rt][v], (_Float16)s[rt][v + 1]};
                 asm("v_fma_mix_f32 %0, %1, 1.0, %0 op_sel_hi:[1,0,0]" : "+v"(l[rt]) : "v"(w));
                 asm("v_fma_mix_f32 %0, %1, 1.0, %0 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "+v"(l_odd[rt]) : "v"(w));
-                p_next[rt][v >> 3][(v & 7) - 1] = w[0];
-                p_next[rt][v >> 3][v & 7] = w[1];
+                p_next[rt][v >> 3][v & 7] = w[0];
+                p_next[rt][v >> 3][(v & 7) + 1] = w[1];
             }
         }
     };
     auto hide = [&](int rt, int block) __attribute__((always_inline)) {
+        int base = (block << 5) + 4 * g;
+        asm volatile("" : "+v"(base));  // (or the keys' numbers are made in front of the branch, in every step)
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
-            const int key = (block << 5) + 8 * (v >> 2) + 4 * g + (v & 3);
+            const int key = base + 8 * (v >> 2) + (v & 3);
             if (key >= lim[rt] || key < lo[rt]) s[rt][v] = -INFINITY;
         }
     };
-    auto masked = [&](int i) { return jb + i >= first_masked || jb + i <= last_below; };
     // Keys of block i that some row of the workgroup sees, bit by bit.
     auto seen_of = [&](int i) { return keys_between(first_key - ((jb + i) << 5), end - ((jb + i) << 5)); };
     // Values of keys that no row sees, whatever the cache holds there, as zeros: a weight of zero would make NaN of an infinite one.  Every wavefront
@@ -238,32 +251,31 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void attn_maps_chunk_kernel(c
         }
     };
     auto read_v = [&](int i, int f) { return *reinterpret_cast<const h8 *>(smem + (i % kVRing) * C::V_BYTES + f * 1024 + lane * 16); };
-    auto take_weights = [&]() __attribute__((always_inline)) {
-#pragma unroll
-        for (int rt = 0; rt < 2; ++rt)
-#pragma unroll
-            for (int t = 0; t < 2; ++t) p_now[rt][t] = p_next[rt][t];
-    };
-    constexpr int AHEAD = 4;  // V fragments on their way out of LDS
     // Step i: the scores of block i, and between their products and those of block i - 1's values the softmax of block i.
-    auto step = [&](int i) __attribute__((always_inline)) {
-        constexpr int SLOTS = KS + 2 * VF, FROM = 2;  // (a tile's scores are read behind the third product after their last)
+    unsigned ring = 0;  // where block i - 1's values lie in LDS
+    auto step = [&](int i, const h8 (&p_now)[2][2], h8 (&p_next)[2][2]) __attribute__((always_inline)) {
+        constexpr int SLOTS = KS + 4 * MT, FROM = 2;  // (a tile's scores are read behind the third product after their last)
         // V of block i - 1 has landed (K and V of the two blocks since may be on their way), and every wavefront is done with the block whose place
         // the copies of this step take.
         TT_WAIT_VMCNT(2 * (KS + CPW));
         __syncthreads();
         const unsigned next_k = k_at.at;
-        const bool hidden = masked(i);
-        h8 vf[AHEAD];
+        const bool hidden = jb + i >= first_masked || jb + i <= last_below;
+        const char *const v_block = smem + ring + lane * 16, *const v_next = reinterpret_cast<const char *>(v_page) + v_at.at;
+        ring = (ring + C::V_BYTES) & (C::RING_BYTES - 1);
+        const unsigned v_to = lds0 + ((ring + 2 * C::V_BYTES) & (C::RING_BYTES - 1)) + (unsigned)(wave * CPW) * 1024u;  // block i + 2's place
+        h8 vf[2][2];  // two tiles of dims
+        auto read_v = [&](int mt) __attribute__((always_inline)) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) vf[mt & 1][t] = *reinterpret_cast<const h8 *>(v_block + (2 * mt + t) * 1024);
+        };
 #pragma unroll
         for (int t = 0; t < KS; ++t) {
             if (t == 0) first_score(s[0], kf[0], q[0][0]);
             else next_score(s[0], kf[t], q[0][t]);
-            if (t < AHEAD) vf[t] = read_v(i - 1, t);
+            if (t < 2) read_v(t);
             __builtin_amdgcn_sched_barrier(0);
         }
-#pragma unroll
-        for (int t = KS; t < AHEAD; ++t) vf[t] = read_v(i - 1, t);
         if (hidden) {
             settle(s[0]);
             hide(0, jb + i);
@@ -273,33 +285,39 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void attn_maps_chunk_kernel(c
             if constexpr (slot < KS) {
                 if constexpr (slot == 0) first_score(s[1], kf[0], q[1][0]);
                 else next_score(s[1], kf[slot], q[1][slot]);
-                kf[slot] = buf_load_h8<0>(rk, k_lane, next_k + slot * 1024);
+                kf[slot] = buf_load_h8<0>(rk, k_lane + (slot & 3) * 1024, next_k + (slot >> 2) * 4096);
             } else {
-                constexpr int u = slot - KS, f = u >> 1, rt = u & 1;
+                // (two products in a row to a sum: 32 cycles each, 36 where the sum is another every time)
+                constexpr int u = slot - KS, mt = u >> 2, rt = (u >> 1) & 1, t = u & 1;
                 if constexpr (u == 0) {
                     if (hidden) {
                         settle(s[1]);
                         hide(1, jb + i);
                     }
                 }
-                o[rt][f >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[f % AHEAD], p_now[rt][f & 1], o[rt][f >> 1], 0, 0, 0);
-                keep_sum(o[rt][f >> 1]);
-                if constexpr (rt == 1 && f + AHEAD < VF) vf[f % AHEAD] = read_v(i - 1, f + AHEAD);
-                constexpr int EVERY = 2 * VF / CPW;
-                if constexpr (u % EVERY == 2) copy_v(i + 2, u / EVERY);
+                o[rt][mt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[mt & 1][t], p_now[rt][t], o[rt][mt], 0, 0, 0);
+                keep_sum(o[rt][mt]);
+                if constexpr (rt == 1 && t == 1 && mt + 2 < MT) read_v(mt + 2);
+                constexpr int EVERY = 4 * MT / CPW;
+                if constexpr (u % EVERY == 2) copy16_global_to_lds(v_next, v_from[u / EVERY], v_to + (u / EVERY) * 1024u);
             }
             constexpr int first = piece_of_slot(slot, FROM, SLOTS, 2 * PIECES), behind = piece_of_slot(slot + 1, FROM, SLOTS, 2 * PIECES);
             if constexpr (first < behind && first <= PIECES && behind > PIECES) static_assert(slot >= KS + 2, "the other tile's scores");
             unrolled<behind - first>([&](auto at) __attribute__((always_inline)) {
                 constexpr int piece = first + decltype(at)::value;
                 if constexpr (piece % PIECES == 0) asm volatile("" : "+v"(s[piece / PIECES]));  // (not read before here)
-                soften(std::integral_constant<int, piece / PIECES>{}, std::integral_constant<int, piece % PIECES>{});
+                soften(std::integral_constant<int, piece / PIECES>{}, std::integral_constant<int, piece % PIECES>{}, p_next);
             });
             __builtin_amdgcn_sched_barrier(0);
         });
         k_at.next();
         v_at.next();
-        take_weights();
+    };
+    auto copy_weights = [&](const h8 (&from)[2][2], h8 (&to)[2][2]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) to[rt][t] = from[rt][t];
     };
 
     // Block 0's scores and softmax.
@@ -317,14 +335,13 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void attn_maps_chunk_kernel(c
     k_at.next();
     settle(s[0]);
     settle(s[1]);
-#pragma unroll
-    for (int rt = 0; rt < 2; ++rt) {
-        if (masked(0)) hide(rt, jb);
+    if (jb >= first_masked || jb <= last_below) {
+        hide(0, jb);
+        hide(1, jb);
     }
     unrolled<2 * PIECES>([&](auto piece) __attribute__((always_inline)) {
-        soften(std::integral_constant<int, decltype(piece)::value / PIECES>{}, std::integral_constant<int, decltype(piece)::value % PIECES>{});
+        soften(std::integral_constant<int, decltype(piece)::value / PIECES>{}, std::integral_constant<int, decltype(piece)::value % PIECES>{}, p);
     });
-    take_weights();  // (no sums yet that a moved reference would mean)
     const int last = nb - 1;
     if (last > 0 && seen_of(0) != ~0u) {
         TT_WAIT_VMCNT(0);
@@ -336,16 +353,19 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void attn_maps_chunk_kernel(c
     for (int i = 1; i <= last;) {
         bool scale_sums;
 #pragma nounroll
-        do {
-            step(i);
+        do {  // (two steps a turn, with the weights' registers in turn, were 5 % slower at heads of 128 and do not fit at heads of 256)
+            h8 p_next[2][2];
+            step(i, p, p_next);
             ++i;
             scale_sums = __any(alpha[0] != 1.0f || alpha[1] != 1.0f);
+            copy_weights(p_next, p);
         } while (!scale_sums && i <= last);
         if (scale_sums) {
 #pragma unroll
             for (int rt = 0; rt < 2; ++rt)
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
+                    // (one at a time, and each kept where it is: no registers are left to have several on their way)
                     keep_sum(o[rt][mt]);
                     o[rt][mt] *= alpha[rt];
                     keep_sum(o[rt][mt]);
@@ -363,7 +383,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void attn_maps_chunk_kernel(c
         const h8 x = read_v(last, f);
 #pragma unroll
         for (int rt = 0; rt < 2; ++rt) {
-            o[rt][f >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, p_now[rt][f & 1], o[rt][f >> 1], 0, 0, 0);
+            o[rt][f >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, p[rt][f & 1], o[rt][f >> 1], 0, 0, 0);
             keep_sum(o[rt][f >> 1]);
         }
     }

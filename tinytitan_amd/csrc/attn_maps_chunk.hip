@@ -69,6 +69,13 @@ __device__ __forceinline__ float max3(float x, float y, float z) {  // (written 
 // A sum over V stays in accumulation registers, wherever control flow comes from: told so behind everything that writes it, or the compiler moves
 // the sums to vector registers and back around every block.
 __device__ __forceinline__ void keep_sum(f16v &o) { asm volatile("" : "+a"(o)); }
+// ... where it is read in a branch of the first or the second map's wavefronts, in words of its own: else the two are made one that selects
+// every register.
+template <bool SECOND>
+__device__ __forceinline__ void keep_sum_of(const f16v &o) {
+    if constexpr (SECOND) asm volatile("; the second map" ::"a"(o));
+    else asm volatile("; the first map" ::"a"(o));
+}
 
 template <typename F, int... I>
 __device__ __forceinline__ void unrolled_over(std::integer_sequence<int, I...>, F f) {
@@ -351,6 +358,10 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void attn_maps_chunk_kernel(c
     // A run of steps is a loop of its own, left where a row's reference moves: with the rare scaling of the sums inside it the compiler moved them
     // about in every step.
     for (int i = 1; i <= last;) {
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) keep_sum(o[rt][mt]);
         bool scale_sums;
 #pragma nounroll
         do {  // (two steps a turn, with the weights' registers in turn, were 5 % slower at heads of 128 and do not fit at heads of 256)
@@ -373,6 +384,10 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void attn_maps_chunk_kernel(c
                 }
         }
     }
+#pragma unroll
+    for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) keep_sum(o[rt][mt]);
     // The last block's values.
     TT_WAIT_VMCNT(0);
     asm volatile("" ::: "memory");
@@ -412,73 +427,95 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void attn_maps_chunk_kernel(c
         return;
     }
 
-    // The maps of a tile meet: wavefront (pair, map) takes the pair's tile `map` and hands the other one over.  Written out per tile of
-    // 32 dims, so that no register is indexed by what is not known here.
+    // The maps of a tile meet: wavefront (pair, map) takes the pair's tile `map` and hands its sums of the other one over, as they are.  What follows
+    // is done once a workgroup, straight on, so that its time goes by its length: the sums are chosen by branches, no select of each register,
+    // and the tile's difference lies in LDS, so that norm, gate and stores are a short loop over tiles of 32 dims.
     __syncthreads();  // (the ring's place is the sums')
     f4 *const to_partner = reinterpret_cast<f4 *>(smem + wave * C::X_BYTES) + lane;
-    const f4 *const from_partner = reinterpret_cast<const f4 *>(smem + (wave ^ 1) * C::X_BYTES) + lane;
-    const float inv[2] = {l[0] > 0.0f ? 1.0f / l[0] : 0.0f, l[1] > 0.0f ? 1.0f / l[1] : 0.0f};
-    const float inv_mine = map ? inv[1] : inv[0], inv_theirs = map ? inv[0] : inv[1];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-        for (int vq = 0; vq < 4; ++vq) {
-            f4 x;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = (map ? o[0][mt][4 * vq + e] : o[1][mt][4 * vq + e]) * inv_theirs;
-            to_partner[(mt * 4 + vq) * 64] = x;
-        }
-    }
+    f4 *const from_partner = reinterpret_cast<f4 *>(smem + (wave ^ 1) * C::X_BYTES) + lane;
+    float *const sums = reinterpret_cast<float *>(smem + C::STAGE_OFF);
+    const float my_l = map ? l[1] : l[0];
     const int my_tok = map ? tok[1] : tok[0], my_head = map ? head[1] : head[0];
     const bool my_valid = map ? valid[1] : valid[0];
     const float lambda = a.maps.lambda[(long long)(my_valid ? my_tok : 0) * a.maps.lambda_stride + my_head];
-    __syncthreads();
-    float squares = 0.0f;
-    f16v mine[MT];
+    auto hand_over = [&](const f16v (&x)[MT], auto second) __attribute__((always_inline)) {
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+        for (int mt = 0; mt < MT; ++mt) {
+            keep_sum_of<decltype(second)::value>(x[mt]);
 #pragma unroll
-        for (int vq = 0; vq < 4; ++vq) {
-            const f4 theirs = from_partner[(mt * 4 + vq) * 64];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float x = (map ? o[1][mt][4 * vq + e] : o[0][mt][4 * vq + e]) * inv_mine;
-                const float d = map_difference(map ? theirs[e] : x, map ? x : theirs[e], lambda);
-                squares += d * d;
-                mine[mt][4 * vq + e] = d;
-            }
+            for (int vq = 0; vq < 4; ++vq) to_partner[(mt * 4 + vq) * 64] = f4{x[mt][4 * vq], x[mt][4 * vq + 1], x[mt][4 * vq + 2], x[mt][4 * vq + 3]};
+            __builtin_amdgcn_sched_barrier(0);
         }
+    };
+    if (map) hand_over(o[0], std::true_type{});
+    else hand_over(o[1], std::false_type{});
+    sums[wave * 64 + lane] = map ? l[0] : l[1];
+    __syncthreads();
+    const float their_l = sums[(wave ^ 1) * 64 + lane];
+    const float my_inv = my_l > 0.0f ? 1.0f / my_l : 0.0f, their_inv = their_l > 0.0f ? 1.0f / their_l : 0.0f;
+    float squares = 0.0f;
+    auto subtract = [&](const f16v (&x)[MT], auto second) __attribute__((always_inline)) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            keep_sum_of<decltype(second)::value>(x[mt]);
+#pragma unroll
+            for (int vq = 0; vq < 4; ++vq) {
+                const f4 theirs = from_partner[(mt * 4 + vq) * 64];
+                f4 d;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float mine = x[mt][4 * vq + e] * my_inv, other = theirs[e] * their_inv;
+                    d[e] = decltype(second)::value ? map_difference(other, mine, lambda) : map_difference(mine, other, lambda);
+                    squares += d[e] * d[e];
+                }
+                from_partner[(mt * 4 + vq) * 64] = d;  // (what this lane alone reads)
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    if (map) subtract(o[1], std::true_type{});
+    else subtract(o[0], std::false_type{});
     float scale = a.maps.out_scale;
     if (a.maps.norm) {
         squares = sum_across_halves(squares);
         scale *= squares == 0.0f ? 0.0f : 1.0f / sqrtf(squares * (1.0f / D) + a.maps.eps);
     }
+    __syncthreads();  // (the sums of the weights have been read: their place is the rows')
     // Norm weight and gate, and the rows out through LDS, 32 dims at a time: a store writes 64 bytes of 16 rows.
     char *const stage = smem + C::STAGE_OFF + wave * C::STAGE_BYTES;
     const int out_row = lane >> 2, out_piece = lane & 3, tile_tok = my_tok - li;
     const global_halves gate_row = (global_halves)(a.gate + (long long)(my_valid ? my_tok : 0) * a.g_stride + (long long)my_head * D + 4 * g);
-    h4 gate[2][4];
-    auto load_gate = [&](int mt) {
-#pragma unroll
-        for (int vq = 0; vq < 4; ++vq) gate[mt & 1][vq] = *(const __attribute__((address_space(1))) h4_unaligned *)(gate_row + 32 * mt + 8 * vq);
-    };
-    if (a.gate) load_gate(0);
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-        if (a.gate && mt + 1 < MT) load_gate(mt + 1);
+    h4 gate[4];
+    uint16_t weight[16];
+    auto load = [&](int mt) __attribute__((always_inline)) {
 #pragma unroll
         for (int vq = 0; vq < 4; ++vq) {
-            h4 x;
+            if (a.gate) gate[vq] = *(const __attribute__((address_space(1))) h4_unaligned *)(gate_row + 32 * mt + 8 * vq);
+            if (a.maps.norm) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int d = 32 * mt + 8 * vq + 4 * g + e;
-                float y = mine[mt][4 * vq + e] * scale;
-                if (a.maps.norm) y *= __builtin_bit_cast(float, (unsigned)a.maps.norm[d] << 16);
-                if (a.gate) y *= sigmoid((float)gate[mt & 1][vq][e]);
-                x[e] = (_Float16)y;
+                for (int e = 0; e < 4; ++e) weight[4 * vq + e] = a.maps.norm[32 * mt + 8 * vq + 4 * g + e];
             }
+        }
+    };
+    load(0);
+#pragma nounroll
+    for (int mt = 0; mt < MT; ++mt) {
+        f4 y[4];
+#pragma unroll
+        for (int vq = 0; vq < 4; ++vq) {
+            y[vq] = from_partner[(mt * 4 + vq) * 64] * scale;
+            if (a.maps.norm) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[vq][e] *= __builtin_bit_cast(float, (unsigned)weight[4 * vq + e] << 16);
+            }
+            if (a.gate) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[vq][e] *= sigmoid((float)gate[vq][e]);
+            }
+            const h4 x = {(_Float16)y[vq][0], (_Float16)y[vq][1], (_Float16)y[vq][2], (_Float16)y[vq][3]};
             *reinterpret_cast<h4 *>(stage + li * C::STAGE_PITCH + (8 * vq + 4 * g) * 2) = x;
         }
+        if (mt + 1 < MT) load(mt + 1);
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int half = 0; half < 2; ++half) {

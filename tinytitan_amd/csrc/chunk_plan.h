@@ -3,6 +3,7 @@
 #pragma once
 
 #include <algorithm>
+#include <cmath>
 
 namespace tt {
 
@@ -165,6 +166,67 @@ inline double splitk_rounds_us(int n_cus, int n_q_heads, int n_kv_heads, int q_l
     if (blocks < 64 || tiles <= 0) return even_us;
     const long long splits = std::max<long long>(n_cus / tiles, 1), rounds = (tiles * splits + n_cus - 1) / n_cus;
     return 5.0 + (even_us - 5.0) * ((double)rounds * n_cus / ((double)tiles * splits));
+}
+
+// Differential attention of a chunk: over the split-K tiles (n_splits 0), whose rows are both maps', or by the chunk kernel of attn_maps_chunk.hip over
+// n_splits ranges of the keys (1: all of a tile's), whichever is estimated fastest.  From timings at 16/2 heads of 256, 32/8 of 128, 12/4 of 128 and
+// 16/4 of 64, 33 to 4,096 rows behind 0 to 32,000 keys, some behind a window.  us, split-K tiles / whole / the best number of ranges:
+//   16/2 of 256: 33 rows behind 4,000 keys 22.1 / 137.9 / 37.0 (8), 333 behind 9,000 191.0 / 314 / 113 (4), 777 behind 9,000 395 / 321 / 203 (2),
+//   777 of a prompt 61.3 / 41.6 / 43.9 (2), 4,096 behind 4,500 1,162 / 586 / 682 (2); over 8 bits, whose pages are dequantised first, 333 behind 9,000
+//   270.9 / 335.5 / 132.0 (4), 33 behind 4,000 26.2 / 166.6 / 49.0 (16);
+//   32/8 of 128: 100 behind 8,000 56.8 / 203 / 48.0 (8), 777 behind 9,000 400 / 237 / 256 (2); 16/4 of 64: 777 behind 2,500 53.1 / 73.1 / 46.6 (3).
+struct MapsPlan {
+    int n_splits = 0, split_blocks = 0;
+};
+constexpr long long kMapsRangeRows = 1ll << 19;  // partial results of the ranges at a time (512 MiB)
+inline MapsPlan plan_maps_chunk(int n_cus, int D, int n_q_heads, int n_kv_heads, int start, int q_len, int window, int bits) {
+    const int group = n_q_heads / n_kv_heads, hs = group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1, span = 128 / hs;
+    const int n_tiles = (q_len + span - 1) / span;
+    // At most this many blocks a tile of `span` tokens walks, and the shortest of them.
+    const long long all = ((long long)start + q_len + 31) / 32;
+    const int most = (int)(window > 0 ? std::min<long long>(all, ((long long)window + span + 60) / 32 + 1) : all);
+    const int least = window > 0 ? most : (int)std::min<long long>(all, ((long long)start + span + 31) / 32);
+    const double mean = (most + least) / 2.0;
+    // A KV head's workgroups run on its own XCDs where it has whole ones; of heads of 64 two fit a CU.
+    const bool own = n_kv_heads <= 8 && 8 % n_kv_heads == 0;
+    const int slots = (own ? n_cus / n_kv_heads : n_cus) * (D == 64 ? 2 : 1);
+    const int per_tile = (own ? group : n_q_heads) / hs;  // workgroups
+    const double start_us = D == 256 ? 13.0 : D == 128 ? 9.0 : 7.0;
+    auto step_us = [&](double workgroups) {
+        const double fill = std::min(1.0, workgroups / slots);
+        return D == 256 ? 0.95 + 0.42 * fill * fill : D == 128 ? 0.70 + 0.12 * fill : fill > 0.5 ? 0.88 : 0.60;
+    };
+    // Whole tiles, the longest first: no CU is done before its longest tile, its share of all of them, or, with k rounds begun, k + 1 tiles of
+    // the length that the last of those begins with.
+    const int singles = n_tiles * per_tile;
+    double blocks = std::max<double>(most, singles * mean / slots);
+    for (int k = 1; k * slots < singles; ++k) blocks = std::max(blocks, (k + 1) * (most - (most - least) * (double)(k * slots) / (singles - 1)));
+    const int rounds = (singles + slots - 1) / slots;
+    double best = start_us + (rounds - 1) * (start_us - 4.0) + blocks * step_us(singles);
+    if (D == 64 && singles <= slots && 2 * singles > slots) best -= (most - least) * 0.13;  // (a long tile's neighbour on its CU is done before it)
+    MapsPlan p;
+    p.n_splits = 1;
+    p.split_blocks = most;
+    const long long range_rows = 2ll * n_q_heads * n_tiles * span;
+    const double part_us = 2.0 * n_q_heads * q_len * D * 8.0 / 5.0e6;  // a range's partial results, written and read
+    for (int s = 2; s <= 32 && most / s >= 4 && s * range_rows <= kMapsRangeRows; ++s) {
+        const int len = (most + s - 1) / s;
+        const double ranges = mean / len + 0.5 * (1.0 - (double)least / most), workgroups = singles * std::max(1.0, ranges);
+        const double some = std::ceil(workgroups / slots);
+        const double us = start_us + (some - 1) * (start_us - 4.0) + some * len * step_us(workgroups) + 5.0 + ranges * part_us;
+        if (us < best) {
+            best = us;
+            p.split_blocks = len;
+            p.n_splits = (most + len - 1) / len;
+        }
+    }
+    double tiles = 4.0 + 1.08 * estimate_splitk_chunk_us(n_cus, D, 2 * n_q_heads, n_kv_heads, q_len, least, most);
+    if (bits != 16) {
+        tiles *= 1.3;
+        best += 3.0 + (double)(window > 0 ? std::min<long long>(all, ((long long)window + q_len) / 32 + 2) : all) * 32.0 * n_kv_heads * D * 6.0 / 4.5e6;
+    }
+    if (tiles < best) p = MapsPlan{};
+    return p;
 }
 
 }  // namespace tt

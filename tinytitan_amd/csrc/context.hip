@@ -1774,30 +1774,81 @@ int tt_hip_attn_prefill_diff(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int slot
     if (st != TT_HIP_OK) return st;
     BusyGuard guard(ctx);
     if (!guard.ok) return TT_HIP_ERR_BUSY;
-    if (scale > 0.0f && kv->bits == 16 && !getenv("TT_TILES")) {
-        if (hipSetDevice(ctx->device) != hipSuccess) return TT_HIP_ERR_HIP;
-        MapsChunk c{};
+    if (hipSetDevice(ctx->device) != hipSuccess) return TT_HIP_ERR_HIP;
+    const long long end = (long long)start_pos + q_len;
+    const MapsPlan plan = plan_maps_chunk(ctx->n_cus, kv->head_dim, n_q_heads, kv->n_kv_heads, start_pos, q_len, window, kv->bits);
+    bool chunk = scale > 0.0f && plan.n_splits > 0;
+    const int group = n_q_heads / kv->n_kv_heads, span = 128 / maps_chunk_heads(group), tok_tiles = (q_len + span - 1) / span;
+    // (no memory for partial results or dequantised pages, or a capture in which they would have to grow: the tiles)
+    auto room = [&](int got) {
+        if (got == TT_HIP_ERR_BUSY || got == TT_HIP_ERR_OUT_OF_MEMORY) {
+            chunk = false;
+            return (int)TT_HIP_OK;
+        }
+        return got;
+    };
+    if (chunk && plan.n_splits > 1) st = room(ensure_partials(ctx, (size_t)plan.n_splits * 2 * n_q_heads * tok_tiles * span, kv->head_dim));
+    if (st != TT_HIP_OK) return st;
+    // Quantised pages: the blocks that some row sees, dequantised once, and positions counted from the first of them.
+    const int skipped = kv->bits == 16 ? 0 : (int)(window > 0 && start_pos + 1LL > window ? start_pos + 1LL - window : 0) / kBlockTokens;
+    const int staged_blocks = (int)((end + kBlockTokens - 1) / kBlockTokens) - skipped;
+    const size_t staged_page = (size_t)staged_blocks * kBlockTokens * kv->head_dim;
+    if (chunk && kv->bits != 16) st = room(ensure_stage(ctx, staged_page * kv->n_kv_heads));
+    if (st != TT_HIP_OK) return st;
+    if (!chunk)
+        return run_maps_tiles(ctx, kv, layer, 1, &slot, &start_pos, &kv_valid, q_len, n_q_heads, q, 0, (long long)q_stride, gate, 0,
+                              (long long)gate_stride, scale, window, maps, out, 0, (long long)o_stride);
+    MapsChunk c{};
+    if (kv->bits == 16) {
         const size_t slot_elems = (size_t)slot * kv->n_kv_heads * kv->page_elems();
         c.pages = PageSource{kv->k[layer] + slot_elems, kv->v[layer] + slot_elems, (long long)kv->page_elems(), kv->ring_blocks()};
-        c.q = reinterpret_cast<const _Float16 *>(q);
-        c.gate = reinterpret_cast<const _Float16 *>(gate);
-        c.out = reinterpret_cast<_Float16 *>(out);
-        c.q_stride = (long long)q_stride;
-        c.g_stride = (long long)gate_stride;
-        c.o_stride = (long long)o_stride;
-        c.aligned = aligned16(out) && o_stride % 8 == 0;
-        c.maps = maps;
-        c.n_q_heads = n_q_heads;
-        c.start = start_pos;
-        c.q_len = q_len;
-        c.kv_valid = kv_valid;
-        c.window = window;
-        c.scale = scale;
-        c.n_splits = 1;
-        return launch_maps_chunk(ctx, kv->head_dim, kv->n_kv_heads, c);
+    } else {
+        const DequantPieces from{0, slot, skipped};
+        st = launch_kvq_dequant_blocks(kv, layer, slot, staged_blocks, ctx->stage_k, ctx->stage_v, staged_page, &from);
+        if (st != TT_HIP_OK) return st;
+        c.pages = PageSource{ctx->stage_k, ctx->stage_v, (long long)staged_page, 0};
     }
-    return run_maps_tiles(ctx, kv, layer, 1, &slot, &start_pos, &kv_valid, q_len, n_q_heads, q, 0, (long long)q_stride, gate, 0,
-                          (long long)gate_stride, scale, window, maps, out, 0, (long long)o_stride);
+    c.q = reinterpret_cast<const _Float16 *>(q);
+    c.gate = reinterpret_cast<const _Float16 *>(gate);
+    c.out = reinterpret_cast<_Float16 *>(out);
+    c.q_stride = (long long)q_stride;
+    c.g_stride = (long long)gate_stride;
+    c.o_stride = (long long)o_stride;
+    c.aligned = aligned16(out) && o_stride % 8 == 0;
+    c.maps = maps;
+    c.n_q_heads = n_q_heads;
+    c.start = start_pos - kBlockTokens * skipped;
+    c.q_len = q_len;
+    c.kv_valid = (int)end - kBlockTokens * skipped;
+    c.window = window;
+    c.scale = scale;
+    c.n_splits = plan.n_splits;
+    c.split_blocks = plan.split_blocks;
+    c.part_o = ctx->part_o;
+    c.part_ml = ctx->part_ml;
+    st = launch_maps_chunk(ctx, kv->head_dim, kv->n_kv_heads, c);
+    if (st != TT_HIP_OK || plan.n_splits == 1) return st;
+    MapsJoinArgs a;
+    std::memset(static_cast<void *>(&a), 0, sizeof(a));
+    a.parts.o = ctx->part_o;
+    a.parts.ml = ctx->part_ml;
+    a.parts.nt = a.parts.tt = span;  // (a tile of the join is a workgroup's rows of one map)
+    a.parts.gh = 1;
+    a.parts.hsubs = a.group2 = 2 * group;
+    a.parts.tok_tiles = tok_tiles;
+    a.parts.n_tiles = 2 * n_q_heads * tok_tiles;
+    a.parts.split_len = plan.split_blocks * kBlockTokens;
+    a.window = window;
+    a.rows = q_len;
+    a.heads = n_q_heads;
+    a.maps = maps;
+    a.gate = c.gate;
+    a.out = c.out;
+    a.g_tok_stride = c.g_stride;
+    a.o_tok_stride = c.o_stride;
+    a.aligned = c.aligned;
+    a.seq[0] = JoinSeq{c.start, c.kv_valid, 0};
+    return launch_maps_join(ctx, kv->head_dim, 1, a, plan.n_splits);
 }
 
 // ---- sequences that share a prefix ------------------------------------------

@@ -331,7 +331,7 @@ int launch_splitk_maps(tt_hip_ctx *ctx, const LaunchPlan &plan, int head_dim, in
 int launch_maps_join(tt_hip_ctx *ctx, int head_dim, int n_seq, const MapsJoinArgs &args, int most_splits);
 
 // A chunk of one sequence by the kernel of attn_maps_chunk.hip, over fp16 pages; with n_splits > 1 each workgroup takes a range of split_blocks
-// key blocks and leaves partial results for launch_maps_join (maps_chunk_parts).
+// key blocks and leaves partial results for launch_maps_join, a tile of which is then a workgroup's tokens of one map.
 struct MapsChunk {
     PageSource pages;
     const _Float16 *q, *gate;

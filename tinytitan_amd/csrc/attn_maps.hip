@@ -17,14 +17,6 @@ namespace {
 
 typedef float f2 __attribute__((ext_vector_type(2)));
 
-// Row n of tile `tile` in split 0 of the pass, for token `tok` of a sequence and row `row` of the heads' maps.
-__device__ __forceinline__ size_t part_row(const PassParts &p, int group, int tok, int row) {
-    const int kvh = row / group, in_group = row - kvh * group;
-    const int hsub = in_group / p.gh, tok_tile = tok / p.tt;
-    const int tile = (kvh * p.hsubs + hsub) * p.tok_tiles + tok_tile;
-    return (size_t)tile * p.nt + (tok - tok_tile * p.tt) * p.gh + (in_group - hsub * p.gh);
-}
-
 // A (token, head) item is D / 4 threads of four dims each, and G of those that share its splits; a workgroup is ITEMS of them.
 template <int D, int G>
 __global__ __launch_bounds__(G * D / 4 > 256 ? G * D / 4 : 256) void attn_maps_join_kernel(const MapsJoinArgs a) {
@@ -33,9 +25,9 @@ __global__ __launch_bounds__(G * D / 4 > 256 ? G * D / 4 : 256) void attn_maps_j
     __shared__ f2 stats[G > 1 ? 2 : 1][G][ITEMS];
     const int lane = threadIdx.x % LANES, in_group = threadIdx.x / LANES, item = in_group % ITEMS, g = in_group / ITEMS;
     const int d = lane * 4, seq = blockIdx.y;
-    const long long at_item = (long long)blockIdx.x * ITEMS + item;
-    const bool real = at_item < (long long)a.rows * a.heads;
-    const int row = real ? (int)(at_item / a.heads) : 0, head = real ? (int)(at_item - (long long)row * a.heads) : 0;
+    const unsigned at_item = blockIdx.x * ITEMS + item, heads = a.heads;  // (rows x heads fit 31 bits)
+    const bool real = at_item < (unsigned)a.rows * heads;
+    const int row = real ? (int)(at_item / heads) : 0, head = real ? (int)(at_item - row * heads) : 0;
     const JoinSeq sq = a.seq[seq];
     // (asked for here, in front of the partial results)
     const float lambda = a.maps.lambda[seq * a.lambda_seq_stride + row * a.maps.lambda_stride + head];
@@ -43,14 +35,10 @@ __global__ __launch_bounds__(G * D / 4 > 256 ? G * D / 4 : 256) void attn_maps_j
     if (a.gate) {
         gate = *(const __attribute__((address_space(1))) h4_unaligned *)(global_halves)(a.gate + seq * a.g_seq_stride + row * a.g_tok_stride + (long long)head * D + d);
     }
-    f4 weight = (f4)1.0f;
-    if (a.maps.norm) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) weight[i] = __builtin_bit_cast(float, (unsigned)a.maps.norm[d + i] << 16);
-    }
+    const f4 weight = map_weight4(a.maps, d);
     // The tile's splits, as the pass counted them.
     const PassParts &p = a.parts;
-    const int t0 = row / p.tt * p.tt, tile_end = max(0, min(sq.total, sq.start + min(t0 + p.tt, a.rows)));
+    const int tok_tile = (unsigned)row / (unsigned)p.tt, t0 = tok_tile * p.tt, tile_end = max(0, min(sq.total, sq.start + min(t0 + p.tt, a.rows)));
     const int first_lim = min(sq.total, sq.start + t0 + 1);
     const int k0 = a.window > 0 && first_lim > a.window ? (first_lim - a.window) & ~31 : 0;
     const int n = (int)((unsigned)(max(tile_end - k0, 1) + p.split_len - 1) / (unsigned)p.split_len);
@@ -63,18 +51,29 @@ __global__ __launch_bounds__(G * D / 4 > 256 ? G * D / 4 : 256) void attn_maps_j
         m[map] = kNegBig;
         l[map] = 0.0f;
     }
-    const size_t at[2] = {part_row(p, a.group2, row, 2 * head) + (size_t)sq.first_split * stride,
-                          part_row(p, a.group2, row, 2 * head + 1) + (size_t)sq.first_split * stride};
+    // The maps' rows in split 0: next to each other, but where a tile ends between them.
+    const int kvh = (unsigned)(2 * head) / (unsigned)a.group2, in_kvh = 2 * head - kvh * a.group2;
+    const int hsub = (unsigned)in_kvh / (unsigned)p.gh, in_tile = in_kvh - hsub * p.gh;
+    const size_t first_row = (size_t)((kvh * p.hsubs + hsub) * p.tok_tiles + tok_tile) * p.nt + (row - t0) * p.gh + in_tile + (size_t)sq.first_split * stride;
+    const size_t at[2] = {first_row, in_tile + 1 < p.gh ? first_row + 1 : first_row + (size_t)p.tok_tiles * p.nt - in_tile};
     for (int first = g; first < n; first += G * BATCH) {
         f4 o[2][BATCH];
         f2 ml[2][BATCH];
+        // (a split that is not there is not asked for: read as the last one again, they were most of what a workgroup fetched)
 #pragma unroll
         for (int i = 0; i < BATCH; ++i) {
-            const size_t s = (size_t)min(first + i * G, n - 1) * stride;
 #pragma unroll
             for (int map = 0; map < 2; ++map) {
-                ml[map][i] = *reinterpret_cast<const f2 *>(p.ml + (at[map] + s) * 2);
-                o[map][i] = *reinterpret_cast<const f4 *>(p.o + (at[map] + s) * D + d);
+                ml[map][i] = f2{kNegBig, 0.0f};
+                o[map][i] = (f4)0.0f;
+            }
+            if (first + i * G < n) {
+                const size_t s = (size_t)(first + i * G) * stride;
+#pragma unroll
+                for (int map = 0; map < 2; ++map) {
+                    ml[map][i] = *reinterpret_cast<const f2 *>(p.ml + (at[map] + s) * 2);
+                    o[map][i] = *reinterpret_cast<const f4 *>(p.o + (at[map] + s) * D + d);
+                }
             }
         }
 #pragma unroll
@@ -88,7 +87,6 @@ __global__ __launch_bounds__(G * D / 4 > 256 ? G * D / 4 : 256) void attn_maps_j
             m[map] = top;
 #pragma unroll
             for (int i = 0; i < BATCH; ++i) {
-                if (first + i * G >= n) break;  // (not a factor of zero, which an infinite value makes NaN of)
                 const float f = fast_exp2(ml[map][i][0] - top);
                 l[map] += f * ml[map][i][1];
                 acc[map] += f * o[map][i];
@@ -122,14 +120,7 @@ __global__ __launch_bounds__(G * D / 4 > 256 ? G * D / 4 : 256) void attn_maps_j
     f4 out;
 #pragma unroll
     for (int i = 0; i < 4; ++i) out[i] = map_difference(a1[i], a2[i], lambda);
-    float scale = a.maps.out_scale;
-    if (a.maps.norm) {
-        float squares = out[0] * out[0] + out[1] * out[1] + out[2] * out[2] + out[3] * out[3];
-#pragma unroll
-        for (int step = 1; step < LANES; step *= 2) squares += __shfl_xor(squares, step);
-        // (a row of zeros stays one, whatever eps is)
-        scale *= squares == 0.0f ? 0.0f : 1.0f / sqrtf(squares * (1.0f / D) + a.maps.eps);
-    }
+    const float scale = map_row_scale<LANES>(a.maps, out);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         out[i] *= scale * weight[i];
@@ -177,7 +168,7 @@ void launch_join_by_splits(tt_hip_ctx *ctx, int n_seq, const MapsJoinArgs &args,
 }
 
 template <int D, int NT, int BITS, int STREAM>
-int launch_pass(tt_hip_ctx *ctx, const LaunchPlan &plan, int n_seq, const SplitKArgs &args) {
+int launch_pass(tt_hip_ctx *ctx, const LaunchPlan &plan, int n_seq, const SplitKMaps &args) {
     auto kernel = attn_splitk_kernel<D, NT, 4, BITS, kKeepMaps, STREAM>;
     dim3 grid((unsigned)plan.n_splits_max, (unsigned)plan.n_tiles, (unsigned)n_seq);
     if (plan.packed_splits > 0) grid = dim3((unsigned)plan.packed_splits, (unsigned)plan.n_tiles);
@@ -202,7 +193,7 @@ int configure_maps_kernels(tt_hip_ctx *ctx) {
     return e == hipSuccess ? TT_HIP_OK : hip_fail(ctx, e, "hipFuncSetAttribute(split-K max dynamic LDS)");
 }
 
-int launch_splitk_maps(tt_hip_ctx *ctx, const LaunchPlan &plan, int head_dim, int n_seq, const SplitKArgs &args, int kv_bits) {
+int launch_splitk_maps(tt_hip_ctx *ctx, const LaunchPlan &plan, int head_dim, int n_seq, const SplitKMaps &args, int kv_bits) {
 #define TT_CASE(DD, NN)                                                                                        \
     if (head_dim == DD && plan.nt == NN) {                                                                     \
         if (kv_bits == 16) return plan.stream ? launch_pass<DD, NN, 16, 1>(ctx, plan, n_seq, args) : launch_pass<DD, NN, 16, 0>(ctx, plan, n_seq, args); \

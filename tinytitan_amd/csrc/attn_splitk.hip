@@ -364,7 +364,6 @@ int launch_splitk_pair(tt_hip_ctx *ctx, int head_dim, int nt, int kv_bits, bool 
 int launch_splitk(tt_hip_ctx *ctx, const LaunchPlan &plan, int head_dim, int n_seq, const SplitKArgs &args, int kv_bits) {
     if (n_seq > kMaxSeqPerLaunch || plan.waves != 4) return TT_HIP_ERR_INVALID_ARGUMENT;
     if (plan.n_tiles > 65535 || n_seq > 65535) return TT_HIP_ERR_SHAPE;
-    if (args.hot.flags & kHotMaps) return launch_splitk_maps(ctx, plan, head_dim, n_seq, args, kv_bits);
 #define TT_CASE(DD, NN)                                                                              \
     if (head_dim == DD && plan.nt == NN) {                                                           \
         if constexpr (NN == 32) {                                                                    \

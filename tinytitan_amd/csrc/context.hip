@@ -307,7 +307,9 @@ struct KeyPiece {
     int first_block = 0;  // the pages' blocks in front of the piece: starts and totals count from here
     PassParts parts{};
     int first_split[kMaxSeqPerLaunch] = {};
-    bool maps = false;  // the rows are those of two maps a head: n_q_heads counts both, q's rows are the heads'
+    const MapHeads *maps = nullptr;  // the rows are those of two maps a head: n_q_heads counts both, q's, gate's and out's rows are the heads'
+    long long lambda_seq_stride = 0;
+    bool finished = false;  // ... and the launch has written them: no join
 };
 static int run_attention(tt_hip_ctx *ctx, tt_hip_kv *kv, int kind, int layer, int n_seq, const int *slots,
                          const int *starts, const int *totals, int rows, int n_q_heads, const tt_half *q,
@@ -548,7 +550,9 @@ static int run_attention(tt_hip_ctx *ctx, tt_hip_kv *kv, int kind, int layer, in
         h.n_splits_max = plan.n_splits_max;
         if (piece) {
             // (a launch of one split would write the final rows: it is told of a second one, which no tile has)
-            if (h.n_splits_max == 1) h.n_splits_max = 2;
+            // (two maps' rows: it writes those, where a head's two are in one tile)
+            if (piece->maps && h.n_splits_max == 1 && plan.gh % 2 == 0) piece->finished = true;
+            else if (h.n_splits_max == 1) h.n_splits_max = 2;
             piece->parts = PassParts{h.part_o, h.part_ml, plan.nt, plan.gh, plan.tt, plan.hsubs, plan.tok_tiles, plan.n_tiles, plan.split_len};
             std::copy(first_split, first_split + n, piece->first_split);
         }
@@ -556,7 +560,6 @@ static int run_attention(tt_hip_ctx *ctx, tt_hip_kv *kv, int kind, int layer, in
                              q_tok_stride % 8 == 0 && g_seq_stride % 8 == 0 && g_tok_stride % 8 == 0 && o_seq_stride % 8 == 0 &&
                              o_tok_stride % 8 == 0;
         h.flags = (aligned ? kHotAligned : 0) | (plan.xcd_grid ? kHotXcdGrid : 0) | (plan.packed_splits > 0 ? kHotPackedSplits : 0);
-        if (piece && piece->maps) h.flags |= kHotMaps;
         h.scale_log2e = scale * 1.4426950408889634f;
         h.window = window;
         h.ring_blocks = walks_pages ? pages->ring_blocks : kv->ring_blocks();
@@ -628,7 +631,8 @@ static int run_attention(tt_hip_ctx *ctx, tt_hip_kv *kv, int kind, int layer, in
                                 chunk_pieces);
             if (st == TT_HIP_OK && !piece) st = launch_combine(ctx, plan, D, n, a);
         } else {
-            st = launch_splitk(ctx, plan, D, n, a, kv_bits);
+            if (piece && piece->maps) st = launch_splitk_maps(ctx, plan, D, n, SplitKMaps{a, *piece->maps, piece->lambda_seq_stride}, kv_bits);
+            else st = launch_splitk(ctx, plan, D, n, a, kv_bits);
         }
         if (st != TT_HIP_OK) return st;
     }
@@ -1681,11 +1685,16 @@ static int run_maps_tiles(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, 
             const int some = std::min(rows - r, rows_at_once);
             const long long q_at = base * q_seq_stride + r * q_tok_stride, o_at = base * o_seq_stride + r * o_tok_stride;
             KeyPiece piece{};
-            piece.maps = true;
+            MapHeads heads = maps;
+            heads.lambda += ((long long)base * rows + r) * maps.lambda_stride;
+            piece.maps = &heads;
+            piece.lambda_seq_stride = rows * maps.lambda_stride;
+            const tt_half *const some_gate = gate ? gate + base * g_seq_stride + r * g_tok_stride : nullptr;
             const int st = run_attention(ctx, kv, 0, layer, n, slots + base, first, totals + base, some, 2 * n_q_heads, q + q_at, q_seq_stride,
-                                         q_tok_stride, nullptr, 0, 0, scale, out + o_at, o_seq_stride, o_tok_stride, 1, 0, nullptr, window, nullptr,
-                                         0, 0, false, nullptr, -1, &piece);
+                                         q_tok_stride, some_gate, g_seq_stride, g_tok_stride, scale, out + o_at, o_seq_stride, o_tok_stride, 1, 0,
+                                         nullptr, window, nullptr, 0, 0, false, nullptr, -1, &piece);
             if (st != TT_HIP_OK) return st;
+            if (piece.finished) continue;
             MapsJoinArgs a;
             std::memset(static_cast<void *>(&a), 0, sizeof(a));
             a.parts = piece.parts;
@@ -1693,10 +1702,9 @@ static int run_maps_tiles(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, 
             a.rows = some;
             a.heads = n_q_heads;
             a.group2 = 2 * (n_q_heads / kv->n_kv_heads);
-            a.maps = maps;
-            a.maps.lambda += ((long long)base * rows + r) * maps.lambda_stride;
-            a.lambda_seq_stride = rows * maps.lambda_stride;
-            a.gate = gate ? reinterpret_cast<const _Float16 *>(gate) + base * g_seq_stride + r * g_tok_stride : nullptr;
+            a.maps = heads;
+            a.lambda_seq_stride = piece.lambda_seq_stride;
+            a.gate = reinterpret_cast<const _Float16 *>(some_gate);
             a.out = reinterpret_cast<_Float16 *>(out) + o_at;
             a.g_seq_stride = g_seq_stride;
             a.g_tok_stride = g_tok_stride;

@@ -40,7 +40,6 @@ constexpr int kHotSinks = 8, kHotPinnedShift = 8;
 // The same kernel for a prefix in another slot: keep_words is that slot, and from kHotPinnedShift on the flags hold the prefix's blocks.
 constexpr int kHotFront = 16;
 // Two softmax maps a head (kKeepMaps).
-constexpr int kHotMaps = 32;
 constexpr int kKeepSinks = 6;  // that kernel's KEEP (splitk_kernel.h)
 constexpr int kKeepPieces = 7;  // ... and of two passes in one launch, over the keys that sequences share and over their own
 constexpr int kKeepMaps = 9;    // ... of two softmax maps a head: `group` counts two rows a head
@@ -128,6 +127,11 @@ struct MapHeads {
     long long lambda_stride;  // floats from a token's row to the next token's; 0: one row for all
     const uint16_t *norm;     // bfloat16 [D]
     float eps, out_scale;
+};
+// The pass over both maps' rows (kKeepMaps): with hot.n_splits_max of one it writes the heads' finished rows itself.
+struct alignas(64) SplitKMaps : SplitKArgs {
+    MapHeads maps;
+    long long lambda_seq_stride;  // floats from a sequence's first row of factors to the next one's
 };
 
 // Where a pass over one piece of the keys has left its partial results: row n of a tile's split lies at
@@ -327,7 +331,7 @@ struct MapsJoinArgs {
 // Rows of maps whose partial results of a split are kept at a time (128 MiB with heads of 256).
 constexpr int kMapsRowsAtOnce = 131072;
 int configure_maps_kernels(tt_hip_ctx *ctx);
-int launch_splitk_maps(tt_hip_ctx *ctx, const LaunchPlan &plan, int head_dim, int n_seq, const SplitKArgs &args, int kv_bits);
+int launch_splitk_maps(tt_hip_ctx *ctx, const LaunchPlan &plan, int head_dim, int n_seq, const SplitKMaps &args, int kv_bits);
 int launch_maps_join(tt_hip_ctx *ctx, int head_dim, int n_seq, const MapsJoinArgs &args, int most_splits);
 
 // A chunk of one sequence by the kernel of attn_maps_chunk.hip, over fp16 pages; with n_splits > 1 each workgroup takes a range of split_blocks

@@ -124,6 +124,37 @@ __device__ __forceinline__ void store_out4_gated(const Args &a, int seq, int tok
     }
 }
 
+// a1 - lambda a2 of two maps' results.  Either is rounded before the difference, no product is fused into it: maps that are the same then cancel
+// to zero, and not to a rounding that a norm behind makes a row of.
+__device__ __forceinline__ float map_difference(float a1, float a2, float lambda) {
+    asm("" : "+v"(a1));
+    asm("" : "+v"(a2));
+    return __builtin_fmaf(-lambda, a2, a1);
+}
+
+// What a head's row of differences is multiplied by: out_scale, and under a norm 1 / rms.  LANES lanes next to each other hold four dims each.
+template <int LANES>
+__device__ __forceinline__ float map_row_scale(const MapHeads &maps, f4 d) {
+    float scale = maps.out_scale;
+    if (maps.norm) {
+        float squares = d[0] * d[0] + d[1] * d[1] + d[2] * d[2] + d[3] * d[3];
+#pragma unroll
+        for (int step = 1; step < LANES; step *= 2) squares += __shfl_xor(squares, step);
+        // (a row of zeros stays one, whatever eps is)
+        scale *= squares == 0.0f ? 0.0f : 1.0f / sqrtf(squares * (1.0f / (4 * LANES)) + maps.eps);
+    }
+    return scale;
+}
+// Four values of the norm's weight, or ones.
+__device__ __forceinline__ f4 map_weight4(const MapHeads &maps, int d) {
+    f4 w = (f4)1.0f;
+    if (maps.norm) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = __builtin_bit_cast(float, (unsigned)maps.norm[d + i] << 16);
+    }
+    return w;
+}
+
 // ---------------------------------------------------------------------------
 // Register tiles of one 32-key block and the per-row online-softmax state.
 // NT = 32 uses v_mfma_f32_32x32x16_f16 (32 query rows per wave), NT = 16 uses
@@ -1326,7 +1357,7 @@ __device__ __forceinline__ void front_rows(const SplitKHot &a, const SplitKSeq &
 
 template <int D, int NT, int WAVES, int BITS, int KEEP = 0, int STREAM = 0>
 __global__ __launch_bounds__(WAVES * 64, ((NT == 16 && (KEEP < 2 || KEEP == kKeepSinks || KEEP == kKeepPieces || KEEP == kKeepMaps)) || (KEEP == kKeepRows && D < 256) ? 2 : 1)) void
-    attn_splitk_kernel(const std::conditional_t<KEEP == kKeepPieces || KEEP == kKeepRows, SplitKPair, SplitKArgs> args) {
+    attn_splitk_kernel(const std::conditional_t<KEEP == kKeepPieces || KEEP == kKeepRows, SplitKPair, std::conditional_t<KEEP == kKeepMaps, SplitKMaps, SplitKArgs>> args) {
     constexpr bool PAIR = KEEP == kKeepPieces || KEEP == kKeepRows;
     constexpr bool MAPS = KEEP == kKeepMaps;
     constexpr bool PAIRED = STREAM == 2;
@@ -1820,7 +1851,24 @@ __global__ __launch_bounds__(WAVES * 64, ((NT == 16 && (KEEP < 2 || KEEP == kKee
     constexpr int D4 = D / 4, ITEMS = NT * D4 / (WAVES * 64), ROUND = WAVES * 64 / D4;
     const bool last = a.n_splits_max == 1;
     h4 gate[ITEMS];
-    if (last && out.gate) {
+    // Two maps' rows: an item is a head's two rows.
+    [[maybe_unused]] constexpr int PAIRS = ITEMS > 1 ? ITEMS / 2 : 1;
+    [[maybe_unused]] float lambda[PAIRS];
+    [[maybe_unused]] f4 weight = (f4)1.0f;
+    if constexpr (MAPS) {
+        if (last) {
+            const int d = threadIdx.x % D4 * 4, pairs = n_valid >> 1;
+            weight = map_weight4(args.maps, d);
+#pragma unroll
+            for (int i = 0; i < PAIRS; ++i) {
+                if (i * ROUND >= pairs) break;
+                const int n = 2 * min(i * ROUND + (int)threadIdx.x / D4, pairs - 1), tl = (n * a.gh_inv) >> 16;
+                const int hh = ti.kvh * (a.group >> 1) + ((ti.hsub * a.gh + (n - tl * a.gh)) >> 1);
+                lambda[i] = args.maps.lambda[seq * args.lambda_seq_stride + (ti.t0 + tl) * args.maps.lambda_stride + hh];
+                gate[i] = load_gate4(out, seq, ti.t0 + tl, hh, d, D);
+            }
+        }
+    } else if (last && out.gate) {
         const global_halves rows = (global_halves)(out.gate + seq * out.g_seq_stride + ti.t0 * out.g_tok_stride + (long long)(ti.kvh * a.group + ti.hsub * a.gh) * D);
         const int d = threadIdx.x % D4 * 4;
 #pragma unroll
@@ -1856,6 +1904,41 @@ __global__ __launch_bounds__(WAVES * 64, ((NT == 16 && (KEEP < 2 || KEEP == kKee
     __syncthreads();
 
     // Merge the waves' states; every thread takes (row, 4 dims) items.
+    if constexpr (MAPS) {
+        if (last) {
+            // (the row's result of one map)
+            auto merged = [&](int n, int d) __attribute__((always_inline)) {
+                float mw[WAVES], ms = kNegBig, lsum = 0.0f;
+#pragma unroll
+                for (int w = 0; w < WAVES; ++w) {
+                    mw[w] = lds[w * REGION + NT * ROW + 2 * n];
+                    ms = fmaxf(ms, mw[w]);
+                }
+                f4 acc = (f4)0.0f;
+#pragma unroll
+                for (int w = 0; w < WAVES; ++w) {
+                    const float f = fast_exp2(mw[w] - ms);
+                    lsum += f * lds[w * REGION + NT * ROW + 2 * n + 1];
+                    acc += f * *reinterpret_cast<const f4 *>(lds + w * REGION + n * ROW + d);
+                }
+                return acc * (lsum > 0.0f ? 1.0f / lsum : 0.0f);
+            };
+            const int d = threadIdx.x % D4 * 4, pairs = n_valid >> 1;
+#pragma unroll
+            for (int i = 0; i < PAIRS; ++i) {
+                const int n = 2 * (i * ROUND + (int)threadIdx.x / D4);
+                if (n >= 2 * pairs) break;
+                const f4 a1 = merged(n, d), a2 = merged(n + 1, d);
+                f4 x;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = map_difference(a1[e], a2[e], lambda[i]);
+                const float scale = map_row_scale<D4>(args.maps, x);
+                const int tl = (n * a.gh_inv) >> 16, hh = ti.kvh * (a.group >> 1) + ((ti.hsub * a.gh + (n - tl * a.gh)) >> 1);
+                store_out4_gated(out, seq, ti.t0 + tl, hh, d, D, x * weight, scale, (a.flags & kHotAligned) != 0, gate[i]);
+            }
+            return;
+        }
+    }
     const size_t pbase = (((size_t)sq.first_split + split) * a.n_tiles + tile) * NT;
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
@@ -1888,14 +1971,6 @@ __global__ __launch_bounds__(WAVES * 64, ((NT == 16 && (KEEP < 2 || KEEP == kKee
             }
         }
     }
-}
-
-// a1 - lambda a2 of two maps' results.  Either is rounded before the difference, no product is fused into it: maps that are the same then cancel
-// to zero, and not to a rounding that a norm behind makes a row of.
-__device__ __forceinline__ float map_difference(float a1, float a2, float lambda) {
-    asm("" : "+v"(a1));
-    asm("" : "+v"(a2));
-    return __builtin_fmaf(-lambda, a2, a1);
 }
 
 constexpr size_t keep_list_bytes(int keep, int waves) { return keep == 2 ? (size_t)waves * kKeepWindows * (64 + 1) * sizeof(int) : 0; }

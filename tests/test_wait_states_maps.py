@@ -1,0 +1,94 @@
+"""Wait states of the assembly blocks in the 8-bit products and in differential attention's chunk kernel, in the device code the compiler makes of
+them: those of the copies into LDS (test_wait_states.py), and those of the score products, matrix instructions of 32 x 32 x 16 whose sums vector
+instructions read.  Such a read wants 18 wait states behind the last product into those registers; a product of that size holds
+the matrix pipe for eight, so that it counts as eight where it is issued behind another one."""
+import os
+import re
+import shutil
+import subprocess
+
+import pytest
+
+from tests.test_wait_states import _missing
+from tinytitan_amd import build
+
+pytestmark = pytest.mark.skipif(shutil.which(build.HIPCC) is None, reason="no hipcc")
+
+ENOUGH, PRODUCT = 18, 8
+
+
+def _vectors(operand):
+    """The vector registers that an operand names."""
+    m = re.match(r"\s*-?\|?v\[(\d+):(\d+)\]|\s*-?\|?v(\d+)\b", operand)
+    if not m:
+        return set()
+    return set(range(int(m[1]), int(m[2]) + 1)) if m[1] else {int(m[3])}
+
+
+def early_reads(listing):
+    """Instructions that read or write a score product's registers too early, and how many such products there are.  A product may take the
+    registers of the one before it as its own sum."""
+    function, found, products, in_block = "", [], 0, False
+    written, now = {}, 0  # register -> states at the last product into it
+    for line in listing.splitlines():
+        label = re.match(r"(_Z\w+):", line)
+        if label:
+            function, written = label[1], {}
+        if "#ASMSTART" in line or "#ASMEND" in line:
+            in_block = "#ASMSTART" in line
+        text = line.split(";")[0].strip()
+        if not text or text.startswith(".") or text.endswith(":"):
+            continue
+        op, _, operands = text.partition(" ")
+        parts = operands.split(",")
+        if op.startswith("v_mfma") and in_block:
+            target = _vectors(parts[0])
+            assert target, text  # (a score product's sum is in vector registers)
+            for part in parts[1:3]:
+                found += [(function, text) for reg in _vectors(part) if now - written.get(reg, -99) < ENOUGH]
+            third = _vectors(parts[3])
+            assert not third or third == target, text
+            if not third:  # (the first of a sum: nobody may still be reading the old one, which was read behind its own products)
+                found += [(function, text) for reg in target if now - written.get(reg, -99) < ENOUGH]
+            now += PRODUCT
+            written.update({reg: now - PRODUCT + 1 for reg in target})
+            products += 1
+            continue
+        if op.startswith(("v_", "ds_", "global_", "buffer_", "flat_", "scratch_")):
+            for part in parts:
+                found += [(function, text) for reg in _vectors(part) if now - written.get(reg, -99) < ENOUGH]
+        now += PRODUCT if op.startswith("v_mfma") else int(operands, 0) + 1 if op == "s_nop" else 1
+    return found, products
+
+
+def _listing(tmp_path, source):
+    listing = tmp_path / "device.s"
+    subprocess.run([build.HIPCC, *build.FLAGS, "--cuda-device-only", "-S", os.path.join(build.CSRC, source), "-o", str(listing)], check=True,
+                   capture_output=True)
+    return listing.read_text()
+
+
+@pytest.mark.parametrize("source", ["attn_maps_chunk.hip", "int8_proj.hip"])
+def test_copies_into_lds_wait_for_what_they_read(tmp_path, source):
+    missing, copies, clobbered = _missing(_listing(tmp_path, source))
+    assert copies > 20
+    assert not clobbered
+    assert not missing, f"{len(missing)}, e.g. {missing[0]}"
+
+
+def test_scores_are_read_behind_their_products(tmp_path):
+    listing = _listing(tmp_path, "attn_maps_chunk.hip")
+    found, products = early_reads(listing)
+    assert products == (2 + 4 + 8) * 2 * 2  # heads of 64, 128 and 256, two tiles, in front of the loop and in it
+    assert not found, f"{len(found)}, e.g. {found[0]}"
+    assert "v_cmpx" not in listing  # (a product behind a change of the lanes at work would want wait states, too)
+
+
+def test_the_check_sees_an_early_read():
+    product = "\t;;#ASMSTART\n\tv_mfma_f32_32x32x16_f16 v[0:15], v[20:23], v[24:27], 0\n\t;;#ASMEND\n"
+    read = "\tv_max3_f32 v30, v3, v31, v32\n"
+    other = "\tv_mfma_f32_32x32x16_f16 a[0:15], v[40:43], v[44:47], a[0:15]\n"
+    assert early_reads("_Zf:\n" + product + read)[0]
+    assert early_reads("_Zf:\n" + product + other + read)[0]
+    assert not early_reads("_Zf:\n" + product + other * 2 + "\ts_nop 1\n" + read)[0]
+    assert not early_reads("_Zf:\n" + product + "\ts_nop 15\n\ts_nop 7\n" + read)[0]

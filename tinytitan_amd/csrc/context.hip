@@ -1694,7 +1694,7 @@ static int run_maps_tiles(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, 
                                          q_tok_stride, some_gate, g_seq_stride, g_tok_stride, scale, out + o_at, o_seq_stride, o_tok_stride, 1, 0,
                                          nullptr, window, nullptr, 0, 0, false, nullptr, -1, &piece);
             if (st != TT_HIP_OK) return st;
-            if (piece.finished) continue;
+            if (piece.finished || ctx->pass_only) continue;
             MapsJoinArgs a;
             std::memset(static_cast<void *>(&a), 0, sizeof(a));
             a.parts = piece.parts;
@@ -1835,7 +1835,7 @@ int tt_hip_attn_prefill_diff(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int slot
     c.part_o = ctx->part_o;
     c.part_ml = ctx->part_ml;
     st = launch_maps_chunk(ctx, kv->head_dim, kv->n_kv_heads, c);
-    if (st != TT_HIP_OK || plan.n_splits == 1) return st;
+    if (st != TT_HIP_OK || plan.n_splits == 1 || ctx->pass_only) return st;
     MapsJoinArgs a;
     std::memset(static_cast<void *>(&a), 0, sizeof(a));
     a.parts.o = ctx->part_o;

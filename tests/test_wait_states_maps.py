@@ -79,7 +79,7 @@ def test_copies_into_lds_wait_for_what_they_read(tmp_path, source):
 def test_scores_are_read_behind_their_products(tmp_path):
     listing = _listing(tmp_path, "attn_maps_chunk.hip")
     found, products = early_reads(listing)
-    assert products == (2 + 4 + 8) * 2 * 2  # heads of 64, 128 and 256, two tiles, in front of the loop and in it
+    assert products == (2 * 2 + 4 + 8 * 2) * 2  # heads of 64, 128 and 256, two tiles or one, in front of the loop and in it
     assert not found, f"{len(found)}, e.g. {found[0]}"
     assert "v_cmpx" not in listing  # (a product behind a change of the lanes at work would want wait states, too)
 

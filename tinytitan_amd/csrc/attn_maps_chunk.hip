@@ -3,21 +3,23 @@
 // Transposed as the other attention kernels are, a lane owns a query row:
 //   S^T[key][row] = K_m . Q_m^T      A = K fragment, of map m's half of the dims,  B = Q^T fragment, both in registers
 //   O^T[d][row]  += V^T . P^T        A = V^T fragment out of LDS,                  B = P^T as it left S^T's registers
-// with v_mfma_f32_32x32x16_f16.  A workgroup is four wavefronts over 128 rows, four tiles of 32 (heads that share a KV head, of one or more tiles
-// of tokens): wavefront 2 p + m takes map m of tiles 2 p and 2 p + 1, all dims of both.  The maps of a tile meet at the end.
+// with v_mfma_f32_32x32x16_f16.  A workgroup takes 128 rows, four tiles of 32 (heads that share a KV head, of one or more tiles of tokens).  Heads of 256
+// and 64: four wavefronts, 2 p + m with map m of tiles 2 p and 2 p + 1; heads of 128: eight, 2 p + m with map m of tile p.  The maps of a tile
+// meet at the end.
 //
-// What shapes it: LDS hands out 64 bytes a cycle and CU, half of what a matrix product wants whose operand comes from there each time.  So an
-// operand of V is used for two tiles, and K, whose blocks lie in memory as the operands are, comes straight into registers, a block ahead.
+// What shapes it: LDS hands out 64 bytes a cycle and CU, half of what a matrix product wants whose operand comes from there each time.  So with two tiles an
+// operand of V is used twice, and K, whose blocks lie in memory as the operands are, comes straight into registers, a block ahead.
 // Of heads of 256 a block of keys is 48 products a wavefront, 1,536 cycles, beside 80 KiB of LDS traffic a CU, 1,280, and 48 KiB through the
 // vector memory path, 768.  One wavefront a SIMD has all 512 registers (256 of them sums over V), so nothing but its own order hides one kind of work
 // behind another: the softmax of block i is cut into pieces of a few instructions each, one between any two of the products of block i's
-// scores and block i - 1's values.
+// scores and block i - 1's values.  Heads of 128 leave room for two wavefronts a SIMD with a tile each, which hide each other's waits (one wavefront with
+// two tiles issued 68 % of its cycles, with the matrix pipe busy for 41, and waited 19) at twice the LDS traffic, 1,024 cycles beside 768 of products.
 //
 // Measured, us a call: 4,096 rows behind 4,500 keys 586 - 605 with 16/2 heads of 256 (1.09 - 1.12 PFLOP/s, of 1.22 that a library product reaches),
-// 705 - 730 with 32/8 of 128 (0.90 - 0.93), 240 - 249 with 16/4 of 64 (0.66 - 0.69).  With heads of 128 a step is 1,860 cycles, of which the matrix pipe is
-// busy 41 %, instructions are issued 68 % -- an exponential takes four slots, a product two -- and waits are 19 %.  Tried and not kept, heads of 256 / 128:
-// the copies of V before the reads of K +16 / +23 %, among them +2 / +1; a barrier every second step, eight blocks of V, +2 / +1;
-// the sums of the weights by dot products of pairs +4 / +6; two workgroups a CU for heads of 128, in 256 registers, +23.
+// 704 with 32/8 of 128 (0.94; two tiles a wavefront 716), 240 - 249 with 16/4 of 64 (0.66 - 0.69); 777 rows behind 9,000 of 32/8 heads of 128 230 - 235
+// (two tiles 252).  Tried and not kept, heads of 256 / of 128 with two tiles: the copies of V in front of all reads of K +16 / +23 %, each in
+// front of one +2 / +1; a barrier every second step, eight blocks of V, +2 / +1; the sums of the weights by dot products of pairs
+// +4 / +6; two workgroups a CU for heads of 128, in 256 registers, +23.
 #include <algorithm>
 
 #include "lds_copy.h"
@@ -49,7 +51,8 @@ struct MapsChunkArgs {
 
 template <int D>
 struct ChunkShape {
-    static constexpr int KS = D / 32, MT = D / 32, VF = 2 * MT, CPW = VF / 4;  // score steps of a map, tiles of dims, V fragments of a block, copies a wavefront
+    static constexpr int RT = D == 128 ? 1 : 2, WAVES = 8 / RT;  // row tiles of a wavefront, wavefronts
+    static constexpr int KS = D / 32, MT = D / 32, VF = 2 * MT, CPW = VF / WAVES;  // score steps of a map, tiles of dims, V fragments of a block, copies a wavefront
     static constexpr int V_BYTES = 64 * D, RING_BYTES = kVRing * V_BYTES;
     static constexpr int X_BYTES = 128 * D;               // a tile's sums on their way to the other map's wavefront
     static constexpr int STAGE_PITCH = 64 + 16, STAGE_BYTES = 32 * STAGE_PITCH;
@@ -97,9 +100,9 @@ constexpr int piece_of_slot(int slot, int from, int slots, int pieces) {
 }
 
 template <int D>
-__global__ __launch_bounds__(256, D == 64 ? 2 : 1) void attn_maps_chunk_kernel(const MapsChunkArgs a) {
+__global__ __launch_bounds__(64 * ChunkShape<D>::WAVES, D == 256 ? 1 : 2) void attn_maps_chunk_kernel(const MapsChunkArgs a) {
     typedef ChunkShape<D> C;
-    constexpr int KS = C::KS, MT = C::MT, VF = C::VF, CPW = C::CPW, BLOCK = 64 * D;
+    constexpr int RT = C::RT, KS = C::KS, MT = C::MT, VF = C::VF, CPW = C::CPW, BLOCK = 64 * D;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 31, g = lane >> 5;
     const int map = wave & 1, pair = wave >> 1;
@@ -126,12 +129,12 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void attn_maps_chunk_kernel(c
     const int nb = a.n_splits > 1 ? min(nb_all, a.split_blocks) : nb_all;
     if (nb <= 0) return;
 
-    // This wavefront's rows: two tiles, 2 pair and 2 pair + 1.
-    int head[2], tok[2], lim[2], lo[2];
-    bool valid[2];
+    // This wavefront's rows: RT tiles, from RT pair on.
+    int head[RT], tok[RT], lim[RT], lo[RT];
+    bool valid[RT];
 #pragma unroll
-    for (int rt = 0; rt < 2; ++rt) {
-        const int u = 2 * pair + rt;
+    for (int rt = 0; rt < RT; ++rt) {
+        const int u = RT * pair + rt;
         head[rt] = kvh * a.group + set * a.hs + u % a.hs;
         tok[rt] = t0 + 32 * (u / a.hs) + li;
         valid[rt] = tok[rt] < a.q_len;
@@ -140,7 +143,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void attn_maps_chunk_kernel(c
         lo[rt] = valid[rt] && a.window > 0 && a.start + tok[rt] + 1 > a.window ? a.start + tok[rt] + 1 - a.window : 0;
     }
     // Blocks from first_masked on, and with a window those up to last_below, hide keys from some row of the wavefront.
-    const int wave_t0 = t0 + 32 * (2 * pair / a.hs), wave_t1 = t0 + 32 * ((2 * pair + 1) / a.hs) + 31;
+    const int wave_t0 = t0 + 32 * (RT * pair / a.hs), wave_t1 = t0 + 32 * ((RT * pair + RT - 1) / a.hs) + 31;
     const int first_masked = min(a.start + wave_t0 + 1, a.kv_valid) >> 5;
     const int last_below = a.window > 0 && a.start + wave_t1 + 1 > a.window ? (a.start + wave_t1 - a.window) >> 5 : -1;
 
@@ -170,9 +173,9 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void attn_maps_chunk_kernel(c
         copy16_global_to_lds(reinterpret_cast<const char *>(v_page) + v_at.at, v_from[c], lds0 + (unsigned)((i % kVRing) * C::V_BYTES + (wave * CPW + c) * 1024));
     };
 
-    h8 q[2][KS], kf[KS];
+    h8 q[RT][KS], kf[KS];
 #pragma unroll
-    for (int rt = 0; rt < 2; ++rt) {
+    for (int rt = 0; rt < RT; ++rt) {
         const global_halves row = (global_halves)(a.q + (long long)(valid[rt] ? tok[rt] : 0) * a.q_stride + (long long)head[rt] * D + map * (D / 2) + 8 * g);
 #pragma unroll
         for (int t = 0; t < KS; ++t) q[rt][t] = load_h8(row + 16 * t);
@@ -187,15 +190,15 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void attn_maps_chunk_kernel(c
         v_at.next();
     }
 #pragma unroll
-    for (int rt = 0; rt < 2; ++rt)
+    for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
         for (int t = 0; t < KS; ++t) q[rt][t] = valid[rt] ? q[rt][t] : (h8)(_Float16)0;
 
-    f16v o[2][MT], s[2];
-    float m[2], l[2], l_odd[2], mx[2], alpha[2];
-    h8 p[2][2];  // weights of the block whose values are next
+    f16v o[RT][MT], s[RT];
+    float m[RT], l[RT], l_odd[RT], mx[RT], alpha[RT];
+    h8 p[RT][2];  // weights of the block whose values are next
 #pragma unroll
-    for (int rt = 0; rt < 2; ++rt) {
+    for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
             o[rt][mt] = (f16v)0.0f;
@@ -207,7 +210,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void attn_maps_chunk_kernel(c
     // The softmax of a tile's block in PIECES pieces: two of the maximum, two of the reference, and of each of the lane's eight pairs of keys two, so
     // that no piece reads an exponential of its own.
     constexpr int PIECES = 2 + 2 + 2 * 8;
-    auto soften = [&](auto rt_c, auto piece_c, h8 (&p_next)[2][2]) __attribute__((always_inline)) {
+    auto soften = [&](auto rt_c, auto piece_c, h8 (&p_next)[RT][2]) __attribute__((always_inline)) {
         constexpr int rt = decltype(rt_c)::value, piece = decltype(piece_c)::value;
         if constexpr (piece < 2) {
             constexpr int v = 8 * piece;
@@ -266,8 +269,8 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void attn_maps_chunk_kernel(c
     auto read_v = [&](int i, int f) { return *reinterpret_cast<const h8 *>(smem + (i % kVRing) * C::V_BYTES + f * 1024 + lane * 16); };
     // Step i: the scores of block i, and between their products and those of block i - 1's values the softmax of block i.
     unsigned ring = 0;  // where block i - 1's values lie in LDS
-    auto step = [&](int i, const h8 (&p_now)[2][2], h8 (&p_next)[2][2]) __attribute__((always_inline)) {
-        constexpr int SLOTS = KS + 4 * MT, FROM = 2;  // (a tile's scores are read behind the third product after their last)
+    auto step = [&](int i, const h8 (&p_now)[RT][2], h8 (&p_next)[RT][2]) __attribute__((always_inline)) {
+        constexpr int CHAIN = (RT - 1) * KS, SLOTS = CHAIN + 2 * RT * MT, FROM = 2;  // (a tile's scores are read behind the third product after their last)
         // V of block i - 1 has landed (K and V of the two blocks since may be on their way), and every wavefront is done with the block whose place
         // the copies of this step take.
         TT_WAIT_VMCNT(2 * (KS + CPW));
@@ -287,6 +290,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void attn_maps_chunk_kernel(c
             if (t == 0) first_score(s[0], kf[0], q[0][0]);
             else next_score(s[0], kf[t], q[0][t]);
             if (t < 2) read_v(t);
+            if constexpr (RT == 1) kf[t] = buf_load_h8<0>(rk, k_lane + (t & 3) * 1024, next_k + (t >> 2) * 4096);
             __builtin_amdgcn_sched_barrier(0);
         }
         if (hidden) {
@@ -295,27 +299,27 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void attn_maps_chunk_kernel(c
         }
         unrolled<SLOTS>([&](auto slot_c) __attribute__((always_inline)) {
             constexpr int slot = decltype(slot_c)::value;
-            if constexpr (slot < KS) {
-                if constexpr (slot == 0) first_score(s[1], kf[0], q[1][0]);
-                else next_score(s[1], kf[slot], q[1][slot]);
+            if constexpr (slot < CHAIN) {
+                if constexpr (slot == 0) first_score(s[RT - 1], kf[0], q[RT - 1][0]);
+                else next_score(s[RT - 1], kf[slot], q[RT - 1][slot]);
                 kf[slot] = buf_load_h8<0>(rk, k_lane + (slot & 3) * 1024, next_k + (slot >> 2) * 4096);
             } else {
                 // (two products in a row to a sum: 32 cycles each, 36 where the sum is another every time)
-                constexpr int u = slot - KS, mt = u >> 2, rt = (u >> 1) & 1, t = u & 1;
-                if constexpr (u == 0) {
+                constexpr int u = slot - CHAIN, mt = u / (2 * RT), rt = (u >> 1) % RT, t = u & 1;
+                if constexpr (RT == 2 && u == 0) {
                     if (hidden) {
-                        settle(s[1]);
-                        hide(1, jb + i);
+                        settle(s[RT - 1]);
+                        hide(RT - 1, jb + i);
                     }
                 }
                 o[rt][mt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[mt & 1][t], p_now[rt][t], o[rt][mt], 0, 0, 0);
                 keep_sum(o[rt][mt]);
-                if constexpr (rt == 1 && t == 1 && mt + 2 < MT) read_v(mt + 2);
-                constexpr int EVERY = 4 * MT / CPW;
+                if constexpr (rt == RT - 1 && t == 1 && mt + 2 < MT) read_v(mt + 2);
+                constexpr int EVERY = 2 * RT * MT / CPW;
                 if constexpr (u % EVERY == 2) copy16_global_to_lds(v_next, v_from[u / EVERY], v_to + (u / EVERY) * 1024u);
             }
-            constexpr int first = piece_of_slot(slot, FROM, SLOTS, 2 * PIECES), behind = piece_of_slot(slot + 1, FROM, SLOTS, 2 * PIECES);
-            if constexpr (first < behind && first <= PIECES && behind > PIECES) static_assert(slot >= KS + 2, "the other tile's scores");
+            constexpr int first = piece_of_slot(slot, FROM, SLOTS, RT * PIECES), behind = piece_of_slot(slot + 1, FROM, SLOTS, RT * PIECES);
+            if constexpr (RT == 2 && first < behind && first <= PIECES && behind > PIECES) static_assert(slot >= KS + 2, "the other tile's scores");
             unrolled<behind - first>([&](auto at) __attribute__((always_inline)) {
                 constexpr int piece = first + decltype(at)::value;
                 if constexpr (piece % PIECES == 0) asm volatile("" : "+v"(s[piece / PIECES]));  // (not read before here)
@@ -326,9 +330,9 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void attn_maps_chunk_kernel(c
         k_at.next();
         v_at.next();
     };
-    auto copy_weights = [&](const h8 (&from)[2][2], h8 (&to)[2][2]) __attribute__((always_inline)) {
+    auto copy_weights = [&](const h8 (&from)[RT][2], h8 (&to)[RT][2]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int rt = 0; rt < 2; ++rt)
+        for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
             for (int t = 0; t < 2; ++t) to[rt][t] = from[rt][t];
     };
@@ -338,21 +342,21 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void attn_maps_chunk_kernel(c
     for (int t = 0; t < KS; ++t) {
         if (t == 0) {
             first_score(s[0], kf[0], q[0][0]);
-            first_score(s[1], kf[0], q[1][0]);
+            if constexpr (RT == 2) first_score(s[1], kf[0], q[1][0]);
         } else {
             next_score(s[0], kf[t], q[0][t]);
-            next_score(s[1], kf[t], q[1][t]);
+            if constexpr (RT == 2) next_score(s[1], kf[t], q[1][t]);
         }
         kf[t] = buf_load_h8<0>(rk, k_lane, k_at.at + t * 1024);
     }
     k_at.next();
-    settle(s[0]);
-    settle(s[1]);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) settle(s[rt]);
     if (jb >= first_masked || jb <= last_below) {
-        hide(0, jb);
-        hide(1, jb);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) hide(rt, jb);
     }
-    unrolled<2 * PIECES>([&](auto piece) __attribute__((always_inline)) {
+    unrolled<RT * PIECES>([&](auto piece) __attribute__((always_inline)) {
         soften(std::integral_constant<int, decltype(piece)::value / PIECES>{}, std::integral_constant<int, decltype(piece)::value % PIECES>{}, p);
     });
     const int last = nb - 1;
@@ -365,21 +369,21 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void attn_maps_chunk_kernel(c
     // about in every step.
     for (int i = 1; i <= last;) {
 #pragma unroll
-        for (int rt = 0; rt < 2; ++rt)
+        for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) keep_sum(o[rt][mt]);
         bool scale_sums;
 #pragma nounroll
         do {  // (two steps a turn, with the weights' registers in turn, were 5 % slower at heads of 128 and do not fit at heads of 256)
-            h8 p_next[2][2];
+            h8 p_next[RT][2];
             step(i, p, p_next);
             ++i;
-            scale_sums = __any(alpha[0] != 1.0f || alpha[1] != 1.0f);
+            scale_sums = __any(alpha[0] != 1.0f || alpha[RT - 1] != 1.0f);
             copy_weights(p_next, p);
         } while (!scale_sums && i <= last);
         if (scale_sums) {
 #pragma unroll
-            for (int rt = 0; rt < 2; ++rt)
+            for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
                     // (one at a time, and each kept where it is: no registers are left to have several on their way)
@@ -391,7 +395,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void attn_maps_chunk_kernel(c
         }
     }
 #pragma unroll
-    for (int rt = 0; rt < 2; ++rt)
+    for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) keep_sum(o[rt][mt]);
     // The last block's values.
@@ -403,18 +407,18 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void attn_maps_chunk_kernel(c
     for (int f = 0; f < VF; ++f) {
         const h8 x = read_v(last, f);
 #pragma unroll
-        for (int rt = 0; rt < 2; ++rt) {
+        for (int rt = 0; rt < RT; ++rt) {
             o[rt][f >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, p[rt][f & 1], o[rt][f >> 1], 0, 0, 0);
             keep_sum(o[rt][f >> 1]);
         }
     }
 #pragma unroll
-    for (int rt = 0; rt < 2; ++rt) l[rt] = sum_across_halves(l[rt] + l_odd[rt]);
+    for (int rt = 0; rt < RT; ++rt) l[rt] = sum_across_halves(l[rt] + l_odd[rt]);
 
     // Lane (li, g), register v of tile mt holds dim 32 mt + 8 (v / 4) + 4 g + v % 4 of row li.
     if (a.n_splits > 1) {
 #pragma unroll
-        for (int rt = 0; rt < 2; ++rt) {
+        for (int rt = 0; rt < RT; ++rt) {
             if (!valid[rt]) continue;
             const size_t row = (((size_t)split * (2 * a.group * a.n_kv_heads) + 2 * head[rt] + map) * a.tok_tiles + tile) * span + (tok[rt] - t0);
             float *const po = a.part_o + row * D + 4 * g;
@@ -433,16 +437,18 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void attn_maps_chunk_kernel(c
         return;
     }
 
-    // The maps of a tile meet: wavefront (pair, map) takes the pair's tile `map` and hands its sums of the other one over, as they are.  What follows
+    // The maps of a tile meet: of two tiles wavefront (pair, map) takes the pair's tile `map` and hands its sums of the other one over, as they are; of one
+    // tile the second map's wavefront hands them to the first's.  What follows
     // is done once a workgroup, straight on, so that its time goes by its length: the sums are chosen by branches, no select of each register,
     // and the tile's difference lies in LDS, so that norm, gate and stores are a short loop over tiles of 32 dims.
     __syncthreads();  // (the ring's place is the sums')
-    f4 *const to_partner = reinterpret_cast<f4 *>(smem + wave * C::X_BYTES) + lane;
-    f4 *const from_partner = reinterpret_cast<f4 *>(smem + (wave ^ 1) * C::X_BYTES) + lane;
+    f4 *const to_partner = reinterpret_cast<f4 *>(smem + (RT == 2 ? wave : pair) * C::X_BYTES) + lane;
+    f4 *const from_partner = reinterpret_cast<f4 *>(smem + (RT == 2 ? wave ^ 1 : pair) * C::X_BYTES) + lane;
     float *const sums = reinterpret_cast<float *>(smem + C::STAGE_OFF);
-    const float my_l = map ? l[1] : l[0];
-    const int my_tok = map ? tok[1] : tok[0], my_head = map ? head[1] : head[0];
-    const bool my_valid = map ? valid[1] : valid[0];
+    const bool second_tile = RT == 2 && map;
+    const float my_l = second_tile ? l[RT - 1] : l[0];
+    const int my_tok = second_tile ? tok[RT - 1] : tok[0], my_head = second_tile ? head[RT - 1] : head[0];
+    const bool my_valid = second_tile ? valid[RT - 1] : valid[0];
     const float lambda = a.maps.lambda[(long long)(my_valid ? my_tok : 0) * a.maps.lambda_stride + my_head];
     auto hand_over = [&](const f16v (&x)[MT], auto second) __attribute__((always_inline)) {
 #pragma unroll
@@ -453,9 +459,13 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void attn_maps_chunk_kernel(c
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    if (map) hand_over(o[0], std::true_type{});
-    else hand_over(o[1], std::false_type{});
-    sums[wave * 64 + lane] = map ? l[0] : l[1];
+    if constexpr (RT == 2) {
+        if (map) hand_over(o[0], std::true_type{});
+        else hand_over(o[1], std::false_type{});
+    } else if (map) {
+        hand_over(o[0], std::true_type{});
+    }
+    sums[wave * 64 + lane] = map ? l[0] : l[RT - 1];
     __syncthreads();
     const float their_l = sums[(wave ^ 1) * 64 + lane];
     const float my_inv = my_l > 0.0f ? 1.0f / my_l : 0.0f, their_inv = their_l > 0.0f ? 1.0f / their_l : 0.0f;
@@ -479,16 +489,21 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void attn_maps_chunk_kernel(c
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    if (map) subtract(o[1], std::true_type{});
-    else subtract(o[0], std::false_type{});
+    if constexpr (RT == 2) {
+        if (map) subtract(o[1], std::true_type{});
+        else subtract(o[0], std::false_type{});
+    } else if (!map) {
+        subtract(o[0], std::false_type{});
+    }
     float scale = a.maps.out_scale;
     if (a.maps.norm) {
         squares = sum_across_halves(squares);
         scale *= squares == 0.0f ? 0.0f : 1.0f / sqrtf(squares * (1.0f / D) + a.maps.eps);
     }
     __syncthreads();  // (the sums of the weights have been read: their place is the rows')
+    if (RT == 1 && map) return;
     // Norm weight and gate, and the rows out through LDS, 32 dims at a time: a store writes 64 bytes of 16 rows.
-    char *const stage = smem + C::STAGE_OFF + wave * C::STAGE_BYTES;
+    char *const stage = smem + C::STAGE_OFF + (RT == 2 ? wave : pair) * C::STAGE_BYTES;
     const int out_row = lane >> 2, out_piece = lane & 3, tile_tok = my_tok - li;
     const global_halves gate_row = (global_halves)(a.gate + (long long)(my_valid ? my_tok : 0) * a.g_stride + (long long)my_head * D + 4 * g);
     h4 gate[4];
@@ -588,9 +603,9 @@ int launch_maps_chunk(tt_hip_ctx *ctx, int head_dim, int n_kv_heads, const MapsC
     a.xs = n_kv_heads <= 8 && 8 % n_kv_heads == 0 ? 8 / n_kv_heads : 0;
     const unsigned grid = a.xs > 0 ? 8u * (unsigned)((a.per_kvh + a.xs - 1) / a.xs) : (unsigned)(a.per_kvh * n_kv_heads);
     switch (head_dim) {
-        case 256: launch_profiled(ctx, attn_maps_chunk_kernel<256>, dim3(grid), dim3(256), (unsigned)ChunkShape<256>::LDS, a); break;
-        case 128: launch_profiled(ctx, attn_maps_chunk_kernel<128>, dim3(grid), dim3(256), (unsigned)ChunkShape<128>::LDS, a); break;
-        case 64: launch_profiled(ctx, attn_maps_chunk_kernel<64>, dim3(grid), dim3(256), (unsigned)ChunkShape<64>::LDS, a); break;
+        case 256: launch_profiled(ctx, attn_maps_chunk_kernel<256>, dim3(grid), dim3(64 * ChunkShape<256>::WAVES), (unsigned)ChunkShape<256>::LDS, a); break;
+        case 128: launch_profiled(ctx, attn_maps_chunk_kernel<128>, dim3(grid), dim3(64 * ChunkShape<128>::WAVES), (unsigned)ChunkShape<128>::LDS, a); break;
+        case 64: launch_profiled(ctx, attn_maps_chunk_kernel<64>, dim3(grid), dim3(64 * ChunkShape<64>::WAVES), (unsigned)ChunkShape<64>::LDS, a); break;
         default: return TT_HIP_ERR_SHAPE;
     }
     const hipError_t e = hipGetLastError();

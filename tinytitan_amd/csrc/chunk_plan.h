@@ -194,7 +194,7 @@ inline MapsPlan plan_maps_chunk(int n_cus, int D, int n_q_heads, int n_kv_heads,
     const double start_us = D == 256 ? 13.0 : D == 128 ? 9.0 : 7.0;
     auto step_us = [&](double workgroups) {
         const double fill = std::min(1.0, workgroups / slots);
-        return D == 256 ? 0.95 + 0.42 * fill * fill : D == 128 ? 0.70 + 0.12 * fill : fill > 0.5 ? 0.88 : 0.60;
+        return D == 256 ? 0.95 + 0.42 * fill * fill : D == 128 ? 0.62 + 0.20 * fill * fill : fill > 0.5 ? 0.88 : 0.60;
     };
     // Whole tiles, the longest first: no CU is done before its longest tile, its share of all of them, or, with k rounds begun, k + 1 tiles of
     // the length that the last of those begins with.

@@ -429,6 +429,205 @@ void launch_gemm(tt_hip_ctx *ctx, const ProductArgs &a) {
                     n_tiles, per_xcd);
 }
 
+// The smallest tiles: the four wavefronts take a stage's four steps of 32 columns, one each, of the WHOLE tile, and add up their sums (exact in
+// integers, in any order) at the end.  A stage's operands then leave LDS once, not for two wavefronts each, and there is a barrier for four times the
+// products.  Every wavefront owns OWN tiles of 32 x 32 behind each other in channels, whose sums of the other three it adds to its own.  Two workgroups fit
+// a CU with four buffers.  us, tiles of 64 x 64 with TM / 2 x TN / 2 a wavefront / these: 512 tokens 2,048 x 4,096 11.6 / 9.8, 333 2,048 x 2,048 7.4 / 6.5,
+// 100 2,048 x 2,048 6.9 / 6.1, 300 300 x 8,192 18.2 / 15.1, 70 6,144 x 5,120 13.6 / 12.3.  Of 128 x 64 they are even (777 tokens, 2,311 x 4,096 19.4 / 18.8, 200
+// 5,120 x 5,120 16.6 / 18.3 the other way): there the copies' way from the L2s bounds both, 12 TB/s.
+template <int TM, int TN, int BUFFERS>
+struct StepsShape {
+    static constexpr int MT = TM / 32, NT = TN / 32, OWN = MT * NT / 4, BUFFER = (TM + TN) * kStageBytes;
+    static constexpr int PITCH = OWN * 32 * 2 + 16, STAGING = 4 * 32 * PITCH;
+    static constexpr size_t LDS = std::max<size_t>({(size_t)BUFFERS * BUFFER, (size_t)12 * OWN * 4096, (size_t)STAGING + TM * sizeof(float)});
+    static_assert(OWN >= 1 && NT <= 4 && 4 % NT == 0 && MT % OWN == 0);
+};
+template <int TM, int TN, int BUFFERS>
+__global__ __launch_bounds__(256, 1) void int8_steps_kernel(const ProductArgs a, int m_tiles, int n_tiles, int per_xcd) {
+    typedef StepsShape<TM, TN, BUFFERS> C;
+    constexpr int MT = C::MT, NT = C::NT, OWN = C::OWN, BUFFER = C::BUFFER;
+    constexpr int COPIES = (TM + TN) / 32;  // of 1 KiB (eight rows) that a wavefront issues a stage
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 31, g = lane >> 5;
+
+    // (workgroups, copies and the order of a line's pieces as above)
+    const int at = (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
+    if (at >= m_tiles * n_tiles) return;
+    const int group = at / (8 * n_tiles), in_group = at - group * 8 * n_tiles, group_m = min(m_tiles - group * 8, 8);
+    const int n_tile = in_group / group_m, m_tile = group * 8 + in_group - n_tile * group_m;
+    const int row0 = m_tile * TM, token0 = n_tile * TN;
+    const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) void *)smem;
+    const int in_copy = lane >> 3, piece = 16 * ((lane & 7) ^ in_copy);
+    unsigned from[COPIES];
+#pragma unroll
+    for (int c = 0; c < COPIES; ++c) {
+        const int r = (c * 4 + wave) * 8 + in_copy;
+        from[c] = c * 32 < TM ? (unsigned)min(r, a.rows - 1 - row0) * (unsigned)a.columns + (unsigned)piece
+                              : (unsigned)min(r - TM, a.tokens - 1 - token0) * (unsigned)a.levels_stride + (unsigned)piece;
+    }
+    const int8_t *w = a.weights + (long long)row0 * a.columns, *x = a.levels + (long long)token0 * a.levels_stride;
+    const int stages = (a.columns + kStageBytes - 1) / kStageBytes;
+    auto copy = [&](int c, int s, int buffer) {
+        const unsigned back = s * kStageBytes + piece < a.columns ? 0u : (unsigned)piece;
+        copy16_global_to_lds((c * 32 < TM ? w : x) + (size_t)s * kStageBytes, from[c] - back, lds0 + (unsigned)buffer * BUFFER + (unsigned)(c * 4 + wave) * 1024u);
+    };
+    i16v acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = (i16v)0;
+    // A stage's operands of this wavefront: 16 bytes of a row each, its piece 2 wave + g.
+    const int in_line = li * kStageBytes + ((2 * wave + g) ^ (li & 7)) * 16;
+    struct Operands {
+        i4 w[MT], x[NT];
+    };
+    auto read = [&](Operands &into, int buffer, int r) {
+        const char *const line = smem + buffer * BUFFER + in_line;
+        if (r < MT) into.w[r < MT ? r : 0] = *reinterpret_cast<const i4 *>(line + 32 * r * kStageBytes);
+        else into.x[r < MT ? 0 : r - MT] = *reinterpret_cast<const i4 *>(line + (TM + 32 * (r - MT)) * kStageBytes);
+    };
+    // Stage s: behind the barrier the next stage has landed and every wavefront holds this one's operands, so that its place is filled again.  (Past
+    // the last stage: that again, into a place that nobody reads.)
+    auto run_stage = [&](auto last_one, int s, int buffer, Operands &now, Operands &next) __attribute__((always_inline)) {
+        constexpr bool LAST = decltype(last_one)::value;
+        constexpr int PRODUCTS = MT * NT, WORK = MT + NT + COPIES;
+        if constexpr (LAST) {  // the columns behind the row's end: levels of zero, whatever the weights' place holds
+            const int k = s * kStageBytes + 32 * wave + 16 * g;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) now.x[j] = k < a.columns ? now.x[j] : (i4)0;
+        } else {
+            TT_WAIT_VMCNT((BUFFERS - 2) * COPIES);
+            __syncthreads();
+        }
+        const int behind = buffer + 1 == BUFFERS ? 0 : buffer + 1, copied = min(s + BUFFERS, stages - 1);
+#pragma unroll
+        for (int u = 0; u < PRODUCTS; ++u) {
+            const int i = u / NT, j = u % NT;
+            acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(now.w[i], now.x[j], acc[i][j], 0, 0, 0);
+            if constexpr (!LAST) {
+#pragma unroll
+                for (int r = 0; r < WORK; ++r) {
+                    if (r * PRODUCTS / WORK != u) continue;
+                    if (r < MT + NT) read(next, behind, r);
+                    else copy(r - MT - NT, copied, buffer);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    static_assert(BUFFERS >= 3);
+#pragma unroll
+    for (int s = 0; s < BUFFERS; ++s)
+#pragma unroll
+        for (int c = 0; c < COPIES; ++c) copy(c, min(s, stages - 1), s);
+    TT_WAIT_VMCNT((BUFFERS - 1) * COPIES);
+    __syncthreads();
+    Operands even, odd;
+#pragma unroll
+    for (int r = 0; r < MT + NT; ++r) read(even, 0, r);
+    int buffer = 0, s = 0;
+    auto step_on = [&] { buffer = buffer + 1 == BUFFERS ? 0 : buffer + 1; };
+#pragma nounroll
+    for (; s + 2 < stages; s += 2) {
+        run_stage(std::false_type{}, s, buffer, even, odd);
+        step_on();
+        run_stage(std::false_type{}, s + 1, buffer, odd, even);
+        step_on();
+    }
+    if (s + 1 < stages) {
+        run_stage(std::false_type{}, s, buffer, even, odd);
+        run_stage(std::true_type{}, s + 1, buffer, odd, even);
+    } else {
+        run_stage(std::true_type{}, s, buffer, even, odd);
+    }
+    TT_WAIT_VMCNT(0);
+    __syncthreads();
+
+    // The sums to their owners: owner o's tiles are (i0 .. i0 + OWN, j), i0 = o / NT * OWN, j = o % NT.
+    i16v mine[OWN];
+#pragma unroll
+    for (int o = 0; o < 4; ++o) {
+        const int i0 = o / NT * OWN, j = o % NT;
+        if (wave == o) {
+#pragma unroll
+            for (int t = 0; t < OWN; ++t) mine[t] = acc[i0 + t][j];
+        } else {
+            i4 *const to = reinterpret_cast<i4 *>(smem + (3 * o + (wave < o ? wave : wave - 1)) * OWN * 4096) + lane;
+#pragma unroll
+            for (int t = 0; t < OWN; ++t)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    const i16v &x = acc[i0 + t][j];
+                    to[(t * 4 + v) * 64] = i4{x[4 * v], x[4 * v + 1], x[4 * v + 2], x[4 * v + 3]};
+                }
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int other = 0; other < 3; ++other) {
+        const i4 *const of = reinterpret_cast<const i4 *>(smem + (3 * wave + other) * OWN * 4096) + lane;
+#pragma unroll
+        for (int t = 0; t < OWN; ++t)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                const i4 x = of[(t * 4 + v) * 64];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mine[t][4 * v + e] += x[e];
+            }
+    }
+    __syncthreads();
+
+    // The rows out through LDS, as above.
+    constexpr int PITCH = C::PITCH, LANES = OWN * 32 / 8, ROWS = 64 / LANES;
+    float *const channel_scales = reinterpret_cast<float *>(smem + C::STAGING);
+    if (threadIdx.x < TM) channel_scales[threadIdx.x] = a.weight_scales[min(row0 + (int)threadIdx.x, a.rows - 1)];
+    __syncthreads();
+    char *const stage = smem + wave * 32 * PITCH;
+    const int wave_row = wave / NT * OWN * 32, wave_token0 = token0 + 32 * (wave % NT);
+    const bool whole = (a.y_stride % 8 == 0) && (reinterpret_cast<size_t>(a.y) & 15) == 0;
+    const float scale = a.scales[min(wave_token0 + li, a.tokens - 1)];
+#pragma unroll
+    for (int t = 0; t < OWN; ++t)
+#pragma unroll
+        for (int v = 0; v < 16; v += 4) {
+            const int r = 32 * t + 8 * (v >> 2) + 4 * g;
+            const f4 channel = *reinterpret_cast<const f4 *>(channel_scales + wave_row + r);
+            h4 out;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) out[e] = (_Float16)((float)mine[t][v + e] * channel[e] * scale);
+            *reinterpret_cast<h4 *>(stage + li * PITCH + r * 2) = out;
+        }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int t = 0; t < 32; t += ROWS) {
+        const int row = t + lane / LANES, first = (lane % LANES) * 8, to_token = wave_token0 + row, r = row0 + wave_row + first;
+        const h8 out = *reinterpret_cast<const h8 *>(stage + row * PITCH + first * 2);
+        if (to_token < a.tokens) {
+            _Float16 *const to = a.y + to_token * a.y_stride + r;
+            if (whole && r + 8 <= a.rows) {
+                *reinterpret_cast<h8 *>(to) = out;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (r + e < a.rows) to[e] = out[e];
+            }
+        }
+    }
+}
+template <int TM, int TN, int BUFFERS>
+hipError_t configure_steps() {
+    return hipFuncSetAttribute(reinterpret_cast<const void *>(int8_steps_kernel<TM, TN, BUFFERS>), hipFuncAttributeMaxDynamicSharedMemorySize,
+                               (int)StepsShape<TM, TN, BUFFERS>::LDS);
+}
+template <int TM, int TN, int BUFFERS>
+void launch_steps(tt_hip_ctx *ctx, const ProductArgs &a) {
+    static_assert(BUFFERS * ((TM + TN) / 32) <= 63 && StepsShape<TM, TN, BUFFERS>::LDS <= 160 * 1024, "what vmcnt counts to; LDS");
+    const int m_tiles = (a.rows + TM - 1) / TM, n_tiles = (a.tokens + TN - 1) / TN;
+    const int per_xcd = (int)(((long long)m_tiles * n_tiles + 7) / 8);
+    launch_profiled(ctx, int8_steps_kernel<TM, TN, BUFFERS>, dim3((unsigned)per_xcd * 8u), dim3(256), (unsigned)StepsShape<TM, TN, BUFFERS>::LDS, a, m_tiles,
+                    n_tiles, per_xcd);
+}
+
 bool aligned(const void *p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
 // (the sums of products of two levels, at most 2^14 each, stay below 2^31)
@@ -473,7 +672,7 @@ struct GemmTile {
     int tm, tn;
     double stage_us, fixed_us;
 };
-constexpr GemmTile kGemmTiles[] = {{256, 256, 1.75, 10.0}, {128, 256, 0.95, 5.0}, {128, 128, 0.62, 3.0}, {128, 64, 0.5, 2.0}, {64, 128, 0.46, 2.0}, {64, 64, 0.36, 1.5}};
+constexpr GemmTile kGemmTiles[] = {{256, 256, 1.75, 10.0}, {128, 256, 0.95, 5.0}, {128, 128, 0.62, 3.0}, {128, 64, 0.5, 2.0}, {64, 128, 0.46, 2.0}, {64, 64, 0.25, 3.0}};
 int gemm_tile(const tt_hip_ctx *ctx, const ProductArgs &a) {
     int best = 0;
     double best_us = 0.0;
@@ -511,7 +710,7 @@ void launch_by_rule(tt_hip_ctx *ctx, const ProductArgs &a) {
         case 2: return launch_gemm<128, 128, 4>(ctx, a);
         case 3: return launch_gemm<128, 64, 3>(ctx, a);
         case 4: return launch_gemm<64, 128, 6>(ctx, a);
-        default: return launch_gemm<64, 64, 8>(ctx, a);
+        default: return launch_steps<64, 64, 4>(ctx, a);
     }
 }
 
@@ -563,7 +762,7 @@ int configure_int8_kernels(tt_hip_ctx *ctx) {
 #define TT_CFG(...) \
     if (e == hipSuccess) e = __VA_ARGS__();
     TT_CFG(configure_gemm<256, 256, 2>) TT_CFG(configure_gemm<128, 256, 3>) TT_CFG(configure_gemm<128, 128, 4>) TT_CFG(configure_gemm<128, 64, 3>)
-    TT_CFG(configure_gemm<64, 128, 6>) TT_CFG(configure_gemm<64, 64, 8>)
+    TT_CFG(configure_gemm<64, 128, 6>) TT_CFG(configure_steps<64, 64, 4>)
     TT_CFG(configure_ring<1, 1, 8, 2, false>) TT_CFG(configure_ring<1, 2, 8, 3, false>) TT_CFG(configure_ring<1, 3, 4, 4, false>)
     TT_CFG(configure_ring<1, 4, 4, 4, false>) TT_CFG(configure_ring<2, 1, 8, 2, false>) TT_CFG(configure_ring<2, 2, 8, 2, false>)
     TT_CFG(configure_ring<2, 3, 8, 2, false>) TT_CFG(configure_ring<2, 4, 4, 3, false>) TT_CFG(configure_ring<4, 1, 4, 3, false>)

@@ -9,8 +9,8 @@
 // the pass behind those of several splits, which adds up their partial results of both maps (as attn_join.hip does: the rows' o and l about a common
 // maximum), subtracts, and applies norm and gate in fp32 with one rounding.  A row that sees no key gives zeros.
 //
-// Memory bounds a long decode: 205 MB behind 100,001 keys of 16/2 heads of 256 take 40.4 - 42 us, the pass alone 32 (6.4 TB/s).  The join reads 2 KiB
-// a (token, head) and split, by one CU an item, since the norm needs the whole row: 112 splits, 7.9 us.
+// Memory bounds a long decode: 205 MB behind 100,001 keys of 16/2 heads of 256 take 40 us, the pass alone 32 (6.4 TB/s).  The join reads 2 KiB
+// a (token, head) and split, by one CU an item, since the norm needs the whole row: 112 splits, 7 us.
 //
 // Roundings: a weight of either map is rounded to fp16 for the second product, as in every kernel here (its sum is that of the rounded weights over fp16
 // pages), and over quantised pages a K operand is.  Against 64 bits 2.5 - 3e-4 over fp16 pages (2-norm; the final rounding alone is 2.0e-4) and
@@ -25,13 +25,19 @@ namespace {
 
 typedef float f2 __attribute__((ext_vector_type(2)));
 
-// A (token, head) item is D / 4 threads of four dims each, and G of those that share its splits; a workgroup is ITEMS of them.
-template <int D, int G>
-__global__ __launch_bounds__(G * D / 4 > 256 ? G * D / 4 : 256) void attn_maps_join_kernel(const MapsJoinArgs a) {
-    constexpr int LANES = D / 4, THREADS = G * LANES > 256 ? G * LANES : 256, ITEMS = THREADS / (G * LANES), BATCH = 4;
+// A (token, head) item is D / 4 threads of four dims each, and G of those that share its splits, for both maps or (BY_MAP) for each; a workgroup is
+// ITEMS of them.  With many splits it waits for memory, and then for one item's sums behind each other: BY_MAP, a thread has most of what it asks for
+// on its way at once (8 x 14 splits; of heads of 256, whose 1,024 threads have 128 registers each, 8 x 8) and adds up half as many.  us a decode step, 16 groups
+// for both maps / 8 for each: 16/2 heads of 256 behind 20,000 keys 18.1 / 17.3, behind 100,000 40.5 / 39.6, 3 rows behind 9,000 14.4 / 13.6, 32/8 of 128 behind
+// 40,000 30.3 / 29.6, 16/4 of 64 behind 60,000 15.2 / 14.4.
+template <int D, int G, bool BY_MAP>
+__global__ __launch_bounds__((BY_MAP ? 2 : 1) * G * D / 4 > 256 ? (BY_MAP ? 2 : 1) * G * D / 4 : 256) void attn_maps_join_kernel(const MapsJoinArgs a) {
+    constexpr int LANES = D / 4, PER_ITEM = (BY_MAP ? 2 : 1) * G * LANES, THREADS = PER_ITEM > 256 ? PER_ITEM : 256, ITEMS = THREADS / PER_ITEM;
+    constexpr int BATCH = BY_MAP ? (D == 256 ? 8 : 14) : 4, MAPS = BY_MAP ? 1 : 2;
     __shared__ f4 sums[G > 1 ? 2 : 1][G][G > 1 ? ITEMS * LANES : 1];
     __shared__ f2 stats[G > 1 ? 2 : 1][G][ITEMS];
-    const int lane = threadIdx.x % LANES, in_group = threadIdx.x / LANES, item = in_group % ITEMS, g = in_group / ITEMS;
+    const int lane = threadIdx.x % LANES, in_group = threadIdx.x / LANES, item = in_group % ITEMS, g = in_group / ITEMS % G;
+    const int first_map = BY_MAP ? in_group / (ITEMS * G) : 0;  // this thread's, of MAPS
     const int d = lane * 4, seq = blockIdx.y;
     const unsigned at_item = blockIdx.x * ITEMS + item, heads = a.heads;  // (rows x heads fit 31 bits)
     const bool real = at_item < (unsigned)a.rows * heads;
@@ -51,10 +57,10 @@ __global__ __launch_bounds__(G * D / 4 > 256 ? G * D / 4 : 256) void attn_maps_j
     const int k0 = a.window > 0 && first_lim > a.window ? (first_lim - a.window) & ~31 : 0;
     const int n = (int)((unsigned)(max(tile_end - k0, 1) + p.split_len - 1) / (unsigned)p.split_len);
     const size_t stride = (size_t)p.n_tiles * p.nt;
-    f4 acc[2];
-    float m[2], l[2];
+    f4 acc[MAPS];
+    float m[MAPS], l[MAPS];
 #pragma unroll
-    for (int map = 0; map < 2; ++map) {
+    for (int map = 0; map < MAPS; ++map) {
         acc[map] = (f4)0.0f;
         m[map] = kNegBig;
         l[map] = 0.0f;
@@ -63,29 +69,30 @@ __global__ __launch_bounds__(G * D / 4 > 256 ? G * D / 4 : 256) void attn_maps_j
     const int kvh = (unsigned)(2 * head) / (unsigned)a.group2, in_kvh = 2 * head - kvh * a.group2;
     const int hsub = (unsigned)in_kvh / (unsigned)p.gh, in_tile = in_kvh - hsub * p.gh;
     const size_t first_row = (size_t)((kvh * p.hsubs + hsub) * p.tok_tiles + tok_tile) * p.nt + (row - t0) * p.gh + in_tile + (size_t)sq.first_split * stride;
-    const size_t at[2] = {first_row, in_tile + 1 < p.gh ? first_row + 1 : first_row + (size_t)p.tok_tiles * p.nt - in_tile};
+    const size_t second_row = in_tile + 1 < p.gh ? first_row + 1 : first_row + (size_t)p.tok_tiles * p.nt - in_tile;
+    const size_t at[2] = {first_map ? second_row : first_row, second_row};
     for (int first = g; first < n; first += G * BATCH) {
-        f4 o[2][BATCH];
-        f2 ml[2][BATCH];
+        f4 o[MAPS][BATCH];
+        f2 ml[MAPS][BATCH];
         // (a split that is not there is not asked for: read as the last one again, they were most of what a workgroup fetched)
 #pragma unroll
         for (int i = 0; i < BATCH; ++i) {
 #pragma unroll
-            for (int map = 0; map < 2; ++map) {
+            for (int map = 0; map < MAPS; ++map) {
                 ml[map][i] = f2{kNegBig, 0.0f};
                 o[map][i] = (f4)0.0f;
             }
             if (first + i * G < n) {
                 const size_t s = (size_t)(first + i * G) * stride;
 #pragma unroll
-                for (int map = 0; map < 2; ++map) {
+                for (int map = 0; map < MAPS; ++map) {
                     ml[map][i] = *reinterpret_cast<const f2 *>(p.ml + (at[map] + s) * 2);
                     o[map][i] = *reinterpret_cast<const f4 *>(p.o + (at[map] + s) * D + d);
                 }
             }
         }
 #pragma unroll
-        for (int map = 0; map < 2; ++map) {
+        for (int map = 0; map < MAPS; ++map) {
             float top = m[map];
 #pragma unroll
             for (int i = 0; i < BATCH; ++i) top = fmaxf(top, ml[map][i][0]);
@@ -103,28 +110,36 @@ __global__ __launch_bounds__(G * D / 4 > 256 ? G * D / 4 : 256) void attn_maps_j
     }
     if constexpr (G > 1) {
 #pragma unroll
-        for (int map = 0; map < 2; ++map) {
-            sums[map][g][item * LANES + lane] = acc[map];
-            if (lane == 0) stats[map][g][item] = f2{m[map], l[map]};
+        for (int map = 0; map < MAPS; ++map) {
+            sums[first_map + map][g][item * LANES + lane] = acc[map];
+            if (lane == 0) stats[first_map + map][g][item] = f2{m[map], l[map]};
         }
         __syncthreads();
-        if (g != 0) return;
+        if (!BY_MAP && g != 0) return;
+        if (g == 0) {
 #pragma unroll
-        for (int map = 0; map < 2; ++map) {
-            float top = kNegBig;
-#pragma unroll 4
-            for (int i = 0; i < G; ++i) top = fmaxf(top, stats[map][i][item][0]);
-            acc[map] = (f4)0.0f;
-            l[map] = 0.0f;
-#pragma unroll 4
-            for (int i = 0; i < G; ++i) {
-                const float f = fast_exp2(stats[map][i][item][0] - top);
-                l[map] += f * stats[map][i][item][1];
-                acc[map] += f * sums[map][i][item * LANES + lane];
+            for (int map = 0; map < MAPS; ++map) {
+                float top = kNegBig;
+#pragma unroll
+                for (int i = 0; i < G; ++i) top = fmaxf(top, stats[first_map + map][i][item][0]);
+                acc[map] = (f4)0.0f;
+                l[map] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < G; ++i) {
+                    const float f = fast_exp2(stats[first_map + map][i][item][0] - top);
+                    l[map] += f * stats[first_map + map][i][item][1];
+                    acc[map] += f * sums[first_map + map][i][item * LANES + lane];
+                }
             }
         }
     }
-    const f4 a1 = acc[0] * (l[0] > 0.0f ? 1.0f / l[0] : 0.0f), a2 = acc[1] * (l[1] > 0.0f ? 1.0f / l[1] : 0.0f);
+    f4 a1 = acc[0] * (l[0] > 0.0f ? 1.0f / l[0] : 0.0f), a2 = acc[MAPS - 1] * (l[MAPS - 1] > 0.0f ? 1.0f / l[MAPS - 1] : 0.0f);
+    if constexpr (BY_MAP) {
+        if (g == 0 && first_map) sums[1][0][item * LANES + lane] = a2;  // (which this thread alone has read)
+        __syncthreads();
+        if (g != 0 || first_map) return;
+        a2 = sums[1][0][item * LANES + lane];
+    }
     f4 out;
 #pragma unroll
     for (int i = 0; i < 4; ++i) out[i] = map_difference(a1[i], a2[i], lambda);
@@ -162,17 +177,17 @@ __global__ __launch_bounds__(64) void diff_lambda_kernel(const float *q1, const 
     if (threadIdx.x == 0) lambda[blockIdx.x] = expf(first) - expf(second) + init;
 }
 
-template <int D, int G>
+template <int D, int G, bool BY_MAP>
 void launch_join_of(tt_hip_ctx *ctx, int n_seq, const MapsJoinArgs &args) {
-    constexpr int THREADS = G * D / 4 > 256 ? G * D / 4 : 256, ITEMS = THREADS * 4 / (G * D);
+    constexpr int PER_ITEM = (BY_MAP ? 2 : 1) * G * D / 4, THREADS = PER_ITEM > 256 ? PER_ITEM : 256, ITEMS = THREADS / PER_ITEM;
     const long long items = (long long)args.rows * args.heads;
-    hipLaunchKernelGGL((attn_maps_join_kernel<D, G>), dim3((unsigned)((items + ITEMS - 1) / ITEMS), (unsigned)n_seq), dim3(THREADS), 0, ctx->stream, args);
+    hipLaunchKernelGGL((attn_maps_join_kernel<D, G, BY_MAP>), dim3((unsigned)((items + ITEMS - 1) / ITEMS), (unsigned)n_seq), dim3(THREADS), 0, ctx->stream, args);
 }
 template <int D>
 void launch_join_by_splits(tt_hip_ctx *ctx, int n_seq, const MapsJoinArgs &args, int most_splits) {
-    if (most_splits <= 4) launch_join_of<D, 1>(ctx, n_seq, args);
-    else if (most_splits <= 16 || (long long)args.rows * args.heads * n_seq >= 4 * ctx->n_cus) launch_join_of<D, 4>(ctx, n_seq, args);
-    else launch_join_of<D, 16>(ctx, n_seq, args);
+    if (most_splits <= 4) launch_join_of<D, 1, false>(ctx, n_seq, args);
+    else if (most_splits <= 16 || (long long)args.rows * args.heads * n_seq >= 4 * ctx->n_cus) launch_join_of<D, 4, false>(ctx, n_seq, args);
+    else launch_join_of<D, 8, true>(ctx, n_seq, args);
 }
 
 template <int D, int NT, int BITS, int STREAM>

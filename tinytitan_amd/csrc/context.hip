@@ -1666,6 +1666,9 @@ int tt_hip_attn_prefill_swa(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int slot,
 
 // ---- differential attention --------------------------------------------------
 
+// Halves of a staged page: as many as a cache's own pages have at most (tt_hip_kv_create).
+static constexpr size_t kMostPageHalves = 0x7ff00000 / 2;
+
 // What a call reads of its sequences' slots: the keys [first, end), rows of the slot's own.
 static int check_maps_keys(const tt_hip_kv *kv, int slot, int window, long long start, long long end) {
     if (slot < 0 || slot >= kv->n_slots) return TT_HIP_ERR_INVALID_ARGUMENT;
@@ -1797,8 +1800,12 @@ int tt_hip_attn_prefill_diff(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int slot
     if (hipSetDevice(ctx->device) != hipSuccess) return TT_HIP_ERR_HIP;
     const long long end = (long long)start_pos + q_len;
     const MapsPlan plan = plan_maps_chunk(ctx->n_cus, kv->head_dim, n_q_heads, kv->n_kv_heads, start_pos, q_len, window, kv->bits);
-    bool chunk = scale > 0.0f && plan.n_splits > 0;
     const int group = n_q_heads / kv->n_kv_heads, span = 128 / maps_chunk_heads(group), tok_tiles = (q_len + span - 1) / span;
+    // Quantised pages: the blocks that some row sees, dequantised once, and positions counted from the first of them.
+    const int skipped = kv->bits == 16 ? 0 : (int)(window > 0 && start_pos + 1LL > window ? start_pos + 1LL - window : 0) / kBlockTokens;
+    const int staged_blocks = (int)((end + kBlockTokens - 1) / kBlockTokens) - skipped;
+    const size_t staged_page = (size_t)staged_blocks * kBlockTokens * kv->head_dim;
+    bool chunk = scale > 0.0f && plan.n_splits > 0 && (kv->bits == 16 || staged_page <= kMostPageHalves);
     // (no memory for partial results or dequantised pages, or a capture in which they would have to grow: the tiles)
     auto room = [&](int got) {
         if (got == TT_HIP_ERR_BUSY || got == TT_HIP_ERR_OUT_OF_MEMORY) {
@@ -1809,10 +1816,6 @@ int tt_hip_attn_prefill_diff(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int slot
     };
     if (chunk && plan.n_splits > 1) st = room(ensure_partials(ctx, (size_t)plan.n_splits * 2 * n_q_heads * tok_tiles * span, kv->head_dim));
     if (st != TT_HIP_OK) return st;
-    // Quantised pages: the blocks that some row sees, dequantised once, and positions counted from the first of them.
-    const int skipped = kv->bits == 16 ? 0 : (int)(window > 0 && start_pos + 1LL > window ? start_pos + 1LL - window : 0) / kBlockTokens;
-    const int staged_blocks = (int)((end + kBlockTokens - 1) / kBlockTokens) - skipped;
-    const size_t staged_page = (size_t)staged_blocks * kBlockTokens * kv->head_dim;
     if (chunk && kv->bits != 16) st = room(ensure_stage(ctx, staged_page * kv->n_kv_heads));
     if (st != TT_HIP_OK) return st;
     if (!chunk)

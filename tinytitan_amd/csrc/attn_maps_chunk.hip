@@ -65,6 +65,9 @@ struct ChunkShape {
 //   a product reads the sum of the one before it as it comes (the same registers), and the first takes a zero for it, not one that was just written;
 //   a vector instruction that reads a sum wants 19 cycles of four clocks behind the last of its products.  Every product of this size holds the
 //   matrix pipe for eight of those cycles, so that two more products issued in between are room enough.
+//   a product wants two cycles of four clocks behind a vector instruction that writes one of its operands; K's come from memory, the queries' are not
+//   written in the loop (an operand parked in an accumulation register and fetched right here gave wrong scores).
+// tests/test_wait_states_maps.py looks for each in the compiler's listing.
 __device__ __forceinline__ void first_score(f16v &s, h8 k, h8 q) { asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, 0" : "=&v"(s) : "v"(k), "v"(q)); }
 __device__ __forceinline__ void next_score(f16v &s, h8 k, h8 q) { asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(s) : "v"(k), "v"(q)); }
 // ... where no two products follow.
@@ -271,8 +274,8 @@ __global__ __launch_bounds__(64 * ChunkShape<D>::WAVES, D == 256 ? 1 : 2) void a
     unsigned ring = 0;  // where block i - 1's values lie in LDS
     auto step = [&](int i, const h8 (&p_now)[RT][2], h8 (&p_next)[RT][2]) __attribute__((always_inline)) {
         constexpr int CHAIN = (RT - 1) * KS, SLOTS = CHAIN + 2 * RT * MT, FROM = 2;  // (a tile's scores are read behind the third product after their last)
-        // V of block i - 1 has landed (K and V of the two blocks since may be on their way), and every wavefront is done with the block whose place
-        // the copies of this step take.
+        // V of block i - 1 has landed (K and V of the two steps since may be on their way; block 0's: see in front of the loop), and every wavefront
+        // is done with the block whose place the copies of this step take.
         TT_WAIT_VMCNT(2 * (KS + CPW));
         __syncthreads();
         const unsigned next_k = k_at.at;
@@ -359,6 +362,9 @@ __global__ __launch_bounds__(64 * ChunkShape<D>::WAVES, D == 256 ? 1 : 2) void a
     unrolled<RT * PIECES>([&](auto piece) __attribute__((always_inline)) {
         soften(std::integral_constant<int, decltype(piece)::value / PIECES>{}, std::integral_constant<int, decltype(piece)::value % PIECES>{}, p);
     });
+    // Block 0's values have landed: behind their copies there are only two blocks' and one block's K, not the two that the first step's wait lets be
+    // on their way.  (The compiler's own waits for K, which count the copies without knowing them, say so too, in another place in every build.)
+    TT_WAIT_VMCNT(KS + 2 * CPW);
     const int last = nb - 1;
     if (last > 0 && seen_of(0) != ~0u) {
         TT_WAIT_VMCNT(0);

@@ -73,6 +73,11 @@ def _listing(tmp_path, source):
     return listing.read_text()
 
 
+@pytest.fixture(scope="module")
+def int8_listing(tmp_path_factory):
+    return _listing(tmp_path_factory.mktemp("int8"), "int8_proj.hip")
+
+
 @pytest.mark.parametrize("source", ["attn_maps_chunk.hip", "int8_proj.hip"])
 def test_copies_into_lds_wait_for_what_they_read(tmp_path, source):
     missing, copies, clobbered = _missing(_listing(tmp_path, source))
@@ -158,6 +163,15 @@ def test_values_have_landed_by_the_barrier_in_front_of_them(tmp_path, dim):
     name = re.search(r"^(_ZN2tt\w*attn_maps_chunk_kernelILi%dE\w*):" % dim, listing, re.M)[1]
     late, reached = late_copies(listing, name, COPIES[dim], 5)
     assert reached == 5
+    assert not late
+
+
+@pytest.mark.parametrize("kernel,tm,tn", [("int8_gemm", 256, 256), ("int8_gemm", 128, 256), ("int8_gemm", 128, 128), ("int8_gemm", 128, 64),
+                                          ("int8_gemm", 64, 128), ("int8_steps", 64, 64)])
+def test_stages_of_a_product_have_landed_by_their_barriers(int8_listing, kernel, tm, tn):
+    name = re.search(r"^(_ZN2tt\w*%s_kernelILi%dELi%dE\w*):" % (kernel, tm, tn), int8_listing, re.M)[1]
+    late, reached = late_copies(int8_listing, name, (tm + tn) // 32, 4)
+    assert reached == 4
     assert not late
 
 

@@ -105,3 +105,23 @@ def test_a_row_that_is_not_finite_stays_alone(gpu_ctx, rows):
     got[2, 5] = want[2, 5].half()
     check(got, (want, bound + (torch.arange(len(some), device="cuda") == 2)[:, None, None] * 1.0), f"{rows} rows")
     layer.close()
+
+
+@pytest.mark.parametrize("scale", [-0.05, 0.0])
+def test_a_chunk_by_tiles_in_several_passes(gpu_ctx, scale):
+    # more rows of both maps than partial results are kept of at a time (131,072 of them), by the way that a scale which is not positive takes
+    H, KH, D, rows, start = 64, 8, 64, 1500, 40
+    layer = Layer(gpu_ctx, H, KH, D, [start + rows])
+    layer.scale = scale
+    heads = layer.heads(np.random.default_rng(3).random((rows, H)).astype(np.float32), normed=False)
+    q, gate = _randn(1, rows, H, D), _randn(2, rows, H, D)
+    from tinytitan_amd.engine import PrefillAttentionParams
+    import torch
+    out = torch.full_like(q, float("nan"))
+    torch.cuda.synchronize()
+    layer.attention.encode_causal(layer.kv, 0, 0, q, out, PrefillAttentionParams(start, rows, start + rows, H, scale, H * D, H * D), heads, gate=gate)
+    gpu_ctx.synchronize()
+    assert torch.isfinite(out).all()
+    some = [0, 1, 500, 1022, 1023, 1024, 1025, 1300, 1499]
+    check(out[some], layer.want(q[some], 0, [start + i for i in some], heads, gate[some], heads.lambdas[some]), f"scale {scale}")
+    layer.close()

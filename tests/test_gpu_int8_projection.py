@@ -350,7 +350,8 @@ def test_refusals(gpu_ctx):
     refused(shape, p.encode_levels, w, ws, levels, scales, y, 10, 64, 4, levels_stride=48)
     refused(bad, p.encode_levels, w, ws, levels, None, y, 10, 64, 4)
     refused(bad, p.encode_levels, w, ws, None, scales, y, 10, 64, 4)
-    for args in ((w.float(), ws, x, y), (w, ws.double(), x, y), (w, ws, x.float(), y), (w, ws, x, y.float()), (w.cpu(), ws, x, y), (w.T, ws, x, y)):
+    for args in ((w.float(), ws, x, y), (w, ws.double(), x, y), (w, ws, x.float(), y), (w, ws, x, y.float()), (w.cpu(), ws, x, y), (w.T, ws, x, y),
+                 (torch.ones(10, 80, dtype=torch.int8, device="cuda")[:, :64], ws, x, y)):
         with pytest.raises(TypeError):
             p.encode(*args, 10, 64, 4, x_stride=80)
     gpu_ctx.synchronize()

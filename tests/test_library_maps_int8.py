@@ -53,6 +53,9 @@ def test_rows_of_factors():
     for norm in (torch.zeros(32, dtype=torch.bfloat16), torch.zeros(128, dtype=torch.bfloat16)[::2]):
         with pytest.raises(TinyTitanHIPError):
             DifferentialHeads(torch.zeros(8), norm).check(64)
+    with pytest.raises(TinyTitanHIPError) as e:
+        DifferentialHeads(torch.zeros(8), torch.zeros(64, dtype=torch.float16)).check(64)
+    assert e.value.status == capi.ERR_INVALID_ARGUMENT
 
 
 def test_signatures_match_the_header():

@@ -109,6 +109,8 @@ struct Args {
     float *floats() { return static_cast<float *>(typed(at::kFloat, "expected an fp32 device tensor with a contiguous last dimension")); }
     // an int8 device tensor of that kind, or None
     int8_t *levels() { return static_cast<int8_t *>(typed(at::kChar, "expected an int8 device tensor with a contiguous last dimension")); }
+    // an int8 device tensor without gaps between its rows, or None
+    int8_t *levels_in_one() { return static_cast<int8_t *>(typed(at::kChar, "expected a contiguous int8 device tensor", true)); }
     // a contiguous device tensor of any type, or None
     void *raw() {
         const at::Tensor *t = tensor();
@@ -182,12 +184,12 @@ private:
         Py_DECREF(whole);
         return v;
     }
-    void *typed(at::ScalarType type, const char *what) {
+    void *typed(at::ScalarType type, const char *what, bool in_one = false) {
         const at::Tensor *t = tensor();
         if (!t) return nullptr;
         if (!t->is_cuda() || t->scalar_type() != type) return fail<void>(what);
         try {
-            if (t->dim() > 0 && t->size(-1) > 1 && t->stride(-1) != 1) return fail<void>(what);
+            if (in_one ? !t->is_contiguous() : t->dim() > 0 && t->size(-1) > 1 && t->stride(-1) != 1) return fail<void>(what);
         } catch (const std::exception &e) {
             ok = false;
             PyErr_SetString(PyExc_RuntimeError, e.what());
@@ -740,7 +742,7 @@ TT_CALL(int8_projection) {
     Args a(args, n, 10);
     if (!a.ok) return nullptr;
     auto *ctx = a.handle<tt_hip_ctx>();
-    const int8_t *weights = a.levels();
+    const int8_t *weights = a.levels_in_one();
     const float *weight_scales = a.floats();
     const tt_half *x = a.half();
     const size_t x_stride = a.size();
@@ -769,7 +771,7 @@ TT_CALL(int8_projection_levels) {
     Args a(args, n, 11);
     if (!a.ok) return nullptr;
     auto *ctx = a.handle<tt_hip_ctx>();
-    const int8_t *weights = a.levels();
+    const int8_t *weights = a.levels_in_one();
     const float *weight_scales = a.floats();
     const int8_t *levels = a.levels();
     const size_t levels_stride = a.size();

@@ -541,8 +541,12 @@ class DifferentialHeads:
 
     def check(self, head_dim: int) -> None:
         w = self.norm_weight
-        if w is not None and (w.numel() != head_dim or not w.is_contiguous()):
+        if w is None:
+            return
+        if w.numel() != head_dim or not w.is_contiguous():
             raise TinyTitanHIPError(capi.ERR_SHAPE, "DifferentialHeads")
+        if w.dtype == torch.float16:  # (16 bits, too, but not those of a bfloat16)
+            raise TinyTitanHIPError(capi.ERR_INVALID_ARGUMENT, "DifferentialHeads")
 
 
 class DifferentialAttention:

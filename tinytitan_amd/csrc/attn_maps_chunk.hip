@@ -20,7 +20,8 @@
 // 704 with 32/8 of 128 (0.94; two tiles a wavefront 716), 240 - 249 with 16/4 of 64 (0.66 - 0.69); 777 rows behind 9,000 of 32/8 heads of 128 230 - 235
 // (two tiles 252).  Tried and not kept, heads of 256 / of 128 with two tiles: the copies of V in front of all reads of K +16 / +23 %, each in
 // front of one +2 / +1; a barrier every second step, eight blocks of V, +2 / +1; the sums of the weights by dot products of pairs
-// +4 / +6; two workgroups a CU for heads of 128, in 256 registers, +23.
+// +4 / +6; two workgroups a CU for heads of 128, in 256 registers, +23.  Those sums as one more tile of values, of ones, which takes an eleventh of the vector
+// instructions away and makes two products of them: heads of 128 +2 on a full chip and even below, of 64 even.
 #include <algorithm>
 
 #include "lds_copy.h"

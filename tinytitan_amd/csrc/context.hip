@@ -34,12 +34,12 @@ int ensure_partials(tt_hip_ctx *ctx, size_t rows, int head_dim, bool front) {
     if (ctx->capturing) return TT_HIP_ERR_BUSY;  // growing would synchronise and allocate inside a capture
     hipError_t e = hipStreamSynchronize(ctx->stream);
     if (e != hipSuccess) return hip_fail(ctx, e, "hipStreamSynchronize");
+    if (part_o) ++ctx->generation;  // (a store that there was not yet is in no graph)
     if (part_o) (void)hipFree(part_o);
     if (part_ml) (void)hipFree(part_ml);
     part_o = nullptr;
     part_ml = nullptr;
     part_rows = 0;
-    ++ctx->generation;
     size_t want = rows + rows / 4;
     e = hipMalloc(reinterpret_cast<void **>(&part_o), want * 256 * sizeof(float));
     if (e != hipSuccess) return hip_fail(ctx, e, "hipMalloc(split partial O)");
@@ -58,11 +58,11 @@ int ensure_stage(tt_hip_ctx *ctx, size_t elems) {
     if (ctx->capturing) return TT_HIP_ERR_BUSY;
     hipError_t e = hipStreamSynchronize(ctx->stream);
     if (e != hipSuccess) return hip_fail(ctx, e, "hipStreamSynchronize");
+    if (ctx->stage_k) ++ctx->generation;
     if (ctx->stage_k) (void)hipFree(ctx->stage_k);
     if (ctx->stage_v) (void)hipFree(ctx->stage_v);
     ctx->stage_k = ctx->stage_v = nullptr;
     ctx->stage_elems = 0;
-    ++ctx->generation;
     const size_t want = elems + elems / 4;
     e = hipMalloc(reinterpret_cast<void **>(&ctx->stage_k), want * sizeof(_Float16));
     if (e != hipSuccess) return hip_fail(ctx, e, "hipMalloc(dequantised K pages)");
@@ -520,7 +520,10 @@ static int run_attention(tt_hip_ctx *ctx, tt_hip_kv *kv, int kind, int layer, in
         if (plan.packed_splits > 0 && plan.tok_tiles > 1) plan.packed_splits = (plan.packed_splits + 7) & ~7;
         plan.partials_only = piece != nullptr;
         const bool front = piece && piece->front;
-        if (plan.n_splits_max > 1 || piece) {
+        // (two maps' rows in one split, where a head's two are in one tile: the launch writes the finished rows, and no store is asked for -- one that
+        // nobody reads would refuse a first capture, and grown it would make every captured graph stale)
+        const bool finishes = piece && piece->maps && plan.n_splits_max == 1 && plan.gh % 2 == 0;
+        if ((plan.n_splits_max > 1 || piece) && !finishes) {
             const size_t part_rows = total_splits * plan.n_tiles * plan.nt;
             if (static_partials) {
                 if (part_rows > kStaticPartialRows) return TT_HIP_ERR_SCRATCH;
@@ -563,9 +566,8 @@ static int run_attention(tt_hip_ctx *ctx, tt_hip_kv *kv, int kind, int layer, in
         h.n_splits_max = plan.n_splits_max;
         if (piece) {
             // (a launch of one split would write the final rows: it is told of a second one, which no tile has)
-            // (two maps' rows: it writes those, where a head's two are in one tile)
-            if (piece->maps && h.n_splits_max == 1 && plan.gh % 2 == 0) piece->finished = true;
-            else if (h.n_splits_max == 1) h.n_splits_max = 2;
+            piece->finished = finishes;
+            if (!finishes && h.n_splits_max == 1) h.n_splits_max = 2;
             piece->parts = PassParts{h.part_o, h.part_ml, plan.nt, plan.gh, plan.tt, plan.hsubs, plan.tok_tiles, plan.n_tiles, plan.split_len};
             std::copy(first_split, first_split + n, piece->first_split);
         }

@@ -539,9 +539,10 @@ TT_HIP_API int tt_hip_attn_prefill_shared(tt_hip_ctx *ctx, tt_hip_kv *kv, int la
  * Softmax statistics, sums, difference and norm are in fp32, with one rounding to fp16.  A row without a visible key (a sequence of
  * length 0) gives zeros.  Values of keys that no row of a call sees do not reach it, whatever the cache holds there; a value that is not
  * finite and that some row sees may reach the sequence's other rows of the call.
- * Both maps come from one pass over the cache.  A chunk's partial results and, over quantised pages, its dequantised blocks live in stores
- * that the context owns (grown on demand; inside a graph capture in which they would have to grow the call takes a way that does without, or
- * is refused with TT_HIP_ERR_BUSY).  No counterpart in the reference.
+ * Both maps come from one pass over the cache.  Partial results of a pass over several ranges of keys and, over quantised pages, a chunk's
+ * dequantised blocks live in stores that the context owns, grown on demand.  Inside a graph capture in which they would have to grow a chunk
+ * takes a way that does without (over quantised pages where its dequantised blocks have room, or its tiles' keys are one range), a slower one
+ * as a rule; other calls are refused with TT_HIP_ERR_BUSY.  A call in one range (a few hundred keys) keeps none.  No counterpart in the reference.
  * TT_HIP_ERR_INVALID_ARGUMENT: a NULL lambda, an eps below zero or NaN; TT_HIP_ERR_SHAPE: a lambda_stride between 0 and n_q_heads;
  * TT_HIP_ERR_CURSOR: a slot that starts from another slot's prefix (tt_hip_kv_share_prefix); TT_HIP_ERR_CAPACITY as for the _swa calls, and
  * for a ring that keeps sinks as soon as a sequence has outgrown it. */

@@ -1,5 +1,6 @@
 """What differential attention asks of the stores that a context owns: a call whose launch writes the finished rows keeps no partial results, so that
-it can be captured on a context that has run nothing, and leaves captured graphs as they are."""
+it can be captured on a context that has run nothing, and leaves captured graphs as they are; and a chunk whose partial results find no room takes a way
+that keeps none."""
 import numpy as np
 import pytest
 
@@ -112,5 +113,45 @@ def test_a_launch_that_finishes_its_rows_leaves_graphs_as_they_are(new_ctx):
         check(got[7], layer.want(rows[7], 8, list(range(236, 300)), heads), "many rows")
 
     check(replayed(new_ctx, graph, out, others), layer.want(q, 0, [4999], heads), "replays")
+    graph.close()
+    layer.close()
+
+
+# rows, start, bits: by the tiles in several splits, or by ranges of keys
+@pytest.mark.parametrize("H,KH,D,bits,rows,start,staged,status", [
+    (16, 2, 256, 16, 24, 3000, False, "OK"), (16, 4, 64, 16, 20, 3000, False, "OK"), (32, 8, 128, 16, 16, 3000, False, "OK"),
+    (16, 2, 256, 16, 333, 2500, False, "OK"), (32, 8, 128, 16, 130, 6000, False, "OK"), (16, 2, 256, 16, 100, 17000, False, "OK"),
+    (16, 2, 256, 8, 333, 2500, False, "OK"),        # (the tiles: one split)
+    (16, 2, 256, 8, 100, 4500, True, "OK"), (16, 2, 256, 4, 20, 3000, True, "OK"),
+    (16, 2, 256, 8, 100, 17000, False, "ERR_BUSY"), (16, 2, 256, 4, 20, 3000, False, "ERR_BUSY")])
+def test_a_chunk_captured_before_there_is_a_store(new_ctx, H, KH, D, bits, rows, start, staged, status):
+    import torch
+    from tinytitan_amd import capi
+    from tinytitan_amd.engine import PrefillAttentionParams
+    layer = Layer(new_ctx, H, KH, D, [max(start + rows, 4500)], bits)
+    heads = layer.heads(normed=False)
+    if staged:  # by a chunk that leaves dequantised blocks and no partial results: of all keys a workgroup, in the chunk kernel
+        layer.chunk(_randn(9, 1500, H, D), 3000, heads)
+    q = _randn(1, rows, H, D)
+    out = torch.zeros_like(q)
+    params = PrefillAttentionParams(start, rows, start + rows, H, layer.scale, H * D, H * D)
+    torch.cuda.synchronize()
+    step = lambda: layer.attention.encode_causal(layer.kv, 0, 0, q, out, params, heads)  # noqa: E731
+    graph = captured(new_ctx, step)
+    if status != "OK":
+        assert graph == getattr(capi, status)
+    else:
+        assert not isinstance(graph, int), graph
+        some = sorted(set(range(0, rows, 9)) | {rows - 1})
+        at = torch.tensor(some, device="cuda")
+        # (between the replays the same call makes its stores)
+        got = replayed(new_ctx, graph, out, lambda: layer.chunk(q, start, heads))
+        check(got[at], layer.want(q[at], 0, [start + r for r in some], heads), "captured")
+        graph.close()
+    step()
+    new_ctx.synchronize()
+    graph = captured(new_ctx, step)
+    eager = layer.chunk(q, start, heads)
+    assert torch.equal(replayed(new_ctx, graph, out), eager)
     graph.close()
     layer.close()

@@ -1802,28 +1802,31 @@ int tt_hip_attn_prefill_diff(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int slot
     if (!guard.ok) return TT_HIP_ERR_BUSY;
     if (hipSetDevice(ctx->device) != hipSuccess) return TT_HIP_ERR_HIP;
     const long long end = (long long)start_pos + q_len;
-    const MapsPlan plan = plan_maps_chunk(ctx->n_cus, kv->head_dim, n_q_heads, kv->n_kv_heads, start_pos, q_len, window, kv->bits);
+    MapsPlan plan = plan_maps_chunk(ctx->n_cus, kv->head_dim, n_q_heads, kv->n_kv_heads, start_pos, q_len, window, kv->bits);
     const int group = n_q_heads / kv->n_kv_heads, span = 128 / maps_chunk_heads(group), tok_tiles = (q_len + span - 1) / span;
     // Quantised pages: the blocks that some row sees, dequantised once, and positions counted from the first of them.
     const int skipped = kv->bits == 16 ? 0 : (int)(window > 0 && start_pos + 1LL > window ? start_pos + 1LL - window : 0) / kBlockTokens;
     const int staged_blocks = (int)((end + kBlockTokens - 1) / kBlockTokens) - skipped;
     const size_t staged_page = (size_t)staged_blocks * kBlockTokens * kv->head_dim;
-    bool chunk = scale > 0.0f && plan.n_splits > 0 && (kv->bits == 16 || staged_page <= kMostPageHalves);
+    const bool served = scale > 0.0f && (kv->bits == 16 || staged_page <= kMostPageHalves);
+    bool chunk = served && plan.n_splits > 0;
+    const auto no_room = [](int got) { return got == TT_HIP_ERR_BUSY || got == TT_HIP_ERR_OUT_OF_MEMORY; };
     // (no memory for partial results or dequantised pages, or a capture in which they would have to grow: the tiles)
     auto room = [&](int got) {
-        if (got == TT_HIP_ERR_BUSY || got == TT_HIP_ERR_OUT_OF_MEMORY) {
-            chunk = false;
-            return (int)TT_HIP_OK;
-        }
-        return got;
+        if (no_room(got)) chunk = false;
+        return no_room(got) ? (int)TT_HIP_OK : got;
     };
     if (chunk && plan.n_splits > 1) st = room(ensure_partials(ctx, (size_t)plan.n_splits * 2 * n_q_heads * tok_tiles * span, kv->head_dim));
     if (st != TT_HIP_OK) return st;
     if (chunk && kv->bits != 16) st = room(ensure_stage(ctx, staged_page * kv->n_kv_heads));
     if (st != TT_HIP_OK) return st;
-    if (!chunk)
-        return run_maps_tiles(ctx, kv, layer, 1, &slot, &start_pos, &kv_valid, q_len, n_q_heads, q, 0, (long long)q_stride, gate, 0,
-                              (long long)gate_stride, scale, window, maps, out, 0, (long long)o_stride);
+    if (!chunk) {
+        st = run_maps_tiles(ctx, kv, layer, 1, &slot, &start_pos, &kv_valid, q_len, n_q_heads, q, 0, (long long)q_stride, gate, 0,
+                            (long long)gate_stride, scale, window, maps, out, 0, (long long)o_stride);
+        // (nor for the tiles' partial results: the chunk kernel over all of a tile's keys, which keeps none)
+        if (!served || !no_room(st) || (kv->bits != 16 && ensure_stage(ctx, staged_page * kv->n_kv_heads) != TT_HIP_OK)) return st;
+        plan.n_splits = 1;
+    }
     MapsChunk c{};
     if (kv->bits == 16) {
         const size_t slot_elems = (size_t)slot * kv->n_kv_heads * kv->page_elems();

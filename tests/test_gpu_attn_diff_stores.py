@@ -1,6 +1,6 @@
 """What differential attention asks of the stores that a context owns: a call whose launch writes the finished rows keeps no partial results, so that
-it can be captured on a context that has run nothing, and leaves captured graphs as they are; and a chunk whose partial results find no room takes a way
-that keeps none."""
+it can be captured on a context that has run nothing, and leaves captured graphs as they are; a chunk whose partial results find no room takes a way
+that keeps none; and of many sequences' rows some are served at a time, so that what is kept of them has a bound."""
 import numpy as np
 import pytest
 
@@ -154,4 +154,48 @@ def test_a_chunk_captured_before_there_is_a_store(new_ctx, H, KH, D, bits, rows,
     eager = layer.chunk(q, start, heads)
     assert torch.equal(replayed(new_ctx, graph, out), eager)
     graph.close()
+    layer.close()
+
+
+def _several_passes(layer, starts, rows, some):
+    """Verify rows with factors by token: `some` of each sequence's against the definition.  Returns what the call has left on the device."""
+    import torch
+
+    def used():
+        torch.cuda.synchronize()
+        free, total = torch.cuda.mem_get_info()
+        return total - free - torch.cuda.memory_reserved()
+
+    H, n = layer.H, len(starts)
+    q, gate = _randn(1, n, rows, H, layer.D), _randn(2, n, rows, H, layer.D)
+    lambdas = np.random.default_rng(3).random((n * rows, H)).astype(np.float32)
+    heads = layer.heads(lambdas)
+    before = used()
+    got = layer.verify(q, starts, rows, heads, gate)
+    grown = used() - before
+    for i, start in enumerate(starts):
+        of = heads.lambdas[i * rows:(i + 1) * rows]
+        check(got[i, some], layer.want(q[i, some], i, [start + r for r in some], heads, gate[i, some], of[some]), f"sequence {i}")
+    return grown
+
+
+def test_rows_of_many_sequences_in_several_passes(new_ctx):
+    # 17 heads, whose 34 rows of maps are tiles of 17: a head's maps may part, and their partial results are kept whatever the keys are
+    H, KH, D, n, rows = 17, 1, 64, 32, 512
+    starts = [int(s) for s in np.random.default_rng(1).integers(0, 90, n)]
+    layer = Layer(new_ctx, H, KH, D, [s + rows for s in starts])
+    at_once = 131072 // (2 * H * n)
+    grown = _several_passes(layer, starts, rows, [0, at_once - 1, at_once, at_once + 1, 2 * at_once, rows - 1])
+    # 131,072 rows, of 32 a tile 17 in use, 256 values and two statistics each, the store a quarter larger than asked for
+    assert grown <= 131072 * 32 / 17 * 1.25 * (256 + 2) * 4 + (32 << 20), grown
+    layer.close()
+
+
+def test_rows_of_unlike_sequences_in_several_passes(new_ctx):
+    H, KH, D, n, rows = 16, 2, 256, 20, 300
+    starts = [20 * i for i in range(n - 1)] + [20000]
+    layer = Layer(new_ctx, H, KH, D, [s + rows for s in starts])
+    at_once = 131072 // (2 * H * n)
+    assert at_once < rows
+    _several_passes(layer, starts, rows, [0, at_once - 1, at_once, rows - 1])
     layer.close()

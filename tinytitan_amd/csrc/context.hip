@@ -1694,9 +1694,9 @@ static int run_maps_tiles(tt_hip_ctx *ctx, tt_hip_kv *kv, int layer, int n_seq, 
                           int n_q_heads, const tt_half *q, long long q_seq_stride, long long q_tok_stride, const tt_half *gate,
                           long long g_seq_stride, long long g_tok_stride, float scale, int window, const MapHeads &maps, tt_half *out,
                           long long o_seq_stride, long long o_tok_stride) {
-    const int rows_at_once = std::max(kMapsRowsAtOnce / (2 * n_q_heads), 16);
     for (int base = 0; base < n_seq; base += kMaxSeqPerLaunch) {
         const int n = std::min(n_seq - base, kMaxSeqPerLaunch);
+        const int rows_at_once = (int)std::max(kMapsRowsAtOnce / (2ll * n_q_heads * n), 16ll);
         for (int r = 0; r < rows; r += rows_at_once) {
             int first[kMaxSeqPerLaunch];
             for (int i = 0; i < n; ++i) first[i] = starts[base + i] + r;

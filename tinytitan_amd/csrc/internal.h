@@ -328,7 +328,7 @@ struct MapsJoinArgs {
     long long g_seq_stride, g_tok_stride, o_seq_stride, o_tok_stride;
     JoinSeq seq[kMaxSeqPerLaunch];
 };
-// Rows of maps whose partial results of a split are kept at a time (128 MiB with heads of 256).
+// Rows of maps, of all sequences of a launch, whose partial results of a split are kept at a time: 128 MiB, and the rows that tiles leave empty.
 constexpr int kMapsRowsAtOnce = 131072;
 int configure_maps_kernels(tt_hip_ctx *ctx);
 int launch_splitk_maps(tt_hip_ctx *ctx, const LaunchPlan &plan, int head_dim, int n_seq, const SplitKMaps &args, int kv_bits);

@@ -19,6 +19,7 @@ through ctypes.
 from __future__ import annotations
 
 import ctypes
+import weakref
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
@@ -62,6 +63,7 @@ class HIPContext:
         if not self.handle:
             raise TinyTitanHIPError(err.value, "tt_hip_ctx_create")
         self.device = device
+        self._caches = weakref.WeakSet()
 
     def _check(self, status: int, where: str) -> None:
         if status != capi.OK:
@@ -141,7 +143,10 @@ class HIPContext:
         return a.value, b.value, c.value
 
     def close(self) -> None:
+        """Closes the context's caches, too: they live on its device and stream."""
         if getattr(self, "handle", None):
+            for kv in list(self._caches):
+                kv.close()
             self._lib.tt_hip_ctx_destroy(self.handle)
             self.handle = None
 
@@ -207,6 +212,7 @@ class KVCacheManager:
                                     "tt_hip_kv_create_ring" if ring_capacity > 0 else "tt_hip_kv_create_quantized")
         self.layers, self.kv_heads, self.head_dim, self.slots = layers, kv_heads, head_dim, slots
         self.precision_bits = precision_bits
+        ctx._caches.add(self)
 
     # -- bookkeeping ---------------------------------------------------------
     @property
@@ -340,7 +346,8 @@ class KVCacheManager:
 
     def close(self) -> None:
         if getattr(self, "handle", None):
-            self._lib.tt_hip_kv_destroy(self.handle)
+            if self.ctx.handle:  # (a context that the collector has finalised before its cache is not there to wait for)
+                self._lib.tt_hip_kv_destroy(self.handle)
             self.handle = None
 
     def __del__(self):  # pragma: no cover

@@ -1,0 +1,89 @@
+"""Tensors of the 8-bit products that are views of wider ones: scales that are a column are refused, not read as if they lay next to each other."""
+import numpy as np
+import pytest
+
+from tests.test_gpu_int8_projection import _dev, _tokens, _weights, check, quantised
+
+pytestmark = pytest.mark.gpu
+
+TOKENS, ROWS, COLUMNS = 6, 40, 256
+
+
+@pytest.fixture
+def products(gpu_ctx):
+    """(projection, x, weights, weight scales, numpy of the last three)."""
+    import torch
+    from tinytitan_amd.engine import Int8Projection
+    r = np.random.default_rng(1)
+    w, ws = _weights(r, ROWS, COLUMNS)
+    x = _tokens(r, TOKENS, COLUMNS)
+    made = Int8Projection(gpu_ctx), _dev(x), _dev(w), _dev(ws), x, w, ws
+    torch.cuda.synchronize()
+    return made
+
+
+def _column(values):
+    """`values` as a column of a wider tensor: [n, 1], two elements from one to the next."""
+    import torch
+    wide = torch.stack([values, torch.full_like(values, 7.0)], 1).contiguous()
+    return wide[:, :1]
+
+
+def test_scales_that_are_a_column(gpu_ctx, products):
+    import torch
+    projection, x, weights, weight_scales, nx, nw, nws = products
+    y = torch.full((TOKENS, ROWS), 3.0, dtype=torch.float16, device="cuda")
+    levels, scales = torch.full((TOKENS, COLUMNS), 9, dtype=torch.int8, device="cuda"), torch.full((TOKENS,), 9.0, device="cuda")
+    torch.cuda.synchronize()
+    for strided in (_column(weight_scales), _column(weight_scales)[:, 0]):
+        with pytest.raises(TypeError):
+            projection.encode(weights, strided, x, y, ROWS, COLUMNS, TOKENS)
+        with pytest.raises(TypeError):
+            projection.encode_levels(weights, strided, levels, scales, y, ROWS, COLUMNS, TOKENS)
+    for strided in (_column(scales), _column(scales)[:, 0]):
+        with pytest.raises(TypeError):
+            projection.quantise(x, levels, strided, COLUMNS, TOKENS)
+        with pytest.raises(TypeError):
+            projection.encode_levels(weights, weight_scales, levels, strided, y, ROWS, COLUMNS, TOKENS)
+        assert (strided == 9.0).all()
+    gpu_ctx.synchronize()
+    assert (y == 3.0).all() and (levels == 9).all() and (scales == 9.0).all()
+    # a column by itself is a vector
+    projection.quantise(x, levels, scales[:, None], COLUMNS, TOKENS)
+    projection.encode_levels(weights, weight_scales[:, None], levels, scales[:, None], y, ROWS, COLUMNS, TOKENS)
+    gpu_ctx.synchronize()
+    exact_levels, exact_scales = quantised(nx)
+    assert np.array_equal(scales.cpu().numpy(), exact_scales)
+    check(y.cpu().numpy(), exact_levels, exact_scales, nw, nws)
+
+
+def test_levels_that_are_a_column(gpu_ctx, products):
+    import torch
+    projection, x, weights, weight_scales, _, _, _ = products
+    wide = torch.full((COLUMNS, 2), 9, dtype=torch.int8, device="cuda")
+    y, scale = torch.full((1, ROWS), 3.0, dtype=torch.float16, device="cuda"), torch.full((1,), 9.0, device="cuda")
+    torch.cuda.synchronize()
+    for strided in (wide[:, :1], wide[:, 0], wide[:, :1].T):
+        with pytest.raises(TypeError):
+            projection.quantise(x[:1], strided, scale, COLUMNS, 1)
+        with pytest.raises(TypeError):
+            projection.encode_levels(weights, weight_scales, strided, scale, y, ROWS, COLUMNS, 1)
+    gpu_ctx.synchronize()
+    assert (wide == 9).all() and (y == 3.0).all() and (scale == 9.0).all()
+
+
+def test_factors_of_one_head_in_a_wider_buffer(gpu_ctx):
+    # (the factors of differential attention are rows of any stride, those of one head a column)
+    import torch
+    from tests.exact_maps import check as check_maps
+    from tests.test_gpu_attn_diff import Layer, _randn
+    from tinytitan_amd.engine import DifferentialHeads
+    layer = Layer(gpu_ctx, 1, 1, 64, [40, 700, 90])
+    wide = _dev(np.random.default_rng(1).random((3, 5)).astype(np.float32))
+    heads = DifferentialHeads(wide[:, 2:3])
+    q = _randn(5, 3, 1, 64)
+    torch.cuda.synchronize()
+    got = layer.decode(q, [40, 700, 90], heads)
+    for i, length in enumerate((40, 700, 90)):
+        check_maps(got[i:i + 1], layer.want(q[i:i + 1], i, [length - 1], heads, lambdas=wide[i, 2:3]), f"sequence {i}")
+    layer.close()

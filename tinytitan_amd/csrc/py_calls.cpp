@@ -107,10 +107,14 @@ struct Args {
     }
     // an fp32 device tensor whose last dimension is contiguous, or None
     float *floats() { return static_cast<float *>(typed(at::kFloat, "expected an fp32 device tensor with a contiguous last dimension")); }
-    // an int8 device tensor of that kind, or None
-    int8_t *levels() { return static_cast<int8_t *>(typed(at::kChar, "expected an int8 device tensor with a contiguous last dimension")); }
+    // an fp32 device vector without gaps, or None: a column of a wider tensor, [n, 1], is none
+    float *floats_in_one() { return static_cast<float *>(typed(at::kFloat, "expected a contiguous fp32 device tensor", Layout::InOne)); }
+    // an int8 device tensor whose last dimension of more than one element is contiguous, or None
+    int8_t *levels() {
+        return static_cast<int8_t *>(typed(at::kChar, "expected an int8 device tensor with a contiguous last dimension", Layout::Rows));
+    }
     // an int8 device tensor without gaps between its rows, or None
-    int8_t *levels_in_one() { return static_cast<int8_t *>(typed(at::kChar, "expected a contiguous int8 device tensor", true)); }
+    int8_t *levels_in_one() { return static_cast<int8_t *>(typed(at::kChar, "expected a contiguous int8 device tensor", Layout::InOne)); }
     // a contiguous device tensor of any type, or None
     void *raw() {
         const at::Tensor *t = tensor();
@@ -184,12 +188,23 @@ private:
         Py_DECREF(whole);
         return v;
     }
-    void *typed(at::ScalarType type, const char *what, bool in_one = false) {
+    enum class Layout {
+        LastDimension,  // next to each other in the last dimension, which may be a column of one
+        Rows,           // ... in the last one of more than one element
+        InOne,
+    };
+    static bool laid_out(const at::Tensor &t, Layout layout) {
+        if (layout == Layout::InOne) return t.is_contiguous();
+        int64_t at = t.dim() - 1;
+        while (layout == Layout::Rows && at > 0 && t.size(at) == 1) --at;
+        return at < 0 || t.size(at) <= 1 || t.stride(at) == 1;
+    }
+    void *typed(at::ScalarType type, const char *what, Layout layout = Layout::LastDimension) {
         const at::Tensor *t = tensor();
         if (!t) return nullptr;
         if (!t->is_cuda() || t->scalar_type() != type) return fail<void>(what);
         try {
-            if (in_one ? !t->is_contiguous() : t->dim() > 0 && t->size(-1) > 1 && t->stride(-1) != 1) return fail<void>(what);
+            if (!laid_out(*t, layout)) return fail<void>(what);
         } catch (const std::exception &e) {
             ok = false;
             PyErr_SetString(PyExc_RuntimeError, e.what());
@@ -743,7 +758,7 @@ TT_CALL(int8_projection) {
     if (!a.ok) return nullptr;
     auto *ctx = a.handle<tt_hip_ctx>();
     const int8_t *weights = a.levels_in_one();
-    const float *weight_scales = a.floats();
+    const float *weight_scales = a.floats_in_one();
     const tt_half *x = a.half();
     const size_t x_stride = a.size();
     tt_half *y = a.half();
@@ -762,7 +777,7 @@ TT_CALL(int8_quantise_rows) {
     const int tokens = a.i(), columns = a.i();
     int8_t *levels = a.levels();
     const size_t levels_stride = a.size();
-    float *scales = a.floats();
+    float *scales = a.floats_in_one();
     return finish(a, [&] { return lib.tt_hip_int8_quantise_rows(ctx, x, x_stride, tokens, columns, levels, levels_stride, scales); });
 }
 
@@ -772,10 +787,10 @@ TT_CALL(int8_projection_levels) {
     if (!a.ok) return nullptr;
     auto *ctx = a.handle<tt_hip_ctx>();
     const int8_t *weights = a.levels_in_one();
-    const float *weight_scales = a.floats();
+    const float *weight_scales = a.floats_in_one();
     const int8_t *levels = a.levels();
     const size_t levels_stride = a.size();
-    const float *scales = a.floats();
+    const float *scales = a.floats_in_one();
     tt_half *y = a.half();
     const int rows = a.i(), columns = a.i(), tokens = a.i();
     const size_t y_stride = a.size();

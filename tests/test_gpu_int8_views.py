@@ -1,4 +1,5 @@
-"""Tensors of the 8-bit products that are views of wider ones: scales that are a column are refused, not read as if they lay next to each other."""
+"""Tensors of the 8-bit products that are views of wider ones: scales that are a column are refused, not read as if they lay next to each other,
+and rows without a named stride have their tensor's."""
 import numpy as np
 import pytest
 
@@ -87,3 +88,29 @@ def test_factors_of_one_head_in_a_wider_buffer(gpu_ctx):
     for i, length in enumerate((40, 700, 90)):
         check_maps(got[i:i + 1], layer.want(q[i:i + 1], i, [length - 1], heads, lambdas=wide[i, 2:3]), f"sequence {i}")
     layer.close()
+
+
+@pytest.mark.parametrize("tokens", [1, 2, 6, 80])
+def test_rows_of_wider_buffers_without_a_named_stride(gpu_ctx, tokens):
+    import torch
+    from tinytitan_amd.engine import Int8Projection
+    r = np.random.default_rng(tokens)
+    w, ws = _weights(r, ROWS, COLUMNS)
+    nx = _tokens(r, tokens, COLUMNS)
+    exact_levels, exact_scales = quantised(nx)
+    projection, weights, weight_scales = Int8Projection(gpu_ctx), _dev(w), _dev(ws)
+    wide = [torch.full((tokens, width), fill, dtype=kind, device="cuda") for width, fill, kind in (
+        (COLUMNS + 24, float("nan"), torch.float16), (COLUMNS + 48, 9, torch.int8), (ROWS + 5, 3.0, torch.float16), (ROWS + 5, 3.0, torch.float16))]
+    x, levels, first, second = wide[0][:, 8:8 + COLUMNS], wide[1][:, 16:16 + COLUMNS], wide[2][:, 3:3 + ROWS], wide[3][:, 3:3 + ROWS].unflatten(1, (8, 5))
+    x.copy_(_dev(nx))
+    scales = torch.full((tokens,), 9.0, device="cuda")
+    torch.cuda.synchronize()
+    projection.encode(weights, weight_scales, x, first, ROWS, COLUMNS, tokens)
+    projection.quantise(x, levels, scales, COLUMNS, tokens)
+    projection.encode_levels(weights, weight_scales, levels, scales, second, ROWS, COLUMNS, tokens)
+    gpu_ctx.synchronize()
+    assert np.array_equal(levels.cpu().numpy(), exact_levels) and np.array_equal(scales.cpu().numpy(), exact_scales)
+    check(first.cpu().numpy(), exact_levels, exact_scales, w, ws)
+    assert torch.equal(second.flatten(1), first)
+    for buffer, at, width, fill in ((wide[1], 16, COLUMNS, 9), (wide[2], 3, ROWS, 3.0), (wide[3], 3, ROWS, 3.0)):
+        assert (buffer[:, :at] == fill).all() and (buffer[:, at + width:] == fill).all()

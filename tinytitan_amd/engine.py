@@ -668,10 +668,23 @@ class AffineProjection:
             self.ctx._check(status, "tt_hip_affine_projection")
 
 
+def _row_stride(t: torch.Tensor, width: int, named: Optional[int]) -> int:
+    """Elements from one of ``t``'s rows of ``width`` to the next: as named; without a name those of a tensor without gaps, or of a view of a
+    wider one, whose rows ``t[i]`` are ``width`` elements next to each other, its own."""
+    if named:
+        return named
+    if not isinstance(t, torch.Tensor) or t.is_contiguous():
+        return width
+    if t.dim() > 1 and t[0].numel() == width and t[0].is_contiguous():
+        return t.stride(0)
+    raise TypeError("expected rows of contiguous elements, or their stride")
+
+
 class Int8Projection:
     """``y[t] = W x[t]`` in 8-bit integers, with a scale for each token and each output channel (no counterpart in the reference, whose
     8-bit weights are affine: ``AffineProjection``).  ``weights`` is an int8 device tensor ``[rows][columns]``, ``weight_scales`` fp32
-    ``[rows]``; a token's scale is ``max |x| / 127``, its levels ``round(x / scale)``, their sum of products exact in integers."""
+    ``[rows]``; a token's scale is ``max |x| / 127``, its levels ``round(x / scale)``, their sum of products exact in integers.  Without a
+    named stride the rows of ``x``, ``levels`` and ``y`` lie without gaps, or are those of a view ``[tokens, ...]``."""
 
     def __init__(self, ctx: HIPContext):
         self.ctx = ctx
@@ -680,16 +693,18 @@ class Int8Projection:
     def encode(self, weights: torch.Tensor, weight_scales: torch.Tensor, x: torch.Tensor, y: torch.Tensor, rows: int, columns: int,
                token_count: int, x_stride: Optional[int] = None, y_stride: Optional[int] = None) -> None:
         """From fp16 tokens, which the call quantises."""
-        status = self._calls.int8_projection(self.ctx.handle, weights, weight_scales, x, x_stride or columns, y, rows, columns, token_count,
-                                             y_stride or rows)
+        x_stride = _row_stride(x, columns, x_stride)
+        y_stride = _row_stride(y, rows, y_stride)
+        status = self._calls.int8_projection(self.ctx.handle, weights, weight_scales, x, x_stride, y, rows, columns, token_count, y_stride)
         if status:
             self.ctx._check(status, "tt_hip_int8_projection")
 
     def quantise(self, x: torch.Tensor, levels: torch.Tensor, scales: torch.Tensor, columns: int, token_count: int,
                  x_stride: Optional[int] = None, levels_stride: Optional[int] = None) -> None:
         """fp16 tokens into ``levels`` (int8) and ``scales`` (fp32), once for all projections of the same input."""
-        status = self._calls.int8_quantise_rows(self.ctx.handle, x, x_stride or columns, token_count, columns, levels,
-                                                levels_stride or columns, scales)
+        x_stride = _row_stride(x, columns, x_stride)
+        levels_stride = _row_stride(levels, columns, levels_stride)
+        status = self._calls.int8_quantise_rows(self.ctx.handle, x, x_stride, token_count, columns, levels, levels_stride, scales)
         if status:
             self.ctx._check(status, "tt_hip_int8_quantise_rows")
 
@@ -697,8 +712,10 @@ class Int8Projection:
                       rows: int, columns: int, token_count: int, levels_stride: Optional[int] = None,
                       y_stride: Optional[int] = None) -> None:
         """From tokens that ``quantise`` has made; the same results as ``encode``."""
-        status = self._calls.int8_projection_levels(self.ctx.handle, weights, weight_scales, levels, levels_stride or columns, scales, y, rows,
-                                                    columns, token_count, y_stride or rows)
+        levels_stride = _row_stride(levels, columns, levels_stride)
+        y_stride = _row_stride(y, rows, y_stride)
+        status = self._calls.int8_projection_levels(self.ctx.handle, weights, weight_scales, levels, levels_stride, scales, y, rows, columns,
+                                                    token_count, y_stride)
         if status:
             self.ctx._check(status, "tt_hip_int8_projection_levels")
 

@@ -48,11 +48,11 @@ def test_dequantised_pages_of_two_gibibytes(gpu_ctx, total, bits):
     out, bound = attend_maps(q[some], k, v, KH, [start + i for i in some], at, 0, layer.scale, heads.lambdas, bits, None, heads.eps, heads.out_scale)
     # (the zeros': 2^-22 of either map's values, which are at most 8)
     check(got[some], (out, bound + 2.0 ** -22 * 8 * 2), f"{total} keys")
-    # (what the test notices: zeros in the rows' place, and in most of them a key that was left out or stood in another's place)
+    # (what the test notices: zeros in the rows' place, and a third of the keys left out)
     assert ((out.abs() > bound).double().mean(-1) > 0.5).all()
-    for j in range(0, sum(p <= start for p in at), 7):
-        others = [i for i in range(len(at)) if i != j]
+    for j in range(3):
+        others = [i for i in range(len(at)) if i * 3 // len(at) != j]
         less, _ = attend_maps(q[some], k[others], v[others], KH, [start + i for i in some], [at[i] for i in others], 0, layer.scale, heads.lambdas, bits, None,
                               heads.eps, heads.out_scale)
-        assert ((less - out).abs() > bound).any(-1).double().mean() > 0.5, j
+        assert ((less - out).abs() > bound).any(-1).all(), j
     layer.close()

@@ -347,18 +347,10 @@ static int run_attention(tt_hip_ctx *ctx, tt_hip_kv *kv, int kind, int layer, in
         int st = plan_launch(ctx, kind, n, n_q_heads, kv->n_kv_heads, D, rows, total_keys, min_keys, max_keys, &plan, kv_bits,
                              small_tiles_ok);
         if (st != TT_HIP_OK) return st;
-        // Two maps' rows: one split, whose launch writes the finished rows, up to more keys than the planner's 384, since the launch it saves is dearer:
-        // five key blocks a wavefront of heads of 256, six of 128, eight of 64.  us, several splits / one, fp16: 16/2 heads of 256 512 keys 10.3 / 9.2, 600 10.3 /
-        // 10.0, 700 9.7 / 10.9; 32/8 of 128 600 8.4 / 7.1, 768 8.2 / 7.8, 900 8.3 / 8.7; 16/4 of 64 768 7.3 / 6.5, 1,024 7.4 / 7.3, 1,280 7.7 / 8.2; 8
-        // sequences of 32/8 heads 600 10.1 / 8.9, 768 10.1 / 10.9.  Blocks of quantised pages cost a wavefront more: 8 bits, 16/2 of 256, 448 keys 10.3 / 11.1, 4
-        // bits, 32/8 of 128, 512 8.8 / 8.4, 600 8.9 / 9.4.
-        if (piece && piece->maps && ctx->split_override <= 0 && plan.n_splits_max > 1) {
-            const int blocks = kv_bits == 16 ? (D == 256 ? 5 : D == 128 ? 6 : 8) : D == 256 ? 3 : 4, one_up_to = blocks * 32 * plan.waves;
-            if (max_keys <= one_up_to && plan.gh % 2 == 0) {
-                plan.split_len = (max_keys + 31) / 32 * 32;
-                plan.n_splits_max = 1;
-                plan.workgroups = (long long)plan.n_tiles * n;
-            }
+        if (piece && piece->maps && ctx->split_override <= 0 && plan.n_splits_max > 1 && max_keys <= maps_one_split_up_to(D, kv_bits) && plan.gh % 2 == 0) {
+            plan.split_len = (max_keys + 31) / 32 * 32;
+            plan.n_splits_max = 1;
+            plan.workgroups = (long long)plan.n_tiles * n;
         }
         if (chunk_splits > 1) {  // the chunk kernel's geometry: 32-row one-head tiles, its own key ranges
             // (a tile that walked past the launched ranges would lose keys, and the combine pass would count a partial result more)

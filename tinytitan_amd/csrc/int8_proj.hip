@@ -6,6 +6,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "int8_plan.h"
 #include "internal.h"
 #include "lds_copy.h"
 #include "wave_ops.h"
@@ -658,14 +659,6 @@ int launch_quantise(tt_hip_ctx *ctx, const tt_half *x, size_t x_stride, int toke
     return e == hipSuccess ? TT_HIP_OK : hip_fail(ctx, e, "quantise_rows_kernel launch");
 }
 
-// Channels of a workgroup of the few tokens' kernel, in tiles of 16: as many as leave 9/16 of the CUs a workgroup.  us by one tile /
-// two / four: one token, 2,048 x 4,096 (128, 64, 32 workgroups) 5.2 / 5.8 / 7.6; 5,120 x 6,144 9.0 / 8.2 / 11.0; 9,216 x 2,048 7.1 / 8.0 / 6.8; 64
-// tokens, 4,096 x 4,096 9.5 / 10.9 / 15.0; 48, 5,120 x 6,144 18.5 / 12.4 / 18.3.
-int ring_tiles(const tt_hip_ctx *ctx, int rows) {
-    for (int tiles = 4; tiles > 1; tiles /= 2)
-        if (16ll * ((rows + 16 * tiles - 1) / (16 * tiles)) >= 9ll * ctx->n_cus) return tiles;
-    return 1;
-}
 // Tiles of the many tokens' kernel: what they are estimated to take, rounds of workgroups times their stages, us as measured with every CU
 // at work (4,096 tokens, 9,216 x 5,120; 777, 2,311 x 4,096; 1,024 and 128, 4,096 x 4,096).
 struct GemmTile {
@@ -688,7 +681,7 @@ int gemm_tile(const tt_hip_ctx *ctx, const ProductArgs &a) {
     return best;
 }
 void launch_by_rule(tt_hip_ctx *ctx, const ProductArgs &a) {
-    const int tiles = ring_tiles(ctx, a.rows), token_tiles = (a.tokens + 15) / 16;
+    const int tiles = int8_ring_tiles(ctx->n_cus, a.rows), token_tiles = (a.tokens + 15) / 16;
     if (token_tiles <= 4 && !(tiles == 4 && token_tiles == 4)) {
         switch (tiles * 10 + token_tiles) {
             case 11: return launch_ring<1, 1, 8, 2, false>(ctx, a);
@@ -726,7 +719,7 @@ int launch_product(tt_hip_ctx *ctx, const ProductArgs &a) {
 // less, of 3 us, for what every workgroup spends on them (us on the device, with it / by two launches: one token, 2,048 x 4,096 5.9 /
 // 9.2, four 7.4 / 9.5, 9,216 x 2,048 7.6 / 11.3, four 7.9 / 11.1, 5,120 x 6,144 8.6 / 13.1).
 int launch_fused(tt_hip_ctx *ctx, const ProductArgs &a, const _Float16 *halves, long long halves_stride, bool *served) {
-    const int tiles = ring_tiles(ctx, a.rows);
+    const int tiles = int8_ring_tiles(ctx->n_cus, a.rows);
     const size_t lds = tiles == 4   ? ring_lds_bytes<4, 1, 4, 3, true>(a.tokens, a.columns)
                        : tiles == 2 ? ring_lds_bytes<2, 1, 8, 3, true>(a.tokens, a.columns)
                                     : ring_lds_bytes<1, 1, 8, 4, true>(a.tokens, a.columns);

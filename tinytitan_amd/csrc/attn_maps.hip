@@ -12,9 +12,12 @@
 // Memory bounds a long decode: 205 MB behind 100,001 keys of 16/2 heads of 256 take 40 us, the pass alone 32 (6.4 TB/s).  The join reads 2 KiB
 // a (token, head) and split, by one CU an item, since the norm needs the whole row: 112 splits, 7 us.
 //
-// Roundings: a weight of either map is rounded to fp16 for the second product, as in every kernel here (its sum is that of the rounded weights over fp16
-// pages), and over quantised pages a K operand is.  Against 64 bits 2.5 - 3e-4 over fp16 pages (2-norm; the final rounding alone is 2.0e-4) and
-// 4.6 - 7e-4 over 8 and 4 bits: a difference of maps keeps the errors of both and little of their sums.
+// Roundings, beside the last one of a row: the matrix instructions' operands are fp16, as in every kernel here.  A weight of either map is rounded to it for
+// the second product (its sum is that of the rounded weights over fp16 pages).  Over quantised pages so is a K operand, level * scale + bias, and in
+// the split-K kernel a weight once more behind its product with a group's V scale, once for the group's 64 dims where a widened V operand would be
+// rounded in each; in front of the chunk kernel every value of K and V is, whose pages are dequantised to fp16.  Against 64 bits 2.5 - 3e-4 over fp16
+// pages (2-norm; the final rounding alone is 2.0e-4) and 4.6 - 7e-4 over 8 and 4 bits: a difference of maps keeps the errors of both and little of
+// their sums.
 #include <algorithm>
 
 #include "splitk_kernel.h"

@@ -13,8 +13,10 @@
 // vector memory path, 768.  One wavefront a SIMD has all 512 registers (256 of them sums over V), so nothing but its own order hides one kind of work
 // behind another: the softmax of block i is cut into pieces of a few instructions each, one between any two of the products of block i's
 // scores and block i - 1's values.  Heads of 128 leave room for two wavefronts a SIMD with a tile each, which hide each other's waits (one wavefront with
-// two tiles issued 68 % of its cycles, with the matrix pipe busy for 41, and waited 19; the two issue 92 % of their SIMD's, the matrix pipe 48) at twice
-// the LDS traffic, 1,024 cycles beside 768 of products.
+// two tiles issued 68 % of its cycles, with the matrix pipe busy for 41, and waited 19; the two issue 92 % of their SIMD's, the matrix pipe 48) at nearly twice
+// the LDS traffic, 72 KiB a block with the copies, 1,152 cycles, in place of 40, beside 768 of products.  Heads of 64 are bound by their instructions: a
+// product has twice the exponentials, conversions and maxima of one of 128, the two wavefronts of a SIMD issue 112 cycles in 100 (of different kinds
+// side by side), and the matrix pipe is busy for 38.
 //
 // Measured, us a call: 4,096 rows behind 4,500 keys 586 - 605 with 16/2 heads of 256 (1.09 - 1.12 PFLOP/s, of 1.22 that a library product reaches),
 // 704 with 32/8 of 128 (0.94; two tiles a wavefront 716), 240 - 249 with 16/4 of 64 (0.66 - 0.69); 777 rows behind 9,000 of 32/8 heads of 128 230 - 235

@@ -101,7 +101,7 @@ struct ProductArgs {
 // the many tokens' kernel has them in: a load of v_mfma_i32_16x16x64_i8's operands from memory takes sixteen rows in pieces of 16 bytes that
 // the vector memory path handles one by one, a quarter of its rate (one token, 9,216 x 2,048: 11.8 us so).
 // Tokens' rows go the same way, or, FUSED, are quantised into LDS by the workgroup itself beside its first weights' way (up to four
-// tokens, whose pieces fit a wavefront's registers).
+// tokens, a wavefront each or more, whose halves and levels lie in LDS behind the rings).
 constexpr int kStageBytes = 128;
 constexpr int kFusedTokens = 4;
 // Tokens that a workgroup shares its wavefronts out to: a power of two.

@@ -538,8 +538,8 @@ TT_HIP_API int tt_hip_attn_prefill_shared(tt_hip_ctx *ctx, tt_hip_kv *kv, int la
  *   gate           the sigmoid gate behind that, or NULL.
  * Softmax statistics, sums, difference and norm are in fp32, with one rounding to fp16.  A row without a visible key (a sequence of
  * length 0) gives zeros.  Values of keys that no row of a call sees do not reach it, whatever the cache holds there; a value that is not
- * finite and that some row sees may reach the sequence's other rows of the call, and a key that is not finite makes NaN of the rows that see it,
- * in either map.
+ * finite and that some row sees may reach the sequence's other rows of the call, and a key that is not finite may make NaN of the
+ * rows that see it, in either map.
  * Both maps come from one pass over the cache.  Partial results of a pass over several ranges of keys and, over quantised pages, a chunk's
  * dequantised blocks live in stores that the context owns, grown on demand.  Inside a graph capture in which they would have to grow a chunk
  * takes a way that does without (over quantised pages where its dequantised blocks have room, or its tiles' keys are one range), a slower one

@@ -82,10 +82,10 @@ static int ensure_keep_rows(tt_hip_ctx *ctx, size_t bytes) {
     if (ctx->capturing) return TT_HIP_ERR_BUSY;
     hipError_t e = hipStreamSynchronize(ctx->stream);
     if (e != hipSuccess) return hip_fail(ctx, e, "hipStreamSynchronize");
+    if (ctx->keep_rows) ++ctx->generation;
     if (ctx->keep_rows) (void)hipFree(ctx->keep_rows);
     ctx->keep_rows = nullptr;
     ctx->keep_rows_bytes = 0;
-    ++ctx->generation;
     const size_t want = bytes + bytes / 4;
     e = hipMalloc(reinterpret_cast<void **>(&ctx->keep_rows), want);
     if (e != hipSuccess) return hip_fail(ctx, e, "hipMalloc(selection rows)");

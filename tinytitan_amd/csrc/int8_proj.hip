@@ -737,10 +737,10 @@ int ensure_levels(tt_hip_ctx *ctx, size_t bytes) {
     if (ctx->capturing) return TT_HIP_ERR_BUSY;
     hipError_t e = hipStreamSynchronize(ctx->stream);
     if (e != hipSuccess) return hip_fail(ctx, e, "hipStreamSynchronize");
+    if (ctx->levels) ++ctx->generation;  // (a store that there was not yet is in no graph)
     if (ctx->levels) (void)hipFree(ctx->levels);
     ctx->levels = nullptr;
     ctx->levels_bytes = 0;
-    ++ctx->generation;
     const size_t want = bytes + bytes / 4;
     e = hipMalloc(reinterpret_cast<void **>(&ctx->levels), want);
     if (e != hipSuccess) return hip_fail(ctx, e, "hipMalloc(token levels)");

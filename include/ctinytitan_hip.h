@@ -682,7 +682,8 @@ TT_HIP_API int tt_hip_affine_projection(tt_hip_ctx *ctx, int weight_bits, const 
  * TT_HIP_ERR_BUSY inside a graph capture if it has to grow).  No counterpart in the reference, whose 8-bit weights are affine
  * (tt_hip_affine_projection).
  * TT_HIP_ERR_SHAPE: columns not a multiple of 16 or 131,072 and more (whose sums could leave 32 bits), strides below the row widths, x,
- * levels or weights not 16-byte aligned, x_stride not a multiple of 8, levels_stride not one of 16 or, in front of a product, 2^24 and more. */
+ * levels or weights not 16-byte aligned, x_stride not a multiple of 8, levels_stride not one of 16 or, in front of a product, 2^24 and more,
+ * 2^24 tokens and more to be quantised. */
 TT_HIP_API int tt_hip_int8_projection(tt_hip_ctx *ctx, const int8_t *weights, const float *weight_scales, const tt_half *x, size_t x_stride,
                                       tt_half *y, int rows, int columns, int token_count, size_t y_stride);
 TT_HIP_API int tt_hip_int8_quantise_rows(tt_hip_ctx *ctx, const tt_half *x, size_t x_stride, int token_count, int columns, int8_t *levels,

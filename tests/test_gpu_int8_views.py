@@ -114,3 +114,16 @@ def test_rows_of_wider_buffers_without_a_named_stride(gpu_ctx, tokens):
     assert torch.equal(second.flatten(1), first)
     for buffer, at, width, fill in ((wide[1], 16, COLUMNS, 9), (wide[2], 3, ROWS, 3.0), (wide[3], 3, ROWS, 3.0)):
         assert (buffer[:, :at] == fill).all() and (buffer[:, at + width:] == fill).all()
+
+
+def test_more_tokens_than_a_launch_has_workgroups_are_refused(gpu_ctx, products):
+    from tinytitan_amd import capi
+    projection, x, weights, weight_scales, _, _, _ = products
+    import torch
+    y, levels, scales = torch.zeros(TOKENS, ROWS, dtype=torch.float16, device="cuda"), torch.zeros(TOKENS, COLUMNS, dtype=torch.int8, device="cuda"), torch.zeros(TOKENS, device="cuda")
+    lib, many = gpu_ctx._lib, 1 << 24
+    assert lib.tt_hip_int8_quantise_rows(gpu_ctx.handle, x.data_ptr(), COLUMNS, many, COLUMNS, levels.data_ptr(), COLUMNS, scales.data_ptr()) == capi.ERR_SHAPE
+    assert lib.tt_hip_int8_projection(gpu_ctx.handle, weights.data_ptr(), weight_scales.data_ptr(), x.data_ptr(), COLUMNS, y.data_ptr(), ROWS, COLUMNS, many,
+                                      ROWS) == capi.ERR_SHAPE
+    gpu_ctx.synchronize()
+    assert not levels.any() and not y.any()

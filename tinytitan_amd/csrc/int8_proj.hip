@@ -631,12 +631,14 @@ void launch_steps(tt_hip_ctx *ctx, const ProductArgs &a) {
 
 bool aligned(const void *p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
+// Tokens that a call quantises: a workgroup of 256 threads each, of which a launch has fewer than 2^32.
+bool tokens_served(int tokens) { return tokens < 1 << 24; }
 // (the sums of products of two levels, at most 2^14 each, stay below 2^31)
 bool columns_served(int columns) { return columns % 16 == 0 && columns < 131072; }
 
 int check_quantise(const tt_half *x, size_t x_stride, int token_count, int columns, const int8_t *levels, size_t levels_stride, const float *scales) {
     if (!x || !levels || !scales || token_count <= 0 || columns <= 0) return TT_HIP_ERR_INVALID_ARGUMENT;
-    if (!columns_served(columns) || x_stride < (size_t)columns || x_stride % 8 != 0 || levels_stride < (size_t)columns || levels_stride % 16 != 0 ||
+    if (!columns_served(columns) || !tokens_served(token_count) || x_stride < (size_t)columns || x_stride % 8 != 0 || levels_stride < (size_t)columns || levels_stride % 16 != 0 ||
         !aligned(x, 16) || !aligned(levels, 16))
         return TT_HIP_ERR_SHAPE;
     return TT_HIP_OK;
@@ -802,7 +804,7 @@ int tt_hip_int8_projection(tt_hip_ctx *ctx, const int8_t *weights, const float *
     const int st = check_product(weights, weight_scales, y, rows, columns, token_count, y_stride);
     if (st != TT_HIP_OK) return st;
     if (!x) return TT_HIP_ERR_INVALID_ARGUMENT;
-    if (x_stride < (size_t)columns || x_stride % 8 != 0 || !aligned(x, 16)) return TT_HIP_ERR_SHAPE;
+    if (!tokens_served(token_count) || x_stride < (size_t)columns || x_stride % 8 != 0 || !aligned(x, 16)) return TT_HIP_ERR_SHAPE;
     BusyGuard guard(ctx);
     if (!guard.ok) return TT_HIP_ERR_BUSY;
     if (hipSetDevice(ctx->device) != hipSuccess) return TT_HIP_ERR_HIP;

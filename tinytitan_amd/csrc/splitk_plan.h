@@ -126,7 +126,8 @@ inline int plan_splitk(int n_cus, int split_override, int kind, int n_seq, int n
 //   32/8 heads of 128, one sequence 640 keys 8.5 / 7.1, 704 9.0 / 7.5, 768 8.7 / 8.1; four 576 9.1 / 9.2, 640 9.2 / 9.9, 704 9.4 / 10.4, 768 9.5 / 11.1; eight 640
 //   10.4 / 10.2, 704 10.6 / 10.7, 768 10.7 / 11.5; sixteen 640 13.3 / 11.1, 704 13.6 / 11.7, 768 14.2 / 12.5; four rows of four sequences 640 10.8 / 10.2, 768 10.9 / 11.3
 //   16/4 of 64, one 1,024 7.6 / 7.1; four 896 8.7 / 7.4, 1,024 8.0 / 8.2; sixteen 1,024 9.5 / 8.8
-//   16/2 of 256, one 448 9.5 / 9.4, 512 9.5 / 10.0, 640 9.7 / 11.2; four 448 10.9 / 12.2, 640 11.2 / 16.2; sixteen 448 12.2 / 14.0, 640 12.3 / 17.6
+//   16/2 of 256, one 448 9.5 / 9.4, 512 9.5 / 10.0, 640 9.7 / 11.2; four 448 10.9 / 12.2, 640 11.2 / 16.2; sixteen 448 12.2 / 14.0, 640 12.3 / 17.6;
+//   8/2 of 256, one 448 8.9 / 8.5, 600 9.0 / 10.0, four 600 10.4 / 14.6
 // and 512 keys over 8 bits, 32/8 of 128, one 8.3 / 7.5, sixteen 10.2 / 8.2; 4 bits 8.8 / 8.1, 10.1 / 8.8.
 inline int maps_one_split_up_to(int head_dim, int kv_bits) {
     if (head_dim == 256) return 0;  // (the planner's own)

@@ -62,7 +62,8 @@ enum tt_hip_status {
 
 /* Replaces MetalContext + the per-Attention split scratch
  * (sources/TinyTitan/Kernels/Attention/Attention.swift:59-71,140-156): owns a
- * HIP stream, the split-K partial buffers and timing events. */
+ * HIP stream, the split-K partial buffers and timing events.  A context's
+ * caches are destroyed before it. */
 TT_HIP_API tt_hip_ctx *tt_hip_ctx_create(int device, int *out_err);
 TT_HIP_API void tt_hip_ctx_destroy(tt_hip_ctx *ctx);
 
